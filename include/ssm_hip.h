@@ -215,6 +215,70 @@ ssm_status ssm_m1_xproj_dt(const float* x, long ldx, const float* Wx, const floa
                            float* dbl, long lddbl, float* dt, long lddt, int T, int D, int R,
                            int N, void* stream);
 
+/* ---- A linear-attention layer with 8-bit projections (no counterpart in the reference). Element
+ * types are SSM_F32 and SSM_BF16; one call's q, k, v and outputs share theirs. */
+
+/* RMS norm of every query and key head, with the position rotation, in one pass:
+ *   x' = x / sqrt(mean x^2 + eps) * w over the D elements of a head; then the pairs of its first R
+ *   elements, with t = pos freq_i (i < R/2): (a, b) <- (a cos t - b sin t, b cos t + a sin t).
+ * Pairs are (i, i + R/2), with `interleaved` (2i, 2i + 1). q (T,H,D), k (T,G,D) with row strides
+ * (heads of a row follow one another); wq, wk (D) float or NULL (ones); pos (T) int32; freq (R/2)
+ * doubles, radians per position; all on the device. R even, R <= D <= 512 (R 0: norm alone, pos
+ * and freq may be NULL; H or G may be 0). qo, ko may be q, k. Angles are formed in double, the
+ * rest in fp32, outputs rounded once. */
+ssm_status ssm_qk_norm_rope(int dtype, const void* q, long ldq, const void* k, long ldk,
+                            const float* wq, const float* wk, const int* pos, const double* freq,
+                            int interleaved, float eps, void* qo, long ldqo, void* ko, long ldko,
+                            int T, int H, int G, int D, int R, void* stream);
+
+/* Linear attention with a constant decay for each head, over whole prompts:
+ *   S_t = e^{g_h} S_{t-1} + v_t k_t^T  (V x K, fp32);  y_t = scale S_t q_t
+ * q (B,L,H,K), k (B,L,G,K), v (B,L,G,V), y (B,L,H,V) with row strides; query head h reads the keys
+ * and values of head h / (H / G). g (H) float, log decays (<= 0; -inf keeps nothing). lengths (B)
+ * int32 on the device or NULL: sequence b has lengths[b] tokens (held to 0 .. L); rows of y from
+ * there on are not written, and what q, k and v hold there is not used. h0, hT (B,H,V,K) float: the
+ * states before the first and after each sequence's last token; either may be NULL, hT may be h0.
+ * K <= 256 (SSM_ERR_UNSUPPORTED above). An inf or NaN changes no earlier token (from its own token
+ * on, results that it touches are inf or NaN). `workspace` (16-byte aligned) holds
+ * ssm_linear_attention_workspace(...) bytes and serves one stream at a time. */
+size_t ssm_linear_attention_workspace(int dtype, int B, int L, int H, int K, int V);
+ssm_status ssm_linear_attention(int dtype, const void* q, long ldq, const void* k, long ldk,
+                                const void* v, long ldv, const float* g, float scale,
+                                const int* lengths, void* y, long ldy, int B, int L, int H, int G,
+                                int K, int V, const float* h0, float* hT, void* workspace,
+                                size_t workspace_bytes, void* stream);
+/* The same for one token of B sequences, h (B,H,V,K) in place. q (B,H,K), k (B,G,K), v (B,G,V),
+ * y (B,H,V) with row strides. */
+ssm_status ssm_linear_attention_step(int dtype, const void* q, long ldq, const void* k, long ldk,
+                                     const void* v, long ldv, const float* g, float scale, void* y,
+                                     long ldy, float* h, int B, int H, int G, int K, int V,
+                                     void* stream);
+
+/* Rows to 8-bit integers: scale_m = max_k |x_mk| / 127 (fp32), q_mk = x_mk / scale_m to the nearest
+ * integer (of the exact quotient; ties to even), held to -127 .. 127. A row of zeros gets scale 0; a
+ * row with an inf or NaN gets zeros and that scale, so that its products are NaN. */
+ssm_status ssm_quantize_rows(int dtype, const void* x, long ldx, int8_t* q, long ldq, float* scale,
+                             int M, int K, void* stream);
+/* y[m,n] = beta*y[m,n] + sx[m] sw[n] sum_k x[m,k] W[n,k] (+ bias[n]) with 8-bit x (M,K), W (N,K):
+ * exact 32-bit integer sums, so K <= 131071. beta 0 does not read y. y of `out_dtype` (SSM_F32,
+ * SSM_BF16). 16-byte aligned rows (ldw % 16 == 0; K % 4 == 0, for x K % 256 == 0) are read in
+ * place; others are laid out in the workspace first. Row strides below 2^22.
+ * workspace: 16-byte aligned, ssm_linear_i8_workspace(...) bytes (0 where nothing is laid out), one
+ * stream at a time. */
+size_t ssm_linear_i8_workspace(const int8_t* x, long ldx, const int8_t* W, long ldw, int M, int N,
+                               int K);
+ssm_status ssm_linear_i8(const int8_t* x, long ldx, const float* sx, const int8_t* W, long ldw,
+                         const float* sw, const float* bias, int out_dtype, void* y, long ldy, int M,
+                         int N, int K, float beta, void* workspace, size_t workspace_bytes,
+                         void* stream);
+/* ssm_quantize_rows of x (M,K), elements of in_dtype, then ssm_linear_i8, in one call: the
+ * activations' scales are found as they come. Bit-equal to the two calls. */
+size_t ssm_linear_q8_workspace(const int8_t* W, long ldw, int M, int N, int K);
+ssm_status ssm_linear_q8(int in_dtype, const void* x, long ldx, const int8_t* W, long ldw,
+                         const float* sw, const float* bias, int out_dtype, void* y, long ldy, int M,
+                         int N, int K, float beta, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 /* Greedy pick per row (sampleToken with topK = 1, src/session/streaming.ts:74-75): index
  * of the largest value, lowest index among equal maxima; NaN never wins (0 for an all-NaN
  * row). x (rows, n) with row stride ldx; out (rows) uint32. */

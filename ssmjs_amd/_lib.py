@@ -108,6 +108,20 @@ PROTOTYPES = {
                              _vp]),
     "ssm_linear": (_i, [_fp, _l, _fp, _l, _fp, _fp, _l, _i, _i, _i, _f, _vp]),
     "ssm_m1_xproj_dt": (_i, [_fp, _l, _fp, _fp, _fp, _l, _fp, _l, _i, _i, _i, _i, _vp]),
+    "ssm_qk_norm_rope": (_i, [_i, _vp, _l, _vp, _l, _fp, _fp, _vp, _vp, _i, _f, _vp, _l, _vp, _l,
+                              _i, _i, _i, _i, _i, _vp]),
+    "ssm_linear_attention_workspace": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "ssm_linear_attention": (_i, [_i, _vp, _l, _vp, _l, _vp, _l, _fp, _f, _vp, _vp, _l, _i, _i, _i,
+                                  _i, _i, _i, _fp, _fp, _vp, _sz, _vp]),
+    "ssm_linear_attention_step": (_i, [_i, _vp, _l, _vp, _l, _vp, _l, _fp, _f, _vp, _l, _fp, _i, _i,
+                                       _i, _i, _i, _vp]),
+    "ssm_quantize_rows": (_i, [_i, _vp, _l, _vp, _l, _fp, _i, _i, _vp]),
+    "ssm_linear_i8_workspace": (_sz, [_vp, _l, _vp, _l, _i, _i, _i]),
+    "ssm_linear_i8": (_i, [_vp, _l, _fp, _vp, _l, _fp, _fp, _i, _vp, _l, _i, _i, _i, _f, _vp, _sz,
+                           _vp]),
+    "ssm_linear_q8_workspace": (_sz, [_vp, _l, _i, _i, _i]),
+    "ssm_linear_q8": (_i, [_i, _vp, _l, _vp, _l, _fp, _fp, _i, _vp, _l, _i, _i, _i, _f, _vp, _sz,
+                           _vp]),
     "ssm_argmax": (_i, [_fp, _l, _i, _i, _vp, _vp]),
     "ssm_sample_workspace": (_sz, [_i, _i]),
     "ssm_sample": (_i, [_fp, _l, _i, _i, _d, _i, _d, _vp, _vp, _vp, _sz, _vp]),

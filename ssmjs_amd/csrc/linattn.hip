@@ -1,0 +1,968 @@
+// Linear attention with a constant decay for each head, chunked for prompts and recurrent for
+// single tokens (Katharopoulos et al. 2020; decays as in Sun et al. 2023, section 2):
+//   S_t = e^g S_{t-1} + v_t k_t^T  (V x K, fp32);   y_t = scale S_t q_t.
+// Query heads h share the keys and values of head h / (H / G).
+//
+// Chunked form. With C tokens a chunk, S the state before it and i, j its tokens:
+//   y_i = scale e^{g (i + 1)} S q_i + sum_{j <= i} scale e^{g (i - j)} (q_i . k_j) v_j
+//   S  <- e^{g C} S + sum_j (e^{g (C - 1 - j)} v_j) k_j^T
+// One workgroup walks the chunks of a segment of one (sequence, head, part of V) with S in its
+// MFMA accumulators. Sequences are cut into segments where (sequence, head, part) alone would
+// not fill the chip: a state pass forms each segment's own state, a combine pass the states that
+// enter the segments, and the full pass starts from those.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.hpp"
+
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+
+constexpr unsigned kOut = 0x80000000u;   // a buffer offset past any descriptor
+
+struct LaArgs {
+    const void* q; long ldq;
+    const void* k; long ldk;
+    const void* v; long ldv;
+    const float* g;
+    float scale;
+    const int* lengths;      // (B) or null: L for all
+    void* y; long ldy;
+    int B, L, H, G, K, V;
+    const float* h0;         // (B,H,V,K) or null
+    float* hT;               // (B,H,V,K) or null
+    float* seg;              // (nseg,B,H,V,K): own states, then entering states
+    int nseg, seglen, vparts;
+};
+
+// e^{g n} - 1 and e^{g n}. g = -inf keeps nothing (and n = 0 everything).
+__device__ __forceinline__ float decay_m1(float g, int n) { return expm1f(g * (float)n); }
+__device__ __forceinline__ float clamp_g(float g) { return fmaxf(g, -1e30f); }
+
+__device__ __forceinline__ int seq_len(const LaArgs& a, int b) {
+    if (!a.lengths) return a.L;
+    return max(0, min(a.lengths[b], a.L));
+}
+
+// Workgroup order: consecutive ids (the parts of V and the heads of a group, which read the same
+// keys and values) on one XCD.
+__device__ __forceinline__ int xcd_order(int b, int T) {
+    const int xcd = b & 7, per = T >> 3, rem = T & 7;
+    return xcd * per + min(xcd, rem) + (b >> 3);
+}
+
+// ---------------------------------------------------------------- bf16
+// Tiles of v_mfma_f32_16x16x32_bf16 (A: row lane % 16, 8 k at 8 (lane / 16); D: column lane % 16,
+// rows 4 (lane / 16) + r). Wave w owns VT / 4 columns of V in S^T (rows k, columns v). The
+// accumulators of two of its 16 x 16 tiles are, rounded, the A operand of S q^T with the 32 k of
+// the block taken in the order (16 t + 4 g + r, 16 (t + 1) + 4 g + r); q is read from LDS in that
+// order. The 64 x 64 products q k^T are shared out over the waves by rows i and go through LDS.
+//
+// Roundings to bf16: the products q k^T with their decay, and S as an operand (in two parts, hi +
+// lo, 16 bits): S itself stays fp32. The values of the state update are e^{..} v in three parts
+// (24 bits), so that the state carries fp32 rounding only.
+__device__ __forceinline__ floatx4 mfma(bf16x8 a, bf16x8 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// M[row0 .. + 3][col0 + lane % 16] of a row-major LDS tile: inside each 16-lane group lane 4a + b
+// receives element b of the 8-byte pieces that lanes a, a + 4, a + 8, a + 12 address.
+template <int PITCH>
+__device__ __forceinline__ bf16x4 tr_read(const __bf16* base, int row0, int col0, int l16) {
+    const __bf16* p = base + (row0 + (l16 >> 2)) * PITCH + col0 + 4 * (l16 & 3);
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p);
+}
+
+__device__ __forceinline__ bf16x8 cat(bf16x4 a, bf16x4 b) {
+    return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// Whether a dword of two bf16 holds an inf or NaN: bit 15 or 31 set.
+__device__ __forceinline__ unsigned odd_bf16(unsigned u) {
+    return ((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+
+constexpr int CB = 64;   // tokens per chunk
+
+template <int KD, int VT>
+struct SmemB {
+    static constexpr int KP = KD + 8, VP = VT + 8, PP = CB + 8;
+    alignas(16) __bf16 q[CB][KP];
+    alignas(16) __bf16 k[CB][KP];
+    alignas(16) __bf16 v[CB][VP];
+    alignas(16) __bf16 p[CB][PP];   // scale e^{g (i - j)} q_i . k_j, row i
+    int odd[2];                     // an inf or NaN in the chunk's v (by the chunk's parity)
+};
+
+// 16 bytes (8 elements) of row `row`, columns col .. + 7, zeros past the descriptor and from
+// column `width` on.
+template <bool VEC>
+__device__ __forceinline__ uint4 fetch_b(__amdgpu_buffer_rsrc_t r, unsigned row, unsigned ld,
+                                         int col, int width) {
+    const unsigned o = (row * ld + (unsigned)col) * 2u;
+    if constexpr (VEC) {
+        return ssm::bload16<uint4>(r, col < width ? o : kOut);
+    } else {
+        unsigned u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const unsigned lo = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(
+                r, col + 2 * e < width ? o + 4u * e : kOut, 0, 0);
+            const unsigned hi = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(
+                r, col + 2 * e + 1 < width ? o + 4u * e + 2u : kOut, 0, 0);
+            u[e] = lo | hi << 16;
+        }
+        return make_uint4(u[0], u[1], u[2], u[3]);
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ floatx4 load_state4(const float* p, int left) {
+    if constexpr (VEC) {
+        return left > 0 ? *reinterpret_cast<const floatx4*>(p) : floatx4{0.f, 0.f, 0.f, 0.f};
+    } else {
+        floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < left) s[e] = p[e];
+        return s;
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_state4(float* p, floatx4 s, int left) {
+    if constexpr (VEC) {
+        if (left > 0) *reinterpret_cast<floatx4*>(p) = s;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < left) p[e] = s[e];
+    }
+}
+
+// STATE: only the segment's own state (from zero), into its slot.
+template <int KD, int VT, bool VEC, bool STATE>
+__global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs a) {
+    using Smem = SmemB<KD, VT>;
+    constexpr int KT = KD / 16, KB = KD / 32, VW = VT / 64;
+    constexpr int KP = Smem::KP, VP = Smem::VP, PP = Smem::PP;
+    constexpr int NK = CB * KD / 8 / 256, NV = CB * VT / 8 / 256;
+    __shared__ Smem s;
+
+    const int id = xcd_order(blockIdx.x, gridDim.x);
+    const int part = id % a.vparts, bh_s = id / a.vparts;
+    const int h = bh_s % a.H, b = bh_s / a.H % a.B, seg = bh_s / a.H / a.B;
+    const int grp = h / (a.H / a.G);
+    const int len = seq_len(a, b);
+    const int t_begin = seg * a.seglen, t_end = min(len, t_begin + a.seglen);
+    // the segment that ends the sequence writes the final state (segment 0 of an empty one)
+    const bool last = seg == (len > 0 ? (len - 1) / a.seglen : 0);
+    if (STATE ? last || t_begin >= len : !last && t_begin >= len) return;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g4 = lane >> 4, l16 = lane & 15;
+    const int v0 = part * VT + 16 * VW * w;     // the wave's first column of V
+    const float g = clamp_g(a.g[h]), gl = g * ssm::kLog2e;
+    const long state = ((long)b * a.H + h) * a.V * a.K;
+    const long slot = (long)a.B * a.H * a.V * a.K;
+
+    floatx4 S[KT][VW];
+    auto each_state = [&](auto&& f) {
+#pragma unroll
+        for (int x = 0; x < VW; ++x) {
+            const int v = v0 + 16 * x + l16;
+            if (v < a.V) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int kk = 16 * kt + 4 * g4;
+                    f(S[kt][x], (long)v * a.K + kk, a.K - kk);
+                }
+            }
+        }
+    };
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int x = 0; x < VW; ++x) S[kt][x] = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (!STATE) {
+        const float* from = a.nseg > 1 ? (seg || a.h0 ? a.seg + seg * slot : nullptr) : a.h0;
+        if (from)
+            each_state([&](floatx4& r, long o, int left) {
+                r = load_state4<VEC>(from + state + o, left);
+            });
+    }
+
+    // ---- a chunk's rows in registers, ahead of their staging
+    uint4 rq[STATE ? 1 : NK], rk[NK], rv[NV];
+    auto base = [&](const void* p, long ld, int head, int width, int t) {
+        return static_cast<const __bf16*>(p) + ((long)b * a.L + t) * ld + (long)head * width;
+    };
+    auto bytes = [&](long ld, int width, int n) {
+        return n > 0 ? (unsigned)(((long)(n - 1) * ld + width) * 2) : 0u;
+    };
+    auto fetch = [&](int t) {
+        const int n = max(0, min(CB, t_end - t));
+        const int tt = min(t, a.L - 1);
+        const auto dk = ssm::rsrc(base(a.k, a.ldk, grp, a.K, tt), bytes(a.ldk, a.K, n));
+        const auto dv = ssm::rsrc(base(a.v, a.ldv, grp, a.V, tt), bytes(a.ldv, a.V, n));
+#pragma unroll
+        for (int u = 0; u < NK; ++u) {
+            const int e = tid + 256 * u, row = e / (KD / 8), col = e % (KD / 8) * 8;
+            rk[u] = fetch_b<VEC>(dk, row, (unsigned)a.ldk, col, a.K);
+        }
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            const int e = tid + 256 * u, row = e / (VT / 8), col = part * VT + e % (VT / 8) * 8;
+            rv[u] = fetch_b<VEC>(dv, row, (unsigned)a.ldv, col, a.V);
+        }
+        if constexpr (!STATE) {
+            const auto dq = ssm::rsrc(base(a.q, a.ldq, h, a.K, tt), bytes(a.ldq, a.K, n));
+#pragma unroll
+            for (int u = 0; u < NK; ++u) {
+                const int e = tid + 256 * u, row = e / (KD / 8), col = e % (KD / 8) * 8;
+                rq[u] = fetch_b<VEC>(dq, row, (unsigned)a.ldq, col, a.K);
+            }
+        }
+    };
+    if (tid < 2) s.odd[tid] = 0;
+    if (t_begin < t_end) fetch(t_begin);
+    __syncthreads();
+
+    // e^{g (n - 1 - j)} of the lane's j of each 32: the state update's weights
+    float wj[2][8], em1 = 0.f;
+    int wn = -1;
+    int parity = 0;
+    for (int t = t_begin; t < t_end; t += CB, parity ^= 1) {
+        const int n = min(CB, t_end - t);
+        // ---- staging
+        unsigned odd = 0;
+#pragma unroll
+        for (int u = 0; u < NK; ++u) {
+            const int e = tid + 256 * u, row = e / (KD / 8), col = e % (KD / 8) * 8;
+            *reinterpret_cast<uint4*>(&s.k[row][col]) = rk[u];
+            if constexpr (!STATE) *reinterpret_cast<uint4*>(&s.q[row][col]) = rq[u];
+        }
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            const int e = tid + 256 * u, row = e / (VT / 8), col = e % (VT / 8) * 8;
+            *reinterpret_cast<uint4*>(&s.v[row][col]) = rv[u];
+            if constexpr (!STATE)
+                odd |= odd_bf16(rv[u].x) | odd_bf16(rv[u].y) | odd_bf16(rv[u].z) | odd_bf16(rv[u].w);
+        }
+        if (!STATE && odd) s.odd[parity] = 1;
+        __syncthreads();
+        if (t + CB < t_end) fetch(t + CB);
+        if (wn != n) {
+            wn = n;
+            em1 = decay_m1(g, n);
+#pragma unroll
+            for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    wj[jb][e] = ssm::ex2(gl * (float)max(0, n - 1 - (32 * jb + 8 * g4 + e)));
+        }
+
+        floatx4 Y[STATE ? 1 : VW][4];
+        bool any_odd = false;
+        if constexpr (!STATE) {
+            any_odd = s.odd[parity] != 0;
+            if (tid == 0) s.odd[parity ^ 1] = 0;   // (the next chunk sets it past two barriers)
+            // ---- q k^T: wave w forms the rows i of tile w, j up to the diagonal
+            {
+                floatx4 acc[4];
+#pragma unroll
+                for (int jt = 0; jt < 4; ++jt) acc[jt] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    const bf16x8 qf = *reinterpret_cast<const bf16x8*>(&s.q[16 * w + l16][32 * kb + 8 * g4]);
+#pragma unroll
+                    for (int jt = 0; jt < 4; ++jt)
+                        if (jt <= w)
+                            acc[jt] = mfma(*reinterpret_cast<const bf16x8*>(&s.k[16 * jt + l16][32 * kb + 8 * g4]),
+                                           qf, acc[jt]);
+                }
+                const int i = 16 * w + l16;
+#pragma unroll
+                for (int jt = 0; jt < 4; ++jt) {
+                    bf16x4 o = {};
+                    if (jt <= w) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int gap = i - (16 * jt + 4 * g4 + r);
+                            const float f = a.scale * ssm::ex2(gl * (float)max(gap, 0));
+                            o[r] = (__bf16)(gap >= 0 ? acc[jt][r] * f : 0.f);
+                        }
+                    }
+                    if (jt <= (w | 1)) *reinterpret_cast<bf16x4*>(&s.p[i][16 * jt + 4 * g4]) = o;
+                }
+            }
+            // ---- S q^T
+#pragma unroll
+            for (int x = 0; x < VW; ++x)
+#pragma unroll
+                for (int it = 0; it < 4; ++it) Y[x][it] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                bf16x8 hi[VW], lo[VW];
+#pragma unroll
+                for (int x = 0; x < VW; ++x)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float f = S[2 * kb + (e >> 2)][x][e & 3];
+                        hi[x][e] = (__bf16)f;
+                        lo[x][e] = (__bf16)(f - (float)hi[x][e]);
+                    }
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const __bf16* qr = &s.q[16 * it + l16][32 * kb + 4 * g4];
+                    const bf16x8 qf = cat(*reinterpret_cast<const bf16x4*>(qr),
+                                          *reinterpret_cast<const bf16x4*>(qr + 16));
+#pragma unroll
+                    for (int x = 0; x < VW; ++x) {
+                        Y[x][it] = mfma(lo[x], qf, Y[x][it]);
+                        Y[x][it] = mfma(hi[x], qf, Y[x][it]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                const float f = a.scale * ssm::ex2(gl * (float)(16 * it + l16 + 1));
+#pragma unroll
+                for (int x = 0; x < VW; ++x) Y[x][it] *= f;
+            }
+            __syncthreads();
+        }
+
+        // ---- P v, and the state update
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int x = 0; x < VW; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[kt][x][r] = fmaf(S[kt][x][r], em1, S[kt][x][r]);
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb) {
+            bf16x8 p1[VW], p2[VW], p3[VW];
+#pragma unroll
+            for (int x = 0; x < VW; ++x) {
+                const int col = 16 * (VW * w + x);
+                const bf16x8 vf = cat(tr_read<VP>(&s.v[0][0], 32 * jb + 8 * g4, col, l16),
+                                      tr_read<VP>(&s.v[0][0], 32 * jb + 8 * g4 + 4, col, l16));
+                if constexpr (!STATE) {
+                    if (!any_odd) {
+#pragma unroll
+                        for (int it = 2 * jb; it < 4; ++it)
+                            Y[x][it] = mfma(vf, *reinterpret_cast<const bf16x8*>(&s.p[16 * it + l16][32 * jb + 8 * g4]),
+                                            Y[x][it]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float f = (float)vf[e] * wj[jb][e];
+                    p1[x][e] = (__bf16)f;
+                    const float d = f - (float)p1[x][e];
+                    p2[x][e] = (__bf16)d;
+                    p3[x][e] = (__bf16)(d - (float)p2[x][e]);
+                }
+            }
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const bf16x8 kf = cat(tr_read<KP>(&s.k[0][0], 32 * jb + 8 * g4, 16 * kt, l16),
+                                      tr_read<KP>(&s.k[0][0], 32 * jb + 8 * g4 + 4, 16 * kt, l16));
+#pragma unroll
+                for (int x = 0; x < VW; ++x) {
+                    S[kt][x] = mfma(kf, p3[x], S[kt][x]);
+                    S[kt][x] = mfma(kf, p2[x], S[kt][x]);
+                    S[kt][x] = mfma(kf, p1[x], S[kt][x]);
+                }
+            }
+        }
+
+        if constexpr (!STATE) {
+            if (any_odd) {
+                // an inf or NaN in v: term by term, so that a zero weight never meets it
+#pragma unroll
+                for (int x = 0; x < VW; ++x)
+#pragma unroll
+                    for (int it = 0; it < 4; ++it) {
+                        const int i = 16 * it + l16;
+                        for (int j = 0; j <= i; ++j) {
+                            const float p = (float)s.p[i][j];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                Y[x][it][r] = fmaf(p, (float)s.v[j][16 * (VW * w + x) + 4 * g4 + r], Y[x][it][r]);
+                        }
+                    }
+            }
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                const int i = 16 * it + l16;
+                if (i >= n) continue;
+                __bf16* yr = static_cast<__bf16*>(a.y) + ((long)b * a.L + t + i) * a.ldy + (long)h * a.V;
+#pragma unroll
+                for (int x = 0; x < VW; ++x) {
+                    const int v = v0 + 16 * x + 4 * g4;
+                    bf16x4 o;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[r] = (__bf16)Y[x][it][r];
+                    if constexpr (VEC) {
+                        if (v < a.V) *reinterpret_cast<bf16x4*>(yr + v) = o;
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (v + r < a.V) yr[v + r] = o[r];
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+    float* to = STATE ? a.seg + seg * slot : (last ? a.hT : nullptr);
+    if (to)
+        each_state([&](floatx4& r, long o, int left) { store_state4<VEC>(to + state + o, r, left); });
+}
+
+// ---------------------------------------------------------------- fp32
+// The same on v_mfma_f32_16x16x4_f32 (A: row lane % 16, k lane / 16; D as above), every product
+// and sum in fp32. Chunks of 32: the quadratic part shrinks with the chunk, and a chunk costs
+// nothing else, as S stays in the accumulators. MFMA r of a 16-k block takes k = 4 (lane / 16) + r
+// from every lane, so that S and the products q k^T are read as they lie in the accumulators and
+// q and k as 16-byte pieces.
+constexpr int CF = 32;
+
+template <int KD, int VT>
+struct SmemF {
+    static constexpr int KP = KD + 4, VP = VT + 4, PP = CF + 4;
+    alignas(16) float q[CF][KP];
+    alignas(16) float k[CF][KP];
+    alignas(16) float v[CF][VP];
+    alignas(16) float p[CF][PP];
+    int odd[2];
+};
+
+__device__ __forceinline__ floatx4 mfma4(float a, float b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+template <bool VEC>
+__device__ __forceinline__ floatx4 fetch_f(__amdgpu_buffer_rsrc_t r, unsigned row, unsigned ld,
+                                           int col, int width) {
+    const unsigned o = (row * ld + (unsigned)col) * 4u;
+    if constexpr (VEC) {
+        return ssm::bload16<floatx4>(r, col < width ? o : kOut);
+    } else {
+        floatx4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = ssm::bload4(r, col + e < width ? o + 4u * e : kOut);
+        return x;
+    }
+}
+
+template <int KD, int VT, bool VEC, bool STATE>
+__global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a) {
+    using Smem = SmemF<KD, VT>;
+    constexpr int KT = KD / 16, VW = VT / 64;
+    constexpr int NK = CF * KD / 4 / 256, NV = CF * VT / 4 / 256;
+    __shared__ Smem s;
+
+    const int id = xcd_order(blockIdx.x, gridDim.x);
+    const int part = id % a.vparts, bh_s = id / a.vparts;
+    const int h = bh_s % a.H, b = bh_s / a.H % a.B, seg = bh_s / a.H / a.B;
+    const int grp = h / (a.H / a.G);
+    const int len = seq_len(a, b);
+    const int t_begin = seg * a.seglen, t_end = min(len, t_begin + a.seglen);
+    const bool last = seg == (len > 0 ? (len - 1) / a.seglen : 0);
+    if (STATE ? last || t_begin >= len : !last && t_begin >= len) return;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g4 = lane >> 4, l16 = lane & 15;
+    const int v0 = part * VT + 16 * VW * w;
+    const float g = clamp_g(a.g[h]), gl = g * ssm::kLog2e;
+    const long state = ((long)b * a.H + h) * a.V * a.K;
+    const long slot = (long)a.B * a.H * a.V * a.K;
+
+    floatx4 S[KT][VW];
+    auto each_state = [&](auto&& f) {
+#pragma unroll
+        for (int x = 0; x < VW; ++x) {
+            const int v = v0 + 16 * x + l16;
+            if (v < a.V) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int kk = 16 * kt + 4 * g4;
+                    f(S[kt][x], (long)v * a.K + kk, a.K - kk);
+                }
+            }
+        }
+    };
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int x = 0; x < VW; ++x) S[kt][x] = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (!STATE) {
+        const float* from = a.nseg > 1 ? (seg || a.h0 ? a.seg + seg * slot : nullptr) : a.h0;
+        if (from)
+            each_state([&](floatx4& r, long o, int left) {
+                r = load_state4<VEC>(from + state + o, left);
+            });
+    }
+
+    floatx4 rq[STATE ? 1 : NK], rk[NK], rv[NV];
+    auto base = [&](const void* p, long ld, int head, int width, int t) {
+        return static_cast<const float*>(p) + ((long)b * a.L + t) * ld + (long)head * width;
+    };
+    auto bytes = [&](long ld, int width, int n) {
+        return n > 0 ? (unsigned)(((long)(n - 1) * ld + width) * 4) : 0u;
+    };
+    auto fetch = [&](int t) {
+        const int n = max(0, min(CF, t_end - t));
+        const int tt = min(t, a.L - 1);
+        const auto dk = ssm::rsrc(base(a.k, a.ldk, grp, a.K, tt), bytes(a.ldk, a.K, n));
+        const auto dv = ssm::rsrc(base(a.v, a.ldv, grp, a.V, tt), bytes(a.ldv, a.V, n));
+#pragma unroll
+        for (int u = 0; u < NK; ++u) {
+            const int e = tid + 256 * u, row = e / (KD / 4), col = e % (KD / 4) * 4;
+            rk[u] = fetch_f<VEC>(dk, row, (unsigned)a.ldk, col, a.K);
+        }
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            const int e = tid + 256 * u, row = e / (VT / 4), col = part * VT + e % (VT / 4) * 4;
+            rv[u] = fetch_f<VEC>(dv, row, (unsigned)a.ldv, col, a.V);
+        }
+        if constexpr (!STATE) {
+            const auto dq = ssm::rsrc(base(a.q, a.ldq, h, a.K, tt), bytes(a.ldq, a.K, n));
+#pragma unroll
+            for (int u = 0; u < NK; ++u) {
+                const int e = tid + 256 * u, row = e / (KD / 4), col = e % (KD / 4) * 4;
+                rq[u] = fetch_f<VEC>(dq, row, (unsigned)a.ldq, col, a.K);
+            }
+        }
+    };
+    if (tid < 2) s.odd[tid] = 0;
+    if (t_begin < t_end) fetch(t_begin);
+    __syncthreads();
+
+    float wj[2][4], em1 = 0.f;
+    int wn = -1;
+    int parity = 0;
+    for (int t = t_begin; t < t_end; t += CF, parity ^= 1) {
+        const int n = min(CF, t_end - t);
+        bool odd = false;
+#pragma unroll
+        for (int u = 0; u < NK; ++u) {
+            const int e = tid + 256 * u, row = e / (KD / 4), col = e % (KD / 4) * 4;
+            *reinterpret_cast<floatx4*>(&s.k[row][col]) = rk[u];
+            if constexpr (!STATE) *reinterpret_cast<floatx4*>(&s.q[row][col]) = rq[u];
+        }
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            const int e = tid + 256 * u, row = e / (VT / 4), col = e % (VT / 4) * 4;
+            *reinterpret_cast<floatx4*>(&s.v[row][col]) = rv[u];
+            if constexpr (!STATE) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) odd |= !(fabsf(rv[u][c]) < INFINITY);
+            }
+        }
+        if (!STATE && odd) s.odd[parity] = 1;
+        __syncthreads();
+        if (t + CF < t_end) fetch(t + CF);
+        if (wn != n) {
+            wn = n;
+            em1 = decay_m1(g, n);
+#pragma unroll
+            for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    wj[jt][r] = ssm::ex2(gl * (float)max(0, n - 1 - (16 * jt + 4 * g4 + r)));
+        }
+
+        floatx4 Y[STATE ? 1 : VW][2];
+        bool any_odd = false;
+        if constexpr (!STATE) {
+            any_odd = s.odd[parity] != 0;
+            if (tid == 0) s.odd[parity ^ 1] = 0;
+            // ---- q k^T: wave 0 tile (j 0, i 0), wave 1 (0, 1), wave 2 (1, 1); (1, 0) is masked
+            if (w < 3) {
+                const int jt = w >> 1, it = w > 0;
+                floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const floatx4 kf = *reinterpret_cast<const floatx4*>(&s.k[16 * jt + l16][16 * kt + 4 * g4]);
+                    const floatx4 qf = *reinterpret_cast<const floatx4*>(&s.q[16 * it + l16][16 * kt + 4 * g4]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc = mfma4(kf[r], qf[r], acc);
+                }
+                const int i = 16 * it + l16;
+                floatx4 o;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int gap = i - (16 * jt + 4 * g4 + r);
+                    const float f = a.scale * ssm::ex2(gl * (float)max(gap, 0));
+                    o[r] = gap >= 0 ? acc[r] * f : 0.f;
+                }
+                *reinterpret_cast<floatx4*>(&s.p[i][16 * jt + 4 * g4]) = o;
+            }
+            // ---- S q^T
+#pragma unroll
+            for (int x = 0; x < VW; ++x)
+#pragma unroll
+                for (int it = 0; it < 2; ++it) Y[x][it] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int it = 0; it < 2; ++it) {
+                    const floatx4 qf = *reinterpret_cast<const floatx4*>(&s.q[16 * it + l16][16 * kt + 4 * g4]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int x = 0; x < VW; ++x) Y[x][it] = mfma4(S[kt][x][r], qf[r], Y[x][it]);
+                }
+#pragma unroll
+            for (int it = 0; it < 2; ++it) {
+                const float f = a.scale * ssm::ex2(gl * (float)(16 * it + l16 + 1));
+#pragma unroll
+                for (int x = 0; x < VW; ++x) Y[x][it] *= f;
+            }
+            __syncthreads();
+        }
+
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int x = 0; x < VW; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[kt][x][r] = fmaf(S[kt][x][r], em1, S[kt][x][r]);
+#pragma unroll
+        for (int jt = 0; jt < 2; ++jt) {
+            float vf[VW][4];
+#pragma unroll
+            for (int x = 0; x < VW; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    vf[x][r] = s.v[16 * jt + 4 * g4 + r][16 * (VW * w + x) + l16];
+            if constexpr (!STATE) {
+                if (!any_odd) {
+#pragma unroll
+                    for (int it = jt; it < 2; ++it) {
+                        const floatx4 pf = *reinterpret_cast<const floatx4*>(&s.p[16 * it + l16][16 * jt + 4 * g4]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int x = 0; x < VW; ++x) Y[x][it] = mfma4(vf[x][r], pf[r], Y[x][it]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < VW; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vf[x][r] *= wj[jt][r];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                float kf[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) kf[r] = s.k[16 * jt + 4 * g4 + r][16 * kt + l16];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int x = 0; x < VW; ++x) S[kt][x] = mfma4(kf[r], vf[x][r], S[kt][x]);
+            }
+        }
+
+        if constexpr (!STATE) {
+            if (any_odd) {
+#pragma unroll
+                for (int x = 0; x < VW; ++x)
+#pragma unroll
+                    for (int it = 0; it < 2; ++it) {
+                        const int i = 16 * it + l16;
+                        for (int j = 0; j <= i; ++j) {
+                            const float p = s.p[i][j];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                Y[x][it][r] = fmaf(p, s.v[j][16 * (VW * w + x) + 4 * g4 + r], Y[x][it][r]);
+                        }
+                    }
+            }
+#pragma unroll
+            for (int it = 0; it < 2; ++it) {
+                const int i = 16 * it + l16;
+                if (i >= n) continue;
+                float* yr = static_cast<float*>(a.y) + ((long)b * a.L + t + i) * a.ldy + (long)h * a.V;
+#pragma unroll
+                for (int x = 0; x < VW; ++x) {
+                    const int v = v0 + 16 * x + 4 * g4;
+                    store_state4<VEC>(yr + v, Y[x][it], a.V - v);
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+    float* to = STATE ? a.seg + seg * slot : (last ? a.hT : nullptr);
+    if (to)
+        each_state([&](floatx4& r, long o, int left) { store_state4<VEC>(to + state + o, r, left); });
+}
+
+// Entering states: slot[s] <- E_s, E_0 = h0 (or 0), E_{s+1} = e^{g seglen} E_s + own state of s.
+// (h0 is copied too: hT may alias it, and the last segment may end before the first begins.)
+__global__ __launch_bounds__(256) void la_combine_kernel(LaArgs a) {
+    const long VK = (long)a.V * a.K, slot = (long)a.B * a.H * VK;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= slot) return;
+    const int bh = (int)(i / VK), h = bh % a.H, b = bh / a.H;
+    const int len = seq_len(a, b);
+    const int used = len > 0 ? (len - 1) / a.seglen + 1 : 1;   // segments that run
+    const float em1 = decay_m1(clamp_g(a.g[h]), a.seglen);
+    float e = a.h0 ? a.h0[i] : 0.f;
+    float* p = a.seg + i;
+    constexpr int U = 8;
+    int sgm = 0;
+    for (; sgm + U < used; sgm += U) {
+        float own[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) own[u] = p[(sgm + u) * slot];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            p[(sgm + u) * slot] = e;
+            e = fmaf(e, em1, e) + own[u];
+        }
+    }
+    for (; sgm < used; ++sgm) {
+        const float own = sgm + 1 < used ? p[sgm * slot] : 0.f;
+        p[sgm * slot] = e;
+        e = fmaf(e, em1, e) + own;
+    }
+}
+
+// ---------------------------------------------------------------- plan
+int v_tile(int K, int V) { return V <= 64 || K > 128 ? 64 : 128; }
+
+// Segments: enough workgroups to fill the chip, each of at least kLeast tokens.
+constexpr int kFill = 512, kLeast = 256;
+void la_plan(int dtype, int B, int L, int H, int K, int V, int& nseg, int& seglen, int& vparts) {
+    const int C = dtype == SSM_F32 ? CF : CB;
+    vparts = (int)ssm::cdiv(V, v_tile(K, V));
+    const long wgs = (long)B * H * vparts;
+    long n = std::min<long>(ssm::cdiv(kFill, std::max(wgs, 1L)), ssm::cdiv(std::max(L, 1), kLeast));
+    n = std::max(n, 1L);
+    seglen = (int)(ssm::cdiv(ssm::cdiv(std::max(L, 1), n), C) * C);
+    nseg = (int)std::max(1L, ssm::cdiv(L, seglen));
+}
+
+template <int KD, int VT, bool VEC>
+ssm_status la_launch(int dtype, const LaArgs& a, hipStream_t st) {
+    const unsigned n = (unsigned)((long)a.nseg * a.B * a.H * a.vparts);
+    if (a.nseg > 1) {
+        const unsigned n1 = (unsigned)((long)(a.nseg - 1) * a.B * a.H * a.vparts);
+        if (dtype == SSM_F32) la_f32_kernel<KD, VT, VEC, true><<<n1, 256, 0, st>>>(a);
+        else la_bf16_kernel<KD, VT, VEC, true><<<n1, 256, 0, st>>>(a);
+        if (ssm_status e = ssm::check_launch("ssm_linear_attention (states)")) return e;
+        const long m = (long)a.B * a.H * a.V * a.K;
+        la_combine_kernel<<<(unsigned)ssm::cdiv(m, 256), 256, 0, st>>>(a);
+        if (ssm_status e = ssm::check_launch("ssm_linear_attention (combine)")) return e;
+    }
+    if (dtype == SSM_F32) la_f32_kernel<KD, VT, VEC, false><<<n, 256, 0, st>>>(a);
+    else la_bf16_kernel<KD, VT, VEC, false><<<n, 256, 0, st>>>(a);
+    return ssm::check_launch("ssm_linear_attention");
+}
+
+template <bool VEC>
+ssm_status la_dispatch(int dtype, const LaArgs& a, hipStream_t st) {
+    const int vt = v_tile(a.K, a.V);
+    if (a.K > 128) return la_launch<256, 64, VEC>(dtype, a, st);
+    if (a.K > 64) return vt == 64 ? la_launch<128, 64, VEC>(dtype, a, st)
+                                  : la_launch<128, 128, VEC>(dtype, a, st);
+    return vt == 64 ? la_launch<64, 64, VEC>(dtype, a, st) : la_launch<64, 128, VEC>(dtype, a, st);
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// ---------------------------------------------------------------- one token
+// S is read and written once: memory bound. 16 lanes hold a row of S (LV x 64 columns in float4
+// pieces, or one by one), a wave four rows, a workgroup 16 RV rows of one (sequence, head); the
+// loads of all RV rows are in flight before the first is used.
+struct LaStepArgs {
+    const void* q; long ldq;
+    const void* k; long ldk;
+    const void* v; long ldv;
+    const float* g;
+    float scale;
+    void* y; long ldy;
+    int H, G, K, V, blocks;
+    float* h;
+};
+
+template <typename T, int KU, int RV, bool VEC>
+__global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
+    constexpr int E = 4 * KU;   // columns per lane
+    const int l16 = threadIdx.x & 15, row = threadIdx.x >> 4;
+    const int blk = blockIdx.x % a.blocks, bh = blockIdx.x / a.blocks;
+    const int h = bh % a.H, b = bh / a.H, grp = h / (a.H / a.G);
+    const int v0 = blk * 16 * RV + row;
+    float* S = a.h + (long)bh * a.V * a.K;
+    // column of element e of the lane
+    auto col = [&](int e) { return VEC ? 64 * (e >> 2) + 4 * l16 + (e & 3) : 16 * e + l16; };
+    float s[RV][E];
+#pragma unroll
+    for (int r = 0; r < RV; ++r) {
+        const int v = v0 + 16 * r;
+        const float* p = S + (long)min(v, a.V - 1) * a.K;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int u = 0; u < KU; ++u) {
+                const float4 x = col(4 * u) < a.K ? ssm::load_nt4(p + col(4 * u)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                s[r][4 * u] = x.x; s[r][4 * u + 1] = x.y; s[r][4 * u + 2] = x.z; s[r][4 * u + 3] = x.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) s[r][e] = col(e) < a.K ? p[col(e)] : 0.f;
+        }
+    }
+    const T* qp = static_cast<const T*>(a.q) + b * a.ldq + (long)h * a.K;
+    const T* kp = static_cast<const T*>(a.k) + b * a.ldk + (long)grp * a.K;
+    const T* vp = static_cast<const T*>(a.v) + b * a.ldv + (long)grp * a.V;
+    float q[E], k[E], vv[RV];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const bool in = col(e) < a.K;
+        q[e] = in ? (float)qp[col(e)] : 0.f;
+        k[e] = in ? (float)kp[col(e)] : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < RV; ++r) vv[r] = (float)vp[min(v0 + 16 * r, a.V - 1)];
+    const float em1 = decay_m1(clamp_g(a.g[h]), 1);
+    float o[RV];
+#pragma unroll
+    for (int r = 0; r < RV; ++r) {
+        float acc = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            s[r][e] = fmaf(vv[r], k[e], fmaf(s[r][e], em1, s[r][e]));
+            acc = fmaf(s[r][e], q[e], acc);
+        }
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 16);
+        o[r] = acc * a.scale;
+    }
+    T* yp = static_cast<T*>(a.y) + b * a.ldy + (long)h * a.V;
+#pragma unroll
+    for (int r = 0; r < RV; ++r) {
+        const int v = v0 + 16 * r;
+        if (v >= a.V) continue;
+        float* p = S + (long)v * a.K;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+                if (col(4 * u) < a.K)
+                    ssm::store_nt4(make_float4(s[r][4 * u], s[r][4 * u + 1], s[r][4 * u + 2], s[r][4 * u + 3]),
+                                   p + col(4 * u));
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (col(e) < a.K) p[col(e)] = s[r][e];
+        }
+        if (l16 == 0) yp[v] = (T)o[r];
+    }
+}
+
+template <typename T, int KU, int RV>
+void step_launch(const LaStepArgs& a, bool vec, unsigned n, hipStream_t st) {
+    if (vec) la_step_kernel<T, KU, RV, true><<<n, 256, 0, st>>>(a);
+    else la_step_kernel<T, KU, RV, false><<<n, 256, 0, st>>>(a);
+}
+
+template <typename T, int KU>
+void step_rows(const LaStepArgs& a, int rv, bool vec, unsigned n, hipStream_t st) {
+    if (rv == 4) step_launch<T, KU, 4>(a, vec, n, st);
+    else step_launch<T, KU, 1>(a, vec, n, st);
+}
+
+template <typename T>
+void step_dispatch(const LaStepArgs& a, int rv, bool vec, unsigned n, hipStream_t st) {
+    if (a.K <= 64) step_rows<T, 1>(a, rv, vec, n, st);
+    else if (a.K <= 128) step_rows<T, 2>(a, rv, vec, n, st);
+    else step_rows<T, 4>(a, rv, vec, n, st);
+}
+
+}  // namespace
+
+extern "C" size_t ssm_linear_attention_workspace(int dtype, int B, int L, int H, int K, int V) {
+    if (B <= 0 || L <= 0 || H <= 0 || K <= 0 || V <= 0) return 0;
+    int nseg, seglen, vparts;
+    la_plan(dtype, B, L, H, K, V, nseg, seglen, vparts);
+    return nseg > 1 ? sizeof(float) * (size_t)nseg * B * H * V * K : 0;
+}
+
+extern "C" ssm_status ssm_linear_attention(int dtype, const void* q, long ldq, const void* k,
+                                           long ldk, const void* v, long ldv, const float* g,
+                                           float scale, const int* lengths, void* y, long ldy,
+                                           int B, int L, int H, int G, int K, int V,
+                                           const float* h0, float* hT, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+    SSM_REQUIRE(dtype == SSM_F32 || dtype == SSM_BF16, "ssm_linear_attention: bad dtype");
+    SSM_REQUIRE(B >= 0 && L >= 0 && H > 0 && G > 0 && H % G == 0 && K > 0 && V > 0,
+                "ssm_linear_attention: bad shape");
+    if (K > 256)
+        return ssm::fail(SSM_ERR_UNSUPPORTED, "ssm_linear_attention: head dim %d of the keys above 256", K);
+    if (B == 0) return SSM_OK;
+    SSM_REQUIRE(g && (L == 0 || (q && k && v && y)), "ssm_linear_attention: null input");
+    SSM_REQUIRE(L == 0 || (ldq >= (long)H * K && ldk >= (long)G * K && ldv >= (long)G * V &&
+                           ldy >= (long)H * V),
+                "ssm_linear_attention: row stride below row width");
+    const long esz = dtype == SSM_F32 ? 4 : 2, ev = 16 / esz;
+    const long lim = (1L << 31) / (CB * esz);   // a chunk's byte offsets are 32-bit
+    SSM_REQUIRE(ldq < lim && ldk < lim && ldv < lim, "ssm_linear_attention: row stride too large");
+    LaArgs a{};
+    a.q = q; a.ldq = ldq; a.k = k; a.ldk = ldk; a.v = v; a.ldv = ldv; a.g = g; a.scale = scale;
+    a.lengths = lengths; a.y = y; a.ldy = ldy; a.B = B; a.L = L; a.H = H; a.G = G; a.K = K; a.V = V;
+    a.h0 = h0; a.hT = hT;
+    la_plan(dtype, B, L, H, K, V, a.nseg, a.seglen, a.vparts);
+    SSM_REQUIRE((long)a.nseg * B * H * a.vparts < (1L << 31) &&
+                    (long)B * H * V * K < (1L << 38),
+                "ssm_linear_attention: too many heads");
+    if (a.nseg > 1) {
+        const size_t need = ssm_linear_attention_workspace(dtype, B, L, H, K, V);
+        SSM_REQUIRE(workspace && workspace_bytes >= need,
+                    "ssm_linear_attention: workspace of %zu bytes needed", need);
+        SSM_REQUIRE(aligned16(workspace), "ssm_linear_attention: workspace must be 16-byte aligned");
+        a.seg = (float*)workspace;
+    }
+    const bool vec = K % ev == 0 && V % ev == 0 && (ldq | ldk | ldv | ldy) % ev == 0 &&
+                     aligned16(q) && aligned16(k) && aligned16(v) && aligned16(y) &&
+                     aligned16(h0) && aligned16(hT);
+    return vec ? la_dispatch<true>(dtype, a, (hipStream_t)stream)
+               : la_dispatch<false>(dtype, a, (hipStream_t)stream);
+}
+
+extern "C" ssm_status ssm_linear_attention_step(int dtype, const void* q, long ldq, const void* k,
+                                                long ldk, const void* v, long ldv, const float* g,
+                                                float scale, void* y, long ldy, float* h, int B,
+                                                int H, int G, int K, int V, void* stream) {
+    SSM_REQUIRE(dtype == SSM_F32 || dtype == SSM_BF16, "ssm_linear_attention_step: bad dtype");
+    SSM_REQUIRE(B >= 0 && H > 0 && G > 0 && H % G == 0 && K > 0 && V > 0,
+                "ssm_linear_attention_step: bad shape");
+    if (K > 256)
+        return ssm::fail(SSM_ERR_UNSUPPORTED, "ssm_linear_attention_step: head dim %d of the keys above 256", K);
+    if (B == 0) return SSM_OK;
+    SSM_REQUIRE(q && k && v && g && y && h, "ssm_linear_attention_step: null input");
+    SSM_REQUIRE(B == 1 || (ldq >= (long)H * K && ldk >= (long)G * K && ldv >= (long)G * V &&
+                           ldy >= (long)H * V),
+                "ssm_linear_attention_step: row stride below row width");
+    LaStepArgs a{q, ldq, k, ldk, v, ldv, g, scale, y, ldy, H, G, K, V, 0, h};
+    // four rows a lane group where that still leaves two workgroups a CU
+    const int rv = (long)B * H * ssm::cdiv(V, 64) >= 512 ? 4 : 1;
+    a.blocks = (int)ssm::cdiv(V, 16 * rv);
+    const long n = (long)B * H * a.blocks;
+    SSM_REQUIRE(n < (1L << 31), "ssm_linear_attention_step: too many heads");
+    const bool vec = K % 4 == 0 && aligned16(h);
+    if (dtype == SSM_F32) step_dispatch<float>(a, rv, vec, (unsigned)n, (hipStream_t)stream);
+    else step_dispatch<__bf16>(a, rv, vec, (unsigned)n, (hipStream_t)stream);
+    return ssm::check_launch("ssm_linear_attention_step");
+}
