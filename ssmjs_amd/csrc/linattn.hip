@@ -20,6 +20,7 @@ namespace {
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 constexpr unsigned kOut = 0x80000000u;   // a buffer offset past any descriptor
@@ -35,12 +36,22 @@ struct LaArgs {
     int B, L, H, G, K, V;
     const float* h0;         // (B,H,V,K) or null
     float* hT;               // (B,H,V,K) or null
-    float* seg;              // (nseg,B,H,V,K): own states, then entering states
-    int nseg, seglen, vparts;
+    float* seg;              // (nseg,B,H,V,K): the segments' own states (the last slot: h0), or,
+    int nseg, seglen, vparts;   // combined, the states that enter them
+    int combined;
 };
 
 // e^{g n} - 1 and e^{g n}. g = -inf keeps nothing (and n = 0 everything).
 __device__ __forceinline__ float decay_m1(float g, int n) { return expm1f(g * (float)n); }
+// A value that the compiler forms again in each turn of a loop: the registers that it would hold
+// over the loop are wanted for the state and the next chunk's rows (spills read back from memory
+// wait behind those rows' loads).
+template <typename T>
+__device__ __forceinline__ T fresh(T x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 __device__ __forceinline__ float clamp_g(float g) { return fmaxf(g, -1e30f); }
 
 __device__ __forceinline__ int seq_len(const LaArgs& a, int b) {
@@ -62,9 +73,9 @@ __device__ __forceinline__ int xcd_order(int b, int T) {
 // the block taken in the order (16 t + 4 g + r, 16 (t + 1) + 4 g + r); q is read from LDS in that
 // order. The 64 x 64 products q k^T are shared out over the waves by rows i and go through LDS.
 //
-// Roundings to bf16: the products q k^T with their decay, and S as an operand (in two parts, hi +
-// lo, 16 bits): S itself stays fp32. The values of the state update are e^{..} v in three parts
-// (24 bits), so that the state carries fp32 rounding only.
+// Roundings to bf16: none that a result keeps. S as an operand of its product with q and the products
+// q k^T enter in two parts (16 bits; 2.5% of the time at 8 sequences of 4096 tokens), and the values of
+// the state update, e^{..} v, in two or three, so that the final state carries fp32 rounding only.
 __device__ __forceinline__ floatx4 mfma(bf16x8 a, bf16x8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -81,31 +92,34 @@ __device__ __forceinline__ bf16x8 cat(bf16x4 a, bf16x4 b) {
     return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// Whether a dword of two bf16 holds an inf or NaN: bit 15 or 31 set.
-__device__ __forceinline__ unsigned odd_bf16(unsigned u) {
-    return ((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// The larger magnitudes' bits, of two bf16 a dword: 0x7f80 and more is an inf or NaN.
+__device__ __forceinline__ u16x2 most_bf16(u16x2 m, unsigned u) {
+    return __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u & 0x7fff7fffu));
 }
 
 constexpr int CB = 64;   // tokens per chunk
 
-template <int KD, int VT>
+template <int KD, int VT, bool STATE>
 struct SmemB {
-    static constexpr int KP = KD + 8, VP = VT + 8, PP = CB + 8;
-    alignas(16) __bf16 q[CB][KP];
+    static constexpr int KP = KD + 8, VP = VT + 8, PP = CB + 8, Y = STATE ? 1 : CB;
+    alignas(16) __bf16 q[Y][KP];
     alignas(16) __bf16 k[CB][KP];
     alignas(16) __bf16 v[CB][VP];
-    alignas(16) __bf16 p[CB][PP];   // scale e^{g (i - j)} q_i . k_j, row i
+    // scale e^{g (i - j)} q_i . k_j, row i, in two parts
+    alignas(16) __bf16 p[2][Y][PP];
+    float dec[CB + 17];             // place 64 - d: scale e^{g d}, d = i - j (1 behind d = 0)
+    alignas(16) float wj[CB];       // e^{g (n - 1 - j)}: the state update's weights
     int odd[2];                     // an inf or NaN in the chunk's v (by the chunk's parity)
 };
 
-// 16 bytes (8 elements) of row `row`, columns col .. + 7, zeros past the descriptor and from
-// column `width` on.
+// 16 bytes (8 elements, columns col .. + 7) from byte offset o on: zeros from column `width` and
+// past the descriptor on.
 template <bool VEC>
-__device__ __forceinline__ uint4 fetch_b(__amdgpu_buffer_rsrc_t r, unsigned row, unsigned ld,
-                                         int col, int width) {
-    const unsigned o = (row * ld + (unsigned)col) * 2u;
+__device__ __forceinline__ uint4 fetch_b(__amdgpu_buffer_rsrc_t r, unsigned o, int col, int width) {
     if constexpr (VEC) {
-        return ssm::bload16<uint4>(r, col < width ? o : kOut);
+        return ssm::bload16<uint4>(r, o);   // (whole pieces: o is past the descriptor then)
     } else {
         unsigned u[4];
 #pragma unroll
@@ -120,34 +134,34 @@ __device__ __forceinline__ uint4 fetch_b(__amdgpu_buffer_rsrc_t r, unsigned row,
     }
 }
 
+// Four elements from byte offset o on, `left` of them inside the row (no more than that are
+// touched; an o past the descriptor reads zeros and writes nothing).
 template <bool VEC>
-__device__ __forceinline__ floatx4 load_state4(const float* p, int left) {
+__device__ __forceinline__ floatx4 load_f4(__amdgpu_buffer_rsrc_t r, unsigned o, int left) {
     if constexpr (VEC) {
-        return left > 0 ? *reinterpret_cast<const floatx4*>(p) : floatx4{0.f, 0.f, 0.f, 0.f};
+        return ssm::bload16<floatx4>(r, left > 0 ? o : kOut);
     } else {
-        floatx4 s = {0.f, 0.f, 0.f, 0.f};
+        floatx4 x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < left) s[e] = p[e];
-        return s;
+        for (int e = 0; e < 4; ++e) x[e] = ssm::bload4(r, e < left ? o + 4u * e : kOut);
+        return x;
     }
 }
 
 template <bool VEC>
-__device__ __forceinline__ void store_state4(float* p, floatx4 s, int left) {
+__device__ __forceinline__ void store_f4(__amdgpu_buffer_rsrc_t r, unsigned o, floatx4 x, int left) {
     if constexpr (VEC) {
-        if (left > 0) *reinterpret_cast<floatx4*>(p) = s;
+        ssm::bstore16(make_float4(x[0], x[1], x[2], x[3]), r, left > 0 ? o : kOut);
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < left) p[e] = s[e];
+        for (int e = 0; e < 4; ++e) ssm::bstore4(x[e], r, e < left ? o + 4u * e : kOut);
     }
 }
 
 // STATE: only the segment's own state (from zero), into its slot.
 template <int KD, int VT, bool VEC, bool STATE>
 __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs a) {
-    using Smem = SmemB<KD, VT>;
+    using Smem = SmemB<KD, VT, STATE>;
     constexpr int KT = KD / 16, KB = KD / 32, VW = VT / 64;
     constexpr int KP = Smem::KP, VP = Smem::VP, PP = Smem::PP;
     constexpr int NK = CB * KD / 8 / 256, NV = CB * VT / 8 / 256;
@@ -161,228 +175,242 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
     const int t_begin = seg * a.seglen, t_end = min(len, t_begin + a.seglen);
     // the segment that ends the sequence writes the final state (segment 0 of an empty one)
     const bool last = seg == (len > 0 ? (len - 1) / a.seglen : 0);
-    if (STATE ? last || t_begin >= len : !last && t_begin >= len) return;
+    // (the first segment's state pass also copies h0: hT may alias it, and the last segment may end
+    // before another begins)
+    const bool copy = STATE && seg == 0 && a.h0;
+    if (STATE ? (last || t_begin >= len) && !copy : !last && t_begin >= len) return;
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g4 = lane >> 4, l16 = lane & 15;
+    const int lane_g = lane >> 4, lane_i = lane & 15;
     const int v0 = part * VT + 16 * VW * w;     // the wave's first column of V
     const float g = clamp_g(a.g[h]), gl = g * ssm::kLog2e;
     const long state = ((long)b * a.H + h) * a.V * a.K;
     const long slot = (long)a.B * a.H * a.V * a.K;
 
     floatx4 S[KT][VW];
+    const unsigned sbytes = (unsigned)(a.V * a.K) * 4u;
     auto each_state = [&](auto&& f) {
+        const int vl = v0 + fresh(lane_i), kl = 4 * fresh(lane_g);
 #pragma unroll
-        for (int x = 0; x < VW; ++x) {
-            const int v = v0 + 16 * x + l16;
-            if (v < a.V) {
+        for (int x = 0; x < VW; ++x)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const int kk = 16 * kt + 4 * g4;
-                    f(S[kt][x], (long)v * a.K + kk, a.K - kk);
-                }
-            }
-        }
+            for (int kt = 0; kt < KT; ++kt)
+                f(S[kt][x], (unsigned)((vl + 16 * x) * a.K + kl + 16 * kt) * 4u,
+                  vl + 16 * x < a.V ? a.K - kl - 16 * kt : 0);
     };
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int x = 0; x < VW; ++x) S[kt][x] = floatx4{0.f, 0.f, 0.f, 0.f};
-    if (!STATE) {
-        const float* from = a.nseg > 1 ? (seg || a.h0 ? a.seg + seg * slot : nullptr) : a.h0;
-        if (from)
-            each_state([&](floatx4& r, long o, int left) {
-                r = load_state4<VEC>(from + state + o, left);
-            });
-    }
-
-    // ---- a chunk's rows in registers, ahead of their staging
+    // ---- a chunk's rows in registers, ahead of their staging: piece u of a thread is its column of
+    // row 256 u / (pieces per row) further down
+    constexpr int RK = 256 / (KD / 8), RV = 256 / (VT / 8);
     uint4 rq[STATE ? 1 : NK], rk[NK], rv[NV];
+    const int krow = tid / (KD / 8), kcol = tid % (KD / 8) * 8;
+    const int vrow = tid / (VT / 8), vcol = tid % (VT / 8) * 8;
     auto base = [&](const void* p, long ld, int head, int width, int t) {
         return static_cast<const __bf16*>(p) + ((long)b * a.L + t) * ld + (long)head * width;
     };
     auto bytes = [&](long ld, int width, int n) {
         return n > 0 ? (unsigned)(((long)(n - 1) * ld + width) * 2) : 0u;
     };
+    const unsigned kdown = (unsigned)a.ldk * (2 * RK), qdown = (unsigned)a.ldq * (2 * RK);
+    const unsigned vdown = (unsigned)a.ldv * (2 * RV);
+    auto first = [](int row, long ld, int col, int width) {
+        return col < width ? ((unsigned)row * (unsigned)ld + (unsigned)col) * 2u : kOut;
+    };
+    const unsigned koff = first(krow, a.ldk, kcol, a.K), qoff = first(krow, a.ldq, kcol, a.K);
+    const unsigned voff = first(vrow, a.ldv, part * VT + vcol, a.V);
     auto fetch = [&](int t) {
         const int n = max(0, min(CB, t_end - t));
         const int tt = min(t, a.L - 1);
         const auto dk = ssm::rsrc(base(a.k, a.ldk, grp, a.K, tt), bytes(a.ldk, a.K, n));
         const auto dv = ssm::rsrc(base(a.v, a.ldv, grp, a.V, tt), bytes(a.ldv, a.V, n));
 #pragma unroll
-        for (int u = 0; u < NK; ++u) {
-            const int e = tid + 256 * u, row = e / (KD / 8), col = e % (KD / 8) * 8;
-            rk[u] = fetch_b<VEC>(dk, row, (unsigned)a.ldk, col, a.K);
-        }
+        for (int u = 0; u < NK; ++u) rk[u] = fetch_b<VEC>(dk, koff + u * kdown, kcol, a.K);
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int e = tid + 256 * u, row = e / (VT / 8), col = part * VT + e % (VT / 8) * 8;
-            rv[u] = fetch_b<VEC>(dv, row, (unsigned)a.ldv, col, a.V);
-        }
+        for (int u = 0; u < NV; ++u) rv[u] = fetch_b<VEC>(dv, voff + u * vdown, part * VT + vcol, a.V);
         if constexpr (!STATE) {
             const auto dq = ssm::rsrc(base(a.q, a.ldq, h, a.K, tt), bytes(a.ldq, a.K, n));
 #pragma unroll
-            for (int u = 0; u < NK; ++u) {
-                const int e = tid + 256 * u, row = e / (KD / 8), col = e % (KD / 8) * 8;
-                rq[u] = fetch_b<VEC>(dq, row, (unsigned)a.ldq, col, a.K);
-            }
+            for (int u = 0; u < NK; ++u) rq[u] = fetch_b<VEC>(dq, qoff + u * qdown, kcol, a.K);
         }
     };
+    if (copy) {
+        const auto from = ssm::rsrc(a.h0 + state, sbytes);
+        const auto to = ssm::rsrc(a.seg + (a.nseg - 1) * slot + state, sbytes);
+        each_state([&](floatx4&, unsigned o, int left) {
+            store_f4<VEC>(to, o, load_f4<VEC>(from, o, left), left);
+        });
+        if (last) return;
+    }
     if (tid < 2) s.odd[tid] = 0;
+    if (tid < CB + 17) s.dec[tid] = a.scale * ssm::ex2(gl * (float)max(0, 64 - tid));
     if (t_begin < t_end) fetch(t_begin);
+    if (!STATE) {
+        // h0 (where there are segments, its copy), then the segments' own states, each decayed by a
+        // segment's length; or the sum that the combine pass left
+        const float* h0 = a.nseg > 1 && a.h0 ? a.seg + (a.nseg - 1) * slot : a.h0;
+        if (a.combined) h0 = seg || a.h0 ? a.seg + seg * slot : nullptr;
+        if (h0) {
+            const auto d = ssm::rsrc(h0 + state, sbytes);
+            each_state([&](floatx4& r, unsigned o, int left) { r = load_f4<VEC>(d, o, left); });
+        }
+        const float seg_m1 = decay_m1(g, a.seglen);
+        for (int p = 0; p < seg && !a.combined; ++p) {
+            const auto d = ssm::rsrc(a.seg + p * slot + state, sbytes);
+            each_state([&](floatx4& r, unsigned o, int left) {
+                const floatx4 own = load_f4<VEC>(d, o, left);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r[e] = fmaf(r[e], seg_m1, r[e]) + own[e];
+            });
+        }
+    }
     __syncthreads();
 
-    // e^{g (n - 1 - j)} of the lane's j of each 32: the state update's weights
-    float wj[2][8], em1 = 0.f;
+    float em1 = 0.f;
     int wn = -1;
     int parity = 0;
     for (int t = t_begin; t < t_end; t += CB, parity ^= 1) {
-        const int n = min(CB, t_end - t);
+        const int n = min(CB, t_end - t), g4 = fresh(lane_g), l16 = fresh(lane_i);
+        if (wn != n) {   // (every wave is past its reads of the weights)
+            wn = n;
+            em1 = decay_m1(g, n);
+            if (tid < CB) s.wj[tid] = ssm::ex2(gl * (float)max(0, n - 1 - tid));
+        }
         // ---- staging
-        unsigned odd = 0;
+        u16x2 most = {0, 0};
 #pragma unroll
         for (int u = 0; u < NK; ++u) {
-            const int e = tid + 256 * u, row = e / (KD / 8), col = e % (KD / 8) * 8;
-            *reinterpret_cast<uint4*>(&s.k[row][col]) = rk[u];
-            if constexpr (!STATE) *reinterpret_cast<uint4*>(&s.q[row][col]) = rq[u];
+            *reinterpret_cast<uint4*>(&s.k[krow + RK * u][kcol]) = rk[u];
+            if constexpr (!STATE) *reinterpret_cast<uint4*>(&s.q[krow + RK * u][kcol]) = rq[u];
         }
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            const int e = tid + 256 * u, row = e / (VT / 8), col = e % (VT / 8) * 8;
-            *reinterpret_cast<uint4*>(&s.v[row][col]) = rv[u];
+            *reinterpret_cast<uint4*>(&s.v[vrow + RV * u][vcol]) = rv[u];
             if constexpr (!STATE)
-                odd |= odd_bf16(rv[u].x) | odd_bf16(rv[u].y) | odd_bf16(rv[u].z) | odd_bf16(rv[u].w);
+                most = most_bf16(most_bf16(most_bf16(most_bf16(most, rv[u].x), rv[u].y), rv[u].z), rv[u].w);
         }
-        if (!STATE && odd) s.odd[parity] = 1;
+        if (!STATE && max(most.x, most.y) >= 0x7f80) s.odd[parity] = 1;
         __syncthreads();
         if (t + CB < t_end) fetch(t + CB);
-        if (wn != n) {
-            wn = n;
-            em1 = decay_m1(g, n);
-#pragma unroll
-            for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    wj[jb][e] = ssm::ex2(gl * (float)max(0, n - 1 - (32 * jb + 8 * g4 + e)));
-        }
-
         floatx4 Y[STATE ? 1 : VW][4];
         bool any_odd = false;
         if constexpr (!STATE) {
             any_odd = s.odd[parity] != 0;
             if (tid == 0) s.odd[parity ^ 1] = 0;   // (the next chunk sets it past two barriers)
             // ---- q k^T: wave w forms the rows i of tile w, j up to the diagonal
-            {
-                floatx4 acc[4];
+            auto products = [&](auto wave) {
+                constexpr int W = decltype(wave)::value;
+                bf16x8 qf[KB];
+                floatx4 acc[W + 1];
 #pragma unroll
-                for (int jt = 0; jt < 4; ++jt) acc[jt] = floatx4{0.f, 0.f, 0.f, 0.f};
+                for (int kb = 0; kb < KB; ++kb)
+                    qf[kb] = *reinterpret_cast<const bf16x8*>(&s.q[16 * W + l16][32 * kb + 8 * g4]);
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    const bf16x8 qf = *reinterpret_cast<const bf16x8*>(&s.q[16 * w + l16][32 * kb + 8 * g4]);
+                for (int jt = 0; jt <= W; ++jt) acc[jt] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int jt = 0; jt < 4; ++jt)
-                        if (jt <= w)
-                            acc[jt] = mfma(*reinterpret_cast<const bf16x8*>(&s.k[16 * jt + l16][32 * kb + 8 * g4]),
-                                           qf, acc[jt]);
-                }
-                const int i = 16 * w + l16;
+                for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int jt = 0; jt < 4; ++jt) {
-                    bf16x4 o = {};
-                    if (jt <= w) {
+                    for (int jt = 0; jt <= W; ++jt)
+                        acc[jt] = mfma(*reinterpret_cast<const bf16x8*>(&s.k[16 * jt + l16][32 * kb + 8 * g4]),
+                                       qf[kb], acc[jt]);
+                const float* dec = &s.dec[64 - l16 + 4 * g4];
+                __bf16* pr = &s.p[0][16 * W + l16][4 * g4];
+#pragma unroll
+                for (int jt = 0; jt <= (W | 1); ++jt) {
+                    bf16x4 hi = {}, lo = {};
+                    if (jt <= W) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const int gap = i - (16 * jt + 4 * g4 + r);
-                            const float f = a.scale * ssm::ex2(gl * (float)max(gap, 0));
-                            o[r] = (__bf16)(gap >= 0 ? acc[jt][r] * f : 0.f);
+                            float p = acc[min(jt, W)][r] * dec[r - 16 * (W - jt)];
+                            if (jt == W && l16 < 4 * g4 + r) p = 0.f;
+                            hi[r] = (__bf16)p;
+                            lo[r] = (__bf16)(p - (float)hi[r]);
                         }
                     }
-                    if (jt <= (w | 1)) *reinterpret_cast<bf16x4*>(&s.p[i][16 * jt + 4 * g4]) = o;
+                    *reinterpret_cast<bf16x4*>(pr + 16 * jt) = hi;
+                    *reinterpret_cast<bf16x4*>(pr + CB * PP + 16 * jt) = lo;
                 }
-            }
-            // ---- S q^T
+            };
+            if (w == 0) products(std::integral_constant<int, 0>{});
+            else if (w == 1) products(std::integral_constant<int, 1>{});
+            else if (w == 2) products(std::integral_constant<int, 2>{});
+            else products(std::integral_constant<int, 3>{});
+            // ---- S q^T, the next block's q read ahead of each block's products
+            bf16x8 qf[2][4];
+            auto q_tiles = [&](bf16x8 (&f)[4], int kb) {
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const __bf16* qr = &s.q[16 * it + l16][32 * kb + 4 * g4];
+                    f[it] = cat(*reinterpret_cast<const bf16x4*>(qr), *reinterpret_cast<const bf16x4*>(qr + 16));
+                }
+            };
+            q_tiles(qf[0], 0);
 #pragma unroll
             for (int x = 0; x < VW; ++x)
 #pragma unroll
                 for (int it = 0; it < 4; ++it) Y[x][it] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
-                bf16x8 hi[VW], lo[VW];
+                if (kb + 1 < KB) q_tiles(qf[(kb + 1) & 1], kb + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                bf16x8 sf[VW], sl[VW];
 #pragma unroll
                 for (int x = 0; x < VW; ++x)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const float f = S[2 * kb + (e >> 2)][x][e & 3];
-                        hi[x][e] = (__bf16)f;
-                        lo[x][e] = (__bf16)(f - (float)hi[x][e]);
+                        sf[x][e] = (__bf16)f;
+                        sl[x][e] = (__bf16)(f - (float)sf[x][e]);
                     }
 #pragma unroll
-                for (int it = 0; it < 4; ++it) {
-                    const __bf16* qr = &s.q[16 * it + l16][32 * kb + 4 * g4];
-                    const bf16x8 qf = cat(*reinterpret_cast<const bf16x4*>(qr),
-                                          *reinterpret_cast<const bf16x4*>(qr + 16));
+                for (int it = 0; it < 4; ++it)
 #pragma unroll
-                    for (int x = 0; x < VW; ++x) {
-                        Y[x][it] = mfma(lo[x], qf, Y[x][it]);
-                        Y[x][it] = mfma(hi[x], qf, Y[x][it]);
-                    }
-                }
+                    for (int x = 0; x < VW; ++x) Y[x][it] = mfma(sf[x], qf[kb & 1][it], Y[x][it]);
+#pragma unroll
+                for (int it = 0; it < 4; ++it)
+#pragma unroll
+                    for (int x = 0; x < VW; ++x) Y[x][it] = mfma(sl[x], qf[kb & 1][it], Y[x][it]);
             }
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
-                const float f = a.scale * ssm::ex2(gl * (float)(16 * it + l16 + 1));
+                const float f = s.dec[63 - 16 * it - l16];
 #pragma unroll
                 for (int x = 0; x < VW; ++x) Y[x][it] *= f;
             }
             __syncthreads();
         }
 
-        // ---- P v, and the state update
+        auto v_tile = [&](int jb, int x) {
+            const int col = 16 * (VW * w + x);
+            return cat(tr_read<VP>(&s.v[0][0], 32 * jb + 8 * g4, col, l16),
+                       tr_read<VP>(&s.v[0][0], 32 * jb + 8 * g4 + 4, col, l16));
+        };
+        // ---- P v
+        if constexpr (!STATE) {
+            if (!any_odd) {
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+                for (int jb = 0; jb < 2; ++jb) {
+                    bf16x8 vf[VW], pf[2][4];
 #pragma unroll
-            for (int x = 0; x < VW; ++x)
+                    for (int x = 0; x < VW; ++x) vf[x] = v_tile(jb, x);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[kt][x][r] = fmaf(S[kt][x][r], em1, S[kt][x][r]);
-#pragma unroll
-        for (int jb = 0; jb < 2; ++jb) {
-            bf16x8 p1[VW], p2[VW], p3[VW];
-#pragma unroll
-            for (int x = 0; x < VW; ++x) {
-                const int col = 16 * (VW * w + x);
-                const bf16x8 vf = cat(tr_read<VP>(&s.v[0][0], 32 * jb + 8 * g4, col, l16),
-                                      tr_read<VP>(&s.v[0][0], 32 * jb + 8 * g4 + 4, col, l16));
-                if constexpr (!STATE) {
-                    if (!any_odd) {
+                    for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int it = 2 * jb; it < 4; ++it)
-                            Y[x][it] = mfma(vf, *reinterpret_cast<const bf16x8*>(&s.p[16 * it + l16][32 * jb + 8 * g4]),
-                                            Y[x][it]);
-                    }
-                }
+                            pf[c][it] = *reinterpret_cast<const bf16x8*>(&s.p[c][16 * it + l16][32 * jb + 8 * g4]);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float f = (float)vf[e] * wj[jb][e];
-                    p1[x][e] = (__bf16)f;
-                    const float d = f - (float)p1[x][e];
-                    p2[x][e] = (__bf16)d;
-                    p3[x][e] = (__bf16)(d - (float)p2[x][e]);
-                }
-            }
+                    for (int c = 1; c >= 0; --c)
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                const bf16x8 kf = cat(tr_read<KP>(&s.k[0][0], 32 * jb + 8 * g4, 16 * kt, l16),
-                                      tr_read<KP>(&s.k[0][0], 32 * jb + 8 * g4 + 4, 16 * kt, l16));
+                        for (int it = 2 * jb; it < 4; ++it)
 #pragma unroll
-                for (int x = 0; x < VW; ++x) {
-                    S[kt][x] = mfma(kf, p3[x], S[kt][x]);
-                    S[kt][x] = mfma(kf, p2[x], S[kt][x]);
-                    S[kt][x] = mfma(kf, p1[x], S[kt][x]);
+                            for (int x = 0; x < VW; ++x) Y[x][it] = mfma(vf[x], pf[c][it], Y[x][it]);
                 }
             }
         }
-
         if constexpr (!STATE) {
             if (any_odd) {
                 // an inf or NaN in v: term by term, so that a zero weight never meets it
@@ -392,40 +420,101 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
                     for (int it = 0; it < 4; ++it) {
                         const int i = 16 * it + l16;
                         for (int j = 0; j <= i; ++j) {
-                            const float p = (float)s.p[i][j];
+                            const float p = (float)s.p[0][i][j] + (float)s.p[1][i][j];
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
                                 Y[x][it][r] = fmaf(p, (float)s.v[j][16 * (VW * w + x) + 4 * g4 + r], Y[x][it][r]);
                         }
                     }
             }
+            const auto dy = ssm::rsrc(static_cast<__bf16*>(a.y) + ((long)b * a.L + t) * a.ldy + (long)h * a.V,
+                                      bytes(a.ldy, a.V, n));
 #pragma unroll
-            for (int it = 0; it < 4; ++it) {
-                const int i = 16 * it + l16;
-                if (i >= n) continue;
-                __bf16* yr = static_cast<__bf16*>(a.y) + ((long)b * a.L + t + i) * a.ldy + (long)h * a.V;
+            for (int x = 0; x < VW; ++x) {
+                const int v = v0 + 16 * x + 4 * g4;
+                const unsigned o0 = v < a.V ? ((unsigned)l16 * (unsigned)a.ldy + v) * 2u : kOut;
 #pragma unroll
-                for (int x = 0; x < VW; ++x) {
-                    const int v = v0 + 16 * x + 4 * g4;
-                    bf16x4 o;
+                for (int it = 0; it < 4; ++it) {
+                    const unsigned o = o0 + (unsigned)it * ((unsigned)a.ldy * 32u);
+                    bf16x4 y;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[r] = (__bf16)Y[x][it][r];
+                    for (int r = 0; r < 4; ++r) y[r] = (__bf16)Y[x][it][r];
                     if constexpr (VEC) {
-                        if (v < a.V) *reinterpret_cast<bf16x4*>(yr + v) = o;
+                        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, y), dy, o, 0, 0);
                     } else {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (v + r < a.V) yr[v + r] = o[r];
+                        for (int r = 0; r < 4; ++r) {
+                            const __bf16 e = y[r];   // (a bit_cast of the element itself reads [0])
+                            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, e), dy,
+                                                                  v + r < a.V ? o + 2u * r : kOut, 0, 0);
+                        }
                     }
                 }
             }
         }
+        // ---- the state
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int x = 0; x < VW; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[kt][x][r] = fmaf(S[kt][x][r], em1, S[kt][x][r]);
+        auto update = [&](auto three) {
+            constexpr int NP = decltype(three)::value ? 3 : 2, KH = KT / 2;
+#pragma unroll
+            for (int jb = 0; jb < 2; ++jb) {
+                bf16x8 kf[KH], parts[VW][NP];
+                auto k_tiles = [&](int kt0) {
+#pragma unroll
+                    for (int kt = 0; kt < KH; ++kt)
+                        kf[kt] = cat(tr_read<KP>(&s.k[0][0], 32 * jb + 8 * g4, 16 * (kt0 + kt), l16),
+                                     tr_read<KP>(&s.k[0][0], 32 * jb + 8 * g4 + 4, 16 * (kt0 + kt), l16));
+                };
+                bf16x8 vf[VW];
+#pragma unroll
+                for (int x = 0; x < VW; ++x) vf[x] = v_tile(jb, x);
+                const floatx4 wa = *reinterpret_cast<const floatx4*>(&s.wj[32 * jb + 8 * g4]);
+                const floatx4 wb = *reinterpret_cast<const floatx4*>(&s.wj[32 * jb + 8 * g4 + 4]);
+                k_tiles(0);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 0; x < VW; ++x)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float f = (float)vf[x][e] * (e < 4 ? wa[e & 3] : wb[e & 3]);
+#pragma unroll
+                        for (int c = 0; c < NP; ++c) {
+                            parts[x][c][e] = (__bf16)f;
+                            f -= (float)parts[x][c][e];
+                        }
+                    }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int c = NP - 1; c >= 0; --c)
+#pragma unroll
+                        for (int kt = 0; kt < KH; ++kt)
+#pragma unroll
+                            for (int x = 0; x < VW; ++x)
+                                S[KH * half + kt][x] = mfma(kf[kt], parts[x][c], S[KH * half + kt][x]);
+                    if (half == 0) k_tiles(KH);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // Two parts leave 2^-18 of a term out, which the decay to the sequence's end takes below
+        // 2^-21 in most chunks of most heads; the third is kept where it does not.
+        if (a.hT && gl * (float)(len - t - n) > -3.f) update(std::true_type{});
+        else update(std::false_type{});
+
         __syncthreads();
     }
 
-    float* to = STATE ? a.seg + seg * slot : (last ? a.hT : nullptr);
-    if (to)
-        each_state([&](floatx4& r, long o, int left) { store_state4<VEC>(to + state + o, r, left); });
+    float* to = STATE ? (last ? nullptr : a.seg + seg * slot) : (last ? a.hT : nullptr);
+    if (to) {
+        const auto d = ssm::rsrc(to + state, sbytes);
+        each_state([&](floatx4& r, unsigned o, int left) { store_f4<VEC>(d, o, r, left); });
+    }
 }
 
 // ---------------------------------------------------------------- fp32
@@ -436,13 +525,13 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
 // q and k as 16-byte pieces.
 constexpr int CF = 32;
 
-template <int KD, int VT>
+template <int KD, int VT, bool STATE>
 struct SmemF {
-    static constexpr int KP = KD + 4, VP = VT + 4, PP = CF + 4;
-    alignas(16) float q[CF][KP];
+    static constexpr int KP = KD + 4, VP = VT + 4, PP = CF + 4, Y = STATE ? 1 : CF;
+    alignas(16) float q[Y][KP];
     alignas(16) float k[CF][KP];
     alignas(16) float v[CF][VP];
-    alignas(16) float p[CF][PP];
+    alignas(16) float p[Y][PP];
     int odd[2];
 };
 
@@ -450,23 +539,9 @@ __device__ __forceinline__ floatx4 mfma4(float a, float b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-template <bool VEC>
-__device__ __forceinline__ floatx4 fetch_f(__amdgpu_buffer_rsrc_t r, unsigned row, unsigned ld,
-                                           int col, int width) {
-    const unsigned o = (row * ld + (unsigned)col) * 4u;
-    if constexpr (VEC) {
-        return ssm::bload16<floatx4>(r, col < width ? o : kOut);
-    } else {
-        floatx4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = ssm::bload4(r, col + e < width ? o + 4u * e : kOut);
-        return x;
-    }
-}
-
 template <int KD, int VT, bool VEC, bool STATE>
 __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a) {
-    using Smem = SmemF<KD, VT>;
+    using Smem = SmemF<KD, VT, STATE>;
     constexpr int KT = KD / 16, VW = VT / 64;
     constexpr int NK = CF * KD / 4 / 256, NV = CF * VT / 4 / 256;
     __shared__ Smem s;
@@ -478,7 +553,10 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
     const int len = seq_len(a, b);
     const int t_begin = seg * a.seglen, t_end = min(len, t_begin + a.seglen);
     const bool last = seg == (len > 0 ? (len - 1) / a.seglen : 0);
-    if (STATE ? last || t_begin >= len : !last && t_begin >= len) return;
+    // (the first segment's state pass also copies h0: hT may alias it, and the last segment may end
+    // before another begins)
+    const bool copy = STATE && seg == 0 && a.h0;
+    if (STATE ? (last || t_begin >= len) && !copy : !last && t_begin >= len) return;
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -489,31 +567,20 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
     const long slot = (long)a.B * a.H * a.V * a.K;
 
     floatx4 S[KT][VW];
+    const unsigned sbytes = (unsigned)(a.V * a.K) * 4u;
     auto each_state = [&](auto&& f) {
+        const int vl = v0 + fresh(l16), kl = 4 * fresh(g4);
 #pragma unroll
-        for (int x = 0; x < VW; ++x) {
-            const int v = v0 + 16 * x + l16;
-            if (v < a.V) {
+        for (int x = 0; x < VW; ++x)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const int kk = 16 * kt + 4 * g4;
-                    f(S[kt][x], (long)v * a.K + kk, a.K - kk);
-                }
-            }
-        }
+            for (int kt = 0; kt < KT; ++kt)
+                f(S[kt][x], (unsigned)((vl + 16 * x) * a.K + kl + 16 * kt) * 4u,
+                  vl + 16 * x < a.V ? a.K - kl - 16 * kt : 0);
     };
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int x = 0; x < VW; ++x) S[kt][x] = floatx4{0.f, 0.f, 0.f, 0.f};
-    if (!STATE) {
-        const float* from = a.nseg > 1 ? (seg || a.h0 ? a.seg + seg * slot : nullptr) : a.h0;
-        if (from)
-            each_state([&](floatx4& r, long o, int left) {
-                r = load_state4<VEC>(from + state + o, left);
-            });
-    }
-
     floatx4 rq[STATE ? 1 : NK], rk[NK], rv[NV];
     auto base = [&](const void* p, long ld, int head, int width, int t) {
         return static_cast<const float*>(p) + ((long)b * a.L + t) * ld + (long)head * width;
@@ -523,30 +590,57 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
     };
     auto fetch = [&](int t) {
         const int n = max(0, min(CF, t_end - t));
-        const int tt = min(t, a.L - 1);
+        const int tt = min(t, a.L - 1), ft = fresh(tid);
         const auto dk = ssm::rsrc(base(a.k, a.ldk, grp, a.K, tt), bytes(a.ldk, a.K, n));
         const auto dv = ssm::rsrc(base(a.v, a.ldv, grp, a.V, tt), bytes(a.ldv, a.V, n));
 #pragma unroll
         for (int u = 0; u < NK; ++u) {
-            const int e = tid + 256 * u, row = e / (KD / 4), col = e % (KD / 4) * 4;
-            rk[u] = fetch_f<VEC>(dk, row, (unsigned)a.ldk, col, a.K);
+            const int e = ft + 256 * u, row = e / (KD / 4), col = e % (KD / 4) * 4;
+            rk[u] = load_f4<VEC>(dk, ((unsigned)row * (unsigned)a.ldk + col) * 4u, a.K - col);
         }
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            const int e = tid + 256 * u, row = e / (VT / 4), col = part * VT + e % (VT / 4) * 4;
-            rv[u] = fetch_f<VEC>(dv, row, (unsigned)a.ldv, col, a.V);
+            const int e = ft + 256 * u, row = e / (VT / 4), col = part * VT + e % (VT / 4) * 4;
+            rv[u] = load_f4<VEC>(dv, ((unsigned)row * (unsigned)a.ldv + col) * 4u, a.V - col);
         }
         if constexpr (!STATE) {
             const auto dq = ssm::rsrc(base(a.q, a.ldq, h, a.K, tt), bytes(a.ldq, a.K, n));
 #pragma unroll
             for (int u = 0; u < NK; ++u) {
-                const int e = tid + 256 * u, row = e / (KD / 4), col = e % (KD / 4) * 4;
-                rq[u] = fetch_f<VEC>(dq, row, (unsigned)a.ldq, col, a.K);
+                const int e = ft + 256 * u, row = e / (KD / 4), col = e % (KD / 4) * 4;
+                rq[u] = load_f4<VEC>(dq, ((unsigned)row * (unsigned)a.ldq + col) * 4u, a.K - col);
             }
         }
     };
+    if (copy) {
+        const auto from = ssm::rsrc(a.h0 + state, sbytes);
+        const auto to = ssm::rsrc(a.seg + (a.nseg - 1) * slot + state, sbytes);
+        each_state([&](floatx4&, unsigned o, int left) {
+            store_f4<VEC>(to, o, load_f4<VEC>(from, o, left), left);
+        });
+        if (last) return;
+    }
     if (tid < 2) s.odd[tid] = 0;
     if (t_begin < t_end) fetch(t_begin);
+    if (!STATE) {
+        // h0 (where there are segments, its copy), then the segments' own states, each decayed by a
+        // segment's length; or the sum that the combine pass left
+        const float* h0 = a.nseg > 1 && a.h0 ? a.seg + (a.nseg - 1) * slot : a.h0;
+        if (a.combined) h0 = seg || a.h0 ? a.seg + seg * slot : nullptr;
+        if (h0) {
+            const auto d = ssm::rsrc(h0 + state, sbytes);
+            each_state([&](floatx4& r, unsigned o, int left) { r = load_f4<VEC>(d, o, left); });
+        }
+        const float seg_m1 = decay_m1(g, a.seglen);
+        for (int p = 0; p < seg && !a.combined; ++p) {
+            const auto d = ssm::rsrc(a.seg + p * slot + state, sbytes);
+            each_state([&](floatx4& r, unsigned o, int left) {
+                const floatx4 own = load_f4<VEC>(d, o, left);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r[e] = fmaf(r[e], seg_m1, r[e]) + own[e];
+            });
+        }
+    }
     __syncthreads();
 
     float wj[2][4], em1 = 0.f;
@@ -554,16 +648,17 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
     int parity = 0;
     for (int t = t_begin; t < t_end; t += CF, parity ^= 1) {
         const int n = min(CF, t_end - t);
+        const int ft = fresh(tid);
         bool odd = false;
 #pragma unroll
         for (int u = 0; u < NK; ++u) {
-            const int e = tid + 256 * u, row = e / (KD / 4), col = e % (KD / 4) * 4;
+            const int e = ft + 256 * u, row = e / (KD / 4), col = e % (KD / 4) * 4;
             *reinterpret_cast<floatx4*>(&s.k[row][col]) = rk[u];
             if constexpr (!STATE) *reinterpret_cast<floatx4*>(&s.q[row][col]) = rq[u];
         }
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            const int e = tid + 256 * u, row = e / (VT / 4), col = e % (VT / 4) * 4;
+            const int e = ft + 256 * u, row = e / (VT / 4), col = e % (VT / 4) * 4;
             *reinterpret_cast<floatx4*>(&s.v[row][col]) = rv[u];
             if constexpr (!STATE) {
 #pragma unroll
@@ -626,7 +721,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
                 }
 #pragma unroll
             for (int it = 0; it < 2; ++it) {
-                const float f = a.scale * ssm::ex2(gl * (float)(16 * it + l16 + 1));
+                const float f = a.scale * ssm::ex2(fresh(gl) * (float)(16 * it + l16 + 1));
 #pragma unroll
                 for (int x = 0; x < VW; ++x) Y[x][it] *= f;
             }
@@ -690,28 +785,28 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
                         }
                     }
             }
+            const auto dy = ssm::rsrc(static_cast<float*>(a.y) + ((long)b * a.L + t) * a.ldy + (long)h * a.V,
+                                      bytes(a.ldy, a.V, n));
 #pragma unroll
-            for (int it = 0; it < 2; ++it) {
-                const int i = 16 * it + l16;
-                if (i >= n) continue;
-                float* yr = static_cast<float*>(a.y) + ((long)b * a.L + t + i) * a.ldy + (long)h * a.V;
+            for (int it = 0; it < 2; ++it)
 #pragma unroll
                 for (int x = 0; x < VW; ++x) {
                     const int v = v0 + 16 * x + 4 * g4;
-                    store_state4<VEC>(yr + v, Y[x][it], a.V - v);
+                    store_f4<VEC>(dy, ((unsigned)(16 * it + l16) * (unsigned)a.ldy + v) * 4u, Y[x][it], a.V - v);
                 }
-            }
         }
         __syncthreads();
     }
 
-    float* to = STATE ? a.seg + seg * slot : (last ? a.hT : nullptr);
-    if (to)
-        each_state([&](floatx4& r, long o, int left) { store_state4<VEC>(to + state + o, r, left); });
+    float* to = STATE ? (last ? nullptr : a.seg + seg * slot) : (last ? a.hT : nullptr);
+    if (to) {
+        const auto d = ssm::rsrc(to + state, sbytes);
+        each_state([&](floatx4& r, unsigned o, int left) { store_f4<VEC>(d, o, r, left); });
+    }
 }
 
-// Entering states: slot[s] <- E_s, E_0 = h0 (or 0), E_{s+1} = e^{g seglen} E_s + own state of s.
-// (h0 is copied too: hT may alias it, and the last segment may end before the first begins.)
+// Entering states of many segments: slot s <- E_s, E_0 = h0 (its copy in the last slot) or 0, E_{s+1} =
+// e^{g seglen} E_s + own state of s.
 __global__ __launch_bounds__(256) void la_combine_kernel(LaArgs a) {
     const long VK = (long)a.V * a.K, slot = (long)a.B * a.H * VK;
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
@@ -720,24 +815,28 @@ __global__ __launch_bounds__(256) void la_combine_kernel(LaArgs a) {
     const int len = seq_len(a, b);
     const int used = len > 0 ? (len - 1) / a.seglen + 1 : 1;   // segments that run
     const float em1 = decay_m1(clamp_g(a.g[h]), a.seglen);
-    float e = a.h0 ? a.h0[i] : 0.f;
     float* p = a.seg + i;
+    float e = a.h0 ? p[(a.nseg - 1) * slot] : 0.f;
+    float own = used > 1 ? p[0] : 0.f;   // (own states are read before E takes their slot)
+    if (a.h0) p[0] = e;
     constexpr int U = 8;
     int sgm = 0;
-    for (; sgm + U < used; sgm += U) {
-        float own[U];
+    for (; sgm + U < used - 1; sgm += U) {
+        float next[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) own[u] = p[(sgm + u) * slot];
+        for (int u = 0; u < U; ++u) next[u] = p[(sgm + u + 1) * slot];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            p[(sgm + u) * slot] = e;
-            e = fmaf(e, em1, e) + own[u];
+            e = fmaf(e, em1, e) + own;
+            p[(sgm + u + 1) * slot] = e;
+            own = next[u];
         }
     }
-    for (; sgm < used; ++sgm) {
-        const float own = sgm + 1 < used ? p[sgm * slot] : 0.f;
-        p[sgm * slot] = e;
+    for (; sgm < used - 1; ++sgm) {
+        const float next = sgm + 2 < used ? p[(sgm + 1) * slot] : 0.f;
         e = fmaf(e, em1, e) + own;
+        p[(sgm + 1) * slot] = e;
+        own = next;
     }
 }
 
@@ -756,17 +855,27 @@ void la_plan(int dtype, int B, int L, int H, int K, int V, int& nseg, int& segle
     nseg = (int)std::max(1L, ssm::cdiv(L, seglen));
 }
 
+// A chain of more segments than this is combined once, by a pass of its own.
+constexpr int kChain = 4;
+
 template <int KD, int VT, bool VEC>
-ssm_status la_launch(int dtype, const LaArgs& a, hipStream_t st) {
+ssm_status la_launch(int dtype, LaArgs a, hipStream_t st) {
     const unsigned n = (unsigned)((long)a.nseg * a.B * a.H * a.vparts);
     if (a.nseg > 1) {
-        const unsigned n1 = (unsigned)((long)(a.nseg - 1) * a.B * a.H * a.vparts);
-        if (dtype == SSM_F32) la_f32_kernel<KD, VT, VEC, true><<<n1, 256, 0, st>>>(a);
-        else la_bf16_kernel<KD, VT, VEC, true><<<n1, 256, 0, st>>>(a);
+        // 64 columns a workgroup, whatever the full pass takes: half the registers, so that more of
+        // them share a CU
+        LaArgs s = a;
+        s.vparts = (int)ssm::cdiv(a.V, 64);
+        const unsigned n1 = (unsigned)((long)(a.nseg - 1) * a.B * a.H * s.vparts);
+        if (dtype == SSM_F32) la_f32_kernel<KD, 64, VEC, true><<<n1, 256, 0, st>>>(s);
+        else la_bf16_kernel<KD, 64, VEC, true><<<n1, 256, 0, st>>>(s);
         if (ssm_status e = ssm::check_launch("ssm_linear_attention (states)")) return e;
-        const long m = (long)a.B * a.H * a.V * a.K;
-        la_combine_kernel<<<(unsigned)ssm::cdiv(m, 256), 256, 0, st>>>(a);
-        if (ssm_status e = ssm::check_launch("ssm_linear_attention (combine)")) return e;
+        a.combined = a.nseg > kChain;
+        if (a.combined) {
+            const long m = (long)a.B * a.H * a.V * a.K;
+            la_combine_kernel<<<(unsigned)ssm::cdiv(m, 256), 256, 0, st>>>(a);
+            if (ssm_status e = ssm::check_launch("ssm_linear_attention (combine)")) return e;
+        }
     }
     if (dtype == SSM_F32) la_f32_kernel<KD, VT, VEC, false><<<n, 256, 0, st>>>(a);
     else la_bf16_kernel<KD, VT, VEC, false><<<n, 256, 0, st>>>(a);
@@ -918,13 +1027,14 @@ extern "C" ssm_status ssm_linear_attention(int dtype, const void* q, long ldq, c
                 "ssm_linear_attention: row stride below row width");
     const long esz = dtype == SSM_F32 ? 4 : 2, ev = 16 / esz;
     const long lim = (1L << 31) / (CB * esz);   // a chunk's byte offsets are 32-bit
-    SSM_REQUIRE(ldq < lim && ldk < lim && ldv < lim, "ssm_linear_attention: row stride too large");
+    SSM_REQUIRE(ldq < lim && ldk < lim && ldv < lim && ldy < lim, "ssm_linear_attention: row stride too large");
     LaArgs a{};
     a.q = q; a.ldq = ldq; a.k = k; a.ldk = ldk; a.v = v; a.ldv = ldv; a.g = g; a.scale = scale;
     a.lengths = lengths; a.y = y; a.ldy = ldy; a.B = B; a.L = L; a.H = H; a.G = G; a.K = K; a.V = V;
     a.h0 = h0; a.hT = hT;
     la_plan(dtype, B, L, H, K, V, a.nseg, a.seglen, a.vparts);
-    SSM_REQUIRE((long)a.nseg * B * H * a.vparts < (1L << 31) &&
+    SSM_REQUIRE((long)V * K < (1L << 29), "ssm_linear_attention: state of a head too large");
+    SSM_REQUIRE((long)a.nseg * B * H * ssm::cdiv(V, 64) < (1L << 31) &&
                     (long)B * H * V * K < (1L << 38),
                 "ssm_linear_attention: too many heads");
     if (a.nseg > 1) {
