@@ -261,8 +261,9 @@ ssm_status ssm_quantize_rows(int dtype, const void* x, long ldx, int8_t* q, long
                              int M, int K, void* stream);
 /* y[m,n] = beta*y[m,n] + sx[m] sw[n] sum_k x[m,k] W[n,k] (+ bias[n]) with 8-bit x (M,K), W (N,K):
  * exact 32-bit integer sums, so K <= 131071. beta 0 does not read y. y of `out_dtype` (SSM_F32,
- * SSM_BF16). 16-byte aligned rows (ldw % 16 == 0; K % 4 == 0, for x K % 256 == 0) are read in
- * place; others are laid out in the workspace first. Row strides below 2^22.
+ * SSM_BF16). Read in place are 16-byte aligned rows: of W with K % 4 == 0 and ldw % 16 == 0, of x with
+ * K % 256 == 0, ldx % 16 == 0 and M > 64; others are laid out in the workspace first. Row strides
+ * below 2^22 (y's below 2^21).
  * workspace: 16-byte aligned, ssm_linear_i8_workspace(...) bytes (0 where nothing is laid out), one
  * stream at a time. */
 size_t ssm_linear_i8_workspace(const int8_t* x, long ldx, const int8_t* W, long ldw, int M, int N,

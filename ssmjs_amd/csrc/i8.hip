@@ -10,16 +10,19 @@
 //   - more rows: the matrix cores bound it. i8_gemm_kernel is a tiled product out of LDS.
 //   - rows that are not 16-byte aligned are laid out in the workspace first (pad_rows_kernel).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 
 namespace {
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef int intx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void;
 
+constexpr unsigned kOut = 0x80000000u;   // a buffer offset past any descriptor
 constexpr int kMaxK = 131071;
 constexpr int kPad = 256;          // rows of the workspace are whole blocks of 256 bytes, zeros past K
 constexpr int kRowsMax = 64;       // rows of the few-row kernel
@@ -88,7 +91,16 @@ struct QuantArgs {
     signed char* q; long ldq;
     float* scale;
     int M, K, Kq;   // Kq: bytes written per row (zeros past K)
+    int frag;       // in the order of the few-row kernel's operand
 };
+
+// Byte k of row m in the order of the few-row kernel's operand: the 16-row block m / 16 and the block
+// of 256 k hold four operands of 1 KB, of which lane (g, i) has 16 bytes, row i's from 64 g + 16 u on.
+// (k's 16-byte pieces stay whole.)
+__device__ __forceinline__ long frag_at(long m, int k, int Kp) {
+    return ((m >> 4) * (Kp >> 8) + (k >> 8)) * 4096L + (k >> 4 & 3) * 1024 + (k >> 6 & 3) * 256 +
+           (m & 15) * 16 + (k & 15);
+}
 
 // A row per workgroup of TPR threads' share: 256 / TPR rows a workgroup, U pieces of four held
 // between the two passes (further ones are read again).
@@ -122,11 +134,13 @@ __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
     if (tid == 0) a.scale[m] = s;
     const bool ok = usable(s);
     const Quant z(ok ? s : 1.f);
-    signed char* out = a.q + m * a.ldq;
+    signed char* out = a.q + (a.frag ? 0 : m * a.ldq);
     auto put = [&](int k, float4 x) {
         if (k >= a.Kq) return;
         const unsigned b = ok ? pack4(z, x) : 0u;
-        if constexpr (VEC) {
+        if (a.frag) {   // (Kq is a whole number of pieces)
+            *reinterpret_cast<unsigned*>(out + frag_at(m, k, (int)a.ldq)) = b;
+        } else if constexpr (VEC) {
             *reinterpret_cast<unsigned*>(out + k) = b;
         } else {
 #pragma unroll
@@ -154,15 +168,16 @@ ssm_status run_quant(const QuantArgs& a, bool vec, hipStream_t st) {
 }
 
 ssm_status quantize(int dtype, const void* x, long ldx, signed char* q, long ldq, float* scale,
-                    int M, int K, int Kq, hipStream_t st) {
-    const QuantArgs a{x, ldx, q, ldq, scale, M, K, Kq};
+                    int M, int K, int Kq, bool frag, hipStream_t st) {
+    const QuantArgs a{x, ldx, q, ldq, scale, M, K, Kq, frag};
     const bool vec = K % 4 == 0 && Kq % 4 == 0 && ldx % 4 == 0 && ldq % 4 == 0 &&
                      ((uintptr_t)x & (dtype == SSM_F32 ? 15 : 7)) == 0 && ((uintptr_t)q & 3) == 0;
     return dtype == SSM_F32 ? run_quant<float>(a, vec, st) : run_quant<__bf16>(a, vec, st);
 }
 
-// Rows of K bytes at any alignment -> rows of Kp bytes, zeros past K.
-__global__ __launch_bounds__(256) void pad_rows_kernel(const signed char* __restrict__ x, long ldx,
+// Rows of K bytes at any alignment -> rows of Kp bytes, zeros past K (or the few-row operand's order).
+template <bool FRAG>
+__global__ __launch_bounds__(256) void lay_rows_kernel(const signed char* __restrict__ x, long ldx,
                                                        int K, signed char* __restrict__ o, int Kp) {
     const signed char* row = x + (long)blockIdx.x * ldx;
     for (int k = 4 * threadIdx.x; k < Kp; k += 1024) {
@@ -170,63 +185,75 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const signed char* __rest
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (k + e < K) b |= (unsigned)(unsigned char)row[k + e] << 8 * e;
-        *reinterpret_cast<unsigned*>(o + (long)blockIdx.x * Kp + k) = b;
+        *reinterpret_cast<unsigned*>(o + (FRAG ? frag_at(blockIdx.x, k, Kp) : (long)blockIdx.x * Kp + k)) = b;
     }
 }
 
 // ---------------------------------------------------------------- epilogue
 struct I8Args {
     const signed char* X; long ldx; const float* sx;   // x as integers (null: from Xf)
-    const void* Xf; long ldxf;                         // x to be rounded in the kernel
+    const void* Xf; long ldxf; int x_dtype;            // x to be rounded in the kernel
     const signed char* W; long ldw; const float* sw;
     const float* bias;
     void* y; long ldy;
     int M, N, K;
     float beta;
+    int vec;      // outputs in aligned pieces of 16 bytes
     int mt, nt, gn;
 };
 
-// Four outputs n .. n + 3 of row m.
+// The outputs of a tile, rows m0 .. and columns n0 ..: a descriptor that ends with the last of them.
+template <typename TO>
+struct Out {
+    __amdgpu_buffer_rsrc_t d;
+    unsigned ld;
+    int cols;
+    __device__ __forceinline__ Out(const I8Args& a, int m0, int rows, int n0, int cols_)
+        : d(ssm::rsrc(static_cast<TO*>(a.y) + (long)m0 * a.ldy + n0,
+                      (unsigned)(((long)(rows - 1) * a.ldy + cols_) * (long)sizeof(TO)))),
+          ld((unsigned)a.ldy), cols(cols_) {}
+};
+
+// One output, n of row m of the tile.
 template <typename TO, bool BETA>
-__device__ __forceinline__ void put4(const I8Args& a, int m, int n, intx4 c, float sm, bool vec) {
-    if (m >= a.M || n >= a.N) return;
-    TO* y = static_cast<TO*>(a.y) + (long)m * a.ldy + n;
-    float o[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int nn = min(n + r, a.N - 1);
-        o[r] = (float)c[r] * (sm * a.sw[nn]);
-        if (a.bias) o[r] += a.bias[nn];
-    }
-    if (vec && n + 3 < a.N) {
-        if constexpr (sizeof(TO) == 4) {
-            floatx4 v = {o[0], o[1], o[2], o[3]};
-            if constexpr (BETA) v += a.beta * *reinterpret_cast<const floatx4*>(y);
-            *reinterpret_cast<floatx4*>(y) = v;
-        } else {
-            bf16x4 v;
-            if constexpr (BETA) {
-                const bf16x4 p = *reinterpret_cast<const bf16x4*>(y);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[r] += a.beta * (float)p[r];
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (__bf16)o[r];
-            *reinterpret_cast<bf16x4*>(y) = v;
-        }
+__device__ __forceinline__ void put1(const Out<TO>& o, float beta, int m, int n, float x) {
+    const unsigned off = n < o.cols ? ((unsigned)m * o.ld + (unsigned)n) * (unsigned)sizeof(TO) : kOut;
+    if constexpr (sizeof(TO) == 4) {
+        if constexpr (BETA) x += beta * ssm::bload4(o.d, off);
+        ssm::bstore4(x, o.d, off);
     } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (n + r < a.N) {
-                if constexpr (BETA) o[r] += a.beta * (float)y[r];
-                y[r] = (TO)o[r];
-            }
+        if constexpr (BETA) {
+            const unsigned p = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(o.d, off, 0, 0);
+            x += beta * __builtin_bit_cast(float, p << 16);
+        }
+        const __bf16 y = (__bf16)x;
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, y), o.d, off, 0, 0);
     }
 }
 
-template <typename TO>
-__device__ __forceinline__ bool vec_out(const I8Args& a) {
-    return a.ldy % 4 == 0 && ((uintptr_t)a.y & (4 * sizeof(TO) - 1)) == 0;
+// 16 bytes of outputs, n .. of row m, aligned to their size.
+template <typename TO, bool BETA>
+__device__ __forceinline__ void put(const Out<TO>& o, float beta, int m, int n, float* v) {
+    constexpr int E = 16 / sizeof(TO);
+    const unsigned off = n < o.cols ? ((unsigned)m * o.ld + (unsigned)n) * (unsigned)sizeof(TO) : kOut;
+    if constexpr (sizeof(TO) == 4) {
+        if constexpr (BETA) {
+            const floatx4 y = ssm::bload16<floatx4>(o.d, off);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += beta * y[e];
+        }
+        ssm::bstore16(make_float4(v[0], v[1], v[2], v[3]), o.d, off);
+    } else {
+        bf16x8 y;
+        if constexpr (BETA) {
+            y = ssm::bload16<bf16x8>(o.d, off);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] += beta * (float)y[e];
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = (__bf16)v[e];
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(ssm::u32x4, y), o.d, off, 0, 0);
+    }
 }
 
 // A row's bytes in whole dwords: one that a descriptor ends inside reads as zeros. (Rows that are
@@ -239,48 +266,112 @@ __device__ __forceinline__ intx4 mfma8(intx4 w, intx4 x, intx4 c) {
 
 // ---------------------------------------------------------------- up to 64 rows
 // A workgroup owns NB blocks of 16 output channels; its four waves take the blocks of 256 k in
-// turn. Lane (g, i) = (lane / 16, lane % 16) holds row i's bytes 64 g + 16 u .. of the block for
-// u = 0 .. 3, which is the operand of MFMA u with the block's k in another order, the same for both
-// operands; so a lane reads 64 consecutive bytes. The waves' sums meet in LDS (integers: their order
-// changes nothing).
-template <int MB, int NB, typename TO, bool BETA>
+// turn. Lane (g, i) = (lane / 16, lane % 16) reads W row i's bytes 64 g + 16 u .. of the block for
+// u = 0 .. 3, which is the operand of MFMA u with the block's k in another order, the same for x. So a
+// lane reads 64 consecutive bytes of its row, and x lies in the workspace in the operands' own order (a
+// row-major x took 3 times as long at 64 rows: 16 lines an instruction). The waves' sums meet in
+// LDS (integers: their order changes nothing).
+//
+// FUSED: up to four rows of x of at most kFusedX elements in all are rounded by every workgroup for
+// itself, into LDS, while its weights are on their way: one launch instead of two.
+constexpr int kFusedX = 8192, kFusedRows = 4;
+
+template <int MB, int NB, typename TX, typename TO, bool BETA>
 __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
+    constexpr bool FUSED = !std::is_void<TX>::value;
+    constexpr int kPieces = kFusedX / 1024;
     __shared__ intx4 red[3][NB * MB][64];
+    __shared__ __attribute__((aligned(16))) signed char xs[FUSED ? kFusedX + kFusedRows * kPad : 16];
+    __shared__ unsigned most[FUSED ? 4 : 1][kPieces];
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15;
     const int n0 = blockIdx.x * 16 * NB;
     const int rows = min(16 * NB, a.N - n0);
     const auto rw = ssm::rsrc(a.W + (long)n0 * a.ldw, (unsigned)((long)(rows - 1) * a.ldw + whole(a.K)));
-    const auto rx = ssm::rsrc(a.X, (unsigned)((long)(a.M - 1) * a.ldx + whole(a.K)));
-    const unsigned wo = (unsigned)(i * a.ldw) + 64u * g, xo = (unsigned)(i * a.ldx) + 64u * g;
-    intx4 acc[NB][MB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int m = 0; m < MB; ++m) acc[b][m] = intx4{0, 0, 0, 0};
+    const unsigned wo = (unsigned)(i * a.ldw) + 64u * g;
     const int steps = (a.K + 255) / 256;
-    for (int s = w; s < steps; s += 4) {
-        intx4 wv[NB][4], xv[MB][4];
-        const unsigned k = 256u * s;
+    auto weights = [&](intx4 (&wv)[NB][4], int s) {   // (a step past the last reads zeros)
+        const unsigned k = s < steps ? 256u * s : kOut;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 wv[b][u] = __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(
                     rw, wo + (unsigned)(16 * b * a.ldw) + 16u * u + k, 0, 0));
+    };
+    intx4 acc[NB][MB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) acc[b][m] = intx4{0, 0, 0, 0};
+    intx4 wv[2][NB][4];
+    weights(wv[0], w);
+    weights(wv[1], w + 4);
+
+    float sm[MB];
+    if constexpr (FUSED) {
+        const int per = (a.K + 1023) / 1024;   // pieces of a row; M * per <= kPieces
+        const int Kp = (a.K + kPad - 1) / kPad * kPad;
+        float4 v[kPieces];
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+            const int m = p / per, k = 4 * ((int)threadIdx.x + 256 * (p - m * per));
+            v[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (m < a.M) v[p] = some4<TX, true>(static_cast<const TX*>(a.Xf) + (long)m * a.ldxf, k, a.K);
+            unsigned t = max4(0, v[p]);
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) t = max(t, (unsigned)__shfl_xor((int)t, off));
+            if (lane == 0) most[w][p] = t;
+        }
+        __syncthreads();
+        auto scale = [&](int m) {
+            unsigned t = 0;
+            for (int p = m * per; p < (m + 1) * per; ++p)
+                t = max(max(t, max(most[0][p], most[1][p])), max(most[2][p], most[3][p]));
+            return scale_of(t);
+        };
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+            const int m = p / per, k = 4 * ((int)threadIdx.x + 256 * (p - m * per));
+            if (m < a.M && k < Kp) {
+                const float s = scale(m);
+                const bool ok = usable(s);
+                *reinterpret_cast<unsigned*>(xs + m * Kp + k) = ok ? pack4(Quant(ok ? s : 1.f), v[p]) : 0u;
+            }
+        }
+        sm[0] = scale(min(i, a.M - 1));
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int m = 0; m < MB; ++m) sm[m] = a.sx[min(16 * m + i, a.M - 1)];
+    }
+    auto step = [&](intx4 (&wv)[NB][4], int s) {
+        intx4 xv[MB][4];
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                xv[m][u] = __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(
-                    rx, xo + (unsigned)(16 * m * a.ldx) + 16u * u + k, 0, 0));
+            for (int u = 0; u < 4; ++u) {
+                if constexpr (FUSED) {
+                    const int Kp = (a.K + kPad - 1) / kPad * kPad;
+                    xv[m][u] = intx4{0, 0, 0, 0};
+                    if (i < a.M) xv[m][u] = *reinterpret_cast<const intx4*>(xs + i * Kp + 256 * s + 64 * g + 16 * u);
+                } else {
+                    xv[m][u] = *reinterpret_cast<const intx4*>(a.X + ((long)m * steps + s) * 4096 + u * 1024 + lane * 16);
+                }
+            }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int m = 0; m < MB; ++m) acc[b][m] = mfma8(wv[b][u], xv[m][u], acc[b][m]);
+    };
+    for (int s = w; s < steps; s += 8) {
+        step(wv[0], s);
+        weights(wv[0], s + 8);
+        if (s + 4 < steps) step(wv[1], s + 4);
+        weights(wv[1], s + 12);
     }
     if (w > 0) {
 #pragma unroll
@@ -290,17 +381,27 @@ __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
     }
     __syncthreads();
     if (w > 0) return;
-    const bool vec = vec_out<TO>(a);
+    const Out<TO> out(a, 0, a.M, n0, rows);
 #pragma unroll
-    for (int m = 0; m < MB; ++m) {
-        const int row = 16 * m + i;
-        const float sm = row < a.M ? a.sx[row] : 0.f;
+    for (int b = 0; b < NB; ++b) {
+        const int n = 16 * b + 4 * g;
+        floatx4 s4, b4;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
+        for (int r = 0; r < 4; ++r) {
+            const int k = min(n0 + n + r, a.N - 1);
+            s4[r] = a.sw[k];
+            b4[r] = a.bias ? a.bias[k] : 0.f;
+        }
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            const int row = 16 * m + i;
             intx4 c = acc[b][m];
 #pragma unroll
             for (int o = 0; o < 3; ++o) c += red[o][b * MB + m][lane];
-            put4<TO, BETA>(a, row, n0 + 16 * b + 4 * g, c, sm, vec);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                put1<TO, BETA>(out, a.beta, row < a.M ? row : 0, row < a.M ? n + r : 1 << 30,
+                               (float)c[r] * (sm[m] * s4[r]) + b4[r]);
         }
     }
 }
@@ -310,28 +411,29 @@ __device__ __forceinline__ void to_lds16(__amdgpu_buffer_rsrc_t r, char* lds, un
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)lds, 16, voff, 0, 0, 0);
 }
 
-// All of the wave's loads, then the workgroup barrier: the next stage is whole, and every wave has
-// finished with the stage read before.
-__device__ __forceinline__ void stage_step() {
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-}
-
-// WN x WM waves, each with TN x TM tiles of 16 x 16: a workgroup owns 16 TN WN output channels of
-// 16 TM WM rows and walks k in blocks of 128 bytes through two LDS stages, the next block's loads in
-// flight while one multiplies. A row's 128 bytes lie as eight 16-byte pieces, piece c at place
-// c ^ (row / 2 % 8): the 16 rows of an operand read then fall on all banks. The loads go straight
-// from memory to LDS (eight rows of 128 bytes an instruction), the order of the pieces being that
-// of their addresses.
-template <int WN, int WM, int TN, int TM, typename TO, bool BETA>
-__global__ __launch_bounds__(64 * WN * WM, 2) void i8_gemm_kernel(I8Args a) {
-    constexpr int NW = WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM;
-    constexpr int NL = (BN + BM) / 8, PER = NL / NW, SB = (BN + BM) * 128;
-    static_assert(NL % NW == 0 && BN % 8 == 0, "loads shared out evenly");
-    __shared__ __attribute__((aligned(16))) char s0[SB];
-    __shared__ __attribute__((aligned(16))) char s1[SB];
+// WN x WM waves, each with TN x TM tiles of 32 x 32 (v_mfma_i32_32x32x32_i8): a workgroup owns 32 TN
+// WN output channels of 32 TM WM rows and walks k in blocks of 64 through NS LDS stages. The loads
+// go straight from memory to LDS, sixteen rows of 64 bytes an instruction. A row's 64 bytes lie as
+// four 16-byte pieces, piece c at place c ^ (row / 4 % 4): any 16 consecutive rows of a piece then
+// fall on all banks.
+//
+// A block's k are two steps of 32 (one MFMA deep). While a step multiplies, the operands of the next
+// one are read; so a stage is free once its second step is in registers, a step before its products
+// end. There the wave waits for its loads of the next stage and for the workgroup, issues the loads
+// of the NS-th block on into the stage that came free, and goes on: one barrier a block, with
+// products behind and ahead of it, and a load has NS - 1 blocks' time to land.
+//
+// The outputs go through LDS, 32 rows of a wave at a time, so that they are written as whole lines:
+// written as they lie in the accumulators (16 bytes of 32 rows an instruction) they took 17 us of a
+// tile's 40 at K 2048.
+template <int WN, int WM, int TN, int TM, int NS, typename TO, bool BETA>
+__global__ __launch_bounds__(64 * WN * WM, TN * TM > 8 ? 1 : 2) void i8_gemm_kernel(I8Args a) {
+    constexpr int NW = WN * WM, BN = 32 * TN * WN, BM = 32 * TM * WM;
+    constexpr int PW = BN / 16 / NW, PX = BM / 16 / NW, PER = PW + PX, SB = (BN + BM) * 64;
+    static_assert(BN % (16 * NW) == 0 && BM % (16 * NW) == 0 && (NS == 3 || NS == 4), "loads shared out evenly");
+    // (each its own object: a read of one does not wait for the loads into the others)
+    __shared__ __attribute__((aligned(16))) char s0[SB], s1[SB], s2[SB], s3[NS > 3 ? SB : 16];
+    __shared__ __attribute__((aligned(16))) float chs[BN], chb[BN], rows_s[BM];
 
     // consecutive ids on one XCD, in groups of gn channel tiles
     const int T = a.mt * a.nt, bid = blockIdx.x;
@@ -343,116 +445,226 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void i8_gemm_kernel(I8Args a) {
 
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = lane >> 4, i16 = lane & 15;
+    const int g = lane >> 5, i32 = lane & 31;
     const int wn = w % WN, wm = w / WN;
     const int n0 = tn * BN, m0 = tm * BM;
     const int nrows = min(BN, a.N - n0), mrows = min(BM, a.M - m0);
+    for (int i = threadIdx.x; i < BN + BM; i += 64 * NW) {
+        if (i < BN) {
+            const int n = min(n0 + i, a.N - 1);
+            chs[i] = a.sw[n];
+            chb[i] = a.bias ? a.bias[n] : 0.f;
+        } else {
+            rows_s[i - BN] = a.sx[min(m0 + i - BN, a.M - 1)];
+        }
+    }
+    // a wave loads PW groups of sixteen rows of W and PX of x
     const auto rw = ssm::rsrc(a.W + (long)n0 * a.ldw, (unsigned)((long)(nrows - 1) * a.ldw + whole(a.K)));
     const auto rx = ssm::rsrc(a.X + (long)m0 * a.ldx, (unsigned)((long)(mrows - 1) * a.ldx + whole(a.K)));
-
-    unsigned off[PER];
+    const unsigned piece = 16u * ((lane & 3) ^ (lane >> 4));
+    const unsigned downw = 16u * (unsigned)a.ldw, downx = 16u * (unsigned)a.ldx;
+    const unsigned atw = (unsigned)((lane >> 2) * a.ldw) + piece + PW * w * downw;
+    const unsigned atx = (unsigned)((lane >> 2) * a.ldx) + piece + PX * w * downx;
+    const int KB = (a.K + 63) / 64;
+    auto load = [&](char* s, int kb) {   // (a block past the last reads zeros: past the descriptors)
+        const unsigned k = kb < KB ? 64u * (unsigned)kb : kOut;
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-        const int r = 8 * (PER * w + u) + (lane >> 3);   // row of the stage: W's, then x's
-        const int c = (lane & 7) ^ (r >> 1 & 7);
-        off[u] = 8 * (PER * w + u) < BN ? (unsigned)(r * a.ldw) + 16u * c
-                                        : (unsigned)((r - BN) * a.ldx) + 16u * c;
-    }
-    const int KB = (a.K + 127) / 128;
-    auto load = [&](char* s, int kb) {
-        const unsigned k = 128u * (unsigned)kb;
-        if (kb >= KB) return;
+        for (int u = 0; u < PW; ++u) to_lds16(rw, s + (PW * w + u) * 1024, atw + (k + u * downw));
 #pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            const int f = PER * w + u;
-            to_lds16(8 * f < BN ? rw : rx, s + f * 1024, off[u] + k);
-        }
+        for (int u = 0; u < PX; ++u) to_lds16(rx, s + BN * 64 + (PX * w + u) * 1024, atx + (k + u * downx));
     };
-    intx4 acc[TN][TM];
+    intx16 acc[TN][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = intx4{0, 0, 0, 0};
-    const int l0 = i16 * 128 + 16 * (g ^ (i16 >> 1)), l1 = i16 * 128 + 16 * ((4 + g) ^ (i16 >> 1));
-    auto compute = [&](const char* s) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const char* p = s + (h ? l1 : l0);
-            intx4 wf[TN], xf[TM];
-#pragma unroll
-            for (int j = 0; j < TM; ++j)
-                xf[j] = *reinterpret_cast<const intx4*>(p + (BN + 16 * (TM * wm + j)) * 128);
-#pragma unroll
-            for (int i = 0; i < TN; ++i)
-                wf[i] = *reinterpret_cast<const intx4*>(p + 16 * (TN * wn + i) * 128);
-#pragma unroll
-            for (int i = 0; i < TN; ++i)
-#pragma unroll
-                for (int j = 0; j < TM; ++j) acc[i][j] = mfma8(wf[i], xf[j], acc[i][j]);
+        for (int j = 0; j < TM; ++j) {
+            acc[i][j] = intx16{};
+            asm volatile("" : "+a"(acc[i][j]));   // (in accumulation registers from the start)
         }
-    };
-    load(s0, 0);
-    for (int kb = 0; kb < KB; kb += 2) {
-        stage_step();
-        load(s1, kb + 1);
-        compute(s0);
-        stage_step();
-        load(s0, kb + 2);
-        if (kb + 1 < KB) compute(s1);
-    }
-    const bool vec = vec_out<TO>(a);
+    struct Frags { intx4 w[TN], x[TM]; };
+    const int swz = i32 >> 2 & 3;
+    const int wrow = (32 * TN * wn + i32) * 64, xrow = (BN + 32 * TM * wm + i32) * 64;
+    auto read = [&](Frags& f, const char* s, int step) {
+        const int c = 16 * ((2 * step + g) ^ swz);
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-        const int m = m0 + 16 * (TM * wm + j) + i16;
-        const float sm = m < a.M ? a.sx[m] : 0.f;
+        for (int j = 0; j < TM; ++j) f.x[j] = *reinterpret_cast<const intx4*>(s + xrow + c + 32 * j * 64);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) f.w[i] = *reinterpret_cast<const intx4*>(s + wrow + c + 32 * i * 64);
+    };
+    auto multiply = [&](const Frags& f) {
 #pragma unroll
         for (int i = 0; i < TN; ++i)
-            put4<TO, BETA>(a, m, n0 + 16 * (TN * wn + i) + 4 * g, acc[i][j], sm, vec);
+#pragma unroll
+            for (int j = 0; j < TM; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
+    };
+    // the reads (and L loads) of a step spread over the products of the one before
+    constexpr int NF = TN + TM, NP = TN * TM;
+    auto spread = [&](auto loads) {
+        constexpr int L = decltype(loads)::value;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (i < NF) __builtin_amdgcn_sched_group_barrier(0x100, (NF + NP - 1) / NP, 0);
+            if (L && i >= NP / 2) __builtin_amdgcn_sched_group_barrier(0x020, (2 * L + NP - 1) / NP, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // at most NS - 2 blocks' loads of the wave in flight, its LDS reads done, then the workgroup
+    auto meet = [&]() {
+        constexpr int KEEP = (NS - 2) * PER;
+        static_assert(KEEP < 64, "vmcnt has six bits");
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0x0070 | (KEEP & 15) | ((KEEP >> 4) << 14));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    Frags f0, f1;
+    // one block out of stage s, its first step in f0; leaves the next block's first step there
+    auto block = [&](char* s, char* next, int kb) {
+        read(f1, s, 1);
+        multiply(f0);
+        spread(std::integral_constant<int, 0>{});
+        meet();
+        read(f0, next, 0);
+        load(s, kb + NS);
+        multiply(f1);
+        spread(std::integral_constant<int, PER>{});
+    };
+    load(s0, 0);
+    load(s1, 1);
+    load(s2, 2);
+    if constexpr (NS > 3) load(s3, 3);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070 | ((NS - 1) * PER & 15) | (((NS - 1) * PER >> 4) << 14));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    read(f0, s0, 0);
+    for (int kb = 0; kb < KB; kb += NS) {   // (blocks past the last multiply zeros)
+        block(s0, s1, kb);
+        block(s1, s2, kb + 1);
+        block(s2, NS > 3 ? s3 : s0, kb + 2);
+        if constexpr (NS > 3) block(s3, s0, kb + 3);
     }
+    // no load is in flight into LDS, and no wave reads operands from it, when it takes the outputs
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+
+    constexpr int CW = 32 * TN, UW = CW / 4;   // columns of a wave, in pieces of four
+    static_assert(NW == 4 && 32 * CW * 4 <= SB, "a stage takes the outputs of 32 rows of a wave or two");
+    constexpr bool HALF = NS == 3;   // two waves a stage
+    static_assert(!HALF || 2 * 32 * CW * 4 <= SB, "");
+    float* tile = HALF ? reinterpret_cast<float*>(w < 2 ? s0 : s1) + (w & 1) * 32 * CW
+                       : reinterpret_cast<float*>(w == 0 ? s0 : w == 1 ? s1 : w == 2 ? s2 : s3);
+    // piece u of row r: its 32 rows fall on different banks
+    auto place = [&](int r, int u) { return tile + r * CW + 4 * (u ^ (r & (UW - 1))); };
+    const Out<TO> out(a, m0, mrows, n0, nrows);
+    auto finish = [&](auto vec) {
+        constexpr bool VEC = decltype(vec)::value;
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            const int mw = 32 * (TM * wm + j);
+            const float sm = rows_s[mw + i32];
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {   // channels 8 q + 4 g .. + 3 of the tile, row i32
+                    const int u = 8 * i + 2 * q + g;
+                    const floatx4 s4 = *reinterpret_cast<const floatx4*>(&chs[CW * wn + 4 * u]);
+                    const floatx4 b4 = *reinterpret_cast<const floatx4*>(&chb[CW * wn + 4 * u]);
+                    floatx4 v;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = (float)acc[i][j][4 * q + r] * (sm * s4[r]) + b4[r];
+                    *reinterpret_cast<floatx4*>(place(i32, u)) = v;
+                }
+            __builtin_amdgcn_wave_barrier();
+            if constexpr (VEC) {
+                constexpr int E = 16 / sizeof(TO), LR = CW / E, RR = 64 / LR;   // lanes a row, rows a time
+#pragma unroll
+                for (int r0 = 0; r0 < 32; r0 += RR) {
+                    const int r = r0 + lane / LR, c = lane % LR * E;
+                    float v[E];
+#pragma unroll
+                    for (int p = 0; p < E / 4; ++p) {
+                        const floatx4 x = *reinterpret_cast<const floatx4*>(place(r, c / 4 + p));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[4 * p + e] = x[e];
+                    }
+                    put<TO, BETA>(out, a.beta, mw + r, CW * wn + c, v);
+                }
+            } else {
+#pragma unroll 4
+                for (int r = 0; r < 32; ++r)
+#pragma unroll
+                    for (int c = 0; c < CW; c += 64) {
+                        const int n = c + lane;
+                        put1<TO, BETA>(out, a.beta, mw + r, CW * wn + n, place(r, n / 4)[n & 3]);
+                    }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    };
+    if (a.vec) finish(std::true_type{});
+    else finish(std::false_type{});
 }
 
 // ---------------------------------------------------------------- plan
-template <int MB, int NB, typename TO>
+template <int MB, int NB, typename TX, typename TO>
 void rows_launch(const I8Args& a, hipStream_t st) {
     const unsigned n = (unsigned)ssm::cdiv(a.N, 16 * NB);
-    if (a.beta != 0.f) i8_rows_kernel<MB, NB, TO, true><<<n, 256, 0, st>>>(a);
-    else i8_rows_kernel<MB, NB, TO, false><<<n, 256, 0, st>>>(a);
+    if (a.beta != 0.f) i8_rows_kernel<MB, NB, TX, TO, true><<<n, 256, 0, st>>>(a);
+    else i8_rows_kernel<MB, NB, TX, TO, false><<<n, 256, 0, st>>>(a);
 }
 
-template <int WN, int WM, int TN, int TM, typename TO>
+// Two blocks of channels a workgroup (half the reads of x) where that leaves one for every CU.
+template <int MB, typename TX, typename TO>
+void rows_blocks(const I8Args& a, hipStream_t st) {
+    if (ssm::cdiv(a.N, 32) >= 256) rows_launch<MB, 2, TX, TO>(a, st);
+    else rows_launch<MB, 1, TX, TO>(a, st);
+}
+
+template <int WN, int WM, int TN, int TM, int NS, typename TO>
 void gemm_launch(I8Args a, hipStream_t st) {
-    a.nt = (int)ssm::cdiv(a.N, 16 * TN * WN);
-    a.mt = (int)ssm::cdiv(a.M, 16 * TM * WM);
+    a.nt = (int)ssm::cdiv(a.N, 32 * TN * WN);
+    a.mt = (int)ssm::cdiv(a.M, 32 * TM * WM);
     a.gn = std::min(a.nt, 8);
     const unsigned n = (unsigned)(a.nt * a.mt);
-    if (a.beta != 0.f) i8_gemm_kernel<WN, WM, TN, TM, TO, true><<<n, 64 * WN * WM, 0, st>>>(a);
-    else i8_gemm_kernel<WN, WM, TN, TM, TO, false><<<n, 64 * WN * WM, 0, st>>>(a);
+    if (a.beta != 0.f) i8_gemm_kernel<WN, WM, TN, TM, NS, TO, true><<<n, 64 * WN * WM, 0, st>>>(a);
+    else i8_gemm_kernel<WN, WM, TN, TM, NS, TO, false><<<n, 64 * WN * WM, 0, st>>>(a);
 }
 
 template <typename TO>
 ssm_status product(const I8Args& a, hipStream_t st) {
-    if (a.M <= 16) rows_launch<1, 1, TO>(a, st);
-    else if (a.M <= 32) rows_launch<2, 1, TO>(a, st);
-    else if (a.M <= kRowsMax) rows_launch<4, 2, TO>(a, st);
-    else if (ssm::cdiv(a.N, 256) * ssm::cdiv(a.M, 256) >= 256) gemm_launch<4, 2, 4, 8, TO>(a, st);
-    else gemm_launch<2, 2, 4, 4, TO>(a, st);
+    if (a.Xf && a.x_dtype == SSM_F32) rows_blocks<1, float, TO>(a, st);
+    else if (a.Xf) rows_blocks<1, __bf16, TO>(a, st);
+    else if (a.M <= 16) rows_blocks<1, void, TO>(a, st);
+    else if (a.M <= 32) rows_blocks<2, void, TO>(a, st);
+    else if (a.M <= kRowsMax) rows_blocks<4, void, TO>(a, st);
+    else if (ssm::cdiv(a.N, 256) * ssm::cdiv(a.M, 256) >= 256) gemm_launch<2, 2, 4, 4, 4, TO>(a, st);
+    else gemm_launch<2, 2, 2, 2, 4, TO>(a, st);
     return ssm::check_launch("ssm_linear_i8");
 }
 
-bool direct(const void* p, long ld, int K, bool x) {
-    // x's bytes past K must be zeros (W's then do not matter)
-    return ((uintptr_t)p & 15) == 0 && ld % 16 == 0 && K % (x ? kPad : 4) == 0;
+bool direct_w(const void* p, long ld, int K) { return ((uintptr_t)p & 15) == 0 && ld % 16 == 0 && K % 4 == 0; }
+// (x's bytes past K must be zeros; W's do not matter then)
+bool direct_x(const void* p, long ld, int M, int K) {
+    return M > kRowsMax && ((uintptr_t)p & 15) == 0 && ld % 16 == 0 && K % kPad == 0;
 }
 
-// Workspace: x's rows as integers (Kp bytes each) with their scales, then W's where they have to
-// be laid out.
+// Rows of x that a product reads: the few-row kernel whole blocks of 16 (what the last of them holds
+// past M goes into sums that are not kept).
+long rows_read(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= kRowsMax ? kRowsMax : M; }
+
+// Workspace: x's rows as integers (Kp bytes each) with their scales, then W's where they have to be
+// laid out.
 struct Layout { size_t x, sx, w, all; long Kp; };
 Layout layout(int M, int N, int K, bool x, bool scales, bool w) {
     Layout l{};
     l.Kp = up(K, kPad);
     size_t o = 0;
     l.x = o;
-    if (x) o += (size_t)M * l.Kp;
+    if (x) o += (size_t)rows_read(M) * l.Kp;
     l.sx = o;
     if (scales) o += (size_t)up(4L * M, 256);
     l.w = o;
@@ -470,7 +682,7 @@ ssm_status check_product(const char* who, const void* x, long ldx, const int8_t*
     if (M == 0) return SSM_OK;
     SSM_REQUIRE(x && W && sw && y, "%s: null input", who);
     SSM_REQUIRE(ldx >= K && ldw >= K && ldy >= N, "%s: row stride below row width", who);
-    SSM_REQUIRE(ldw < (1L << 22) && ldx < (1L << 22), "%s: row stride too large", who);
+    SSM_REQUIRE(ldw < (1L << 22) && ldx < (1L << 22) && ldy < (1L << 21), "%s: row stride too large", who);
     return SSM_OK;
 }
 
@@ -478,11 +690,13 @@ ssm_status launch_product(I8Args a, int out_dtype, const Layout& l, bool lay_w, 
                           hipStream_t st) {
     if (lay_w) {
         signed char* o = (signed char*)ws + l.w;
-        pad_rows_kernel<<<a.N, 256, 0, st>>>(a.W, a.ldw, a.K, o, (int)l.Kp);
+        lay_rows_kernel<false><<<a.N, 256, 0, st>>>(a.W, a.ldw, a.K, o, (int)l.Kp);
         if (ssm_status e = ssm::check_launch("ssm_linear_i8 (weight rows)")) return e;
         a.W = o;
         a.ldw = l.Kp;
     }
+    const int e = out_dtype == SSM_F32 ? 4 : 8;
+    a.vec = a.N % e == 0 && a.ldy % e == 0 && ((uintptr_t)a.y & 15) == 0;
     return out_dtype == SSM_F32 ? product<float>(a, st) : product<__bf16>(a, st);
 }
 
@@ -495,13 +709,13 @@ extern "C" ssm_status ssm_quantize_rows(int dtype, const void* x, long ldx, int8
     if (M == 0) return SSM_OK;
     SSM_REQUIRE(x && q && scale, "ssm_quantize_rows: null input");
     SSM_REQUIRE(ldx >= K && ldq >= K, "ssm_quantize_rows: row stride below row width");
-    return quantize(dtype, x, ldx, (signed char*)q, ldq, scale, M, K, K, (hipStream_t)stream);
+    return quantize(dtype, x, ldx, (signed char*)q, ldq, scale, M, K, K, false, (hipStream_t)stream);
 }
 
 extern "C" size_t ssm_linear_i8_workspace(const int8_t* x, long ldx, const int8_t* W, long ldw, int M,
                                           int N, int K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    return layout(M, N, K, !direct(x, ldx, K, true), false, !direct(W, ldw, K, false)).all;
+    return layout(M, N, K, !direct_x(x, ldx, M, K), false, !direct_w(W, ldw, K)).all;
 }
 
 extern "C" ssm_status ssm_linear_i8(const int8_t* x, long ldx, const float* sx, const int8_t* W,
@@ -512,15 +726,18 @@ extern "C" ssm_status ssm_linear_i8(const int8_t* x, long ldx, const float* sx, 
         return e;
     if (M == 0) return SSM_OK;
     SSM_REQUIRE(sx, "ssm_linear_i8: null input");
-    const bool lay_x = !direct(x, ldx, K, true), lay_w = !direct(W, ldw, K, false);
+    const bool lay_x = !direct_x(x, ldx, M, K), lay_w = !direct_w(W, ldw, K);
     const Layout l = layout(M, N, K, lay_x, false, lay_w);
     SSM_REQUIRE(l.all == 0 || (workspace && workspace_bytes >= l.all && ((uintptr_t)workspace & 15) == 0),
                 "ssm_linear_i8: 16-byte aligned workspace of %zu bytes needed", l.all);
-    I8Args a{(const signed char*)x, ldx, sx, nullptr, 0, (const signed char*)W, ldw, sw, bias, y, ldy,
-             M, N, K, beta, 0, 0, 0};
+    I8Args a{(const signed char*)x, ldx, sx, nullptr, 0, 0, (const signed char*)W, ldw, sw, bias, y, ldy,
+             M, N, K, beta, 0, 0, 0, 0};
     if (lay_x) {
         signed char* o = (signed char*)workspace + l.x;
-        pad_rows_kernel<<<M, 256, 0, (hipStream_t)stream>>>(a.X, ldx, K, o, (int)l.Kp);
+        if (M <= kRowsMax)
+            lay_rows_kernel<true><<<M, 256, 0, (hipStream_t)stream>>>(a.X, ldx, K, o, (int)l.Kp);
+        else
+            lay_rows_kernel<false><<<M, 256, 0, (hipStream_t)stream>>>(a.X, ldx, K, o, (int)l.Kp);
         if (ssm_status e = ssm::check_launch("ssm_linear_i8 (rows)")) return e;
         a.X = o;
         a.ldx = l.Kp;
@@ -530,7 +747,7 @@ extern "C" ssm_status ssm_linear_i8(const int8_t* x, long ldx, const float* sx, 
 
 extern "C" size_t ssm_linear_q8_workspace(const int8_t* W, long ldw, int M, int N, int K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    return layout(M, N, K, true, true, !direct(W, ldw, K, false)).all;
+    return layout(M, N, K, true, true, !direct_w(W, ldw, K)).all;
 }
 
 extern "C" ssm_status ssm_linear_q8(int in_dtype, const void* x, long ldx, const int8_t* W, long ldw,
@@ -541,15 +758,19 @@ extern "C" ssm_status ssm_linear_q8(int in_dtype, const void* x, long ldx, const
     if (ssm_status e = check_product("ssm_linear_q8", x, ldx, W, ldw, sw, out_dtype, y, ldy, M, N, K))
         return e;
     if (M == 0) return SSM_OK;
-    const bool lay_w = !direct(W, ldw, K, false);
+    const bool lay_w = !direct_w(W, ldw, K);
     const Layout l = layout(M, N, K, true, true, lay_w);
     SSM_REQUIRE(workspace && workspace_bytes >= l.all && ((uintptr_t)workspace & 15) == 0,
                 "ssm_linear_q8: 16-byte aligned workspace of %zu bytes needed", l.all);
     signed char* q = (signed char*)workspace + l.x;
     float* sx = (float*)((char*)workspace + l.sx);
-    if (ssm_status e = quantize(in_dtype, x, ldx, q, l.Kp, sx, M, K, (int)l.Kp, (hipStream_t)stream))
+    I8Args a{q, l.Kp, sx, nullptr, ldx, in_dtype, (const signed char*)W, ldw, sw, bias, y, ldy,
+             M, N, K, beta, 0, 0, 0, 0};
+    const bool vec = K % 4 == 0 && ldx % 4 == 0 && ((uintptr_t)x & (in_dtype == SSM_F32 ? 15 : 7)) == 0;
+    if (vec && M <= kFusedRows && M * ssm::cdiv(K, 1024) <= kFusedX / 1024)
+        a.Xf = x;
+    else if (ssm_status e = quantize(in_dtype, x, ldx, q, l.Kp, sx, M, K, (int)l.Kp, M <= kRowsMax,
+                                     (hipStream_t)stream))
         return e;
-    const I8Args a{q, l.Kp, sx, nullptr, 0, (const signed char*)W, ldw, sw, bias, y, ldy,
-                   M, N, K, beta, 0, 0, 0};
     return launch_product(a, out_dtype, l, lay_w, (char*)workspace, (hipStream_t)stream);
 }

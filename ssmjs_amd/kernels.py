@@ -247,44 +247,70 @@ def gated_rmsnorm(x, z, w, groups=1, eps=1e-5, out=None):
 
 
 # ---------------------------------------------------------------- a linear-attention layer
-def _code(t):
-    if t.dtype == torch.bfloat16:
-        return _lib.SSM_BF16
-    if t.dtype == torch.float32:
-        return _lib.SSM_F32
-    raise TypeError(f"expected float32 or bfloat16, got {t.dtype}")
+# Small calls cost what the host spends on them, so each operand is checked with as few calls into
+# torch as that takes: contiguous ones (the common case) need no strides.
+_CODES = {torch.float32: _lib.SSM_F32, torch.bfloat16: _lib.SSM_BF16}
+_f32_t, _i32_t, _i8_t, _f64_t = torch.float32, torch.int32, torch.int8, torch.float64
 
 
-def _at(name, t, shape, dtype):
-    """Device pointer of an operand of this shape and type on the current device (None -> NULL)."""
-    if t is None:
-        return None
+def _code(dtype):
+    code = _CODES.get(dtype)
+    if code is None:
+        raise TypeError(f"expected float32 or bfloat16, got {dtype}")
+    return code
+
+
+def _here():
+    return _device() if _device is not None else torch.cuda.current_device()
+
+
+def _refuse(name, t, shape, dtype):
+    """Why an operand is not of this shape and type on the current device."""
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_cuda:
         raise ValueError("ssmjs_amd kernels need HIP device tensors (no CPU path)")
-    if t.get_device() != (_device() if _device is not None else torch.cuda.current_device()):
-        raise ValueError(f"{name}: expected a tensor on the current HIP device, got {t.device}")
+    raise ValueError(f"{name}: expected a tensor on the current HIP device, got {t.device}")
+
+
+def _at(name, t, shape, dtype, dev):
+    """Device pointer of an operand of this shape and type on device `dev`."""
+    if t.dtype != dtype or t.shape != shape or t.get_device() != dev:
+        _refuse(name, t, shape, dtype)
     return t.data_ptr()
 
 
-def _packed(name, t, shape, dtype):
-    """_at, of a contiguous operand."""
-    if t is not None and not t.is_contiguous():
+def _packed(name, t, shape, dtype, dev):
+    """_at, of a contiguous operand (None -> NULL)."""
+    if t is None:
+        return None
+    if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    return _at(name, t, shape, dtype)
+    return _at(name, t, shape, dtype, dev)
+
+
+def _current(name, t):
+    """The device of a call: its first operand's, which has to be the current one."""
+    if not t.is_cuda:
+        raise ValueError("ssmjs_amd kernels need HIP device tensors (no CPU path)")
+    dev = t.get_device()
+    if dev != _here():
+        raise ValueError(f"{name}: expected a tensor on the current HIP device, got {t.device}")
+    return dev
 
 
 def _head_rows(name, t):
     """Row stride of (..., rows, heads, elements): a row's heads follow one another, and the rows
     lie at one distance through all leading dimensions."""
-    size, st = t.shape, t.stride()
-    n = t.dim()
+    size = t.shape
+    if t.is_contiguous():
+        return size[-1] * size[-2]
+    st = t.stride()
     if (size[-1] > 1 and st[-1] != 1) or (size[-2] > 1 and st[-2] != size[-1]):
         raise ValueError(f"{name}: the heads of a row must follow one another")
-    if n == 3:
+    if len(size) == 3:
         return st[0] if size[0] > 1 else size[1] * size[2]
     ld = st[1] if size[1] > 1 else (st[0] if size[0] > 1 else size[2] * size[3])
     if size[0] > 1 and size[1] > 1 and st[0] != size[1] * ld:
@@ -292,39 +318,61 @@ def _head_rows(name, t):
     return ld
 
 
+def _ld(name, t):
+    """Row stride of a (rows, n) view whose rows are contiguous."""
+    if t.is_contiguous():
+        return t.shape[1]
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def qk_norm_rope(q, k, wq, wk, positions, freqs, eps=1e-6, interleaved=False, out=None):
     """RMS norm of every query and key head with the position rotation (ssm_qk_norm_rope): returns
     (q', k'). q (B,L,H,D) or (B,H,D), k (.., G,D), float32 or bfloat16; wq, wk (D) float32 or None;
     positions int32, the shape of q without its heads; freqs (R/2) float64, radians per position: the
-    first R elements of a head turn, in pairs (i, i + R/2) or, interleaved, (2i, 2i + 1). `out`: a
-    pair of tensors, which may be (q, k)."""
-    if q.dim() not in (3, 4) or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2]:
+    first R elements of a head turn, in pairs (i, i + R/2) or, interleaved, (2i, 2i + 1); None: norm
+    alone. `out`: a pair of tensors, which may be (q, k)."""
+    shape, kshape, dt = q.shape, k.shape, q.dtype
+    if len(shape) not in (3, 4) or len(kshape) != len(shape):
         raise ValueError("q (B,L,H,D) or (B,H,D), and k of the same rows")
-    D, G = q.shape[-1], k.shape[-2]
-    if out is None:
-        out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-               torch.empty(k.shape, dtype=k.dtype, device=k.device))
-    qo, ko = out
-    code, dt = _code(q), q.dtype
+    *rows, H, D = shape
+    G = kshape[-2]
+    code, dev = _code(dt), _current("q", q)
+    T = rows[0] if len(rows) == 1 else rows[0] * rows[1]
     R = 2 * freqs.shape[0] if freqs is not None else 0
-    rows = q.shape[:-2]
-    kshape = rows + (G, D)
-    _lib.call("ssm_qk_norm_rope", code, _at("q", q, q.shape, dt), _head_rows("q", q),
-              _at("k", k, kshape, dt), _head_rows("k", k),
-              _packed("wq", wq, (D,), torch.float32), _packed("wk", wk, (D,), torch.float32),
-              _packed("positions", positions, rows, torch.int32),
-              _packed("freqs", freqs, (R // 2,), torch.float64), int(interleaved), eps,
-              _at("out[0]", qo, q.shape, dt), _head_rows("out[0]", qo),
-              _at("out[1]", ko, kshape, dt), _head_rows("out[1]", ko),
-              rows.numel(), q.shape[-2], G, D, R, _stream())
+    pk = _at("k", k, (*rows, G, D), dt, dev)
+    if out is None:
+        qo, ko = q.new_empty(shape), k.new_empty(kshape)
+        pqo, pko, ldqo, ldko = qo.data_ptr(), ko.data_ptr(), H * D, G * D
+    else:
+        qo, ko = out
+        pqo, pko = _at("out[0]", qo, shape, dt, dev), _at("out[1]", ko, kshape, dt, dev)
+        ldqo, ldko = _head_rows("out[0]", qo), _head_rows("out[1]", ko)
+    _lib.call("ssm_qk_norm_rope", code, q.data_ptr(), _head_rows("q", q), pk, _head_rows("k", k),
+              _packed("wq", wq, (D,), _f32_t, dev), _packed("wk", wk, (D,), _f32_t, dev),
+              _packed("positions", positions, tuple(rows), _i32_t, dev),
+              _packed("freqs", freqs, (R // 2,), _f64_t, dev), int(interleaved), eps, pqo, ldqo, pko,
+              ldko, T, H, G, D, R, _raw_stream(dev) if _raw_stream is not None else _stream())
     return qo, ko
 
 
 def linear_attention_workspace(B, L, H, K, V, dtype, device):
     """Workspace for linear_attention (ssm_linear_attention_workspace bytes)."""
-    code = _lib.SSM_BF16 if dtype == torch.bfloat16 else _lib.SSM_F32
-    return torch.empty(max(1, _lib.lib().ssm_linear_attention_workspace(code, B, L, H, K, V)),
+    return torch.empty(max(1, _lib.lib().ssm_linear_attention_workspace(_code(dtype), B, L, H, K, V)),
                        dtype=torch.uint8, device=device)
+
+
+def _own_scratch(workspace, nbytes, t):
+    """(tensor, pointer, bytes) of a call's workspace: the caller's, or one for this call."""
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        return workspace, _p(workspace), workspace.numel() * workspace.element_size()
+    if nbytes == 0:
+        return None, None, 0
+    ws = t.new_empty(nbytes, dtype=torch.uint8)
+    return ws, ws.data_ptr(), nbytes
 
 
 def linear_attention(q, k, v, g, scale=1.0, lengths=None, h0=None, hT=None, out=None,
@@ -337,23 +385,22 @@ def linear_attention(q, k, v, g, scale=1.0, lengths=None, h0=None, hT=None, out=
         raise ValueError("q (B,L,H,K), k (B,L,G,K), v (B,L,G,V)")
     B, L, H, K = q.shape
     G, V = k.shape[2], v.shape[3]
-    code, dt = _code(q), q.dtype
-    y = out if out is not None else torch.empty(B, L, H, V, dtype=dt, device=q.device)
-    if workspace is not None:
-        ws, nbytes = workspace, workspace.numel() * workspace.element_size()
-    else:
-        ws, nbytes = _scratch(_lib.lib().ssm_linear_attention_workspace(code, B, L, H, K, V),
-                              q.device)
+    dt = q.dtype
+    code, dev = _code(dt), _current("q", q)
+    pk, pv = _at("k", k, (B, L, G, K), dt, dev), _at("v", v, (B, L, G, V), dt, dev)
+    if out is None:
+        out = q.new_empty((B, L, H, V))
+    py = _at("out", out, (B, L, H, V), dt, dev)
     state = (B, H, V, K)
-    _lib.call("ssm_linear_attention", code, _at("q", q, (B, L, H, K), dt), _head_rows("q", q),
-              _at("k", k, (B, L, G, K), dt), _head_rows("k", k),
-              _at("v", v, (B, L, G, V), dt), _head_rows("v", v),
-              _packed("g", g, (H,), torch.float32), scale,
-              _packed("lengths", lengths, (B,), torch.int32),
-              _at("out", y, (B, L, H, V), dt), _head_rows("out", y), B, L, H, G, K, V,
-              _packed("h0", h0, state, torch.float32), _packed("hT", hT, state, torch.float32),
-              _p(ws), nbytes, _stream())
-    return y
+    # (held to the end of the call: freed before, it could be given to another stream)
+    ws, pws, nbytes = _own_scratch(
+        workspace, _lib.lib().ssm_linear_attention_workspace(code, B, L, H, K, V), q)
+    _lib.call("ssm_linear_attention", code, q.data_ptr(), _head_rows("q", q), pk,
+              _head_rows("k", k), pv, _head_rows("v", v), _packed("g", g, (H,), _f32_t, dev), scale,
+              _packed("lengths", lengths, (B,), _i32_t, dev), py, _head_rows("out", out), B, L, H, G,
+              K, V, _packed("h0", h0, state, _f32_t, dev), _packed("hT", hT, state, _f32_t, dev),
+              pws, nbytes, _raw_stream(dev) if _raw_stream is not None else _stream())
+    return out
 
 
 def linear_attention_step(q, k, v, g, h, scale=1.0, out=None):
@@ -363,22 +410,20 @@ def linear_attention_step(q, k, v, g, h, scale=1.0, out=None):
         raise ValueError("q (B,H,K), k (B,G,K), v (B,G,V)")
     B, H, K = q.shape
     G, V = k.shape[1], v.shape[2]
-    code, dt = _code(q), q.dtype
-    y = out if out is not None else torch.empty(B, H, V, dtype=dt, device=q.device)
-    _lib.call("ssm_linear_attention_step", code, _at("q", q, (B, H, K), dt), _head_rows("q", q),
-              _at("k", k, (B, G, K), dt), _head_rows("k", k),
-              _at("v", v, (B, G, V), dt), _head_rows("v", v),
-              _packed("g", g, (H,), torch.float32), scale, _at("out", y, (B, H, V), dt),
-              _head_rows("out", y), _packed("h", h, (B, H, V, K), torch.float32), B, H, G, K, V,
-              _stream())
-    return y
-
-
-def _ld(name, t):
-    """Row stride of a (rows, n) view whose rows are contiguous."""
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name}: rows must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    dt = q.dtype
+    code, dev = _code(dt), _current("q", q)
+    pk, pv = _at("k", k, (B, G, K), dt, dev), _at("v", v, (B, G, V), dt, dev)
+    ph = _packed("h", h, (B, H, V, K), _f32_t, dev)
+    if ph is None:
+        raise ValueError("linear_attention_step needs a state")
+    if out is None:
+        out = q.new_empty((B, H, V))
+    py = _at("out", out, (B, H, V), dt, dev)
+    _lib.call("ssm_linear_attention_step", code, q.data_ptr(), _head_rows("q", q), pk,
+              _head_rows("k", k), pv, _head_rows("v", v), _packed("g", g, (H,), _f32_t, dev), scale,
+              py, _head_rows("out", out), ph, B, H, G, K, V,
+              _raw_stream(dev) if _raw_stream is not None else _stream())
+    return out
 
 
 def quantize_rows(x, out=None):
@@ -386,58 +431,61 @@ def quantize_rows(x, out=None):
     (ssm_quantize_rows): returns (q (M,K) int8, scale (M) float32). For weights (N,K) this is a scale
     for each output channel."""
     M, K = x.shape
+    code, dev = _code(x.dtype), _current("x", x)
     if out is None:
-        out = (torch.empty(M, K, dtype=torch.int8, device=x.device),
-               torch.empty(M, dtype=torch.float32, device=x.device))
+        out = x.new_empty((M, K), dtype=_i8_t), x.new_empty(M, dtype=_f32_t)
     q, scale = out
-    _lib.call("ssm_quantize_rows", _code(x), _at("x", x, (M, K), x.dtype), _ld("x", x),
-              _at("out[0]", q, (M, K), torch.int8), _ld("out[0]", q),
-              _packed("out[1]", scale, (M,), torch.float32), M, K, _stream())
+    _lib.call("ssm_quantize_rows", code, x.data_ptr(), _ld("x", x),
+              _at("out[0]", q, (M, K), _i8_t, dev), _ld("out[0]", q),
+              _packed("out[1]", scale, (M,), _f32_t, dev), M, K, _stream())
     return q, scale
 
 
-def _i8_out(out, out_dtype, beta, M, N, device):
+def _product_out(out, out_dtype, M, N, x, dev):
+    """(y, its type's code, pointer, row stride) of a product's outputs."""
     if out is None:
-        if beta != 0:
-            raise ValueError("beta needs `out`")
-        return torch.empty(M, N, dtype=out_dtype, device=device)
-    return out
+        code = _code(out_dtype)
+        out = x.new_empty((M, N), dtype=out_dtype)
+        return out, code, out.data_ptr(), N
+    return out, _code(out.dtype), _at("out", out, (M, N), out.dtype, dev), _ld("out", out)
 
 
 def linear_i8(x, sx, W, sw, bias=None, out=None, out_dtype=torch.float32, beta=0.0,
               workspace=None):
     """y = beta*y + sx sw (x W^T) (+ bias) with 8-bit x (M,K) and W (N,K), a scale for each row of
     both (ssm_linear_i8); y in `out_dtype` (or out's), float32 or bfloat16."""
+    if out is None and beta != 0:
+        raise ValueError("beta needs `out`")
     M, K = x.shape
     N = W.shape[0]
-    y = _i8_out(out, out_dtype, beta, M, N, x.device)
-    px, ldx = _at("x", x, (M, K), torch.int8), _ld("x", x)
-    pw, ldw = _at("W", W, (N, K), torch.int8), _ld("W", W)
-    if workspace is not None:
-        ws, nbytes = workspace, workspace.numel() * workspace.element_size()
-    else:
-        ws, nbytes = _scratch(_lib.lib().ssm_linear_i8_workspace(px, ldx, pw, ldw, M, N, K),
-                              x.device)
-    _lib.call("ssm_linear_i8", px, ldx, _packed("sx", sx, (M,), torch.float32), pw, ldw,
-              _packed("sw", sw, (N,), torch.float32), _packed("bias", bias, (N,), torch.float32),
-              _code(y), _at("out", y, (M, N), y.dtype), _ld("out", y), M, N, K, beta, _p(ws),
-              nbytes, _stream())
+    dev = _current("x", x)
+    px, ldx = _at("x", x, (M, K), _i8_t, dev), _ld("x", x)
+    pw, ldw = _at("W", W, (N, K), _i8_t, dev), _ld("W", W)
+    y, code, py, ldy = _product_out(out, out_dtype, M, N, x, dev)
+    ws, pws, nbytes = _own_scratch(
+        workspace, _lib.lib().ssm_linear_i8_workspace(px, ldx, pw, ldw, M, N, K), x)
+    _lib.call("ssm_linear_i8", px, ldx, _packed("sx", sx, (M,), _f32_t, dev), pw, ldw,
+              _packed("sw", sw, (N,), _f32_t, dev), _packed("bias", bias, (N,), _f32_t, dev), code,
+              py, ldy, M, N, K, beta, pws, nbytes,
+              _raw_stream(dev) if _raw_stream is not None else _stream())
     return y
 
 
 def linear_q8(x, W, sw, bias=None, out=None, out_dtype=None, beta=0.0, workspace=None):
     """linear_i8 of x (M,K) in float32 or bfloat16, rounded to 8 bits with a scale for each row on
     the way (ssm_linear_q8); y in x's type unless `out_dtype` or `out` say otherwise."""
+    if out is None and beta != 0:
+        raise ValueError("beta needs `out`")
     M, K = x.shape
     N = W.shape[0]
-    y = _i8_out(out, out_dtype or x.dtype, beta, M, N, x.device)
-    pw, ldw = _at("W", W, (N, K), torch.int8), _ld("W", W)
-    if workspace is not None:
-        ws, nbytes = workspace, workspace.numel() * workspace.element_size()
-    else:
-        ws, nbytes = _scratch(_lib.lib().ssm_linear_q8_workspace(pw, ldw, M, N, K), x.device)
-    _lib.call("ssm_linear_q8", _code(x), _at("x", x, (M, K), x.dtype), _ld("x", x), pw, ldw,
-              _packed("sw", sw, (N,), torch.float32), _packed("bias", bias, (N,), torch.float32),
-              _code(y), _at("out", y, (M, N), y.dtype), _ld("out", y), M, N, K, beta, _p(ws),
-              nbytes, _stream())
+    dt = x.dtype
+    code_x, dev = _code(dt), _current("x", x)
+    pw, ldw = _at("W", W, (N, K), _i8_t, dev), _ld("W", W)
+    y, code, py, ldy = _product_out(out, out_dtype or dt, M, N, x, dev)
+    ws, pws, nbytes = _own_scratch(
+        workspace, _lib.lib().ssm_linear_q8_workspace(pw, ldw, M, N, K), x)
+    _lib.call("ssm_linear_q8", code_x, x.data_ptr(), _ld("x", x), pw, ldw,
+              _packed("sw", sw, (N,), _f32_t, dev), _packed("bias", bias, (N,), _f32_t, dev), code,
+              py, ldy, M, N, K, beta, pws, nbytes,
+              _raw_stream(dev) if _raw_stream is not None else _stream())
     return y

@@ -109,10 +109,11 @@ def test_linear_q8_refuses(change, status):
 
 def test_product_workspaces_agree_with_the_launches():
     L = _lib.lib()
-    # aligned rows of whole 256-byte blocks are read in place
-    assert L.ssm_linear_i8_workspace(P, 256, P, 256, 5, 64, 256) == 0
+    # aligned rows of whole 256-byte blocks are read in place, x's from 65 rows on
+    assert L.ssm_linear_i8_workspace(P, 256, P, 256, 65, 64, 256) == 0
+    assert L.ssm_linear_i8_workspace(P, 256, P, 256, 64, 64, 256) >= 64 * 256
     assert L.ssm_linear_i8_workspace(P, 240, P, 240, 5, 64, 240) >= 5 * 256
-    assert L.ssm_linear_i8_workspace(P, 256, P + 1, 256, 5, 64, 256) >= 64 * 256
+    assert L.ssm_linear_i8_workspace(P, 256, P + 1, 256, 65, 64, 256) >= 64 * 256
     for change in (dict(K=240, ldx=240, ldw=240), dict(W=P + 8), dict(x=P + 4), dict(ldw=264)):
         c = dict(x=P, ldx=256, W=P, ldw=256, M=2, N=64, K=256) | change
         need = L.ssm_linear_i8_workspace(c["x"], c["ldx"], c["W"], c["ldw"], c["M"], c["N"], c["K"])
