@@ -19,32 +19,60 @@ namespace {
 typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr unsigned kOut = 0x80000000u;   // a buffer offset past any descriptor
 constexpr int kMaxK = 131071;
 constexpr int kPad = 256;          // rows of the workspace are whole blocks of 256 bytes, zeros past K
+constexpr int kCUs = 256;          // workgroups of the large tiles' kernel: one a CU
 constexpr int kRowsMax = 64;       // rows of the few-row kernel
 inline long up(long n, long to) { return (n + to - 1) / to * to; }
 
 // ---------------------------------------------------------------- rows to integers
+// x / s to the nearest integer. t = x inv is within 127 * 2^-23 of the quotient, so its nearest integer
+// is the quotient's unless t is that near to a half; then the exact remainder decides (x - q s has 24
+// bits). Adding 1.5 * 2^23 leaves the integer in the sum's low bits, two's complement.
 struct Quant {
     float f, s, inv;   // x f / (s f), s f in the normal range
+    static constexpr float kMagic = 12582912.f, kSure = 0.4999f;
     __device__ __forceinline__ explicit Quant(float scale) {
         f = scale < 0x1p-100f ? 0x1p120f : 1.f;
         s = scale * f;
         inv = 1.f / s;
     }
-    // nearest integer to x / s: a first guess, then the exact remainder (x - q s has 24 bits)
-    __device__ __forceinline__ int operator()(float x) const {
+    __device__ __forceinline__ unsigned exact(float x) const {
         x *= f;
         float q = rintf(x * inv);
         const float r = fmaf(-q, s, x), d = 2.f * fabsf(r);
         if (d > s || (d == s && ((int)q & 1))) q += copysignf(1.f, r);
-        return (int)fminf(fmaxf(q, -127.f), 127.f);
+        return (unsigned)(int)fminf(fmaxf(q, -127.f), 127.f);
+    }
+    __device__ __forceinline__ unsigned near(float x, float& off) const {
+        const float u = fmaf(x, inv, kMagic);
+        off = fmaxf(off, fabsf(fmaf(x, inv, kMagic - u)));
+        return __builtin_bit_cast(unsigned, u);
+    }
+    static __device__ __forceinline__ unsigned bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+        // (v_perm_b32: the low bytes of two words side by side)
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u),
+                                     __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
+    }
+    __device__ __forceinline__ unsigned pack(float4 v) const {
+        float off = 0.f;
+        const unsigned b = bytes(near(v.x, off), near(v.y, off), near(v.z, off), near(v.w, off));
+        if (off <= kSure && f == 1.f) return b;
+        return bytes(exact(v.x), exact(v.y), exact(v.z), exact(v.w));
     }
 };
+
+// A value that the compiler forms again here: registers for it are not held over a loop.
+__device__ __forceinline__ int fresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 
 __device__ __forceinline__ unsigned abs_bits(float x) { return __builtin_bit_cast(unsigned, x) & 0x7fffffffu; }
 
@@ -82,8 +110,18 @@ __device__ __forceinline__ unsigned max4(unsigned m, float4 v) {
     return max(max(m, max(abs_bits(v.x), abs_bits(v.y))), max(abs_bits(v.z), abs_bits(v.w)));
 }
 
-__device__ __forceinline__ unsigned pack4(const Quant& z, float4 v) {
-    return (z(v.x) & 255) | (z(v.y) & 255) << 8 | (z(v.z) & 255) << 16 | (unsigned)z(v.w) << 24;
+// The largest of a wave's values, in every lane: four steps inside each 16 lanes (quad_perm, half_mirror,
+// mirror), then the four rows.
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+    auto step = [&](auto ctrl) {
+        v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    step(std::integral_constant<int, 0xb1>{});
+    step(std::integral_constant<int, 0x4e>{});
+    step(std::integral_constant<int, 0x141>{});
+    step(std::integral_constant<int, 0x140>{});
+    auto row = [&](int l) { return (unsigned)__builtin_amdgcn_readlane((int)v, l); };
+    return max(max(row(0), row(16)), max(row(32), row(48)));
 }
 
 struct QuantArgs {
@@ -102,26 +140,29 @@ __device__ __forceinline__ long frag_at(long m, int k, int Kp) {
            (m & 15) * 16 + (k & 15);
 }
 
-// A row per workgroup of TPR threads' share: 256 / TPR rows a workgroup, U pieces of four held
-// between the two passes (further ones are read again).
+// TPR threads a row, 256 / TPR rows a workgroup: U pieces of eight elements a thread are held between
+// the two passes (further ones are read again).
 template <typename T, int TPR, bool VEC>
 __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
-    constexpr int U = 8, RPB = 256 / TPR, NW = TPR / 64;
+    constexpr int U = 4, RPB = 256 / TPR, NW = TPR / 64;
     __shared__ unsigned red[4];
     const int tid = threadIdx.x % TPR, rw = threadIdx.x / TPR;
     const long m = (long)blockIdx.x * RPB + rw;
     const bool live = m < a.M;
     const T* row = static_cast<const T*>(a.x) + (live ? m : 0) * a.ldx;
-    float4 v[U];
+    struct Eight { float4 a, b; };
+    auto get = [&](int k) { return Eight{some4<T, VEC>(row, k, a.K), some4<T, VEC>(row, k + 4, a.K)}; };
+    Eight v[U];
     unsigned most = 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        v[u] = some4<T, VEC>(row, 4 * (tid + TPR * u), a.K);
-        most = max4(most, v[u]);
-    }
-    for (int k = 4 * (tid + TPR * U); k < a.K; k += 4 * TPR) most = max4(most, some4<T, VEC>(row, k, a.K));
+    for (int u = 0; u < U; ++u) v[u] = get(8 * (tid + TPR * u));
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) most = max(most, (unsigned)__shfl_xor((int)most, off));
+    for (int u = 0; u < U; ++u) most = max4(max4(most, v[u].a), v[u].b);
+    for (int k = 8 * (tid + TPR * U); k < a.K; k += 8 * TPR) {
+        const Eight e = get(k);
+        most = max4(max4(most, e.a), e.b);
+    }
+    most = wave_max(most);
     if constexpr (NW > 1) {
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
         __syncthreads();
@@ -135,27 +176,27 @@ __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
     const bool ok = usable(s);
     const Quant z(ok ? s : 1.f);
     signed char* out = a.q + (a.frag ? 0 : m * a.ldq);
-    auto put = [&](int k, float4 x) {
+    auto put = [&](int k, const Eight& e) {
         if (k >= a.Kq) return;
-        const unsigned b = ok ? pack4(z, x) : 0u;
+        const uint2 b = ok ? make_uint2(z.pack(e.a), z.pack(e.b)) : make_uint2(0u, 0u);
         if (a.frag) {   // (Kq is a whole number of pieces)
-            *reinterpret_cast<unsigned*>(out + frag_at(m, k, (int)a.ldq)) = b;
+            *reinterpret_cast<uint2*>(out + frag_at(m, k, (int)a.ldq)) = b;
         } else if constexpr (VEC) {
-            *reinterpret_cast<unsigned*>(out + k) = b;
+            *reinterpret_cast<uint2*>(out + k) = b;
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (k + e < a.Kq) out[k + e] = (signed char)(b >> 8 * e);
+            for (int e = 0; e < 8; ++e)
+                if (k + e < a.Kq) out[k + e] = (signed char)((e < 4 ? b.x : b.y) >> 8 * (e & 3));
         }
     };
 #pragma unroll
-    for (int u = 0; u < U; ++u) put(4 * (tid + TPR * u), v[u]);
-    for (int k = 4 * (tid + TPR * U); k < a.Kq; k += 4 * TPR) put(k, some4<T, VEC>(row, k, a.K));
+    for (int u = 0; u < U; ++u) put(8 * (tid + TPR * u), v[u]);
+    for (int k = 8 * (tid + TPR * U); k < a.Kq; k += 8 * TPR) put(k, get(k));
 }
 
 template <typename T>
 ssm_status run_quant(const QuantArgs& a, bool vec, hipStream_t st) {
-    // a wave a row up to 2048 elements (its eight pieces a lane), a workgroup beyond
+    // a wave a row up to 2048 elements (its four pieces a lane), a workgroup beyond
     if (a.K <= 2048 && a.M >= 1024) {
         const unsigned n = (unsigned)ssm::cdiv(a.M, 4);
         if (vec) quant_kernel<T, 64, true><<<n, 256, 0, st>>>(a);
@@ -170,8 +211,8 @@ ssm_status run_quant(const QuantArgs& a, bool vec, hipStream_t st) {
 ssm_status quantize(int dtype, const void* x, long ldx, signed char* q, long ldq, float* scale,
                     int M, int K, int Kq, bool frag, hipStream_t st) {
     const QuantArgs a{x, ldx, q, ldq, scale, M, K, Kq, frag};
-    const bool vec = K % 4 == 0 && Kq % 4 == 0 && ldx % 4 == 0 && ldq % 4 == 0 &&
-                     ((uintptr_t)x & (dtype == SSM_F32 ? 15 : 7)) == 0 && ((uintptr_t)q & 3) == 0;
+    const bool vec = K % 4 == 0 && Kq % 8 == 0 && ldx % 4 == 0 && ldq % 8 == 0 &&
+                     ((uintptr_t)x & (dtype == SSM_F32 ? 15 : 7)) == 0 && ((uintptr_t)q & 7) == 0;
     return dtype == SSM_F32 ? run_quant<float>(a, vec, st) : run_quant<__bf16>(a, vec, st);
 }
 
@@ -256,6 +297,25 @@ __device__ __forceinline__ void put(const Out<TO>& o, float beta, int m, int n, 
     }
 }
 
+// Four outputs, n .. of row m, aligned to their size.
+template <typename TO, bool BETA>
+__device__ __forceinline__ void put4(const Out<TO>& o, float beta, int m, int n, float* v) {
+    if constexpr (sizeof(TO) == 4) {
+        put<TO, BETA>(o, beta, m, n, v);
+    } else {
+        const unsigned off = n < o.cols ? ((unsigned)m * o.ld + (unsigned)n) * 2u : kOut;
+        bf16x4 y;
+        if constexpr (BETA) {
+            y = __builtin_bit_cast(bf16x4, __builtin_amdgcn_raw_buffer_load_b64(o.d, off, 0, 0));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += beta * (float)y[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (__bf16)v[e];
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, y), o.d, off, 0, 0);
+    }
+}
+
 // A row's bytes in whole dwords: one that a descriptor ends inside reads as zeros. (Rows that are
 // read in place have a multiple of four, the workspace's are longer.)
 __device__ __forceinline__ int whole(int K) { return (K + 3) & ~3; }
@@ -265,8 +325,8 @@ __device__ __forceinline__ intx4 mfma8(intx4 w, intx4 x, intx4 c) {
 }
 
 // ---------------------------------------------------------------- up to 64 rows
-// A workgroup owns NB blocks of 16 output channels; its four waves take the blocks of 256 k in
-// turn. Lane (g, i) = (lane / 16, lane % 16) reads W row i's bytes 64 g + 16 u .. of the block for
+// A workgroup owns 16 output channels; its four waves take the blocks of 256 k in turn, two blocks'
+// weights in flight a wave. Lane (g, i) = (lane / 16, lane % 16) reads W row i's bytes 64 g + 16 u .. of the block for
 // u = 0 .. 3, which is the operand of MFMA u with the block's k in another order, the same for x. So a
 // lane reads 64 consecutive bytes of its row, and x lies in the workspace in the operands' own order (a
 // row-major x took 3 times as long at 64 rows: 16 lines an instruction). The waves' sums meet in
@@ -276,132 +336,117 @@ __device__ __forceinline__ intx4 mfma8(intx4 w, intx4 x, intx4 c) {
 // itself, into LDS, while its weights are on their way: one launch instead of two.
 constexpr int kFusedX = 8192, kFusedRows = 4;
 
-template <int MB, int NB, typename TX, typename TO, bool BETA>
+template <int MB, typename TX, typename TO, bool BETA>
 __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
     constexpr bool FUSED = !std::is_void<TX>::value;
     constexpr int kPieces = kFusedX / 1024;
-    __shared__ intx4 red[3][NB * MB][64];
+    __shared__ intx4 red[4][MB][64];
     __shared__ __attribute__((aligned(16))) signed char xs[FUSED ? kFusedX + kFusedRows * kPad : 16];
     __shared__ unsigned most[FUSED ? 4 : 1][kPieces];
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15;
-    const int n0 = blockIdx.x * 16 * NB;
-    const int rows = min(16 * NB, a.N - n0);
+    const int n0 = blockIdx.x * 16;
+    const int rows = min(16, a.N - n0);
     const auto rw = ssm::rsrc(a.W + (long)n0 * a.ldw, (unsigned)((long)(rows - 1) * a.ldw + whole(a.K)));
     const unsigned wo = (unsigned)(i * a.ldw) + 64u * g;
-    const int steps = (a.K + 255) / 256;
-    auto weights = [&](intx4 (&wv)[NB][4], int s) {   // (a step past the last reads zeros)
-        const unsigned k = s < steps ? 256u * s : kOut;
+    const int steps = (a.K + 255) / 256, Kp = steps * 256;
+    intx4 wv[2][4];
+    auto fetch = [&](intx4 (&v)[4], int s) {
+        if (s >= steps) return;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                wv[b][u] = __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(
-                    rw, wo + (unsigned)(16 * b * a.ldw) + 16u * u + k, 0, 0));
+        for (int u = 0; u < 4; ++u)
+            v[u] = __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(rw, wo + 16u * u + 256u * s, 0, 0));
     };
-    intx4 acc[NB][MB];
+    intx4 acc[MB];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int m = 0; m < MB; ++m) acc[b][m] = intx4{0, 0, 0, 0};
-    intx4 wv[2][NB][4];
-    weights(wv[0], w);
-    weights(wv[1], w + 4);
-
+    for (int m = 0; m < MB; ++m) acc[m] = intx4{0, 0, 0, 0};
     float sm[MB];
     if constexpr (FUSED) {
-        const int per = (a.K + 1023) / 1024;   // pieces of a row; M * per <= kPieces
-        const int Kp = (a.K + kPad - 1) / kPad * kPad;
+        // piece p: 1024 elements of row p >> sh, from 1024 (p & (per - 1)) on
+        const int sh = a.K > 4096 ? 3 : a.K > 2048 ? 2 : a.K > 1024 ? 1 : 0, pieces = a.M << sh;
         float4 v[kPieces];
+        auto row = [&](int p) { return p >> sh; };
+        auto col = [&](int p) { return 4 * ((int)threadIdx.x + 256 * (p & ((1 << sh) - 1))); };
 #pragma unroll
-        for (int p = 0; p < kPieces; ++p) {
-            const int m = p / per, k = 4 * ((int)threadIdx.x + 256 * (p - m * per));
-            v[p] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (m < a.M) v[p] = some4<TX, true>(static_cast<const TX*>(a.Xf) + (long)m * a.ldxf, k, a.K);
-            unsigned t = max4(0, v[p]);
+        for (int p = 0; p < kPieces; ++p)
+            if (p < pieces) v[p] = some4<TX, true>(static_cast<const TX*>(a.Xf) + (long)row(p) * a.ldxf, col(p), a.K);
+        fetch(wv[0], w);   // (behind x: loads come back in order)
+        fetch(wv[1], w + 4);
 #pragma unroll
-            for (int off = 32; off > 0; off >>= 1) t = max(t, (unsigned)__shfl_xor((int)t, off));
-            if (lane == 0) most[w][p] = t;
-        }
+        for (int p = 0; p < kPieces; ++p)
+            if (p < pieces) {
+                const unsigned t = wave_max(max4(0, v[p]));
+                if (lane == 0) most[w][p] = t;
+            }
         __syncthreads();
         auto scale = [&](int m) {
             unsigned t = 0;
-            for (int p = m * per; p < (m + 1) * per; ++p)
+            for (int p = m << sh; p < (m + 1) << sh; ++p)
                 t = max(max(t, max(most[0][p], most[1][p])), max(most[2][p], most[3][p]));
             return scale_of(t);
         };
 #pragma unroll
-        for (int p = 0; p < kPieces; ++p) {
-            const int m = p / per, k = 4 * ((int)threadIdx.x + 256 * (p - m * per));
-            if (m < a.M && k < Kp) {
-                const float s = scale(m);
+        for (int p = 0; p < kPieces; ++p)
+            if (p < pieces && col(p) < Kp) {
+                const float s = scale(row(p));
                 const bool ok = usable(s);
-                *reinterpret_cast<unsigned*>(xs + m * Kp + k) = ok ? pack4(Quant(ok ? s : 1.f), v[p]) : 0u;
+                *reinterpret_cast<unsigned*>(xs + row(p) * Kp + col(p)) = ok ? Quant(ok ? s : 1.f).pack(v[p]) : 0u;
             }
-        }
         sm[0] = scale(min(i, a.M - 1));
         __syncthreads();
     } else {
+        fetch(wv[0], w);
+        fetch(wv[1], w + 4);
 #pragma unroll
         for (int m = 0; m < MB; ++m) sm[m] = a.sx[min(16 * m + i, a.M - 1)];
     }
-    auto step = [&](intx4 (&wv)[NB][4], int s) {
-        intx4 xv[MB][4];
+    auto step = [&](const intx4 (&v)[4], int s) {
+        if (s >= steps) return;
+        intx4 x[MB][4];
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 if constexpr (FUSED) {
-                    const int Kp = (a.K + kPad - 1) / kPad * kPad;
-                    xv[m][u] = intx4{0, 0, 0, 0};
-                    if (i < a.M) xv[m][u] = *reinterpret_cast<const intx4*>(xs + i * Kp + 256 * s + 64 * g + 16 * u);
+                    x[m][u] = intx4{0, 0, 0, 0};
+                    if (i < a.M) x[m][u] = *reinterpret_cast<const intx4*>(xs + i * Kp + 256 * s + 64 * g + 16 * u);
                 } else {
-                    xv[m][u] = *reinterpret_cast<const intx4*>(a.X + ((long)m * steps + s) * 4096 + u * 1024 + lane * 16);
+                    x[m][u] = *reinterpret_cast<const intx4*>(a.X + ((long)m * steps + s) * 4096 + u * 1024 + lane * 16);
                 }
             }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int m = 0; m < MB; ++m) acc[b][m] = mfma8(wv[b][u], xv[m][u], acc[b][m]);
+            for (int m = 0; m < MB; ++m) acc[m] = mfma8(v[u], x[m][u], acc[m]);
     };
     for (int s = w; s < steps; s += 8) {
         step(wv[0], s);
-        weights(wv[0], s + 8);
-        if (s + 4 < steps) step(wv[1], s + 4);
-        weights(wv[1], s + 12);
+        fetch(wv[0], s + 8);
+        step(wv[1], s + 4);
+        fetch(wv[1], s + 12);
     }
-    if (w > 0) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int m = 0; m < MB; ++m) red[w - 1][b * MB + m][lane] = acc[b][m];
-    }
+    for (int m = 0; m < MB; ++m) red[w][m][lane] = acc[m];
     __syncthreads();
-    if (w > 0) return;
+    // rows 16 t .. are finished by wave t
     const Out<TO> out(a, 0, a.M, n0, rows);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int n = 16 * b + 4 * g;
-        floatx4 s4, b4;
+    for (int t = 0; t < MB; ++t) {
+        if (t != w) continue;
+        const int n = 4 * g, row = 16 * t + i;
+        const intx4 c = red[0][t][lane] + red[1][t][lane] + red[2][t][lane] + red[3][t][lane];
+        float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int k = min(n0 + n + r, a.N - 1);
-            s4[r] = a.sw[k];
-            b4[r] = a.bias ? a.bias[k] : 0.f;
+            v[r] = (float)c[r] * (sm[t] * a.sw[k]) + (a.bias ? a.bias[k] : 0.f);
         }
+        const int rr = row < a.M ? row : 0, nn = row < a.M ? n : 1 << 30;
+        if (a.vec) put4<TO, BETA>(out, a.beta, rr, nn, v);
+        else {
 #pragma unroll
-        for (int m = 0; m < MB; ++m) {
-            const int row = 16 * m + i;
-            intx4 c = acc[b][m];
-#pragma unroll
-            for (int o = 0; o < 3; ++o) c += red[o][b * MB + m][lane];
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                put1<TO, BETA>(out, a.beta, row < a.M ? row : 0, row < a.M ? n + r : 1 << 30,
-                               (float)c[r] * (sm[m] * s4[r]) + b4[r]);
+            for (int r = 0; r < 4; ++r) put1<TO, BETA>(out, a.beta, rr, nn + r, v[r]);
         }
     }
 }
@@ -412,7 +457,7 @@ __device__ __forceinline__ void to_lds16(__amdgpu_buffer_rsrc_t r, char* lds, un
 }
 
 // WN x WM waves, each with TN x TM tiles of 32 x 32 (v_mfma_i32_32x32x32_i8): a workgroup owns 32 TN
-// WN output channels of 32 TM WM rows and walks k in blocks of 64 through NS LDS stages. The loads
+// WN output channels of 32 TM WM rows and walks k in blocks of 64 through four LDS stages. The loads
 // go straight from memory to LDS, sixteen rows of 64 bytes an instruction. A row's 64 bytes lie as
 // four 16-byte pieces, piece c at place c ^ (row / 4 % 4): any 16 consecutive rows of a piece then
 // fall on all banks.
@@ -420,67 +465,54 @@ __device__ __forceinline__ void to_lds16(__amdgpu_buffer_rsrc_t r, char* lds, un
 // A block's k are two steps of 32 (one MFMA deep). While a step multiplies, the operands of the next
 // one are read; so a stage is free once its second step is in registers, a step before its products
 // end. There the wave waits for its loads of the next stage and for the workgroup, issues the loads
-// of the NS-th block on into the stage that came free, and goes on: one barrier a block, with
-// products behind and ahead of it, and a load has NS - 1 blocks' time to land.
+// of the fourth block on into the stage that came free, and goes on: one barrier a block, with
+// products behind and ahead of it, and a load has three blocks' time to land. At a tile's end these
+// are the next tile's first blocks: its operands land while the outputs are written.
 //
-// The outputs go through LDS, 32 rows of a wave at a time, so that they are written as whole lines:
-// written as they lie in the accumulators (16 bytes of 32 rows an instruction) they took 17 us of a
-// tile's 40 at K 2048.
-template <int WN, int WM, int TN, int TM, int NS, typename TO, bool BETA>
-__global__ __launch_bounds__(64 * WN * WM, TN * TM > 8 ? 1 : 2) void i8_gemm_kernel(I8Args a) {
+// The outputs go through LDS, so that they are written 128 bytes of a row at a time: as they lie in the accumulators (16 bytes of 32 rows an instruction) they took
+// 17 us of a tile's 40 at K 2048.
+struct Tiles {        // tile ids first, first + step, .. below end; id -> place
+    int first, step, end;
+};
+
+template <int WN, int WM, int TN, int TM, bool ONE, typename TO, bool BETA, int SB, typename Place>
+__device__ __forceinline__ void i8_tiles(const I8Args& a, Tiles tiles, Place place_of, char* s0, char* s1,
+                                         char* s2, char* s3, float* chs, float* chb, float* rows_s,
+                                         float* outs) {
     constexpr int NW = WN * WM, BN = 32 * TN * WN, BM = 32 * TM * WM;
-    constexpr int PW = BN / 16 / NW, PX = BM / 16 / NW, PER = PW + PX, SB = (BN + BM) * 64;
-    static_assert(BN % (16 * NW) == 0 && BM % (16 * NW) == 0 && (NS == 3 || NS == 4), "loads shared out evenly");
-    // (each its own object: a read of one does not wait for the loads into the others)
-    __shared__ __attribute__((aligned(16))) char s0[SB], s1[SB], s2[SB], s3[NS > 3 ? SB : 16];
-    __shared__ __attribute__((aligned(16))) float chs[BN], chb[BN], rows_s[BM];
-
-    // consecutive ids on one XCD, in groups of gn channel tiles
-    const int T = a.mt * a.nt, bid = blockIdx.x;
-    const int xcd = bid & 7, per = T >> 3, rem = T & 7;
-    const int id = xcd * per + min(xcd, rem) + (bid >> 3);
-    const int gsz = a.gn * a.mt, grp = id / gsz, gr = id - grp * gsz;
-    const int gn = min(a.gn, a.nt - grp * a.gn);
-    const int tn = grp * a.gn + gr % gn, tm = gr / gn;
-
+    constexpr int PW = BN / 16 / NW, PX = BM / 16 / NW, PER = PW + PX;
+    static_assert(BN % (16 * NW) == 0 && BM % (16 * NW) == 0 && (BN + BM) * 64 <= SB, "loads shared out evenly");
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 5, i32 = lane & 31;
     const int wn = w % WN, wm = w / WN;
-    const int n0 = tn * BN, m0 = tm * BM;
-    const int nrows = min(BN, a.N - n0), mrows = min(BM, a.M - m0);
-    for (int i = threadIdx.x; i < BN + BM; i += 64 * NW) {
-        if (i < BN) {
-            const int n = min(n0 + i, a.N - 1);
-            chs[i] = a.sw[n];
-            chb[i] = a.bias ? a.bias[n] : 0.f;
-        } else {
-            rows_s[i - BN] = a.sx[min(m0 + i - BN, a.M - 1)];
-        }
-    }
     // a wave loads PW groups of sixteen rows of W and PX of x
-    const auto rw = ssm::rsrc(a.W + (long)n0 * a.ldw, (unsigned)((long)(nrows - 1) * a.ldw + whole(a.K)));
-    const auto rx = ssm::rsrc(a.X + (long)m0 * a.ldx, (unsigned)((long)(mrows - 1) * a.ldx + whole(a.K)));
     const unsigned piece = 16u * ((lane & 3) ^ (lane >> 4));
     const unsigned downw = 16u * (unsigned)a.ldw, downx = 16u * (unsigned)a.ldx;
     const unsigned atw = (unsigned)((lane >> 2) * a.ldw) + piece + PW * w * downw;
     const unsigned atx = (unsigned)((lane >> 2) * a.ldx) + piece + PX * w * downx;
-    const int KB = (a.K + 63) / 64;
-    auto load = [&](char* s, int kb) {   // (a block past the last reads zeros: past the descriptors)
+    const int KB = (a.K + 63) / 64, KR = (KB + 3) & ~3;   // (blocks past the last multiply zeros)
+
+    struct Where { int n0, m0, nrows, mrows; };
+    auto where = [&](int id) {
+        int tn, tm;
+        place_of(id, tn, tm);
+        return Where{tn * BN, tm * BM, min(BN, a.N - tn * BN), min(BM, a.M - tm * BM)};
+    };
+    auto rsrc_w = [&](const Where& t) {
+        return ssm::rsrc(a.W + (long)t.n0 * a.ldw, (unsigned)((long)(t.nrows - 1) * a.ldw + whole(a.K)));
+    };
+    auto rsrc_x = [&](const Where& t) {
+        return ssm::rsrc(a.X + (long)t.m0 * a.ldx, (unsigned)((long)(t.mrows - 1) * a.ldx + whole(a.K)));
+    };
+    auto load = [&](char* s, __amdgpu_buffer_rsrc_t rw, __amdgpu_buffer_rsrc_t rx, int kb) {
+        // (a block past the last reads zeros: past the descriptors)
         const unsigned k = kb < KB ? 64u * (unsigned)kb : kOut;
 #pragma unroll
         for (int u = 0; u < PW; ++u) to_lds16(rw, s + (PW * w + u) * 1024, atw + (k + u * downw));
 #pragma unroll
         for (int u = 0; u < PX; ++u) to_lds16(rx, s + BN * 64 + (PX * w + u) * 1024, atx + (k + u * downx));
     };
-    intx16 acc[TN][TM];
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int j = 0; j < TM; ++j) {
-            acc[i][j] = intx16{};
-            asm volatile("" : "+a"(acc[i][j]));   // (in accumulation registers from the start)
-        }
     struct Frags { intx4 w[TN], x[TM]; };
     const int swz = i32 >> 2 & 3;
     const int wrow = (32 * TN * wn + i32) * 64, xrow = (BN + 32 * TM * wm + i32) * 64;
@@ -491,6 +523,7 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM > 8 ? 1 : 2) void i8_gemm_ker
 #pragma unroll
         for (int i = 0; i < TN; ++i) f.w[i] = *reinterpret_cast<const intx4*>(s + wrow + c + 32 * i * 64);
     };
+    intx16 acc[TN][TM];
     auto multiply = [&](const Frags& f) {
 #pragma unroll
         for (int i = 0; i < TN; ++i)
@@ -510,139 +543,259 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM > 8 ? 1 : 2) void i8_gemm_ker
         }
         __builtin_amdgcn_sched_barrier(0);
     };
-    // at most NS - 2 blocks' loads of the wave in flight, its LDS reads done, then the workgroup
-    auto meet = [&]() {
-        constexpr int KEEP = (NS - 2) * PER;
+    // at most KEEP of the wave's loads (and stores) in flight, its LDS reads done, then the workgroup
+    auto meet = [&](auto keep) {
+        constexpr int KEEP = decltype(keep)::value;
         static_assert(KEEP < 64, "vmcnt has six bits");
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(0x0070 | (KEEP & 15) | ((KEEP >> 4) << 14));
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
+    constexpr std::integral_constant<int, 2 * PER> two{};
+    constexpr std::integral_constant<int, 3 * PER> three{};
+
+    int id = tiles.first;
+    if (id >= tiles.end) return;
+    Where t = where(id);
+    auto rw = rsrc_w(t), rx = rsrc_x(t);
+    load(s0, rw, rx, 0);
+    load(s1, rw, rx, 1);
+    load(s2, rw, rx, 2);
+    load(s3, rw, rx, 3);
     Frags f0, f1;
-    // one block out of stage s, its first step in f0; leaves the next block's first step there
-    auto block = [&](char* s, char* next, int kb) {
-        read(f1, s, 1);
-        multiply(f0);
-        spread(std::integral_constant<int, 0>{});
-        meet();
-        read(f0, next, 0);
-        load(s, kb + NS);
-        multiply(f1);
-        spread(std::integral_constant<int, PER>{});
-    };
-    load(s0, 0);
-    load(s1, 1);
-    load(s2, 2);
-    if constexpr (NS > 3) load(s3, 3);
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0x0070 | ((NS - 1) * PER & 15) | (((NS - 1) * PER >> 4) << 14));
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    read(f0, s0, 0);
-    for (int kb = 0; kb < KB; kb += NS) {   // (blocks past the last multiply zeros)
-        block(s0, s1, kb);
-        block(s1, s2, kb + 1);
-        block(s2, NS > 3 ? s3 : s0, kb + 2);
-        if constexpr (NS > 3) block(s3, s0, kb + 3);
+    for (;;) {
+        const int after = id + tiles.step;
+        const bool more = !ONE && after < tiles.end;
+        const Where tn = more ? where(after) : t;
+        const auto nw = rsrc_w(tn), nx = rsrc_x(tn);
+        // one block out of stage s, its first step in f0; leaves the next block's first step there
+        auto block = [&](char* s, char* next, int kb) {
+            read(f1, s, 1);
+            multiply(f0);
+            spread(std::integral_constant<int, 0>{});
+            meet(two);
+            read(f0, next, 0);
+            if (kb + 4 < KR) load(s, rw, rx, kb + 4);
+            else load(s, nw, nx, more ? kb + 4 - KR : KB);
+            multiply(f1);
+            spread(std::integral_constant<int, PER>{});
+        };
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int j = 0; j < TM; ++j) {
+                acc[i][j] = intx16{};
+                asm volatile("" : "+a"(acc[i][j]));   // (in accumulation registers from the start)
+            }
+        meet(three);
+        read(f0, s0, 0);
+        // the tile's scales, for its end (the last tile's were read before the barrier)
+        for (int i = threadIdx.x; i < BN + BM; i += 64 * NW) {
+            if (i < BN) {
+                const int n = min(t.n0 + i, a.N - 1);
+                chs[i] = a.sw[n];
+                chb[i] = a.bias ? a.bias[n] : 0.f;
+            } else {
+                rows_s[i - BN] = a.sx[min(t.m0 + i - BN, a.M - 1)];
+            }
+        }
+        for (int kb = 0; kb < KR; kb += 4) {
+            block(s0, s1, kb);
+            block(s1, s2, kb + 1);
+            block(s2, s3, kb + 2);
+            block(s3, s0, kb + 3);
+        }
+
+        if constexpr (ONE) {   // (the outputs take a stage)
+            __builtin_amdgcn_s_waitcnt(0x0070);
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // ---- outputs, 32 rows of 128 bytes at a time through the wave's own 4 KB of LDS: bf16 as they are
+        // written (two tiles of columns), fp32 and what beta y is added to as fp32 (one). The 16-byte piece
+        // u of row r lies at u ^ (r % 8), so that the rows of a piece fall on all banks.
+        using TL = typename std::conditional<BETA, float, TO>::type;
+        constexpr int UI = 4 / sizeof(TL), CP = 32 * UI;   // tiles and columns a time
+        const int li = fresh(i32), lg = fresh(g), ll = fresh(lane);
+        char* tile = reinterpret_cast<char*>(outs) + w * 4096;
+        auto place = [&](int r, int u) { return tile + r * 128 + 16 * (u ^ (r & 7)); };
+        const Out<TO> out(a, t.m0, t.mrows, t.n0, t.nrows);
+        auto finish = [&](auto vec) {
+            constexpr bool VEC = decltype(vec)::value;
+#pragma unroll
+            for (int j = 0; j < TM; ++j) {
+                const int mw = 32 * (TM * wm + j);
+                const float sm = rows_s[mw + li];
+#pragma unroll
+                for (int i0 = 0; i0 < TN; i0 += UI) {
+                    const int nw = 32 * (TN * wn + i0);
+#pragma unroll
+                    for (int i = 0; i < UI; ++i)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {   // channels 8 q + 4 g .. + 3 of the tile, row i32
+                            const int c = 32 * i + 8 * q + 4 * lg;
+                            const floatx4 s4 = *reinterpret_cast<const floatx4*>(&chs[nw + c]);
+                            const floatx4 b4 = *reinterpret_cast<const floatx4*>(&chb[nw + c]);
+                            floatx4 v;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) v[r] = (float)acc[i0 + i][j][4 * q + r] * (sm * s4[r]) + b4[r];
+                            if constexpr (sizeof(TL) == 4) {
+                                *reinterpret_cast<floatx4*>(place(li, c / 4)) = v;
+                            } else {
+                                bf16x4 y;
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) y[r] = (__bf16)v[r];
+                                *reinterpret_cast<bf16x4*>(place(li, c / 8) + 2 * (c & 4)) = y;
+                            }
+                        }
+                    __builtin_amdgcn_wave_barrier();
+                    if constexpr (VEC) {
+                        constexpr int E = 16 / sizeof(TO), LR = CP / E, RR = 64 / LR;   // lanes a row, rows a time
+#pragma unroll
+                        for (int r0 = 0; r0 < 32; r0 += RR) {
+                            const int r = r0 + ll / LR, c = ll % LR * E;
+                            if constexpr (BETA || sizeof(TO) == 4) {
+                                float v[E];
+#pragma unroll
+                                for (int p = 0; p < E / 4; ++p) {
+                                    const floatx4 x = *reinterpret_cast<const floatx4*>(place(r, c / 4 + p));
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) v[4 * p + e] = x[e];
+                                }
+                                put<TO, BETA>(out, a.beta, mw + r, nw + c, v);
+                            } else {
+                                const unsigned off = nw + c < out.cols ? ((unsigned)(mw + r) * out.ld + (unsigned)(nw + c)) * 2u : kOut;
+                                __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const ssm::u32x4*>(place(r, c / 8)), out.d, off, 0, 0);
+                            }
+                        }
+                    } else {
+#pragma unroll 4
+                        for (int k = 0; k < 32 * CP; k += 64) {
+                            const int r = (k + ll) / CP, c = (k + ll) % CP;
+                            const TL y = reinterpret_cast<const TL*>(place(r, c * (int)sizeof(TL) / 16))[c % (16 / (int)sizeof(TL))];
+                            put1<TO, BETA>(out, a.beta, mw + r, nw + c, (float)y);
+                        }
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                }
+            }
+        };
+        if (a.vec) finish(std::true_type{});
+        else finish(std::false_type{});
+        if (ONE || !more) break;
+        id = after;
+        t = tn;
+        rw = nw;
+        rx = nx;
     }
-    // no load is in flight into LDS, and no wave reads operands from it, when it takes the outputs
+    // no load is in flight into LDS, and no wave reads from it, when it is used otherwise
     __builtin_amdgcn_s_waitcnt(0x0070);
     __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
+}
 
-    constexpr int CW = 32 * TN, UW = CW / 4;   // columns of a wave, in pieces of four
-    static_assert(NW == 4 && 32 * CW * 4 <= SB, "a stage takes the outputs of 32 rows of a wave or two");
-    constexpr bool HALF = NS == 3;   // two waves a stage
-    static_assert(!HALF || 2 * 32 * CW * 4 <= SB, "");
-    float* tile = HALF ? reinterpret_cast<float*>(w < 2 ? s0 : s1) + (w & 1) * 32 * CW
-                       : reinterpret_cast<float*>(w == 0 ? s0 : w == 1 ? s1 : w == 2 ? s2 : s3);
-    // piece u of row r: its 32 rows fall on different banks
-    auto place = [&](int r, int u) { return tile + r * CW + 4 * (u ^ (r & (UW - 1))); };
-    const Out<TO> out(a, m0, mrows, n0, nrows);
-    auto finish = [&](auto vec) {
-        constexpr bool VEC = decltype(vec)::value;
-#pragma unroll
-        for (int j = 0; j < TM; ++j) {
-            const int mw = 32 * (TM * wm + j);
-            const float sm = rows_s[mw + i32];
-#pragma unroll
-            for (int i = 0; i < TN; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {   // channels 8 q + 4 g .. + 3 of the tile, row i32
-                    const int u = 8 * i + 2 * q + g;
-                    const floatx4 s4 = *reinterpret_cast<const floatx4*>(&chs[CW * wn + 4 * u]);
-                    const floatx4 b4 = *reinterpret_cast<const floatx4*>(&chb[CW * wn + 4 * u]);
-                    floatx4 v;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = (float)acc[i][j][4 * q + r] * (sm * s4[r]) + b4[r];
-                    *reinterpret_cast<floatx4*>(place(i32, u)) = v;
-                }
-            __builtin_amdgcn_wave_barrier();
-            if constexpr (VEC) {
-                constexpr int E = 16 / sizeof(TO), LR = CW / E, RR = 64 / LR;   // lanes a row, rows a time
-#pragma unroll
-                for (int r0 = 0; r0 < 32; r0 += RR) {
-                    const int r = r0 + lane / LR, c = lane % LR * E;
-                    float v[E];
-#pragma unroll
-                    for (int p = 0; p < E / 4; ++p) {
-                        const floatx4 x = *reinterpret_cast<const floatx4*>(place(r, c / 4 + p));
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[4 * p + e] = x[e];
-                    }
-                    put<TO, BETA>(out, a.beta, mw + r, CW * wn + c, v);
-                }
-            } else {
-#pragma unroll 4
-                for (int r = 0; r < 32; ++r)
-#pragma unroll
-                    for (int c = 0; c < CW; c += 64) {
-                        const int n = c + lane;
-                        put1<TO, BETA>(out, a.beta, mw + r, CW * wn + n, place(r, n / 4)[n & 3]);
-                    }
-            }
-            __builtin_amdgcn_wave_barrier();
-        }
+// One tile of 128 channels and 64 TM rows a workgroup, several workgroups a CU.
+template <int TM, typename TO, bool BETA>
+__global__ __launch_bounds__(256, 2) void i8_gemm_kernel(I8Args a) {
+    constexpr int SB = (128 + 64 * TM) * 64;
+    // (the stages are objects of their own: a read of one does not wait for the loads into the others;
+    // the first takes the outputs too, 4 KB a wave)
+    constexpr int S0 = SB < 4 * 4096 ? 4 * 4096 : SB;
+    __shared__ __attribute__((aligned(16))) char s0[S0], s1[SB], s2[SB], s3[SB];
+    __shared__ __attribute__((aligned(16))) float chs[128], chb[128], rows_s[64 * TM];
+    // consecutive ids on one XCD, in groups of gn channel tiles
+    const int T = a.mt * a.nt, xcd = blockIdx.x & 7, per = T >> 3, rem = T & 7;
+    const int id = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
+    auto place = [&](int id, int& tn, int& tm) {
+        const int gsz = a.gn * a.mt, grp = id / gsz, gr = id - grp * gsz;
+        const int gn = min(a.gn, a.nt - grp * a.gn);
+        tn = grp * a.gn + gr % gn;
+        tm = gr / gn;
     };
-    if (a.vec) finish(std::true_type{});
-    else finish(std::false_type{});
+    i8_tiles<2, 2, 2, TM, true, TO, BETA, SB>(a, Tiles{id, 1, id + 1}, place, s0, s1, s2, s3, chs, chb, rows_s,
+                                              reinterpret_cast<float*>(s0));
+}
+
+// 256 x 256 tiles, one workgroup a CU that walks its share of them: XCD x's 32 workgroups take its
+// tiles in turn. Tiles of a last turn that would leave three quarters of the CUs idle are shared out
+// in quarters, 128 x 128 a workgroup (8192 x 8512: 1088 tiles are 4.25 turns).
+template <typename TO, bool BETA>
+__global__ __launch_bounds__(256, 1) void i8_gemm_big_kernel(I8Args a) {
+    constexpr int SB = 512 * 64;
+    __shared__ __attribute__((aligned(16))) char s0[SB], s1[SB], s2[SB], s3[SB];
+    __shared__ __attribute__((aligned(16))) float chs[256], chb[256], rows_s[256], outs[4096];
+    const int T = a.mt * a.nt, xcd = blockIdx.x & 7, local = blockIdx.x >> 3, wgs = gridDim.x >> 3;
+    const int per = T >> 3, rem = T & 7;
+    const int lo = xcd * per + min(xcd, rem), n = per + (xcd < rem), tail = n % wgs;
+    const bool quarters = 4 * tail <= wgs;
+    auto place = [&](int id, int& tn, int& tm) {
+        const int gsz = a.gn * a.mt, grp = id / gsz, gr = id - grp * gsz;
+        const int gn = min(a.gn, a.nt - grp * a.gn);
+        tn = grp * a.gn + gr % gn;
+        tm = gr / gn;
+    };
+    const int whole_end = lo + n - (quarters ? tail : 0);
+    i8_tiles<2, 2, 4, 4, false, TO, BETA, SB>(a, Tiles{lo + local, wgs, whole_end}, place, s0, s1, s2, s3, chs, chb,
+                                       rows_s, outs);
+    if (!quarters) return;
+    auto quarter = [&](int id, int& tn, int& tm) {
+        place(whole_end + (id >> 2), tn, tm);
+        tn = 2 * tn + (id & 1);
+        tm = 2 * tm + (id >> 1 & 1);
+    };
+    // (a quarter that lies past the matrix is not begun)
+    int id = local;
+    if (id < 4 * tail) {
+        int tn, tm;
+        quarter(id, tn, tm);
+        if (tn * 128 >= a.N || tm * 128 >= a.M) id = 4 * tail;
+    }
+    i8_tiles<2, 2, 2, 2, true, TO, BETA, SB>(a, Tiles{id, wgs, min(4 * tail, id + 1)}, quarter, s0, s1, s2, s3,
+                                             chs, chb, rows_s, outs);
 }
 
 // ---------------------------------------------------------------- plan
-template <int MB, int NB, typename TX, typename TO>
-void rows_launch(const I8Args& a, hipStream_t st) {
-    const unsigned n = (unsigned)ssm::cdiv(a.N, 16 * NB);
-    if (a.beta != 0.f) i8_rows_kernel<MB, NB, TX, TO, true><<<n, 256, 0, st>>>(a);
-    else i8_rows_kernel<MB, NB, TX, TO, false><<<n, 256, 0, st>>>(a);
-}
-
-// Two blocks of channels a workgroup (half the reads of x) where that leaves one for every CU.
 template <int MB, typename TX, typename TO>
-void rows_blocks(const I8Args& a, hipStream_t st) {
-    if (ssm::cdiv(a.N, 32) >= 256) rows_launch<MB, 2, TX, TO>(a, st);
-    else rows_launch<MB, 1, TX, TO>(a, st);
+void rows_launch(const I8Args& a, hipStream_t st) {
+    const unsigned n = (unsigned)ssm::cdiv(a.N, 16);
+    if (a.beta != 0.f) i8_rows_kernel<MB, TX, TO, true><<<n, 256, 0, st>>>(a);
+    else i8_rows_kernel<MB, TX, TO, false><<<n, 256, 0, st>>>(a);
 }
 
-template <int WN, int WM, int TN, int TM, int NS, typename TO>
-void gemm_launch(I8Args a, hipStream_t st) {
-    a.nt = (int)ssm::cdiv(a.N, 32 * TN * WN);
-    a.mt = (int)ssm::cdiv(a.M, 32 * TM * WM);
+template <int TM, typename TO>
+void tile_launch(I8Args a, hipStream_t st) {
+    a.nt = (int)ssm::cdiv(a.N, 128);
+    a.mt = (int)ssm::cdiv(a.M, 64 * TM);
     a.gn = std::min(a.nt, 8);
     const unsigned n = (unsigned)(a.nt * a.mt);
-    if (a.beta != 0.f) i8_gemm_kernel<WN, WM, TN, TM, NS, TO, true><<<n, 64 * WN * WM, 0, st>>>(a);
-    else i8_gemm_kernel<WN, WM, TN, TM, NS, TO, false><<<n, 64 * WN * WM, 0, st>>>(a);
+    if (a.beta != 0.f) i8_gemm_kernel<TM, TO, true><<<n, 256, 0, st>>>(a);
+    else i8_gemm_kernel<TM, TO, false><<<n, 256, 0, st>>>(a);
+}
+
+template <typename TO>
+void gemm_launch(I8Args a, hipStream_t st) {
+    const long big = ssm::cdiv(a.N, 256) * ssm::cdiv(a.M, 256);
+    if (big >= kCUs) {
+        a.nt = (int)ssm::cdiv(a.N, 256);
+        a.mt = (int)ssm::cdiv(a.M, 256);
+        a.gn = std::min(a.nt, 8);
+        if (a.beta != 0.f) i8_gemm_big_kernel<TO, true><<<kCUs, 256, 0, st>>>(a);
+        else i8_gemm_big_kernel<TO, false><<<kCUs, 256, 0, st>>>(a);
+        return;
+    }
+    // tiles of 64 rows where those of 128 would leave CUs idle (512 x 4096 x 4096: 20.5 -> 17.4 us)
+    if (ssm::cdiv(a.N, 128) * ssm::cdiv(a.M, 128) < kCUs) tile_launch<1, TO>(a, st);
+    else tile_launch<2, TO>(a, st);
 }
 
 template <typename TO>
 ssm_status product(const I8Args& a, hipStream_t st) {
-    if (a.Xf && a.x_dtype == SSM_F32) rows_blocks<1, float, TO>(a, st);
-    else if (a.Xf) rows_blocks<1, __bf16, TO>(a, st);
-    else if (a.M <= 16) rows_blocks<1, void, TO>(a, st);
-    else if (a.M <= 32) rows_blocks<2, void, TO>(a, st);
-    else if (a.M <= kRowsMax) rows_blocks<4, void, TO>(a, st);
-    else if (ssm::cdiv(a.N, 256) * ssm::cdiv(a.M, 256) >= 256) gemm_launch<2, 2, 4, 4, 4, TO>(a, st);
-    else gemm_launch<2, 2, 2, 2, 4, TO>(a, st);
+    if (a.Xf && a.x_dtype == SSM_F32) rows_launch<1, float, TO>(a, st);
+    else if (a.Xf) rows_launch<1, __bf16, TO>(a, st);
+    else if (a.M <= 16) rows_launch<1, void, TO>(a, st);
+    else if (a.M <= 32) rows_launch<2, void, TO>(a, st);
+    else if (a.M <= kRowsMax) rows_launch<4, void, TO>(a, st);
+    else gemm_launch<TO>(a, st);
     return ssm::check_launch("ssm_linear_i8");
 }
 
@@ -767,7 +920,8 @@ extern "C" ssm_status ssm_linear_q8(int in_dtype, const void* x, long ldx, const
     I8Args a{q, l.Kp, sx, nullptr, ldx, in_dtype, (const signed char*)W, ldw, sw, bias, y, ldy,
              M, N, K, beta, 0, 0, 0, 0};
     const bool vec = K % 4 == 0 && ldx % 4 == 0 && ((uintptr_t)x & (in_dtype == SSM_F32 ? 15 : 7)) == 0;
-    if (vec && M <= kFusedRows && M * ssm::cdiv(K, 1024) <= kFusedX / 1024)
+    const int per = K > 4096 ? 8 : K > 2048 ? 4 : K > 1024 ? 2 : 1;
+    if (vec && K <= kFusedX && M <= kFusedRows && M * per <= kFusedX / 1024)
         a.Xf = x;
     else if (ssm_status e = quantize(in_dtype, x, ldx, q, l.Kp, sx, M, K, (int)l.Kp, M <= kRowsMax,
                                      (hipStream_t)stream))

@@ -843,13 +843,15 @@ __global__ __launch_bounds__(256) void la_combine_kernel(LaArgs a) {
 // ---------------------------------------------------------------- plan
 int v_tile(int K, int V) { return V <= 64 || K > 128 ? 64 : 128; }
 
-// Segments: enough workgroups to fill the chip, each of at least kLeast tokens.
-constexpr int kFill = 512, kLeast = 256;
+// Segments: enough workgroups to fill the chip, each of at least so many tokens. (fp32 chunks take four
+// times as long on the matrix cores: 24 sequences and heads of 2000 tokens ran 95 us with segments of
+// 256, 84 with 64; bf16 ones gain nothing below 256, as their states' traffic grows.)
+constexpr int kFill = 512, kLeastB = 256, kLeastF = 64;
 void la_plan(int dtype, int B, int L, int H, int K, int V, int& nseg, int& seglen, int& vparts) {
     const int C = dtype == SSM_F32 ? CF : CB;
     vparts = (int)ssm::cdiv(V, v_tile(K, V));
     const long wgs = (long)B * H * vparts;
-    long n = std::min<long>(ssm::cdiv(kFill, std::max(wgs, 1L)), ssm::cdiv(std::max(L, 1), kLeast));
+    long n = std::min<long>(ssm::cdiv(kFill, std::max(wgs, 1L)), ssm::cdiv(std::max(L, 1), dtype == SSM_F32 ? kLeastF : kLeastB));
     n = std::max(n, 1L);
     seglen = (int)(ssm::cdiv(ssm::cdiv(std::max(L, 1), n), C) * C);
     nseg = (int)std::max(1L, ssm::cdiv(L, seglen));
