@@ -843,17 +843,20 @@ __global__ __launch_bounds__(256) void la_combine_kernel(LaArgs a) {
 // ---------------------------------------------------------------- plan
 int v_tile(int K, int V) { return V <= 64 || K > 128 ? 64 : 128; }
 
-// Segments: enough workgroups to fill the chip, each of at least so many tokens. (fp32 chunks take four
-// times as long on the matrix cores: 24 sequences and heads of 2000 tokens ran 95 us with segments of
-// 256, 84 with 64; bf16 ones gain nothing below 256, as their states' traffic grows.)
-constexpr int kFill = 512, kLeastB = 256, kLeastF = 64;
+// Segments: as many as fill the chip once, two workgroups a CU (one more turn for the rest costs as much
+// as a whole one: 80 sequences and heads of 4096 tokens ran 171 us in 7 segments, 144 in 6), each of
+// at least so many tokens that its states' traffic stays small beside its rows'. bf16: 512 where that
+// leaves a workgroup for every CU (128 sequences and heads of 1024: 72 -> 63 us against 256), else 256.
+// fp32 chunks take four times as long on the matrix cores: 64 (24 of 2000: 95 -> 84 us against 256).
+constexpr int kSlots = 512, kCUs = 256;
 void la_plan(int dtype, int B, int L, int H, int K, int V, int& nseg, int& seglen, int& vparts) {
     const int C = dtype == SSM_F32 ? CF : CB;
     vparts = (int)ssm::cdiv(V, v_tile(K, V));
-    const long wgs = (long)B * H * vparts;
-    long n = std::min<long>(ssm::cdiv(kFill, std::max(wgs, 1L)), ssm::cdiv(std::max(L, 1), dtype == SSM_F32 ? kLeastF : kLeastB));
-    n = std::max(n, 1L);
-    seglen = (int)(ssm::cdiv(ssm::cdiv(std::max(L, 1), n), C) * C);
+    const long wgs = std::max((long)B * H * vparts, 1L), len = std::max(L, 1);
+    const long fit = std::max(kSlots / wgs, 1L), by512 = ssm::cdiv(len, 512);
+    const long most = dtype == SSM_F32 ? ssm::cdiv(len, 64) : by512 * wgs >= kCUs ? by512 : ssm::cdiv(len, 256);
+    const long n = std::min(fit, most);
+    seglen = (int)(ssm::cdiv(ssm::cdiv(len, n), C) * C);
     nseg = (int)std::max(1L, ssm::cdiv(L, seglen));
 }
 
