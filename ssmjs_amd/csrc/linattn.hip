@@ -116,10 +116,10 @@ struct SmemB {
 
 // 16 bytes (8 elements, columns col .. + 7) from byte offset o on: zeros from column `width` and
 // past the descriptor on.
-template <bool VEC>
+template <bool VEC, bool NT = false>
 __device__ __forceinline__ uint4 fetch_b(__amdgpu_buffer_rsrc_t r, unsigned o, int col, int width) {
-    if constexpr (VEC) {
-        return ssm::bload16<uint4>(r, o);   // (whole pieces: o is past the descriptor then)
+    if constexpr (VEC) {   // (whole pieces: o is past the descriptor then)
+        return NT ? ssm::bload16_nt<uint4>(r, o) : ssm::bload16<uint4>(r, o);
     } else {
         unsigned u[4];
 #pragma unroll
@@ -232,9 +232,11 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
 #pragma unroll
         for (int u = 0; u < NV; ++u) rv[u] = fetch_b<VEC>(dv, voff + u * vdown, part * VT + vcol, a.V);
         if constexpr (!STATE) {
+            // (read once: out of the way of k and v, which the state pass has read before and the other
+            // heads of the group read; 5 sequences of 4096 tokens 146 -> 140 us)
             const auto dq = ssm::rsrc(base(a.q, a.ldq, h, a.K, tt), bytes(a.ldq, a.K, n));
 #pragma unroll
-            for (int u = 0; u < NK; ++u) rq[u] = fetch_b<VEC>(dq, qoff + u * qdown, kcol, a.K);
+            for (int u = 0; u < NK; ++u) rq[u] = fetch_b<VEC, true>(dq, qoff + u * qdown, kcol, a.K);
         }
     };
     if (copy) {
