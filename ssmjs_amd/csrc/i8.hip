@@ -95,6 +95,17 @@ __device__ __forceinline__ float4 load4(const __bf16* p) {
                        __builtin_bit_cast(float, u.y << 16), __builtin_bit_cast(float, u.y & 0xffff0000u));
 }
 
+struct Eight { float4 a, b; };
+__device__ __forceinline__ Eight load8(const float* p) { return Eight{load4(p), load4(p + 4)}; }
+__device__ __forceinline__ Eight load8(const __bf16* p) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    auto two = [](unsigned x, unsigned y) {
+        return make_float4(__builtin_bit_cast(float, x << 16), __builtin_bit_cast(float, x & 0xffff0000u),
+                           __builtin_bit_cast(float, y << 16), __builtin_bit_cast(float, y & 0xffff0000u));
+    };
+    return Eight{two(u.x, u.y), two(u.z, u.w)};
+}
+
 // Four consecutive elements from k on, zeros past K.
 template <typename T, bool VEC>
 __device__ __forceinline__ float4 some4(const T* row, int k, int K) {
@@ -141,8 +152,9 @@ __device__ __forceinline__ long frag_at(long m, int k, int Kp) {
 }
 
 // TPR threads a row, 256 / TPR rows a workgroup: U pieces of eight elements a thread are held between
-// the two passes (further ones are read again).
-template <typename T, int TPR, bool VEC>
+// the two passes (further ones are read again). VEC: elements of an aligned load, 8 (K a multiple of it
+// too), 4 or 1. Memory bound; at 8192 x 2048 bf16 (50 MB) 3.5 TB/s.
+template <typename T, int TPR, int VEC>
 __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
     constexpr int U = 4, RPB = 256 / TPR, NW = TPR / 64;
     __shared__ unsigned red[4];
@@ -150,8 +162,14 @@ __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
     const long m = (long)blockIdx.x * RPB + rw;
     const bool live = m < a.M;
     const T* row = static_cast<const T*>(a.x) + (live ? m : 0) * a.ldx;
-    struct Eight { float4 a, b; };
-    auto get = [&](int k) { return Eight{some4<T, VEC>(row, k, a.K), some4<T, VEC>(row, k + 4, a.K)}; };
+    auto get = [&](int k) {
+        if constexpr (VEC == 8) {
+            const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+            return k < a.K ? load8(row + k) : Eight{z, z};
+        } else {
+            return Eight{some4<T, VEC == 4>(row, k, a.K), some4<T, VEC == 4>(row, k + 4, a.K)};
+        }
+    };
     Eight v[U];
     unsigned most = 0;
 #pragma unroll
@@ -181,7 +199,7 @@ __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
         const uint2 b = ok ? make_uint2(z.pack(e.a), z.pack(e.b)) : make_uint2(0u, 0u);
         if (a.frag) {   // (Kq is a whole number of pieces)
             *reinterpret_cast<uint2*>(out + frag_at(m, k, (int)a.ldq)) = b;
-        } else if constexpr (VEC) {
+        } else if constexpr (VEC > 1) {
             *reinterpret_cast<uint2*>(out + k) = b;
         } else {
 #pragma unroll
@@ -194,26 +212,33 @@ __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
     for (int k = 8 * (tid + TPR * U); k < a.Kq; k += 8 * TPR) put(k, get(k));
 }
 
-template <typename T>
-ssm_status run_quant(const QuantArgs& a, bool vec, hipStream_t st) {
-    // a wave a row up to 2048 elements (its four pieces a lane), a workgroup beyond
-    if (a.K <= 2048 && a.M >= 1024) {
-        const unsigned n = (unsigned)ssm::cdiv(a.M, 4);
-        if (vec) quant_kernel<T, 64, true><<<n, 256, 0, st>>>(a);
-        else quant_kernel<T, 64, false><<<n, 256, 0, st>>>(a);
-    } else {
-        if (vec) quant_kernel<T, 256, true><<<a.M, 256, 0, st>>>(a);
-        else quant_kernel<T, 256, false><<<a.M, 256, 0, st>>>(a);
-    }
-    return ssm::check_launch("ssm_quantize_rows");
+template <typename T, int VEC>
+void quant_launch(const QuantArgs& a, hipStream_t st) {
+    // a wave a row up to 2048 elements (its four pieces a lane) where that leaves a workgroup for every
+    // CU, a workgroup a row else
+    if (a.K <= 2048 && a.M >= 1024) quant_kernel<T, 64, VEC><<<(unsigned)ssm::cdiv(a.M, 4), 256, 0, st>>>(a);
+    else quant_kernel<T, 256, VEC><<<a.M, 256, 0, st>>>(a);
 }
 
 ssm_status quantize(int dtype, const void* x, long ldx, signed char* q, long ldq, float* scale,
                     int M, int K, int Kq, bool frag, hipStream_t st) {
     const QuantArgs a{x, ldx, q, ldq, scale, M, K, Kq, frag};
-    const bool vec = K % 4 == 0 && Kq % 8 == 0 && ldx % 4 == 0 && ldq % 8 == 0 &&
-                     ((uintptr_t)x & (dtype == SSM_F32 ? 15 : 7)) == 0 && ((uintptr_t)q & 7) == 0;
-    return dtype == SSM_F32 ? run_quant<float>(a, vec, st) : run_quant<__bf16>(a, vec, st);
+    const bool out8 = Kq % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)q & 7) == 0;
+    auto aligned = [&](int n) {   // n elements, 16 bytes at most
+        const uintptr_t b = std::min(16, n * (dtype == SSM_F32 ? 4 : 2));
+        return out8 && K % n == 0 && ldx % n == 0 && ((uintptr_t)x & (b - 1)) == 0;
+    };
+    const int vec = aligned(8) ? 8 : aligned(4) ? 4 : 1;
+    if (dtype == SSM_F32) {
+        if (vec == 8) quant_launch<float, 8>(a, st);
+        else if (vec == 4) quant_launch<float, 4>(a, st);
+        else quant_launch<float, 1>(a, st);
+    } else {
+        if (vec == 8) quant_launch<__bf16, 8>(a, st);
+        else if (vec == 4) quant_launch<__bf16, 4>(a, st);
+        else quant_launch<__bf16, 1>(a, st);
+    }
+    return ssm::check_launch("ssm_quantize_rows");
 }
 
 // Rows of K bytes at any alignment -> rows of Kp bytes, zeros past K (or the few-row operand's order).
