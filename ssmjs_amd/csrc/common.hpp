@@ -24,6 +24,20 @@ hipError_t dev_malloc(void** p, size_t bytes);
 
 inline long cdiv(long a, long b) { return (a + b - 1) / b; }
 
+// A launch's threads are counted in 32 bits: the most workgroups of 256.
+constexpr long kMaxGroups = (1L << 24) - 1;
+
+// Whether one of `rows` rows of wa bytes, lda bytes apart, shares memory with one of as many of wb, ldb
+// apart. (Column ranges of one buffer lie between each other's rows.)
+inline bool rows_meet(const void* a, long lda, long wa, const void* b, long ldb, long wb, long rows) {
+    if (rows <= 0 || wa <= 0 || wb <= 0) return false;
+    const uintptr_t p = (uintptr_t)a, q = (uintptr_t)b;
+    if (p + (rows - 1) * lda + wa <= q || q + (rows - 1) * ldb + wb <= p) return false;
+    if (lda != ldb || rows == 1) return true;
+    const long d = ((long)(q - p) % lda + lda) % lda;
+    return d < wa || d + wb > lda;
+}
+
 }  // namespace ssm
 
 #define SSM_HIP_TRY(expr)                                                   \

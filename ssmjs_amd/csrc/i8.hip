@@ -8,7 +8,7 @@
 //   - up to 64 rows (one per decoded sequence): the weights' bytes bound it. i8_rows_kernel reads
 //     every weight row once, straight into registers, the k of a row shared by the four waves.
 //   - more rows: the matrix cores bound it. i8_gemm_kernel is a tiled product out of LDS.
-//   - rows that are not 16-byte aligned are laid out in the workspace first (pad_rows_kernel).
+//   - rows that are not 16-byte aligned are laid out in the workspace first (lay_rows_kernel).
 #include <algorithm>
 #include <type_traits>
 
@@ -28,7 +28,7 @@ constexpr unsigned kOut = 0x80000000u;   // a buffer offset past any descriptor
 constexpr int kMaxK = 131071;
 constexpr int kPad = 256;          // rows of the workspace are whole blocks of 256 bytes, zeros past K
 constexpr int kCUs = 256;          // workgroups of the large tiles' kernel: one a CU
-constexpr int kRowsMax = 64;       // rows of the few-row kernel
+constexpr int kRowsMax = 64;       // rows of the few-row kernel (64 x 2048 x 2048: 9.3 us, 11.9 in tiles)
 inline long up(long n, long to) { return (n + to - 1) / to * to; }
 
 // ---------------------------------------------------------------- rows to integers
@@ -153,7 +153,7 @@ __device__ __forceinline__ long frag_at(long m, int k, int Kp) {
 
 // TPR threads a row, 256 / TPR rows a workgroup: U pieces of eight elements a thread are held between
 // the two passes (further ones are read again). VEC: elements of an aligned load, 8 (K a multiple of it
-// too), 4 or 1. Memory bound; at 8192 x 2048 bf16 (50 MB) 3.5 TB/s.
+// too), 4 or 1. Memory bound; at 8192 x 2048 bf16 (50 MB) 13.5 us, 3.7 TB/s.
 template <typename T, int TPR, int VEC>
 __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
     constexpr int U = 4, RPB = 256 / TPR, NW = TPR / 64;
@@ -214,9 +214,10 @@ __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
 
 template <typename T, int VEC>
 void quant_launch(const QuantArgs& a, hipStream_t st) {
-    // a wave a row up to 2048 elements (its four pieces a lane) where that leaves a workgroup for every
-    // CU, a workgroup a row else
-    if (a.K <= 2048 && a.M >= 1024) quant_kernel<T, 64, VEC><<<(unsigned)ssm::cdiv(a.M, 4), 256, 0, st>>>(a);
+    // a wave a row up to 2048 elements (its four pieces a lane) where there are more rows than
+    // elements (bf16, 8192 x 2048: 13.5 us, 15.0 with a workgroup a row; 8192 x 768: 7.1, 12.0), a
+    // workgroup a row else (1000 x 2048: 4.4 us, 6.0 with waves)
+    if (a.K <= 2048 && a.M >= std::max(a.K, 1000)) quant_kernel<T, 64, VEC><<<(unsigned)ssm::cdiv(a.M, 4), 256, 0, st>>>(a);
     else quant_kernel<T, 256, VEC><<<a.M, 256, 0, st>>>(a);
 }
 
@@ -358,8 +359,9 @@ __device__ __forceinline__ intx4 mfma8(intx4 w, intx4 x, intx4 c) {
 // LDS (integers: their order changes nothing).
 //
 // FUSED: up to four rows of x of at most kFusedX elements in all are rounded by every workgroup for
-// itself, into LDS, while its weights are on their way: one launch instead of two.
-constexpr int kFusedX = 8192, kFusedRows = 4;
+// itself, into LDS, while its weights are on their way: one launch instead of two (N 8512, K 2048, bf16:
+// one row 6.0 us, 8.5 in two launches; two rows 7.3, 8.3; four rows, past kFusedX, would take 10.4).
+constexpr int kFusedX = 4096, kFusedRows = 4;
 
 template <int MB, typename TX, typename TO, bool BETA>
 __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
@@ -389,7 +391,7 @@ __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
     float sm[MB];
     if constexpr (FUSED) {
         // piece p: 1024 elements of row p >> sh, from 1024 (p & (per - 1)) on
-        const int sh = a.K > 4096 ? 3 : a.K > 2048 ? 2 : a.K > 1024 ? 1 : 0, pieces = a.M << sh;
+        const int sh = a.K > 2048 ? 2 : a.K > 1024 ? 1 : 0, pieces = a.M << sh;
         float4 v[kPieces];
         auto row = [&](int p) { return p >> sh; };
         auto col = [&](int p) { return 4 * ((int)threadIdx.x + 256 * (p & ((1 << sh) - 1))); };
@@ -494,8 +496,11 @@ __device__ __forceinline__ void to_lds16(__amdgpu_buffer_rsrc_t r, char* lds, un
 // products behind and ahead of it, and a load has three blocks' time to land. At a tile's end these
 // are the next tile's first blocks: its operands land while the outputs are written.
 //
-// The outputs go through LDS, so that they are written 128 bytes of a row at a time: as they lie in the accumulators (16 bytes of 32 rows an instruction) they took
-// 17 us of a tile's 40 at K 2048.
+// Bound by the matrix cores and the LDS reads that feed them: 8192 x 8512 x 2048 to bf16 takes 154 us, 1.86
+// POP/s (a library's product of the integers alone 164 us), 8192 x 8192 x 8192 477 us, 2.3 POP/s (457).
+//
+// The outputs go through LDS, so that they are written 128 bytes of a row at a time: as they lie in the
+// accumulators (16 bytes of 32 rows an instruction) they took 17 us of a tile's 40 at K 2048.
 struct Tiles {        // tile ids first, first + step, .. below end; id -> place
     int first, step, end;
 };
@@ -799,6 +804,8 @@ void tile_launch(I8Args a, hipStream_t st) {
 
 template <typename TO>
 void gemm_launch(I8Args a, hipStream_t st) {
+    // tiles of 256 where every CU has one (4096 x 4096 x 4096: 68 us, 80 in tiles of 128; with half as many,
+    // 2048 x 4096 x 2048: 36 us, 26). gn: 4, 8 and 16 are within 3%.
     const long big = ssm::cdiv(a.N, 256) * ssm::cdiv(a.M, 256);
     if (big >= kCUs) {
         a.nt = (int)ssm::cdiv(a.N, 256);
@@ -808,7 +815,8 @@ void gemm_launch(I8Args a, hipStream_t st) {
         else i8_gemm_big_kernel<TO, false><<<kCUs, 256, 0, st>>>(a);
         return;
     }
-    // tiles of 64 rows where those of 128 would leave CUs idle (512 x 4096 x 4096: 20.5 -> 17.4 us)
+    // tiles of 64 rows where those of 128 would leave CUs idle (512 x 4096 x 4096: 16.0 us, 19.7; a tile
+    // for every CU, 1000 x 4096 x 2048: 15.0 us with 64 rows, 12.1 with 128)
     if (ssm::cdiv(a.N, 128) * ssm::cdiv(a.M, 128) < kCUs) tile_launch<1, TO>(a, st);
     else tile_launch<2, TO>(a, st);
 }
@@ -860,6 +868,7 @@ ssm_status check_product(const char* who, const void* x, long ldx, const int8_t*
     if (M == 0) return SSM_OK;
     SSM_REQUIRE(x && W && sw && y, "%s: null input", who);
     SSM_REQUIRE(ldx >= K && ldw >= K && ldy >= N, "%s: row stride below row width", who);
+    SSM_REQUIRE(M <= ssm::kMaxGroups && N <= ssm::kMaxGroups, "%s: too many rows", who);
     SSM_REQUIRE(ldw < (1L << 22) && ldx < (1L << 22) && ldy < (1L << 21), "%s: row stride too large", who);
     return SSM_OK;
 }
@@ -887,6 +896,9 @@ extern "C" ssm_status ssm_quantize_rows(int dtype, const void* x, long ldx, int8
     if (M == 0) return SSM_OK;
     SSM_REQUIRE(x && q && scale, "ssm_quantize_rows: null input");
     SSM_REQUIRE(ldx >= K && ldq >= K, "ssm_quantize_rows: row stride below row width");
+    SSM_REQUIRE(M <= ssm::kMaxGroups, "ssm_quantize_rows: too many rows");
+    const long es = dtype == SSM_F32 ? 4 : 2;
+    SSM_REQUIRE(!ssm::rows_meet(x, ldx * es, K * es, q, ldq, K, M), "ssm_quantize_rows: q overlaps x");
     return quantize(dtype, x, ldx, (signed char*)q, ldq, scale, M, K, K, false, (hipStream_t)stream);
 }
 
@@ -908,6 +920,8 @@ extern "C" ssm_status ssm_linear_i8(const int8_t* x, long ldx, const float* sx, 
     const Layout l = layout(M, N, K, lay_x, false, lay_w);
     SSM_REQUIRE(l.all == 0 || (workspace && workspace_bytes >= l.all && ((uintptr_t)workspace & 15) == 0),
                 "ssm_linear_i8: 16-byte aligned workspace of %zu bytes needed", l.all);
+    const long es = out_dtype == SSM_F32 ? 4 : 2;
+    SSM_REQUIRE(!ssm::rows_meet(x, ldx, K, y, ldy * es, N * es, M), "ssm_linear_i8: y overlaps x");
     I8Args a{(const signed char*)x, ldx, sx, nullptr, 0, 0, (const signed char*)W, ldw, sw, bias, y, ldy,
              M, N, K, beta, 0, 0, 0, 0};
     if (lay_x) {
@@ -945,8 +959,10 @@ extern "C" ssm_status ssm_linear_q8(int in_dtype, const void* x, long ldx, const
     I8Args a{q, l.Kp, sx, nullptr, ldx, in_dtype, (const signed char*)W, ldw, sw, bias, y, ldy,
              M, N, K, beta, 0, 0, 0, 0};
     const bool vec = K % 4 == 0 && ldx % 4 == 0 && ((uintptr_t)x & (in_dtype == SSM_F32 ? 15 : 7)) == 0;
-    const int per = K > 4096 ? 8 : K > 2048 ? 4 : K > 1024 ? 2 : 1;
-    if (vec && K <= kFusedX && M <= kFusedRows && M * per <= kFusedX / 1024)
+    const int per = K > 2048 ? 4 : K > 1024 ? 2 : 1;
+    // (each workgroup reads all of x there while others write: y has to be elsewhere)
+    const long ei = in_dtype == SSM_F32 ? 4 : 2, eo = out_dtype == SSM_F32 ? 4 : 2;
+    if (vec && !ssm::rows_meet(x, ldx * ei, K * ei, y, ldy * eo, N * eo, M) && K <= kFusedX && M <= kFusedRows && M * per <= kFusedX / 1024)
         a.Xf = x;
     else if (ssm_status e = quantize(in_dtype, x, ldx, q, l.Kp, sx, M, K, (int)l.Kp, M <= kRowsMax,
                                      (hipStream_t)stream))

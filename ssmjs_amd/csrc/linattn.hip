@@ -41,8 +41,26 @@ struct LaArgs {
     int combined;
 };
 
-// e^{g n} - 1 and e^{g n}. g = -inf keeps nothing (and n = 0 everything).
-__device__ __forceinline__ float decay_m1(float g, int n) { return expm1f(g * (float)n); }
+__device__ __forceinline__ float clamp_g(float g) { return g < -1e30f ? -1e30f : g; }   // (a NaN stays)
+
+// x <- e^{g n} x: as x + (e^{g n} - 1) x from 1/2 on, so that a decay too slow for fp32's e^{g n} is kept,
+// and as a product below, where the difference would lose what is left. (Without a branch: the reads
+// around it stay ahead of it, and fp32 prompts took 5% longer.)
+struct Decay {
+    float m, keep;   // (of a whole wave)
+    __device__ __forceinline__ Decay() : m(0.f), keep(0.f) {}
+    __device__ __forceinline__ Decay(float g, int n) {
+        const float e = g * (float)n;
+        const bool slow = !(e < -0.69f);
+        auto whole = [](float x) {
+            return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+        };
+        m = whole(slow ? expm1f(e) : expf(e));
+        keep = whole(slow ? 1.f : 0.f);
+    }
+    __device__ __forceinline__ float of(float x) const { return fmaf(x, m, keep * x); }
+};
+
 // A value that the compiler forms again in each turn of a loop: the registers that it would hold
 // over the loop are wanted for the state and the next chunk's rows (spills read back from memory
 // wait behind those rows' loads).
@@ -51,8 +69,6 @@ __device__ __forceinline__ T fresh(T x) {
     asm volatile("" : "+v"(x));
     return x;
 }
-
-__device__ __forceinline__ float clamp_g(float g) { return fmaxf(g, -1e30f); }
 
 __device__ __forceinline__ int seq_len(const LaArgs& a, int b) {
     if (!a.lengths) return a.L;
@@ -259,26 +275,26 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
             const auto d = ssm::rsrc(h0 + state, sbytes);
             each_state([&](floatx4& r, unsigned o, int left) { r = load_f4<VEC>(d, o, left); });
         }
-        const float seg_m1 = decay_m1(g, a.seglen);
+        const Decay over(g, a.seglen);
         for (int p = 0; p < seg && !a.combined; ++p) {
             const auto d = ssm::rsrc(a.seg + p * slot + state, sbytes);
             each_state([&](floatx4& r, unsigned o, int left) {
                 const floatx4 own = load_f4<VEC>(d, o, left);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = fmaf(r[e], seg_m1, r[e]) + own[e];
+                for (int e = 0; e < 4; ++e) r[e] = over.of(r[e]) + own[e];
             });
         }
     }
     __syncthreads();
 
-    float em1 = 0.f;
+    Decay decay;
     int wn = -1;
     int parity = 0;
     for (int t = t_begin; t < t_end; t += CB, parity ^= 1) {
         const int n = min(CB, t_end - t), g4 = fresh(lane_g), l16 = fresh(lane_i);
         if (wn != n) {   // (every wave is past its reads of the weights)
             wn = n;
-            em1 = decay_m1(g, n);
+            decay = Decay(g, n);
             if (tid < CB) s.wj[tid] = ssm::ex2(gl * (float)max(0, n - 1 - tid));
         }
         // ---- staging
@@ -460,7 +476,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
 #pragma unroll
             for (int x = 0; x < VW; ++x)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[kt][x][r] = fmaf(S[kt][x][r], em1, S[kt][x][r]);
+                for (int r = 0; r < 4; ++r) S[kt][x][r] = decay.of(S[kt][x][r]);
         auto update = [&](auto three) {
             constexpr int NP = decltype(three)::value ? 3 : 2, KH = KT / 2;
 #pragma unroll
@@ -633,19 +649,20 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
             const auto d = ssm::rsrc(h0 + state, sbytes);
             each_state([&](floatx4& r, unsigned o, int left) { r = load_f4<VEC>(d, o, left); });
         }
-        const float seg_m1 = decay_m1(g, a.seglen);
+        const Decay over(g, a.seglen);
         for (int p = 0; p < seg && !a.combined; ++p) {
             const auto d = ssm::rsrc(a.seg + p * slot + state, sbytes);
             each_state([&](floatx4& r, unsigned o, int left) {
                 const floatx4 own = load_f4<VEC>(d, o, left);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = fmaf(r[e], seg_m1, r[e]) + own[e];
+                for (int e = 0; e < 4; ++e) r[e] = over.of(r[e]) + own[e];
             });
         }
     }
     __syncthreads();
 
-    float wj[2][4], em1 = 0.f;
+    float wj[2][4];
+    Decay decay;
     int wn = -1;
     int parity = 0;
     for (int t = t_begin; t < t_end; t += CF, parity ^= 1) {
@@ -672,7 +689,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
         if (t + CF < t_end) fetch(t + CF);
         if (wn != n) {
             wn = n;
-            em1 = decay_m1(g, n);
+            decay = Decay(g, n);
 #pragma unroll
             for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
@@ -735,7 +752,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
 #pragma unroll
             for (int x = 0; x < VW; ++x)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[kt][x][r] = fmaf(S[kt][x][r], em1, S[kt][x][r]);
+                for (int r = 0; r < 4; ++r) S[kt][x][r] = decay.of(S[kt][x][r]);
 #pragma unroll
         for (int jt = 0; jt < 2; ++jt) {
             float vf[VW][4];
@@ -816,7 +833,9 @@ __global__ __launch_bounds__(256) void la_combine_kernel(LaArgs a) {
     const int bh = (int)(i / VK), h = bh % a.H, b = bh / a.H;
     const int len = seq_len(a, b);
     const int used = len > 0 ? (len - 1) / a.seglen + 1 : 1;   // segments that run
-    const float em1 = decay_m1(clamp_g(a.g[h]), a.seglen);
+    const float x = clamp_g(a.g[h]) * (float)a.seglen;   // (threads of a wave may be of several heads)
+    const bool slow = !(x < -0.69f);
+    const float m = slow ? expm1f(x) : expf(x), keep = slow ? 1.f : 0.f;
     float* p = a.seg + i;
     float e = a.h0 ? p[(a.nseg - 1) * slot] : 0.f;
     float own = used > 1 ? p[0] : 0.f;   // (own states are read before E takes their slot)
@@ -829,40 +848,51 @@ __global__ __launch_bounds__(256) void la_combine_kernel(LaArgs a) {
         for (int u = 0; u < U; ++u) next[u] = p[(sgm + u + 1) * slot];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            e = fmaf(e, em1, e) + own;
+            e = fmaf(e, m, keep * e) + own;
             p[(sgm + u + 1) * slot] = e;
             own = next[u];
         }
     }
     for (; sgm < used - 1; ++sgm) {
         const float next = sgm + 2 < used ? p[(sgm + 1) * slot] : 0.f;
-        e = fmaf(e, em1, e) + own;
+        e = fmaf(e, m, keep * e) + own;
         p[(sgm + 1) * slot] = e;
         own = next;
     }
 }
 
 // ---------------------------------------------------------------- plan
-int v_tile(int K, int V) { return V <= 64 || K > 128 ? 64 : 128; }
-
 // Segments: as many as fill the chip once, two workgroups a CU (one more turn for the rest costs as much
 // as a whole one: 80 sequences and heads of 4096 tokens ran 171 us in 7 segments, 144 in 6), each of
 // at least so many tokens that its states' traffic stays small beside its rows'. bf16: 512 where that
 // leaves a workgroup for every CU (128 sequences and heads of 1024: 72 -> 63 us against 256), else 256.
 // fp32 chunks take four times as long on the matrix cores: 64 (24 of 2000: 95 -> 84 us against 256).
+//
+// Columns of V a workgroup: 128, which share a chunk's q k^T and its rows of q and k (512 sequences and
+// heads of 4096 tokens: 484 us, 600 in parts of 64). 64 where V or the registers (K above 128) ask for
+// it; where whole sequences fill the chip in parts of 64 and need no state pass (256 sequences and heads
+// of 1500 tokens: 111 us, 130 in two segments of 128 columns; of 4096: 303, 307); and where the shortest
+// segments would leave CUs idle (8 of 4096: 37 us, 45).
 constexpr int kSlots = 512, kCUs = 256;
-void la_plan(int dtype, int B, int L, int H, int K, int V, int& nseg, int& seglen, int& vparts) {
+struct LaPlan { int nseg, seglen, vt, vparts; };
+LaPlan la_plan(int dtype, int B, int L, int H, int K, int V) {
     const int C = dtype == SSM_F32 ? CF : CB;
-    vparts = (int)ssm::cdiv(V, v_tile(K, V));
-    const long wgs = std::max((long)B * H * vparts, 1L), len = std::max(L, 1);
-    const long fit = std::max(kSlots / wgs, 1L), by512 = ssm::cdiv(len, 512);
-    const long most = dtype == SSM_F32 ? ssm::cdiv(len, 64) : by512 * wgs >= kCUs ? by512 : ssm::cdiv(len, 256);
+    const long heads = (long)B * H, len = std::max(L, 1), by512 = ssm::cdiv(len, 512);
+    const long half = heads * ssm::cdiv(V, 64), full = heads * ssm::cdiv(V, 128);
+    const long shortest = ssm::cdiv(len, dtype == SSM_F32 ? 64 : 256);
+    LaPlan p;
+    p.vt = V <= 64 || K > 128 || (half <= kSlots && 4 * half > 3 * kSlots) || full * shortest < kCUs ? 64 : 128;
+    p.vparts = (int)ssm::cdiv(V, p.vt);
+    const long wgs = std::max(heads * p.vparts, 1L), fit = std::max(kSlots / wgs, 1L);
+    const long most = dtype != SSM_F32 && by512 * wgs >= kCUs ? by512 : shortest;
     const long n = std::min(fit, most);
-    seglen = (int)(ssm::cdiv(ssm::cdiv(len, n), C) * C);
-    nseg = (int)std::max(1L, ssm::cdiv(L, seglen));
+    p.seglen = (int)(ssm::cdiv(ssm::cdiv(len, n), C) * C);
+    p.nseg = (int)std::max(1L, ssm::cdiv(L, p.seglen));
+    return p;
 }
 
-// A chain of more segments than this is combined once, by a pass of its own.
+// A chain of more segments than this is combined once, by a pass of its own (8 sequences of 1500 tokens, 16
+// heads, 3 segments: 94 us in a chain, 100 combined; 24 heads of 4096 tokens, 16 segments: 103 and 64).
 constexpr int kChain = 4;
 
 template <int KD, int VT, bool VEC>
@@ -890,8 +920,7 @@ ssm_status la_launch(int dtype, LaArgs a, hipStream_t st) {
 }
 
 template <bool VEC>
-ssm_status la_dispatch(int dtype, const LaArgs& a, hipStream_t st) {
-    const int vt = v_tile(a.K, a.V);
+ssm_status la_dispatch(int dtype, const LaArgs& a, int vt, hipStream_t st) {
     if (a.K > 128) return la_launch<256, 64, VEC>(dtype, a, st);
     if (a.K > 64) return vt == 64 ? la_launch<128, 64, VEC>(dtype, a, st)
                                   : la_launch<128, 128, VEC>(dtype, a, st);
@@ -901,7 +930,8 @@ ssm_status la_dispatch(int dtype, const LaArgs& a, hipStream_t st) {
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // ---------------------------------------------------------------- one token
-// S is read and written once: memory bound. 16 lanes hold a row of S (LV x 64 columns in float4
+// S is read and written once: memory bound (64 sequences of 32 heads, K = V = 128, 270 MB: 50 us, 5.4
+// TB/s), past the caches, as the next token's call comes after the layer's other work. 16 lanes hold a row of S (LV x 64 columns in float4
 // pieces, or one by one), a wave four rows, a workgroup 16 RV rows of one (sequence, head); the
 // loads of all RV rows are in flight before the first is used.
 struct LaStepArgs {
@@ -953,14 +983,14 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
     }
 #pragma unroll
     for (int r = 0; r < RV; ++r) vv[r] = (float)vp[min(v0 + 16 * r, a.V - 1)];
-    const float em1 = decay_m1(clamp_g(a.g[h]), 1);
+    const Decay decay(clamp_g(a.g[h]), 1);
     float o[RV];
 #pragma unroll
     for (int r = 0; r < RV; ++r) {
         float acc = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            s[r][e] = fmaf(vv[r], k[e], fmaf(s[r][e], em1, s[r][e]));
+            s[r][e] = fmaf(vv[r], k[e], decay.of(s[r][e]));
             acc = fmaf(s[r][e], q[e], acc);
         }
 #pragma unroll
@@ -1011,8 +1041,7 @@ void step_dispatch(const LaStepArgs& a, int rv, bool vec, unsigned n, hipStream_
 
 extern "C" size_t ssm_linear_attention_workspace(int dtype, int B, int L, int H, int K, int V) {
     if (B <= 0 || L <= 0 || H <= 0 || K <= 0 || V <= 0) return 0;
-    int nseg, seglen, vparts;
-    la_plan(dtype, B, L, H, K, V, nseg, seglen, vparts);
+    const int nseg = la_plan(dtype, B, L, H, K, V).nseg;
     return nseg > 1 ? sizeof(float) * (size_t)nseg * B * H * V * K : 0;
 }
 
@@ -1039,10 +1068,12 @@ extern "C" ssm_status ssm_linear_attention(int dtype, const void* q, long ldq, c
     a.q = q; a.ldq = ldq; a.k = k; a.ldk = ldk; a.v = v; a.ldv = ldv; a.g = g; a.scale = scale;
     a.lengths = lengths; a.y = y; a.ldy = ldy; a.B = B; a.L = L; a.H = H; a.G = G; a.K = K; a.V = V;
     a.h0 = h0; a.hT = hT;
-    la_plan(dtype, B, L, H, K, V, a.nseg, a.seglen, a.vparts);
+    const LaPlan plan = la_plan(dtype, B, L, H, K, V);
+    a.nseg = plan.nseg;
+    a.seglen = plan.seglen;
+    a.vparts = plan.vparts;
     SSM_REQUIRE((long)V * K < (1L << 29), "ssm_linear_attention: state of a head too large");
-    SSM_REQUIRE((long)a.nseg * B * H * ssm::cdiv(V, 64) < (1L << 31) &&
-                    (long)B * H * V * K < (1L << 38),
+    SSM_REQUIRE((double)a.nseg * B * H * ssm::cdiv(V, 64) <= (double)ssm::kMaxGroups,
                 "ssm_linear_attention: too many heads");
     if (a.nseg > 1) {
         const size_t need = ssm_linear_attention_workspace(dtype, B, L, H, K, V);
@@ -1051,11 +1082,17 @@ extern "C" ssm_status ssm_linear_attention(int dtype, const void* q, long ldq, c
         SSM_REQUIRE(aligned16(workspace), "ssm_linear_attention: workspace must be 16-byte aligned");
         a.seg = (float*)workspace;
     }
+    const long rows = (long)B * L;
+    auto meets = [&](const void* x, long ldx, long wide) {
+        return ssm::rows_meet(x, ldx * esz, wide * esz, y, ldy * esz, (long)H * V * esz, rows);
+    };
+    SSM_REQUIRE(!meets(q, ldq, (long)H * K) && !meets(k, ldk, (long)G * K) && !meets(v, ldv, (long)G * V),
+                "ssm_linear_attention: y overlaps an input");
     const bool vec = K % ev == 0 && V % ev == 0 && (ldq | ldk | ldv | ldy) % ev == 0 &&
                      aligned16(q) && aligned16(k) && aligned16(v) && aligned16(y) &&
                      aligned16(h0) && aligned16(hT);
-    return vec ? la_dispatch<true>(dtype, a, (hipStream_t)stream)
-               : la_dispatch<false>(dtype, a, (hipStream_t)stream);
+    return vec ? la_dispatch<true>(dtype, a, plan.vt, (hipStream_t)stream)
+               : la_dispatch<false>(dtype, a, plan.vt, (hipStream_t)stream);
 }
 
 extern "C" ssm_status ssm_linear_attention_step(int dtype, const void* q, long ldq, const void* k,
@@ -1073,11 +1110,18 @@ extern "C" ssm_status ssm_linear_attention_step(int dtype, const void* q, long l
                            ldy >= (long)H * V),
                 "ssm_linear_attention_step: row stride below row width");
     LaStepArgs a{q, ldq, k, ldk, v, ldv, g, scale, y, ldy, H, G, K, V, 0, h};
-    // four rows a lane group where that still leaves two workgroups a CU
-    const int rv = (long)B * H * ssm::cdiv(V, 64) >= 512 ? 4 : 1;
+    // four rows a lane group where that still leaves a workgroup for every CU (K = V = 128: 64 sequences of
+    // 32 heads 50 us, 68 with one row; one of 12 heads 3.8 us with one, 4.5 with four)
+    const int rv = (long)B * H * ssm::cdiv(V, 64) >= 256 ? 4 : 1;
     a.blocks = (int)ssm::cdiv(V, 16 * rv);
     const long n = (long)B * H * a.blocks;
-    SSM_REQUIRE(n < (1L << 31), "ssm_linear_attention_step: too many heads");
+    SSM_REQUIRE(n <= ssm::kMaxGroups, "ssm_linear_attention_step: too many heads");
+    const long es = dtype == SSM_F32 ? 4 : 2;
+    auto meets = [&](const void* x, long ldx, long wide) {
+        return ssm::rows_meet(x, ldx * es, wide * es, y, ldy * es, (long)H * V * es, B);
+    };
+    SSM_REQUIRE(!meets(q, ldq, (long)H * K) && !meets(k, ldk, (long)G * K) && !meets(v, ldv, (long)G * V),
+                "ssm_linear_attention_step: y overlaps an input");
     const bool vec = K % 4 == 0 && aligned16(h);
     if (dtype == SSM_F32) step_dispatch<float>(a, rv, vec, (unsigned)n, (hipStream_t)stream);
     else step_dispatch<__bf16>(a, rv, vec, (unsigned)n, (hipStream_t)stream);

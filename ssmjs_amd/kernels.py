@@ -368,7 +368,9 @@ def _own_scratch(workspace, nbytes, t):
     if workspace is not None:
         if not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
-        return workspace, _p(workspace), workspace.numel() * workspace.element_size()
+        if workspace.get_device() != t.get_device():
+            raise ValueError(f"workspace: expected a tensor on {t.device}, got {workspace.device}")
+        return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
     if nbytes == 0:
         return None, None, 0
     ws = t.new_empty(nbytes, dtype=torch.uint8)

@@ -152,3 +152,23 @@ def test_views_and_alignment(M):
         torch.cuda.synchronize()
         assert torch.equal(got, want)
         assert (wide[:, :3] == 5).all() and (wide[:, 3 + N:] == 5).all()
+
+
+@pytest.mark.parametrize("M,K", [(1, 1024), (4, 2048), (9, 512), (200, 256)])
+def test_output_over_the_input(M, K):
+    """y written over x: bit-equal to a call with an output of its own."""
+    print(f"[case] linear_q8 in place {M} x {K}", flush=True)
+    from ssmjs_amd import kernels
+    x = data(M, K, torch.float32, M)
+    W, sw = kernels.quantize_rows(data(K, K, torch.float32, M + 1))
+    y = kernels.linear_q8(x, W, sw)
+    for beta in (0.0, 0.5):
+        mine = x.clone()
+        ref = x.clone()
+        kernels.linear_q8(x, W, sw, out=ref, beta=beta)
+        kernels.linear_q8(mine, W, sw, out=mine, beta=beta)
+        torch.cuda.synchronize()
+        assert torch.equal(mine, ref), beta
+    kernels.linear_q8(x, W, sw, out=x)
+    torch.cuda.synchronize()
+    assert torch.equal(x, y)

@@ -71,6 +71,8 @@ CASES = [   # B, L, H, G, K, V
     (1, 65, 2, 1, 128, 128), (2, 130, 4, 2, 128, 64), (1, 96, 2, 2, 64, 128), (1, 200, 2, 1, 96, 96),
     (1, 77, 2, 1, 256, 64), (1, 70, 1, 1, 200, 136), (1, 130, 2, 2, 33, 17), (1, 67, 1, 1, 129, 65),
     (1, 100, 2, 1, 32, 260), (1, 700, 2, 2, 128, 128), (3, 1100, 1, 1, 64, 64), (1, 2050, 2, 1, 128, 128),
+    # enough heads for 128 columns a workgroup: whole sequences, segments in a chain, odd widths
+    (75, 70, 4, 2, 128, 128), (75, 40, 4, 1, 60, 136), (4, 2050, 16, 4, 128, 128), (5, 1030, 6, 2, 64, 128),
 ]
 
 
@@ -91,14 +93,14 @@ def test_matches_recurrence(B, L, H, G, K, V, dtype, state):
     close(hT, ref[1], bh, "state")
 
 
-@pytest.mark.parametrize("K,V,G", [(128, 128, 1), (64, 64, 2), (40, 72, 1), (33, 17, 2)])
+@pytest.mark.parametrize("K,V,G,H", [(128, 128, 1, 2), (64, 64, 2, 2), (40, 72, 1, 2), (33, 17, 2, 2), (128, 128, 7, 14)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_lengths(K, V, G, dtype):
+def test_lengths(K, V, G, H, dtype):
     """Padded batches: what lies behind a sequence is neither used (NaN there) nor written."""
-    print(f"[case] linear_attention lengths K={K} V={V} {dtype}", flush=True)
+    print(f"[case] linear_attention lengths K={K} V={V} H={H} {dtype}", flush=True)
     from ssmjs_amd import kernels
     n = [0, 1, 63, 64, 65, 255, 256, 257, 600, 2000]
-    B, L, H = len(n), 600, 2
+    B, L = len(n), 600
     q, k, v, g, h0 = make(B, L, H, G, K, V, dtype, 3)
     lengths = torch.tensor(n, dtype=torch.int32, device="cuda")
     n = [min(m, L) for m in n]   # held to 0 .. L
@@ -155,11 +157,12 @@ def test_extreme_decays(dtype):
 @pytest.mark.parametrize("where", ["q", "k", "v"])
 @pytest.mark.parametrize("value", [float("inf"), float("nan")])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_odd_values_are_causal(where, value, dtype):
+@pytest.mark.parametrize("B", [1, 150])   # (64 columns a workgroup, and 128)
+def test_odd_values_are_causal(where, value, dtype, B):
     """An inf or NaN at token 150 of one head changes no earlier token, and no other head."""
     print(f"[case] linear_attention {value} in {where} {dtype}", flush=True)
     from ssmjs_amd import kernels
-    q, k, v, g, _ = make(1, 300, 2, 2, 128, 128, dtype, 4)
+    q, k, v, g, _ = make(B, 300, 2, 2, 128, 128, dtype, 4)
     clean = kernels.linear_attention(q, k, v, g)
     {"q": q, "k": k, "v": v}[where][0, 150, 1, 70] = value
     y = kernels.linear_attention(q, k, v, g)
@@ -221,3 +224,44 @@ def test_step(B, H, G, K, V, dtype):
     b = units * ref[2][:, 0] + (2.0 ** -8 * ref[0][:, 0].abs() if dtype == torch.bfloat16 else 0)
     close(y, ref[0][:, 0], b, "y")
     close(h, ref[1], units * ref[3], "state")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_nan_decay_shows(dtype):
+    """A NaN decay makes its own head's results NaN and no other's."""
+    print(f"[case] NaN decay {dtype}", flush=True)
+    from ssmjs_amd import kernels
+    q, k, v, g, h0 = make(2, 70, 3, 1, 64, 64, dtype, 5)
+    g[1] = float("nan")
+    hT = torch.empty_like(h0)
+    y = kernels.linear_attention(q, k, v, g, h0=h0, hT=hT)
+    h = h0.clone()
+    y1 = kernels.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, h)
+    torch.cuda.synchronize()
+    for t, heads in ((y, 2), (y1, 1)):
+        assert t.select(heads, 1).isnan().all()
+        assert torch.isfinite(t.index_select(heads, torch.tensor([0, 2], device="cuda"))).all()
+    for s in (hT, h):
+        assert s[:, 1].isnan().all() and torch.isfinite(s[:, [0, 2]]).all()
+
+
+@pytest.mark.parametrize("L,g", [(1, -12.0), (2, -9.0), (5, -1.0), (40, -0.6), (600, -0.05), (2000, -0.02), (700, -1e-6)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_what_a_decay_leaves(L, g, dtype):
+    """With no values the state is e^{g L} h0, to within the roundings of each chunk's and segment's decay
+    (its exponent's, relative to it, and four of 2^-24: the function's two, a sum, a product)."""
+    print(f"[case] linear_attention decay of a state L={L} g={g} {dtype}", flush=True)
+    from ssmjs_amd import kernels
+    q, k, v, _, h0 = make(1, L, 2, 1, 64, 64, dtype, 1)
+    v = torch.zeros_like(v)
+    gs = torch.full((2,), g, device="cuda")
+    hT = torch.empty_like(h0)
+    kernels.linear_attention(q, k, v, gs, h0=h0, hT=hT)
+    h = h0.clone()
+    kernels.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], gs, h)
+    torch.cuda.synchronize()
+    g = gs.double()[0]
+    for got, n in ((hT, L), (h, 1)):
+        ref = h0.double() * torch.exp(g * n)
+        units = float(g.abs()) * n + 4 * (-(-n // 32) + 32)   # (at most 32 segments)
+        close(got, ref, units * 2.0 ** -24 * ref.abs(), f"state after {n}")

@@ -163,3 +163,42 @@ def test_python_checks():
     assert k._head_rows("q", z(2, 4, 6, 8)[:, :, 2:5]) == 48
     assert k._head_rows("q", z(3, 1, 6, 8)[:, :, 2:5]) == 48
     assert k._head_rows("q", z(3, 6, 8)[:, :2]) == 48
+
+
+def refused(status, word):
+    assert status == INVALID and word in _lib.lib().ssm_last_error(), _lib.lib().ssm_last_error()
+
+
+def test_overlapping_outputs_are_refused():
+    """An output may be the input it is made of where that is said, and lie between the columns of
+    another tensor's rows; else it shares no memory with an input. (Each call ends at these checks.)"""
+    far = 1 << 30
+    o = b"overlaps"
+    # four rows of 4 x 64 queries (1024 bytes) and 2 x 64 keys
+    a = dict(T=4, q=P, k=far, qo=2 * far, ko=3 * far)
+    refused(rope(**a | dict(qo=P + 4)), o)
+    refused(rope(**a | dict(qo=P, ldqo=260)), o)
+    refused(rope(**a | dict(ko=P + 3 * 1024 + 1020)), o)
+    refused(rope(**a | dict(qo=far - 4)), o)
+    refused(rope(**a | dict(ko=2 * far + 512)), o)
+    # rows of 384 elements that hold queries, keys: keys written into the queries' last column
+    refused(rope(**a | dict(ldq=384, ldko=384, ko=P + 255 * 4)), o)
+    b = dict(q=P, k=far, v=2 * far, y=3 * far, g=P)
+    for name, at in (("q", P), ("k", far), ("v", 2 * far)):
+        refused(attention(**b | dict(y=at)), o)
+        refused(attention(**b | dict(y=at + 511)), o)
+        refused(step(**b | dict(y=at)), o)
+    refused(attention(**b | dict(ldq=1024, ldy=1024, y=P + 1000)), o)   # (the last of a row of q)
+    refused(_lib.lib().ssm_quantize_rows(F32, P, 8, P + 60, 8, far, 2, 8, None), o)
+    need = _lib.lib().ssm_linear_i8_workspace(P, 256, far, 256, 2, 64, 256)
+    refused(i8(W=far, sw=far, sx=far, y=P + 252, ws=far, nws=need), o)
+
+
+def test_more_rows_than_a_launch_counts_are_refused():
+    n = 1 << 24
+    far = 1 << 45
+    refused(_lib.lib().ssm_quantize_rows(F32, P, 8, far, 8, P, n, 8, None), b"too many rows")
+    refused(i8(M=n, y=far), b"too many rows")
+    refused(q8(N=n, ldy=1 << 20), b"row stride")
+    refused(attention(B=n, H=1, G=1, L=1), b"too many heads")
+    refused(step(B=n, H=1, G=1, V=16, K=1), b"too many heads")
