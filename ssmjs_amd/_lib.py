@@ -181,4 +181,6 @@ def check(status: int, what: str = "") -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args), name)
+    status = getattr(_lib or lib(), name)(*args)
+    if status != SSM_OK:
+        check(status, name)

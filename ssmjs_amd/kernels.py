@@ -342,14 +342,19 @@ def qk_norm_rope(q, k, wq, wk, positions, freqs, eps=1e-6, interleaved=False, ou
     T = rows[0] if len(rows) == 1 else rows[0] * rows[1]
     R = 2 * freqs.shape[0] if freqs is not None else 0
     pk = _at("k", k, (*rows, G, D), dt, dev)
+    dense = q.is_contiguous() and k.is_contiguous()
+    ldq, ldk = (H * D, G * D) if dense else (_head_rows("q", q), _head_rows("k", k))
     if out is None:
-        qo, ko = q.new_empty(shape), k.new_empty(kshape)
+        if dense:
+            qo, ko = torch.empty_like(q), torch.empty_like(k)
+        else:
+            qo, ko = q.new_empty(shape), k.new_empty(kshape)
         pqo, pko, ldqo, ldko = qo.data_ptr(), ko.data_ptr(), H * D, G * D
     else:
         qo, ko = out
         pqo, pko = _at("out[0]", qo, shape, dt, dev), _at("out[1]", ko, kshape, dt, dev)
         ldqo, ldko = _head_rows("out[0]", qo), _head_rows("out[1]", ko)
-    _lib.call("ssm_qk_norm_rope", code, q.data_ptr(), _head_rows("q", q), pk, _head_rows("k", k),
+    _lib.call("ssm_qk_norm_rope", code, q.data_ptr(), ldq, pk, ldk,
               _packed("wq", wq, (D,), _f32_t, dev), _packed("wk", wk, (D,), _f32_t, dev),
               _packed("positions", positions, tuple(rows), _i32_t, dev),
               _packed("freqs", freqs, (R // 2,), _f64_t, dev), int(interleaved), eps, pqo, ldqo, pko,
@@ -418,12 +423,17 @@ def linear_attention_step(q, k, v, g, h, scale=1.0, out=None):
     ph = _packed("h", h, (B, H, V, K), _f32_t, dev)
     if ph is None:
         raise ValueError("linear_attention_step needs a state")
+    if q.is_contiguous() and k.is_contiguous() and v.is_contiguous():
+        ldq, ldk, ldv = H * K, G * K, G * V
+    else:
+        ldq, ldk, ldv = _head_rows("q", q), _head_rows("k", k), _head_rows("v", v)
     if out is None:
         out = q.new_empty((B, H, V))
-    py = _at("out", out, (B, H, V), dt, dev)
-    _lib.call("ssm_linear_attention_step", code, q.data_ptr(), _head_rows("q", q), pk,
-              _head_rows("k", k), pv, _head_rows("v", v), _packed("g", g, (H,), _f32_t, dev), scale,
-              py, _head_rows("out", out), ph, B, H, G, K, V,
+        py, ldy = out.data_ptr(), H * V
+    else:
+        py, ldy = _at("out", out, (B, H, V), dt, dev), _head_rows("out", out)
+    _lib.call("ssm_linear_attention_step", code, q.data_ptr(), ldq, pk, ldk, pv, ldv,
+              _packed("g", g, (H,), _f32_t, dev), scale, py, ldy, ph, B, H, G, K, V,
               _raw_stream(dev) if _raw_stream is not None else _stream())
     return out
 
