@@ -37,7 +37,7 @@ struct LaArgs {
     const float* h0;         // (B,H,V,K) or null
     float* hT;               // (B,H,V,K) or null
     float* seg;              // (nseg,B,H,V,K): the segments' own states (the last slot: h0), or,
-    int nseg, seglen, vparts;   // combined, the states that enter them
+    int nseg, seglen, vparts, share;   // combined, the states that enter them
     int combined;
 };
 
@@ -75,11 +75,28 @@ __device__ __forceinline__ int seq_len(const LaArgs& a, int b) {
     return max(0, min(a.lengths[b], a.L));
 }
 
-// Workgroup order: consecutive ids (the parts of V and the heads of a group, which read the same
-// keys and values) on one XCD.
-__device__ __forceinline__ int xcd_order(int b, int T) {
-    const int xcd = b & 7, per = T >> 3, rem = T & 7;
-    return xcd * per + min(xcd, rem) + (b >> 3);
+// Workgroup order: those that read the same keys and values (the parts of V and the heads of a group) on one
+// XCD, the groups, then the sequences and segments, dealt out over the XCDs: a padded batch's long
+// sequences are then shared by all of them (8 sequences of up to 1500 tokens, 32 heads: 112 -> 84 us against
+// a range of ids an XCD). Few groups would leave XCDs idle: then single heads are dealt out.
+struct Place {
+    int part, h, grp, b, seg;   // seg past the last: none
+    __device__ __forceinline__ explicit Place(const LaArgs& a) {
+        const int per = a.share * a.vparts, local = blockIdx.x >> 3, units = a.H / a.share;
+        const int unit = local / per * 8 + (blockIdx.x & 7), in = local % per;
+        part = in % a.vparts;
+        h = unit % units * a.share + in / a.vparts;
+        grp = h / (a.H / a.G);
+        b = unit / units % a.B;
+        seg = unit / units / a.B;
+    }
+};
+
+// The workgroups of a launch over so many segments, and the heads that are dealt out together.
+inline unsigned la_groups(LaArgs& a, int segments) {
+    const long groups = (long)segments * a.B * a.G;
+    a.share = groups % 8 == 0 || groups >= 64 ? a.H / a.G : 1;
+    return (unsigned)(8 * ssm::cdiv((long)segments * a.B * (a.H / a.share), 8) * a.share * a.vparts);
 }
 
 // ---------------------------------------------------------------- bf16
@@ -183,10 +200,9 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
     constexpr int NK = CB * KD / 8 / 256, NV = CB * VT / 8 / 256;
     __shared__ Smem s;
 
-    const int id = xcd_order(blockIdx.x, gridDim.x);
-    const int part = id % a.vparts, bh_s = id / a.vparts;
-    const int h = bh_s % a.H, b = bh_s / a.H % a.B, seg = bh_s / a.H / a.B;
-    const int grp = h / (a.H / a.G);
+    const Place place(a);
+    const int part = place.part, h = place.h, grp = place.grp, b = place.b, seg = place.seg;
+    if (seg >= a.nseg - STATE) return;
     const int len = seq_len(a, b);
     const int t_begin = seg * a.seglen, t_end = min(len, t_begin + a.seglen);
     // the segment that ends the sequence writes the final state (segment 0 of an empty one)
@@ -564,10 +580,9 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
     constexpr int NK = CF * KD / 4 / 256, NV = CF * VT / 4 / 256;
     __shared__ Smem s;
 
-    const int id = xcd_order(blockIdx.x, gridDim.x);
-    const int part = id % a.vparts, bh_s = id / a.vparts;
-    const int h = bh_s % a.H, b = bh_s / a.H % a.B, seg = bh_s / a.H / a.B;
-    const int grp = h / (a.H / a.G);
+    const Place place(a);
+    const int part = place.part, h = place.h, grp = place.grp, b = place.b, seg = place.seg;
+    if (seg >= a.nseg - STATE) return;
     const int len = seq_len(a, b);
     const int t_begin = seg * a.seglen, t_end = min(len, t_begin + a.seglen);
     const bool last = seg == (len > 0 ? (len - 1) / a.seglen : 0);
@@ -897,13 +912,12 @@ constexpr int kChain = 4;
 
 template <int KD, int VT, bool VEC>
 ssm_status la_launch(int dtype, LaArgs a, hipStream_t st) {
-    const unsigned n = (unsigned)((long)a.nseg * a.B * a.H * a.vparts);
     if (a.nseg > 1) {
         // 64 columns a workgroup, whatever the full pass takes: half the registers, so that more of
         // them share a CU
         LaArgs s = a;
         s.vparts = (int)ssm::cdiv(a.V, 64);
-        const unsigned n1 = (unsigned)((long)(a.nseg - 1) * a.B * a.H * s.vparts);
+        const unsigned n1 = la_groups(s, a.nseg - 1);
         if (dtype == SSM_F32) la_f32_kernel<KD, 64, VEC, true><<<n1, 256, 0, st>>>(s);
         else la_bf16_kernel<KD, 64, VEC, true><<<n1, 256, 0, st>>>(s);
         if (ssm_status e = ssm::check_launch("ssm_linear_attention (states)")) return e;
@@ -914,6 +928,7 @@ ssm_status la_launch(int dtype, LaArgs a, hipStream_t st) {
             if (ssm_status e = ssm::check_launch("ssm_linear_attention (combine)")) return e;
         }
     }
+    const unsigned n = la_groups(a, a.nseg);
     if (dtype == SSM_F32) la_f32_kernel<KD, VT, VEC, false><<<n, 256, 0, st>>>(a);
     else la_bf16_kernel<KD, VT, VEC, false><<<n, 256, 0, st>>>(a);
     return ssm::check_launch("ssm_linear_attention");
@@ -1073,7 +1088,7 @@ extern "C" ssm_status ssm_linear_attention(int dtype, const void* q, long ldq, c
     a.seglen = plan.seglen;
     a.vparts = plan.vparts;
     SSM_REQUIRE((long)V * K < (1L << 29), "ssm_linear_attention: state of a head too large");
-    SSM_REQUIRE((double)a.nseg * B * H * ssm::cdiv(V, 64) <= (double)ssm::kMaxGroups,
+    SSM_REQUIRE(((double)a.nseg * B + 7) * H * ssm::cdiv(V, 64) <= (double)ssm::kMaxGroups,
                 "ssm_linear_attention: too many heads");
     if (a.nseg > 1) {
         const size_t need = ssm_linear_attention_workspace(dtype, B, L, H, K, V);
