@@ -6,7 +6,7 @@
 //
 // Three kernels share the work by rows:
 //   - up to 64 rows (one per decoded sequence): the weights' bytes bound it. i8_rows_kernel reads
-//     every weight row once, straight into registers, the k of a row shared by the four waves.
+//     every weight row once, straight into registers, the k of a row shared by its waves.
 //   - more rows: the matrix cores bound it. i8_gemm_kernel is a tiled product out of LDS.
 //   - rows that are not 16-byte aligned are laid out in the workspace first (lay_rows_kernel).
 #include <algorithm>
@@ -351,8 +351,8 @@ __device__ __forceinline__ intx4 mfma8(intx4 w, intx4 x, intx4 c) {
 }
 
 // ---------------------------------------------------------------- up to 64 rows
-// A workgroup owns 16 output channels; its four waves take the blocks of 256 k in turn, two blocks'
-// weights in flight a wave. Lane (g, i) = (lane / 16, lane % 16) reads W row i's bytes 64 g + 16 u .. of the block for
+// A workgroup owns 16 output channels; its NW waves take the blocks of 256 k in turn, two blocks' weights in
+// flight a wave. Lane (g, i) = (lane / 16, lane % 16) reads W row i's bytes 64 g + 16 u .. of the block for
 // u = 0 .. 3, which is the operand of MFMA u with the block's k in another order, the same for x. So a
 // lane reads 64 consecutive bytes of its row, and x lies in the workspace in the operands' own order (a
 // row-major x took 3 times as long at 64 rows: 16 lines an instruction). The waves' sums meet in
@@ -363,11 +363,12 @@ __device__ __forceinline__ intx4 mfma8(intx4 w, intx4 x, intx4 c) {
 // one row 6.0 us, 8.5 in two launches; two rows 7.3, 8.3; four rows, past kFusedX, would take 10.4).
 constexpr int kFusedX = 4096, kFusedRows = 4;
 
-template <int MB, typename TX, typename TO, bool BETA>
-__global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
+template <int MB, typename TX, typename TO, bool BETA, int NW>
+__global__ __launch_bounds__(64 * NW) void i8_rows_kernel(I8Args a) {
     constexpr bool FUSED = !std::is_void<TX>::value;
+    static_assert(!FUSED || NW == 4, "256 threads round x");
     constexpr int kPieces = kFusedX / 1024;
-    __shared__ intx4 red[4][MB][64];
+    __shared__ intx4 red[NW][MB][64];
     __shared__ __attribute__((aligned(16))) signed char xs[FUSED ? kFusedX + kFusedRows * kPad : 16];
     __shared__ unsigned most[FUSED ? 4 : 1][kPieces];
     const int lane = threadIdx.x & 63;
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
         for (int p = 0; p < kPieces; ++p)
             if (p < pieces) v[p] = some4<TX, true>(static_cast<const TX*>(a.Xf) + (long)row(p) * a.ldxf, col(p), a.K);
         fetch(wv[0], w);   // (behind x: loads come back in order)
-        fetch(wv[1], w + 4);
+        fetch(wv[1], w + NW);
 #pragma unroll
         for (int p = 0; p < kPieces; ++p)
             if (p < pieces) {
@@ -424,7 +425,7 @@ __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
         __syncthreads();
     } else {
         fetch(wv[0], w);
-        fetch(wv[1], w + 4);
+        fetch(wv[1], w + NW);
 #pragma unroll
         for (int m = 0; m < MB; ++m) sm[m] = a.sx[min(16 * m + i, a.M - 1)];
     }
@@ -447,11 +448,11 @@ __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
 #pragma unroll
             for (int m = 0; m < MB; ++m) acc[m] = mfma8(v[u], x[m][u], acc[m]);
     };
-    for (int s = w; s < steps; s += 8) {
+    for (int s = w; s < steps; s += 2 * NW) {
         step(wv[0], s);
-        fetch(wv[0], s + 8);
-        step(wv[1], s + 4);
-        fetch(wv[1], s + 12);
+        fetch(wv[0], s + 2 * NW);
+        step(wv[1], s + NW);
+        fetch(wv[1], s + 3 * NW);
     }
 #pragma unroll
     for (int m = 0; m < MB; ++m) red[w][m][lane] = acc[m];
@@ -462,7 +463,9 @@ __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
     for (int t = 0; t < MB; ++t) {
         if (t != w) continue;
         const int n = 4 * g, row = 16 * t + i;
-        const intx4 c = red[0][t][lane] + red[1][t][lane] + red[2][t][lane] + red[3][t][lane];
+        intx4 c = red[0][t][lane];
+#pragma unroll
+        for (int o = 1; o < NW; ++o) c += red[o][t][lane];
         float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -785,11 +788,19 @@ __global__ __launch_bounds__(256, 1) void i8_gemm_big_kernel(I8Args a) {
 }
 
 // ---------------------------------------------------------------- plan
-template <int MB, typename TX, typename TO>
+template <int MB, typename TX, typename TO, int NW>
 void rows_launch(const I8Args& a, hipStream_t st) {
     const unsigned n = (unsigned)ssm::cdiv(a.N, 16);
-    if (a.beta != 0.f) i8_rows_kernel<MB, TX, TO, true><<<n, 256, 0, st>>>(a);
-    else i8_rows_kernel<MB, TX, TO, false><<<n, 256, 0, st>>>(a);
+    if (a.beta != 0.f) i8_rows_kernel<MB, TX, TO, true, NW><<<n, 64 * NW, 0, st>>>(a);
+    else i8_rows_kernel<MB, TX, TO, false, NW><<<n, 64 * NW, 0, st>>>(a);
+}
+
+// Eight waves a workgroup where there is at most one a CU (rounding and product of 64 rows, N 2048, K 4096: 11.2
+// us, 13.1 with four; N 6144: 15.0, 14.7).
+template <int MB, typename TO>
+void rows_of(const I8Args& a, hipStream_t st) {
+    if (a.N <= 16 * kCUs) rows_launch<MB, void, TO, 8>(a, st);
+    else rows_launch<MB, void, TO, 4>(a, st);
 }
 
 template <int TM, typename TO>
@@ -823,11 +834,11 @@ void gemm_launch(I8Args a, hipStream_t st) {
 
 template <typename TO>
 ssm_status product(const I8Args& a, hipStream_t st) {
-    if (a.Xf && a.x_dtype == SSM_F32) rows_launch<1, float, TO>(a, st);
-    else if (a.Xf) rows_launch<1, __bf16, TO>(a, st);
-    else if (a.M <= 16) rows_launch<1, void, TO>(a, st);
-    else if (a.M <= 32) rows_launch<2, void, TO>(a, st);
-    else if (a.M <= kRowsMax) rows_launch<4, void, TO>(a, st);
+    if (a.Xf && a.x_dtype == SSM_F32) rows_launch<1, float, TO, 4>(a, st);
+    else if (a.Xf) rows_launch<1, __bf16, TO, 4>(a, st);
+    else if (a.M <= 16) rows_of<1, TO>(a, st);
+    else if (a.M <= 32) rows_of<2, TO>(a, st);
+    else if (a.M <= kRowsMax) rows_of<4, TO>(a, st);
     else gemm_launch<TO>(a, st);
     return ssm::check_launch("ssm_linear_i8");
 }

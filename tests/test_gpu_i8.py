@@ -88,7 +88,8 @@ def product(q, s, W, sw, bias, beta, y0):
 SHAPES = [   # M, N, K
     (1, 1, 1), (1, 8512, 2048), (2, 17, 64), (16, 100, 256), (17, 33, 300), (33, 4384, 1024), (64, 257, 512),
     (64, 96, 4096), (65, 100, 200), (100, 256, 1000), (127, 513, 768), (200, 130, 999), (300, 1028, 128),
-    (1000, 600, 1536), (4200, 4100, 512), (3, 40, 131071), (70, 40, 131071),
+    (1000, 600, 1536), (4200, 4100, 512), (3, 40, 131071), (70, 40, 131071), (9, 4112, 700), (20, 4100, 2600),
+    (2, 4200, 5000),
 ]
 
 
