@@ -106,6 +106,11 @@ inline unsigned la_groups(LaArgs& a, int segments) {
 // the block taken in the order (16 t + 4 g + r, 16 (t + 1) + 4 g + r); q is read from LDS in that
 // order. The 64 x 64 products q k^T are shared out over the waves by rows i and go through LDS.
 //
+// 8 sequences of 4096 tokens, 16 heads, K = V = 128: the state pass takes 57 us (268 MB, 4.7 TB/s), the full
+// pass 140, of which its loads and stores alone are 120: it is bound by memory and by the three barriers a
+// chunk, between which two waves a SIMD cannot keep the matrix cores fed (a third of their time). Eight
+// waves of 16 columns read S q's queries twice as often: 190 us.
+//
 // Roundings to bf16: none that a result keeps. S as an operand of its product with q and the products
 // q k^T enter in two parts (16 bits; 2.5% of the time at 8 sequences of 4096 tokens), and the values of
 // the state update, e^{..} v, in two or three, so that the final state carries fp32 rounding only.
@@ -556,7 +561,9 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
 // and sum in fp32. Chunks of 32: the quadratic part shrinks with the chunk, and a chunk costs
 // nothing else, as S stays in the accumulators. MFMA r of a 16-k block takes k = 4 (lane / 16) + r
 // from every lane, so that S and the products q k^T are read as they lie in the accumulators and
-// q and k as 16-byte pieces.
+// q and k as 16-byte pieces. Bound by the matrix cores: 8 sequences of 4096 tokens, 16 heads, K = V = 128 take
+// 513 us, 105 TFLOP/s of the 154 that a large product reaches (5.5 K V + 48 (K + V) operations a token, the
+// state pass's among them).
 constexpr int CF = 32;
 
 template <int KD, int VT, bool STATE>
@@ -855,24 +862,18 @@ __global__ __launch_bounds__(256) void la_combine_kernel(LaArgs a) {
     float e = a.h0 ? p[(a.nseg - 1) * slot] : 0.f;
     float own = used > 1 ? p[0] : 0.f;   // (own states are read before E takes their slot)
     if (a.h0) p[0] = e;
-    constexpr int U = 8;
-    int sgm = 0;
-    for (; sgm + U < used - 1; sgm += U) {
+    constexpr int U = 8;   // loads in flight (16 and 32: 2% of the whole longer)
+    for (int sgm = 0; sgm < used - 1; sgm += U) {
         float next[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) next[u] = p[(sgm + u + 1) * slot];
+        for (int u = 0; u < U; ++u) next[u] = sgm + u + 2 < used ? p[(sgm + u + 1) * slot] : 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            if (sgm + u + 1 >= used) break;
             e = fmaf(e, m, keep * e) + own;
             p[(sgm + u + 1) * slot] = e;
             own = next[u];
         }
-    }
-    for (; sgm < used - 1; ++sgm) {
-        const float next = sgm + 2 < used ? p[(sgm + 1) * slot] : 0.f;
-        e = fmaf(e, m, keep * e) + own;
-        p[(sgm + 1) * slot] = e;
-        own = next;
     }
 }
 
