@@ -72,7 +72,7 @@ CASES = [   # B, L, H, G, K, V
     (1, 77, 2, 1, 256, 64), (1, 70, 1, 1, 200, 136), (1, 130, 2, 2, 33, 17), (1, 67, 1, 1, 129, 65),
     (1, 100, 2, 1, 32, 260), (1, 700, 2, 2, 128, 128), (3, 1100, 1, 1, 64, 64), (1, 2050, 2, 1, 128, 128),
     # enough heads for 128 columns a workgroup: whole sequences, segments in a chain, odd widths
-    (75, 70, 4, 2, 128, 128), (75, 40, 4, 1, 60, 136), (4, 2050, 16, 4, 128, 128), (5, 1030, 6, 2, 64, 128),
+    (75, 70, 4, 2, 128, 128), (75, 70, 4, 2, 64, 128), (75, 40, 4, 1, 60, 136), (4, 2050, 16, 4, 128, 128), (5, 1030, 6, 2, 64, 128),
 ]
 
 
