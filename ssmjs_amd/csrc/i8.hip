@@ -429,9 +429,8 @@ __global__ __launch_bounds__(64 * NW) void i8_rows_kernel(I8Args a) {
 #pragma unroll
         for (int m = 0; m < MB; ++m) sm[m] = a.sx[min(16 * m + i, a.M - 1)];
     }
-    auto step = [&](const intx4 (&v)[4], int s) {
+    auto operands = [&](intx4 (&x)[MB][4], int s) {
         if (s >= steps) return;
-        intx4 x[MB][4];
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -443,16 +442,40 @@ __global__ __launch_bounds__(64 * NW) void i8_rows_kernel(I8Args a) {
                     x[m][u] = *reinterpret_cast<const intx4*>(a.X + ((long)m * steps + s) * 4096 + u * 1024 + lane * 16);
                 }
             }
+    };
+    auto step = [&](const intx4 (&v)[4], const intx4 (&x)[MB][4], int s) {
+        if (s >= steps) return;
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int m = 0; m < MB; ++m) acc[m] = mfma8(v[u], x[m][u], acc[m]);
     };
-    for (int s = w; s < steps; s += 2 * NW) {
-        step(wv[0], s);
-        fetch(wv[0], s + 2 * NW);
-        step(wv[1], s + NW);
-        fetch(wv[1], s + 3 * NW);
+    // (one workgroup a CU: x's operands a block ahead, too; 64 x 2048 x 4096 11.3 -> 10.3 us. With more of them
+    // the registers cost as much: 48 x 8512 x 2048 11.4 -> 11.6.)
+    if constexpr (NW == 8) {
+        intx4 xv[2][MB][4];
+        operands(xv[0], w);
+        for (int s = w; s < steps; s += 2 * NW) {
+            operands(xv[1], s + NW);
+            step(wv[0], xv[0], s);
+            fetch(wv[0], s + 2 * NW);
+            operands(xv[0], s + 2 * NW);
+            step(wv[1], xv[1], s + NW);
+            fetch(wv[1], s + 3 * NW);
+        }
+    } else {
+        auto both = [&](const intx4 (&v)[4], int s) {
+            if (s >= steps) return;
+            intx4 x[MB][4];
+            operands(x, s);
+            step(v, x, s);
+        };
+        for (int s = w; s < steps; s += 2 * NW) {
+            both(wv[0], s);
+            fetch(wv[0], s + 2 * NW);
+            both(wv[1], s + NW);
+            fetch(wv[1], s + 3 * NW);
+        }
     }
 #pragma unroll
     for (int m = 0; m < MB; ++m) red[w][m][lane] = acc[m];
@@ -795,7 +818,7 @@ void rows_launch(const I8Args& a, hipStream_t st) {
     else i8_rows_kernel<MB, TX, TO, false, NW><<<n, 64 * NW, 0, st>>>(a);
 }
 
-// Eight waves a workgroup where there is at most one a CU (rounding and product of 64 rows, N 2048, K 4096: 11.2
+// Eight waves a workgroup where there is at most one a CU (rounding and product of 64 rows, N 2048, K 4096: 10.3
 // us, 13.1 with four; N 6144: 15.0, 14.7).
 template <int MB, typename TO>
 void rows_of(const I8Args& a, hipStream_t st) {
