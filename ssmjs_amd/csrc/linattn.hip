@@ -111,9 +111,8 @@ inline unsigned la_groups(LaArgs& a, int segments) {
 // chunk, between which two waves a SIMD cannot keep the matrix cores fed (a third of their time). Eight
 // waves of 16 columns read S q's queries twice as often: 190 us.
 //
-// Roundings to bf16: none that a result keeps. S as an operand of its product with q and the products
-// q k^T enter in two parts (16 bits; 2.5% of the time at 8 sequences of 4096 tokens), and the values of
-// the state update, e^{..} v, in two or three, so that the final state carries fp32 rounding only.
+// Roundings to bf16: the output's alone. What enters a product with 24 bits (S with q, the products q k^T with
+// v, and the values of the state update, e^{..} v, with k) enters in three parts of eight bits each.
 __device__ __forceinline__ floatx4 mfma(bf16x8 a, bf16x8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -128,6 +127,22 @@ __device__ __forceinline__ bf16x4 tr_read(const __bf16* base, int row0, int col0
 
 __device__ __forceinline__ bf16x8 cat(bf16x4 a, bf16x4 b) {
     return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// Pairs of fp32 numbers as three pairs of bf16 whose sums they are: each part has the leading eight bits of
+// what the ones before it leave, cut off, not rounded (so that the largest numbers stay finite, and nothing
+// is left).
+struct Parts { unsigned u[3]; };
+__device__ __forceinline__ Parts split(float a, float b) {
+    Parts p;
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+        const unsigned x = __builtin_bit_cast(unsigned, a), y = __builtin_bit_cast(unsigned, b);
+        p.u[c] = __builtin_amdgcn_perm(y, x, 0x07060302u);   // (v_perm_b32: their upper halves)
+        a -= __builtin_bit_cast(float, x & 0xffff0000u);
+        b -= __builtin_bit_cast(float, y & 0xffff0000u);
+    }
+    return p;
 }
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -145,8 +160,8 @@ struct SmemB {
     alignas(16) __bf16 q[Y][KP];
     alignas(16) __bf16 k[CB][KP];
     alignas(16) __bf16 v[CB][VP];
-    // scale e^{g (i - j)} q_i . k_j, row i, in two parts
-    alignas(16) __bf16 p[2][Y][PP];
+    // scale e^{g (i - j)} q_i . k_j, row i, in three parts
+    alignas(16) __bf16 p[3][Y][PP];
     float dec[CB + 17];             // place 64 - d: scale e^{g d}, d = i - j (1 behind d = 0)
     alignas(16) float wj[CB];       // e^{g (n - 1 - j)}: the state update's weights
     int odd[2];                     // an inf or NaN in the chunk's v (by the chunk's parity)
@@ -359,18 +374,20 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
                 __bf16* pr = &s.p[0][16 * W + l16][4 * g4];
 #pragma unroll
                 for (int jt = 0; jt <= (W | 1); ++jt) {
-                    bf16x4 hi = {}, lo = {};
+                    Parts p[2] = {};
                     if (jt <= W) {
+                        float f[4];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            float p = acc[min(jt, W)][r] * dec[r - 16 * (W - jt)];
-                            if (jt == W && l16 < 4 * g4 + r) p = 0.f;
-                            hi[r] = (__bf16)p;
-                            lo[r] = (__bf16)(p - (float)hi[r]);
+                            f[r] = acc[min(jt, W)][r] * dec[r - 16 * (W - jt)];
+                            if (jt == W && l16 < 4 * g4 + r) f[r] = 0.f;
                         }
+                        p[0] = split(f[0], f[1]);
+                        p[1] = split(f[2], f[3]);
                     }
-                    *reinterpret_cast<bf16x4*>(pr + 16 * jt) = hi;
-                    *reinterpret_cast<bf16x4*>(pr + CB * PP + 16 * jt) = lo;
+#pragma unroll
+                    for (int c = 0; c < 3; ++c)
+                        *reinterpret_cast<u32x2*>(pr + c * CB * PP + 16 * jt) = u32x2{p[0].u[c], p[1].u[c]};
                 }
             };
             if (w == 0) products(std::integral_constant<int, 0>{});
@@ -395,23 +412,26 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
             for (int kb = 0; kb < KB; ++kb) {
                 if (kb + 1 < KB) q_tiles(qf[(kb + 1) & 1], kb + 1);
                 __builtin_amdgcn_sched_barrier(0);
-                bf16x8 sf[VW], sl[VW];
+                bf16x8 sf[3][VW];
 #pragma unroll
-                for (int x = 0; x < VW; ++x)
+                for (int x = 0; x < VW; ++x) {
+                    ssm::u32x4 u[3];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float f = S[2 * kb + (e >> 2)][x][e & 3];
-                        sf[x][e] = (__bf16)f;
-                        sl[x][e] = (__bf16)(f - (float)sf[x][e]);
+                    for (int e = 0; e < 4; ++e) {
+                        const floatx4& t = S[2 * kb + (e >> 1)][x];
+                        const Parts p = split(t[2 * (e & 1)], t[2 * (e & 1) + 1]);
+#pragma unroll
+                        for (int c = 0; c < 3; ++c) u[c][e] = p.u[c];
                     }
 #pragma unroll
-                for (int it = 0; it < 4; ++it)
+                    for (int c = 0; c < 3; ++c) sf[c][x] = __builtin_bit_cast(bf16x8, u[c]);
+                }
 #pragma unroll
-                    for (int x = 0; x < VW; ++x) Y[x][it] = mfma(sf[x], qf[kb & 1][it], Y[x][it]);
+                for (int c = 2; c >= 0; --c)
 #pragma unroll
-                for (int it = 0; it < 4; ++it)
+                    for (int it = 0; it < 4; ++it)
 #pragma unroll
-                    for (int x = 0; x < VW; ++x) Y[x][it] = mfma(sl[x], qf[kb & 1][it], Y[x][it]);
+                        for (int x = 0; x < VW; ++x) Y[x][it] = mfma(sf[c][x], qf[kb & 1][it], Y[x][it]);
             }
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
@@ -432,17 +452,17 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
             if (!any_odd) {
 #pragma unroll
                 for (int jb = 0; jb < 2; ++jb) {
-                    bf16x8 vf[VW], pf[2][4];
+                    bf16x8 vf[VW], pf[3][4];
 #pragma unroll
                     for (int x = 0; x < VW; ++x) vf[x] = v_tile(jb, x);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                    for (int c = 0; c < 3; ++c)
 #pragma unroll
                         for (int it = 2 * jb; it < 4; ++it)
                             pf[c][it] = *reinterpret_cast<const bf16x8*>(&s.p[c][16 * it + l16][32 * jb + 8 * g4]);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int c = 1; c >= 0; --c)
+                    for (int c = 2; c >= 0; --c)
 #pragma unroll
                         for (int it = 2 * jb; it < 4; ++it)
 #pragma unroll
@@ -459,7 +479,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
                     for (int it = 0; it < 4; ++it) {
                         const int i = 16 * it + l16;
                         for (int j = 0; j <= i; ++j) {
-                            const float p = (float)s.p[0][i][j] + (float)s.p[1][i][j];
+                            const float p = (float)s.p[0][i][j] + ((float)s.p[1][i][j] + (float)s.p[2][i][j]);
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
                                 Y[x][it][r] = fmaf(p, (float)s.v[j][16 * (VW * w + x) + 4 * g4 + r], Y[x][it][r]);
@@ -498,53 +518,49 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
             for (int x = 0; x < VW; ++x)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) S[kt][x][r] = decay.of(S[kt][x][r]);
-        auto update = [&](auto three) {
-            constexpr int NP = decltype(three)::value ? 3 : 2, KH = KT / 2;
+        constexpr int KH = KT / 2;
 #pragma unroll
-            for (int jb = 0; jb < 2; ++jb) {
-                bf16x8 kf[KH], parts[VW][NP];
-                auto k_tiles = [&](int kt0) {
+        for (int jb = 0; jb < 2; ++jb) {
+            bf16x8 kf[KH], parts[VW][3];
+            auto k_tiles = [&](int kt0) {
+#pragma unroll
+                for (int kt = 0; kt < KH; ++kt)
+                    kf[kt] = cat(tr_read<KP>(&s.k[0][0], 32 * jb + 8 * g4, 16 * (kt0 + kt), l16),
+                                 tr_read<KP>(&s.k[0][0], 32 * jb + 8 * g4 + 4, 16 * (kt0 + kt), l16));
+            };
+            bf16x8 vf[VW];
+#pragma unroll
+            for (int x = 0; x < VW; ++x) vf[x] = v_tile(jb, x);
+            const floatx4 wa = *reinterpret_cast<const floatx4*>(&s.wj[32 * jb + 8 * g4]);
+            const floatx4 wb = *reinterpret_cast<const floatx4*>(&s.wj[32 * jb + 8 * g4 + 4]);
+            k_tiles(0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < VW; ++x) {
+                ssm::u32x4 u[3];
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const floatx4& wt = e < 4 ? wa : wb;
+                    const Parts p = split((float)vf[x][e] * wt[e & 3], (float)vf[x][e + 1] * wt[(e & 3) + 1]);
+#pragma unroll
+                    for (int c = 0; c < 3; ++c) u[c][e / 2] = p.u[c];
+                }
+#pragma unroll
+                for (int c = 0; c < 3; ++c) parts[x][c] = __builtin_bit_cast(bf16x8, u[c]);
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                for (int c = 2; c >= 0; --c)
 #pragma unroll
                     for (int kt = 0; kt < KH; ++kt)
-                        kf[kt] = cat(tr_read<KP>(&s.k[0][0], 32 * jb + 8 * g4, 16 * (kt0 + kt), l16),
-                                     tr_read<KP>(&s.k[0][0], 32 * jb + 8 * g4 + 4, 16 * (kt0 + kt), l16));
-                };
-                bf16x8 vf[VW];
 #pragma unroll
-                for (int x = 0; x < VW; ++x) vf[x] = v_tile(jb, x);
-                const floatx4 wa = *reinterpret_cast<const floatx4*>(&s.wj[32 * jb + 8 * g4]);
-                const floatx4 wb = *reinterpret_cast<const floatx4*>(&s.wj[32 * jb + 8 * g4 + 4]);
-                k_tiles(0);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int x = 0; x < VW; ++x)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float f = (float)vf[x][e] * (e < 4 ? wa[e & 3] : wb[e & 3]);
-#pragma unroll
-                        for (int c = 0; c < NP; ++c) {
-                            parts[x][c][e] = (__bf16)f;
-                            f -= (float)parts[x][c][e];
-                        }
-                    }
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                    for (int c = NP - 1; c >= 0; --c)
-#pragma unroll
-                        for (int kt = 0; kt < KH; ++kt)
-#pragma unroll
-                            for (int x = 0; x < VW; ++x)
-                                S[KH * half + kt][x] = mfma(kf[kt], parts[x][c], S[KH * half + kt][x]);
-                    if (half == 0) k_tiles(KH);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                        for (int x = 0; x < VW; ++x)
+                            S[KH * half + kt][x] = mfma(kf[kt], parts[x][c], S[KH * half + kt][x]);
+                if (half == 0) k_tiles(KH);
             }
-        };
-        // Two parts leave 2^-18 of a term out, which the decay to the sequence's end takes below
-        // 2^-21 in most chunks of most heads; the third is kept where it does not.
-        if (a.hT && gl * (float)(len - t - n) > -3.f) update(std::true_type{});
-        else update(std::false_type{});
+            __builtin_amdgcn_sched_barrier(0);
+        }
 
         __syncthreads();
     }
