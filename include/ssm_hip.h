@@ -239,7 +239,8 @@ ssm_status ssm_qk_norm_rope(int dtype, const void* q, long ldq, const void* k, l
  * there on are not written, and what q, k and v hold there is not used. h0, hT (B,H,V,K) float: the
  * states before the first and after each sequence's last token; either may be NULL, hT may be h0.
  * y overlaps no input. K <= 256 (SSM_ERR_UNSUPPORTED above). An inf or NaN changes no earlier token (from its own token
- * on, results that it touches are inf or NaN). `workspace` (16-byte aligned) holds
+ * on, results that it touches are inf or NaN). A state that is infinite, as given or from finite tokens that
+ * overflow, stays infinite, of its sign. `workspace` (16-byte aligned) holds
  * ssm_linear_attention_workspace(...) bytes and serves one stream at a time. */
 size_t ssm_linear_attention_workspace(int dtype, int B, int L, int H, int K, int V);
 ssm_status ssm_linear_attention(int dtype, const void* q, long ldq, const void* k, long ldk,

@@ -46,6 +46,14 @@ __device__ __forceinline__ float clamp_g(float g) { return g < -1e30f ? -1e30f :
 // x <- e^{g n} x: as x + (e^{g n} - 1) x from 1/2 on, so that a decay too slow for fp32's e^{g n} is kept,
 // and as a product below, where the difference would lose what is left. (Without a branch: the reads
 // around it stay ahead of it, and fp32 prompts took 5% longer.)
+__device__ __forceinline__ float decayed(float x, float m, float keep) { return fmaf(x, m, keep * x); }
+
+// The same, of a state that may be infinite: it stays so, as it does token by token.
+__device__ __forceinline__ float decayed_any(float x, float m, float keep) {
+    const float y = decayed(x, m, keep);
+    return __builtin_isinf(x) ? x : y;
+}
+
 struct Decay {
     float m, keep;   // (of a whole wave)
     __device__ __forceinline__ Decay() : m(0.f), keep(0.f) {}
@@ -58,7 +66,7 @@ struct Decay {
         m = whole(slow ? expm1f(e) : expf(e));
         keep = whole(slow ? 1.f : 0.f);
     }
-    __device__ __forceinline__ float of(float x) const { return fmaf(x, m, keep * x); }
+    __device__ __forceinline__ float of_any(float x) const { return decayed_any(x, m, keep); }
 };
 
 // A value that the compiler forms again in each turn of a loop: the registers that it would hold
@@ -131,16 +139,21 @@ __device__ __forceinline__ bf16x8 cat(bf16x4 a, bf16x4 b) {
 
 // Pairs of fp32 numbers as three pairs of bf16 whose sums they are: each part has the leading eight bits of
 // what the ones before it leave, cut off, not rounded (so that the largest numbers stay finite, and nothing
-// is left).
+// is left). ANY: an infinite number's first part is infinite and the others finite, of its sign (NaN else).
 struct Parts { unsigned u[3]; };
+template <bool ANY = false>
 __device__ __forceinline__ Parts split(float a, float b) {
+    constexpr float most = 3.402823466e38f;
+    auto held = [](float x) { return __builtin_amdgcn_fmed3f(x, -most, most); };
+    auto head = [](float x) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0xffff0000u); };
     Parts p;
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
         const unsigned x = __builtin_bit_cast(unsigned, a), y = __builtin_bit_cast(unsigned, b);
         p.u[c] = __builtin_amdgcn_perm(y, x, 0x07060302u);   // (v_perm_b32: their upper halves)
-        a -= __builtin_bit_cast(float, x & 0xffff0000u);
-        b -= __builtin_bit_cast(float, y & 0xffff0000u);
+        if (ANY && c == 0) a = held(a), b = held(b);
+        a -= head(a);
+        b -= head(b);
     }
     return p;
 }
@@ -317,7 +330,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
             each_state([&](floatx4& r, unsigned o, int left) {
                 const floatx4 own = load_f4<VEC>(d, o, left);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = over.of(r[e]) + own[e];
+                for (int e = 0; e < 4; ++e) r[e] = over.of_any(r[e]) + own[e];
             });
         }
     }
@@ -351,6 +364,19 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
         if (t + CB < t_end) fetch(t + CB);
         floatx4 Y[STATE ? 1 : VW][4];
         bool any_odd = false;
+        float now = decay.m, keep = decay.keep;
+        auto each = [&](auto&& f) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int x = 0; x < VW; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float e = S[kt][x][r];
+                        f(e);
+                        S[kt][x][r] = e;
+                    }
+        };
         if constexpr (!STATE) {
             any_odd = s.odd[parity] != 0;
             if (tid == 0) s.odd[parity ^ 1] = 0;   // (the next chunk sets it past two barriers)
@@ -403,35 +429,50 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
                     f[it] = cat(*reinterpret_cast<const bf16x4*>(qr), *reinterpret_cast<const bf16x4*>(qr + 16));
                 }
             };
-            q_tiles(qf[0], 0);
+            auto state_products = [&](auto any) {
+                q_tiles(qf[0], 0);
+#pragma unroll
+                for (int x = 0; x < VW; ++x)
+#pragma unroll
+                    for (int it = 0; it < 4; ++it) Y[x][it] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    if (kb + 1 < KB) q_tiles(qf[(kb + 1) & 1], kb + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    bf16x8 sf[3][VW];
+#pragma unroll
+                    for (int x = 0; x < VW; ++x) {
+                        ssm::u32x4 u[3];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const floatx4& t = S[2 * kb + (e >> 1)][x];
+                            const Parts p = split<decltype(any)::value>(t[2 * (e & 1)], t[2 * (e & 1) + 1]);
+#pragma unroll
+                            for (int c = 0; c < 3; ++c) u[c][e] = p.u[c];
+                        }
+#pragma unroll
+                        for (int c = 0; c < 3; ++c) sf[c][x] = __builtin_bit_cast(bf16x8, u[c]);
+                    }
+#pragma unroll
+                    for (int c = 2; c >= 0; --c)
+#pragma unroll
+                        for (int it = 0; it < 4; ++it)
+#pragma unroll
+                            for (int x = 0; x < VW; ++x) Y[x][it] = mfma(sf[c][x], qf[kb & 1][it], Y[x][it]);
+                }
+            };
+            state_products(std::false_type{});
+            // An infinite state makes all outputs of its row NaN there: then once more, with the state taken
+            // apart as it is, and decayed here (the decay below is then one half and one half).
+            float sum = 0.f;
 #pragma unroll
             for (int x = 0; x < VW; ++x)
 #pragma unroll
-                for (int it = 0; it < 4; ++it) Y[x][it] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                if (kb + 1 < KB) q_tiles(qf[(kb + 1) & 1], kb + 1);
-                __builtin_amdgcn_sched_barrier(0);
-                bf16x8 sf[3][VW];
-#pragma unroll
-                for (int x = 0; x < VW; ++x) {
-                    ssm::u32x4 u[3];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const floatx4& t = S[2 * kb + (e >> 1)][x];
-                        const Parts p = split(t[2 * (e & 1)], t[2 * (e & 1) + 1]);
-#pragma unroll
-                        for (int c = 0; c < 3; ++c) u[c][e] = p.u[c];
-                    }
-#pragma unroll
-                    for (int c = 0; c < 3; ++c) sf[c][x] = __builtin_bit_cast(bf16x8, u[c]);
-                }
-#pragma unroll
-                for (int c = 2; c >= 0; --c)
-#pragma unroll
-                    for (int it = 0; it < 4; ++it)
-#pragma unroll
-                        for (int x = 0; x < VW; ++x) Y[x][it] = mfma(sf[c][x], qf[kb & 1][it], Y[x][it]);
+                for (int r = 0; r < 4; ++r) sum = fmaf(Y[x][0][r], 0.f, sum);
+            if (__any(sum != 0.f)) {
+                state_products(std::true_type{});
+                each([&](float& x) { x = decay.of_any(x); });
+                keep = now = 0.5f;
             }
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
@@ -512,12 +553,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
             }
         }
         // ---- the state
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int x = 0; x < VW; ++x)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) S[kt][x][r] = decay.of(S[kt][x][r]);
+        each([&](float& x) { x = STATE ? decay.of_any(x) : decayed(x, now, keep); });
         constexpr int KH = KT / 2;
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb) {
@@ -693,7 +729,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
             each_state([&](floatx4& r, unsigned o, int left) {
                 const floatx4 own = load_f4<VEC>(d, o, left);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = over.of(r[e]) + own[e];
+                for (int e = 0; e < 4; ++e) r[e] = over.of_any(r[e]) + own[e];
             });
         }
     }
@@ -737,6 +773,19 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
 
         floatx4 Y[STATE ? 1 : VW][2];
         bool any_odd = false;
+        float now = decay.m, keep = decay.keep;
+        auto each = [&](auto&& f) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int x = 0; x < VW; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float e = S[kt][x][r];
+                        f(e);
+                        S[kt][x][r] = e;
+                    }
+        };
         if constexpr (!STATE) {
             any_odd = s.odd[parity] != 0;
             if (tid == 0) s.odd[parity ^ 1] = 0;
@@ -776,6 +825,16 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
 #pragma unroll
                         for (int x = 0; x < VW; ++x) Y[x][it] = mfma4(S[kt][x][r], qf[r], Y[x][it]);
                 }
+            // (as in the bf16 kernel; the products need no change)
+            float sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < VW; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum = fmaf(Y[x][0][r], 0.f, sum);
+            if (__any(sum != 0.f)) {
+                each([&](float& x) { x = decay.of_any(x); });
+                keep = now = 0.5f;
+            }
 #pragma unroll
             for (int it = 0; it < 2; ++it) {
                 const float f = a.scale * ssm::ex2(fresh(gl) * (float)(16 * it + l16 + 1));
@@ -785,12 +844,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_f32_kernel(LaArgs a
             __syncthreads();
         }
 
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int x = 0; x < VW; ++x)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) S[kt][x][r] = decay.of(S[kt][x][r]);
+        each([&](float& x) { x = STATE ? decay.of_any(x) : decayed(x, now, keep); });
 #pragma unroll
         for (int jt = 0; jt < 2; ++jt) {
             float vf[VW][4];
@@ -886,7 +940,7 @@ __global__ __launch_bounds__(256) void la_combine_kernel(LaArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (sgm + u + 1 >= used) break;
-            e = fmaf(e, m, keep * e) + own;
+            e = decayed_any(e, m, keep) + own;
             p[(sgm + u + 1) * slot] = e;
             own = next[u];
         }
@@ -1022,7 +1076,7 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
         float acc = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            s[r][e] = fmaf(vv[r], k[e], decay.of(s[r][e]));
+            s[r][e] = fmaf(vv[r], k[e], decay.of_any(s[r][e]));
             acc = fmaf(s[r][e], q[e], acc);
         }
 #pragma unroll
