@@ -262,7 +262,8 @@ ssm_status ssm_linear_attention_step(int dtype, const void* q, long ldq, const v
 ssm_status ssm_quantize_rows(int dtype, const void* x, long ldx, int8_t* q, long ldq, float* scale,
                              int M, int K, void* stream);
 /* y[m,n] = beta*y[m,n] + sx[m] sw[n] sum_k x[m,k] W[n,k] (+ bias[n]) with 8-bit x (M,K), W (N,K):
- * exact 32-bit integer sums, so K <= 131071. beta 0 does not read y. y of `out_dtype` (SSM_F32,
+ * exact 32-bit integer sums, so K <= 131071. The scales' own product may leave fp32's range (a sum of 0 is 0
+ * then, and a result keeps its digits). beta 0 does not read y. y of `out_dtype` (SSM_F32,
  * SSM_BF16). Read in place are 16-byte aligned rows: of W with K % 4 == 0 and ldw % 16 == 0, of x with
  * K % 256 == 0, ldx % 16 == 0 and M > 64; others are laid out in the workspace first. M, N < 2^24, row
  * strides below 2^22 (y's below 2^21). y does not overlap x.

@@ -281,6 +281,23 @@ struct Out {
           ld((unsigned)a.ldy), cols(cols_) {}
 };
 
+// A scale of which a product with another one could leave the normal numbers.
+__device__ __forceinline__ bool far(float scale) {
+    const float m = fabsf(scale);
+    return m != 0.f && !(m >= 0x1p-60f && m <= 0x1p60f);
+}
+
+// The sum times both scales. FAR: where one is far, times the smaller one first: what that leaves is as large
+// as an integer or has all its digits, so the second product is out of range only where the result is.
+template <bool FAR>
+__device__ __forceinline__ float scaled(int sum, float row, float channel) {
+    const float c = (float)sum;
+    if constexpr (FAR)
+        if (far(row) || far(channel))
+            return fabsf(row) < fabsf(channel) ? c * row * channel : c * channel * row;
+    return c * (row * channel);
+}
+
 // One output, n of row m of the tile.
 template <typename TO, bool BETA>
 __device__ __forceinline__ void put1(const Out<TO>& o, float beta, int m, int n, float x) {
@@ -493,7 +510,7 @@ __global__ __launch_bounds__(64 * NW) void i8_rows_kernel(I8Args a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int k = min(n0 + n + r, a.N - 1);
-            v[r] = (float)c[r] * (sm[t] * a.sw[k]) + (a.bias ? a.bias[k] : 0.f);
+            v[r] = scaled<true>(c[r], sm[t], a.sw[k]) + (a.bias ? a.bias[k] : 0.f);
         }
         const int rr = row < a.M ? row : 0, nn = row < a.M ? n : 1 << 30;
         if (a.vec) put4<TO, BETA>(out, a.beta, rr, nn, v);
@@ -677,8 +694,13 @@ __device__ __forceinline__ void i8_tiles(const I8Args& a, Tiles tiles, Place pla
         char* tile = reinterpret_cast<char*>(outs) + w * 4096;
         auto place = [&](int r, int u) { return tile + r * 128 + 16 * (u ^ (r & 7)); };
         const Out<TO> out(a, t.m0, t.mrows, t.n0, t.nrows);
-        auto finish = [&](auto vec) {
-            constexpr bool VEC = decltype(vec)::value;
+        bool any_far = false;   // (of the wave's channels and rows)
+#pragma unroll
+        for (int c = 0; c < 32 * TN; c += 64) any_far |= far(chs[32 * TN * wn + c + ll % (32 * TN)]);
+#pragma unroll
+        for (int r = 0; r < 32 * TM; r += 64) any_far |= far(rows_s[32 * TM * wm + r + ll % (32 * TM)]);
+        auto finish = [&](auto vec, auto fars) {
+            constexpr bool VEC = decltype(vec)::value, FAR = decltype(fars)::value;
 #pragma unroll
             for (int j = 0; j < TM; ++j) {
                 const int mw = 32 * (TM * wm + j);
@@ -695,7 +717,7 @@ __device__ __forceinline__ void i8_tiles(const I8Args& a, Tiles tiles, Place pla
                             const floatx4 b4 = *reinterpret_cast<const floatx4*>(&chb[nw + c]);
                             floatx4 v;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) v[r] = (float)acc[i0 + i][j][4 * q + r] * (sm * s4[r]) + b4[r];
+                            for (int r = 0; r < 4; ++r) v[r] = scaled<FAR>(acc[i0 + i][j][4 * q + r], sm, s4[r]) + b4[r];
                             if constexpr (sizeof(TL) == 4) {
                                 *reinterpret_cast<floatx4*>(place(li, c / 4)) = v;
                             } else {
@@ -737,8 +759,15 @@ __device__ __forceinline__ void i8_tiles(const I8Args& a, Tiles tiles, Place pla
                 }
             }
         };
-        if (a.vec) finish(std::true_type{});
-        else finish(std::false_type{});
+        constexpr std::true_type yes{};
+        constexpr std::false_type no{};
+        if (__any(any_far)) {
+            if (a.vec) finish(yes, yes);
+            else finish(no, yes);
+        } else {
+            if (a.vec) finish(yes, no);
+            else finish(no, no);
+        }
         if (ONE || !more) break;
         id = after;
         t = tn;
