@@ -387,7 +387,7 @@ def linear_attention(q, k, v, g, scale=1.0, lengths=None, h0=None, hT=None, out=
     """Linear attention with a decay for each head over whole prompts (ssm_linear_attention):
     S_t = e^g S_{t-1} + v_t k_t^T, y_t = scale S_t q_t. q (B,L,H,K), k (B,L,G,K), v (B,L,G,V),
     float32 or bfloat16; g (H) float32; y (B,L,H,V) in their type. lengths (B) int32: rows of y from
-    a sequence's length on are not written. h0, hT (B,H,V,K) float32, hT may be h0."""
+    a sequence's length on are zeros, or, in an `out` of the caller's, not written. h0, hT (B,H,V,K) float32, hT may be h0."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("q (B,L,H,K), k (B,L,G,K), v (B,L,G,V)")
     B, L, H, K = q.shape
@@ -396,7 +396,7 @@ def linear_attention(q, k, v, g, scale=1.0, lengths=None, h0=None, hT=None, out=
     code, dev = _code(dt), _current("q", q)
     pk, pv = _at("k", k, (B, L, G, K), dt, dev), _at("v", v, (B, L, G, V), dt, dev)
     if out is None:
-        out = q.new_empty((B, L, H, V))
+        out = (q.new_empty if lengths is None else q.new_zeros)((B, L, H, V))
     py = _at("out", out, (B, L, H, V), dt, dev)
     state = (B, H, V, K)
     # (held to the end of the call: freed before, it could be given to another stream)
