@@ -163,7 +163,7 @@ def run(s):
                                         eps=1e-6, interleaved=s["pair"] == "beside")
         if s["op"] == "prompt":
             y = kernels.linear_attention(s["q"], s["k"], s["v"], s["g"], scale=s["scale"],
-                                         lengths=s["lengths"], h0=s["h0"], hT=s["hT"], out=s["y"])
+                                         lengths=s["lengths"], h0=s["h0"], hT=s["hT"])
             return y, s["hT"]
         if s["op"] == "token":
             return kernels.linear_attention_step(s["q"], s["k"], s["v"], s["g"], s["h"],
