@@ -238,7 +238,7 @@ ssm_status ssm_qk_norm_rope(int dtype, const void* q, long ldq, const void* k, l
  * int32 on the device or NULL: sequence b has lengths[b] tokens (held to 0 .. L); rows of y from
  * there on are not written, and what q, k and v hold there is not used. h0, hT (B,H,V,K) float: the
  * states before the first and after each sequence's last token; either may be NULL, hT may be h0.
- * y overlaps no input. K <= 256 (SSM_ERR_UNSUPPORTED above). An inf or NaN changes no earlier token (from its own token
+ * y and hT overlap no input (but hT h0) nor each other, the workspace nothing. K <= 256 (SSM_ERR_UNSUPPORTED above). An inf or NaN changes no earlier token (from its own token
  * on, results that it touches are inf or NaN). A state that is infinite, as given or from finite tokens that
  * overflow, stays infinite, of its sign. `workspace` (16-byte aligned) holds
  * ssm_linear_attention_workspace(...) bytes and serves one stream at a time. */
@@ -249,7 +249,7 @@ ssm_status ssm_linear_attention(int dtype, const void* q, long ldq, const void* 
                                 int K, int V, const float* h0, float* hT, void* workspace,
                                 size_t workspace_bytes, void* stream);
 /* The same for one token of B sequences, h (B,H,V,K) in place. q (B,H,K), k (B,G,K), v (B,G,V),
- * y (B,H,V) with row strides; y overlaps no input. */
+ * y (B,H,V) with row strides; y and h overlap no input nor each other. */
 ssm_status ssm_linear_attention_step(int dtype, const void* q, long ldq, const void* k, long ldk,
                                      const void* v, long ldv, const float* g, float scale, void* y,
                                      long ldy, float* h, int B, int H, int G, int K, int V,
@@ -257,8 +257,8 @@ ssm_status ssm_linear_attention_step(int dtype, const void* q, long ldq, const v
 
 /* Rows to 8-bit integers: scale_m = max_k |x_mk| / 127 (fp32), q_mk = x_mk / scale_m to the nearest
  * integer (of the exact quotient; ties to even), held to -127 .. 127. A row of zeros gets scale 0; a
- * row with an inf or NaN gets zeros and that scale, so that its products are NaN. M < 2^24; q does not
- * overlap x. */
+ * row with an inf or NaN gets zeros and that scale, so that its products are NaN. M < 2^24; q, scale and x
+ * do not overlap. */
 ssm_status ssm_quantize_rows(int dtype, const void* x, long ldx, int8_t* q, long ldq, float* scale,
                              int M, int K, void* stream);
 /* y[m,n] = beta*y[m,n] + sx[m] sw[n] sum_k x[m,k] W[n,k] (+ bias[n]) with 8-bit x (M,K), W (N,K):
@@ -266,7 +266,7 @@ ssm_status ssm_quantize_rows(int dtype, const void* x, long ldx, int8_t* q, long
  * then, and a result keeps its digits). beta 0 does not read y. y of `out_dtype` (SSM_F32,
  * SSM_BF16). Read in place are 16-byte aligned rows: of W with K % 4 == 0 and ldw % 16 == 0, of x with
  * K % 256 == 0, ldx % 16 == 0 and M > 64; others are laid out in the workspace first. M, N < 2^24, row
- * strides below 2^22 (y's below 2^21). y does not overlap x.
+ * strides below 2^22 (y's below 2^21). y overlaps no other operand, the workspace nothing.
  * workspace: 16-byte aligned, ssm_linear_i8_workspace(...) bytes (0 where nothing is laid out), one
  * stream at a time. */
 size_t ssm_linear_i8_workspace(const int8_t* x, long ldx, const int8_t* W, long ldw, int M, int N,
@@ -276,7 +276,7 @@ ssm_status ssm_linear_i8(const int8_t* x, long ldx, const float* sx, const int8_
                          int N, int K, float beta, void* workspace, size_t workspace_bytes,
                          void* stream);
 /* ssm_quantize_rows of x (M,K), elements of in_dtype, then ssm_linear_i8, in one call: the
- * activations' scales are found as they come. Bit-equal to the two calls. y may be x (of one type). */
+ * activations' scales are found as they come. Bit-equal to the two calls. y may overlap x (be it, of one type). */
 size_t ssm_linear_q8_workspace(const int8_t* W, long ldw, int M, int N, int K);
 ssm_status ssm_linear_q8(int in_dtype, const void* x, long ldx, const int8_t* W, long ldw,
                          const float* sw, const float* bias, int out_dtype, void* y, long ldy, int M,

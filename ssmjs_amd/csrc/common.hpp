@@ -7,6 +7,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <string>
+#include <utility>
 
 #include "../../include/ssm_hip.h"
 
@@ -27,15 +28,29 @@ inline long cdiv(long a, long b) { return (a + b - 1) / b; }
 // A launch's threads are counted in 32 bits: the most workgroups of 256.
 constexpr long kMaxGroups = (1L << 24) - 1;
 
-// Whether one of `rows` rows of wa bytes, lda bytes apart, shares memory with one of as many of wb, ldb
-// apart. (Column ranges of one buffer lie between each other's rows.)
-inline bool rows_meet(const void* a, long lda, long wa, const void* b, long ldb, long wb, long rows) {
-    if (rows <= 0 || wa <= 0 || wb <= 0) return false;
-    const uintptr_t p = (uintptr_t)a, q = (uintptr_t)b;
-    if (p + (rows - 1) * lda + wa <= q || q + (rows - 1) * ldb + wb <= p) return false;
-    if (lda != ldb || rows == 1) return true;
-    const long d = ((long)(q - p) % lda + lda) % lda;
-    return d < wa || d + wb > lda;
+// What an operand covers: rows of `wide` bytes, `ld` bytes apart (a block is one row; null: nothing).
+struct Rows {
+    const void* p;
+    long ld, wide, n;
+};
+inline Rows block(const void* p, size_t bytes) { return Rows{p, 0, (long)bytes, 1}; }
+
+// Whether two operands share memory. (Column ranges of one buffer lie between each other's rows, and so may
+// a block; rows of unlike distances are taken to meet where their ranges do.)
+inline bool meet(Rows a, Rows b) {
+    if (!a.p || !b.p || a.n <= 0 || b.n <= 0 || a.wide <= 0 || b.wide <= 0) return false;
+    if (a.n == 1) std::swap(a, b);
+    const uintptr_t p = (uintptr_t)a.p, q = (uintptr_t)b.p;
+    if (p + (a.n - 1) * a.ld + a.wide <= q || q + (b.n - 1) * b.ld + b.wide <= p) return false;
+    if (a.n == 1 || (b.n > 1 && a.ld != b.ld)) return true;
+    const long d = ((long)(q - p) % a.ld + a.ld) % a.ld;
+    return d < a.wide || d + b.wide > a.ld;
+}
+
+// Whether an output shares memory with one of the others.
+template <typename... R>
+bool meets(const Rows& out, const R&... others) {
+    return (meet(out, others) || ...);
 }
 
 }  // namespace ssm

@@ -242,14 +242,17 @@ extern "C" ssm_status ssm_qk_norm_rope(int dtype, const void* q, long ldq, const
                 "ssm_qk_norm_rope: row stride below row width");
     SSM_REQUIRE((long)T * (H + G) < (1L << 32), "ssm_qk_norm_rope: too many heads");
     const long es = dtype == SSM_F32 ? 4 : 2;
-    auto meet = [&](const void* x, long ldx, long wx, const void* y, long ldy, long wy) {
-        return ssm::rows_meet(x, ldx * es, wx * es, y, ldy * es, wy * es, T);
-    };
-    SSM_REQUIRE(((q == qo && (ldq == ldqo || T == 1)) || !meet(q, ldq, wide_q, qo, ldqo, wide_q)) &&
-                    ((k == ko && (ldk == ldko || T == 1)) || !meet(k, ldk, wide_k, ko, ldko, wide_k)) &&
-                    !meet(q, ldq, wide_q, ko, ldko, wide_k) && !meet(k, ldk, wide_k, qo, ldqo, wide_q) &&
-                    !meet(qo, ldqo, wide_q, ko, ldko, wide_k),
+    auto rows = [&](const void* x, long ld, long wide) { return ssm::Rows{x, ld * es, wide * es, T}; };
+    const ssm::Rows rq = rows(q, ldq, wide_q), rk = rows(k, ldk, wide_k), rqo = rows(qo, ldqo, wide_q),
+                    rko = rows(ko, ldko, wide_k);
+    SSM_REQUIRE(((q == qo && (ldq == ldqo || T == 1)) || !ssm::meet(rq, rqo)) &&
+                    ((k == ko && (ldk == ldko || T == 1)) || !ssm::meet(rk, rko)) &&
+                    !ssm::meet(rq, rko) && !ssm::meet(rk, rqo) && !ssm::meet(rqo, rko),
                 "ssm_qk_norm_rope: an output overlaps an input that it is not, or the other output");
+    const ssm::Rows gq = ssm::block(wq, 4L * D), gk = ssm::block(wk, 4L * D),
+                    at = ssm::block(R ? pos : nullptr, 4L * T), turns = ssm::block(R ? freq : nullptr, 4L * R);
+    SSM_REQUIRE(!ssm::meets(rqo, gq, gk, at, turns) && !ssm::meets(rko, gq, gk, at, turns),
+                "ssm_qk_norm_rope: an output overlaps the weights, positions or frequencies");
     HeadArgs a{q, ldq, k, ldk, wq, wk, pos, freq, qo, ldqo, ko, ldko, T, H, G, D, R, 1, eps};
     // pieces of four elements: 16 bytes in fp32 (and of the weights), 8 in bf16
     const uintptr_t piece = dtype == SSM_F32 ? 15 : 7;

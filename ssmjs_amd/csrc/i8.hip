@@ -936,6 +936,17 @@ ssm_status check_product(const char* who, const void* x, long ldx, const int8_t*
     return SSM_OK;
 }
 
+// y apart from what is read while it is written, the workspace from everything.
+ssm_status check_overlaps(const char* who, const ssm::Rows& y, const int8_t* W, long ldw, const float* sw,
+                          const float* bias, int N, int K, const ssm::Rows& workspace, const ssm::Rows& x,
+                          const ssm::Rows& sx) {
+    const ssm::Rows w{W, ldw, K, N}, s = ssm::block(sw, 4L * N), b = ssm::block(bias, 4L * N);
+    SSM_REQUIRE(!ssm::meets(y, w, s, b), "%s: y overlaps the weights, their scales or the bias", who);
+    SSM_REQUIRE(!ssm::meets(workspace, w, s, b, y, x, sx),
+                "%s: the workspace overlaps another operand", who);
+    return SSM_OK;
+}
+
 ssm_status launch_product(I8Args a, int out_dtype, const Layout& l, bool lay_w, char* ws,
                           hipStream_t st) {
     if (lay_w) {
@@ -961,7 +972,9 @@ extern "C" ssm_status ssm_quantize_rows(int dtype, const void* x, long ldx, int8
     SSM_REQUIRE(ldx >= K && ldq >= K, "ssm_quantize_rows: row stride below row width");
     SSM_REQUIRE(M <= ssm::kMaxGroups, "ssm_quantize_rows: too many rows");
     const long es = dtype == SSM_F32 ? 4 : 2;
-    SSM_REQUIRE(!ssm::rows_meet(x, ldx * es, K * es, q, ldq, K, M), "ssm_quantize_rows: q overlaps x");
+    const ssm::Rows rx{x, ldx * es, K * es, M}, rq{q, ldq, K, M};
+    SSM_REQUIRE(!ssm::meet(rx, rq), "ssm_quantize_rows: q overlaps x");
+    SSM_REQUIRE(!ssm::meets(ssm::block(scale, 4L * M), rx, rq), "ssm_quantize_rows: the scales overlap x or q");
     return quantize(dtype, x, ldx, (signed char*)q, ldq, scale, M, K, K, false, (hipStream_t)stream);
 }
 
@@ -984,7 +997,11 @@ extern "C" ssm_status ssm_linear_i8(const int8_t* x, long ldx, const float* sx, 
     SSM_REQUIRE(l.all == 0 || (workspace && workspace_bytes >= l.all && ((uintptr_t)workspace & 15) == 0),
                 "ssm_linear_i8: 16-byte aligned workspace of %zu bytes needed", l.all);
     const long es = out_dtype == SSM_F32 ? 4 : 2;
-    SSM_REQUIRE(!ssm::rows_meet(x, ldx, K, y, ldy * es, N * es, M), "ssm_linear_i8: y overlaps x");
+    const ssm::Rows rx{x, ldx, K, M}, rs = ssm::block(sx, 4L * M), ry{y, ldy * es, N * es, M};
+    SSM_REQUIRE(!ssm::meets(ry, rx, rs), "ssm_linear_i8: y overlaps x or its scales");
+    if (ssm_status e = check_overlaps("ssm_linear_i8", ry, W, ldw, sw, bias, N, K, ssm::block(workspace, l.all),
+                                      rx, rs))
+        return e;
     I8Args a{(const signed char*)x, ldx, sx, nullptr, 0, 0, (const signed char*)W, ldw, sw, bias, y, ldy,
              M, N, K, beta, 0, 0, 0, 0};
     if (lay_x) {
@@ -1023,9 +1040,13 @@ extern "C" ssm_status ssm_linear_q8(int in_dtype, const void* x, long ldx, const
              M, N, K, beta, 0, 0, 0, 0};
     const bool vec = K % 4 == 0 && ldx % 4 == 0 && ((uintptr_t)x & (in_dtype == SSM_F32 ? 15 : 7)) == 0;
     const int per = K > 2048 ? 4 : K > 1024 ? 2 : 1;
-    // (each workgroup reads all of x there while others write: y has to be elsewhere)
     const long ei = in_dtype == SSM_F32 ? 4 : 2, eo = out_dtype == SSM_F32 ? 4 : 2;
-    if (vec && !ssm::rows_meet(x, ldx * ei, K * ei, y, ldy * eo, N * eo, M) && K <= kFusedX && M <= kFusedRows && M * per <= kFusedX / 1024)
+    const ssm::Rows rx{x, ldx * ei, K * ei, M}, ry{y, ldy * eo, N * eo, M};
+    if (ssm_status e = check_overlaps("ssm_linear_q8", ry, W, ldw, sw, bias, N, K, ssm::block(workspace, l.all),
+                                      rx, ssm::block(nullptr, 0)))
+        return e;
+    // (each workgroup reads all of x there while others write: y has to be elsewhere)
+    if (vec && !ssm::meet(rx, ry) && K <= kFusedX && M <= kFusedRows && M * per <= kFusedX / 1024)
         a.Xf = x;
     else if (ssm_status e = quantize(in_dtype, x, ldx, q, l.Kp, sx, M, K, (int)l.Kp, M <= kRowsMax,
                                      (hipStream_t)stream))

@@ -1168,12 +1168,16 @@ extern "C" ssm_status ssm_linear_attention(int dtype, const void* q, long ldq, c
         SSM_REQUIRE(aligned16(workspace), "ssm_linear_attention: workspace must be 16-byte aligned");
         a.seg = (float*)workspace;
     }
-    const long rows = (long)B * L;
-    auto meets = [&](const void* x, long ldx, long wide) {
-        return ssm::rows_meet(x, ldx * esz, wide * esz, y, ldy * esz, (long)H * V * esz, rows);
-    };
-    SSM_REQUIRE(!meets(q, ldq, (long)H * K) && !meets(k, ldk, (long)G * K) && !meets(v, ldv, (long)G * V),
-                "ssm_linear_attention: y overlaps an input");
+    auto rows = [&](const void* x, long ld, long wide) { return ssm::Rows{x, ld * esz, wide * esz, (long)B * L}; };
+    const ssm::Rows rq = rows(q, ldq, (long)H * K), rk = rows(k, ldk, (long)G * K), rv = rows(v, ldv, (long)G * V),
+                    ry = rows(y, ldy, (long)H * V), rg = ssm::block(g, 4L * H), rl = ssm::block(lengths, 4L * B),
+                    from = ssm::block(h0, 4L * B * H * V * K), to = ssm::block(hT, 4L * B * H * V * K);
+    SSM_REQUIRE(!ssm::meets(ry, rq, rk, rv, rg, rl, from), "ssm_linear_attention: y overlaps an input");
+    SSM_REQUIRE(!ssm::meets(to, rq, rk, rv, rg, rl, ry) && (h0 == hT || !ssm::meet(to, from)),
+                "ssm_linear_attention: hT overlaps y or an input that it is not");
+    SSM_REQUIRE(a.nseg == 1 || !ssm::meets(ssm::block(workspace, ssm_linear_attention_workspace(dtype, B, L, H, K, V)),
+                                           rq, rk, rv, rg, rl, ry, from, to),
+                "ssm_linear_attention: the workspace overlaps another operand");
     const bool vec = K % ev == 0 && V % ev == 0 && (ldq | ldk | ldv | ldy) % ev == 0 &&
                      aligned16(q) && aligned16(k) && aligned16(v) && aligned16(y) &&
                      aligned16(h0) && aligned16(hT);
@@ -1203,11 +1207,13 @@ extern "C" ssm_status ssm_linear_attention_step(int dtype, const void* q, long l
     const long n = (long)B * H * a.blocks;
     SSM_REQUIRE(n <= ssm::kMaxGroups, "ssm_linear_attention_step: too many heads");
     const long es = dtype == SSM_F32 ? 4 : 2;
-    auto meets = [&](const void* x, long ldx, long wide) {
-        return ssm::rows_meet(x, ldx * es, wide * es, y, ldy * es, (long)H * V * es, B);
-    };
-    SSM_REQUIRE(!meets(q, ldq, (long)H * K) && !meets(k, ldk, (long)G * K) && !meets(v, ldv, (long)G * V),
+    auto rows = [&](const void* x, long ld, long wide) { return ssm::Rows{x, ld * es, wide * es, B}; };
+    const ssm::Rows q_rows = rows(q, ldq, (long)H * K), k_rows = rows(k, ldk, (long)G * K),
+                    v_rows = rows(v, ldv, (long)G * V), y_rows = rows(y, ldy, (long)H * V), decays = ssm::block(g, 4L * H);
+    SSM_REQUIRE(!ssm::meets(y_rows, q_rows, k_rows, v_rows, decays),
                 "ssm_linear_attention_step: y overlaps an input");
+    SSM_REQUIRE(!ssm::meets(ssm::block(h, 4L * B * H * V * K), q_rows, k_rows, v_rows, decays, y_rows),
+                "ssm_linear_attention_step: the state overlaps y or an input");
     const bool vec = K % 4 == 0 && aligned16(h);
     if (dtype == SSM_F32) step_dispatch<float>(a, rv, vec, (unsigned)n, (hipStream_t)stream);
     else step_dispatch<__bf16>(a, rv, vec, (unsigned)n, (hipStream_t)stream);
