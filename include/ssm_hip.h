@@ -224,7 +224,7 @@ ssm_status ssm_m1_xproj_dt(const float* x, long ldx, const float* Wx, const floa
  * Pairs are (i, i + R/2), with `interleaved` (2i, 2i + 1). q (T,H,D), k (T,G,D) with row strides
  * (heads of a row follow one another); wq, wk (D) float or NULL (ones); pos (T) int32; freq (R/2)
  * doubles, radians per position; all on the device. R even, R <= D <= 512 (R 0: norm alone, pos
- * and freq may be NULL; H or G may be 0). qo, ko may be q, k and overlap nothing else. Angles are formed in double, the
+ * and freq may be NULL; H or G may be 0; H + G <= 2^30). qo, ko may be q, k and overlap nothing else. Angles are formed in double, the
  * rest in fp32, outputs rounded once. */
 ssm_status ssm_qk_norm_rope(int dtype, const void* q, long ldq, const void* k, long ldk,
                             const float* wq, const float* wk, const int* pos, const double* freq,
@@ -238,7 +238,7 @@ ssm_status ssm_qk_norm_rope(int dtype, const void* q, long ldq, const void* k, l
  * int32 on the device or NULL: sequence b has lengths[b] tokens (held to 0 .. L); rows of y from
  * there on are not written, and what q, k and v hold there is not used. h0, hT (B,H,V,K) float: the
  * states before the first and after each sequence's last token; either may be NULL, hT may be h0.
- * y and hT overlap no input (but hT h0) nor each other, the workspace nothing. K <= 256 (SSM_ERR_UNSUPPORTED above). An inf or NaN changes no earlier token (from its own token
+ * y and hT overlap no input (but hT h0) nor each other, the workspace nothing. K <= 256 (SSM_ERR_UNSUPPORTED above), L <= 2^30. An inf or NaN changes no earlier token (from its own token
  * on, results that it touches are inf or NaN). A state that is infinite, as given or from finite tokens that
  * overflow, stays infinite, of its sign. `workspace` (16-byte aligned) holds
  * ssm_linear_attention_workspace(...) bytes and serves one stream at a time. */
@@ -257,7 +257,7 @@ ssm_status ssm_linear_attention_step(int dtype, const void* q, long ldq, const v
 
 /* Rows to 8-bit integers: scale_m = max_k |x_mk| / 127 (fp32), q_mk = x_mk / scale_m to the nearest
  * integer (of the exact quotient; ties to even), held to -127 .. 127. A row of zeros gets scale 0; a
- * row with an inf or NaN gets zeros and that scale, so that its products are NaN. M < 2^24; q, scale and x
+ * row with an inf or NaN gets zeros and that scale, so that its products are NaN. M < 2^24, K <= 2^30; q, scale and x
  * do not overlap. */
 ssm_status ssm_quantize_rows(int dtype, const void* x, long ldx, int8_t* q, long ldq, float* scale,
                              int M, int K, void* stream);

@@ -28,6 +28,9 @@ inline long cdiv(long a, long b) { return (a + b - 1) / b; }
 // A launch's threads are counted in 32 bits: the most workgroups of 256.
 constexpr long kMaxGroups = (1L << 24) - 1;
 
+// The longest dimension that a kernel steps through with an int, which passes its end by up to a step.
+constexpr long kMaxSteps = 1L << 30;
+
 // What an operand covers: rows of `wide` bytes, `ld` bytes apart (a block is one row; null: nothing).
 struct Rows {
     const void* p;

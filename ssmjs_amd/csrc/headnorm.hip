@@ -234,13 +234,14 @@ extern "C" ssm_status ssm_qk_norm_rope(int dtype, const void* q, long ldq, const
                 "ssm_qk_norm_rope: %d rotated elements of %d (an even number up to all)", R, D);
     if (D > kMaxD)
         return ssm::fail(SSM_ERR_UNSUPPORTED, "ssm_qk_norm_rope: head dim %d above %d", D, kMaxD);
-    if (T == 0 || H + G == 0) return SSM_OK;
+    if (T == 0 || (H == 0 && G == 0)) return SSM_OK;
     SSM_REQUIRE((H == 0 || (q && qo)) && (G == 0 || (k && ko)) && (R == 0 || (pos && freq)),
                 "ssm_qk_norm_rope: null input");
     const long wide_q = (long)H * D, wide_k = (long)G * D;
     SSM_REQUIRE(T == 1 || (ldq >= wide_q && ldqo >= wide_q && ldk >= wide_k && ldko >= wide_k),
                 "ssm_qk_norm_rope: row stride below row width");
-    SSM_REQUIRE((long)T * (H + G) < (1L << 32), "ssm_qk_norm_rope: too many heads");
+    const long heads = (long)H + G;
+    SSM_REQUIRE(heads <= ssm::kMaxSteps && T * heads < (1L << 32), "ssm_qk_norm_rope: too many heads");
     const long es = dtype == SSM_F32 ? 4 : 2;
     auto rows = [&](const void* x, long ld, long wide) { return ssm::Rows{x, ld * es, wide * es, T}; };
     const ssm::Rows rq = rows(q, ldq, wide_q), rk = rows(k, ldk, wide_k), rqo = rows(qo, ldqo, wide_q),

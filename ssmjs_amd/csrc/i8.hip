@@ -971,6 +971,7 @@ extern "C" ssm_status ssm_quantize_rows(int dtype, const void* x, long ldx, int8
     SSM_REQUIRE(x && q && scale, "ssm_quantize_rows: null input");
     SSM_REQUIRE(ldx >= K && ldq >= K, "ssm_quantize_rows: row stride below row width");
     SSM_REQUIRE(M <= ssm::kMaxGroups, "ssm_quantize_rows: too many rows");
+    SSM_REQUIRE(K <= ssm::kMaxSteps, "ssm_quantize_rows: too long");
     const long es = dtype == SSM_F32 ? 4 : 2;
     const ssm::Rows rx{x, ldx * es, K * es, M}, rq{q, ldq, K, M};
     SSM_REQUIRE(!ssm::meet(rx, rq), "ssm_quantize_rows: q overlaps x");

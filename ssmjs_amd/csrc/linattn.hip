@@ -1158,6 +1158,7 @@ extern "C" ssm_status ssm_linear_attention(int dtype, const void* q, long ldq, c
     a.nseg = plan.nseg;
     a.seglen = plan.seglen;
     a.vparts = plan.vparts;
+    SSM_REQUIRE(L <= ssm::kMaxSteps, "ssm_linear_attention: too long");
     SSM_REQUIRE((long)V * K < (1L << 29), "ssm_linear_attention: state of a head too large");
     SSM_REQUIRE(((double)a.nseg * B + 7) * H * ssm::cdiv(V, 64) <= (double)ssm::kMaxGroups,
                 "ssm_linear_attention: too many heads");
