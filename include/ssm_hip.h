@@ -265,7 +265,8 @@ ssm_status ssm_quantize_rows(int dtype, const void* x, long ldx, int8_t* q, long
  * exact 32-bit integer sums, so K <= 131071. The scales' own product may leave fp32's range (a sum of 0 is 0
  * then, and a result keeps its digits). beta 0 does not read y. y of `out_dtype` (SSM_F32,
  * SSM_BF16). Read in place are 16-byte aligned rows: of W with K % 4 == 0 and ldw % 16 == 0, of x with
- * K % 256 == 0, ldx % 16 == 0 and M > 64; others are laid out in the workspace first. M, N < 2^24, row
+ * K % 256 == 0, ldx % 16 == 0 and M > 64; others are laid out in the workspace first, in every call (for
+ * W a read and a write of it and a launch more: keep weights at such a stride). M, N < 2^24, row
  * strides below 2^22 (y's below 2^21). y overlaps no other operand, the workspace nothing.
  * workspace: 16-byte aligned, ssm_linear_i8_workspace(...) bytes (0 where nothing is laid out), one
  * stream at a time. */

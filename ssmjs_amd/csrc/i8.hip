@@ -2,13 +2,16 @@
 //   quantised rows    s_m = max_k |x_mk| / 127 (fp32),  q_mk = x_mk / s_m to the nearest integer,
 //                     ties to even (from the exact quotient), held to -127 .. 127
 //   y_mn = beta y_mn + s_m s_n sum_k q_mk w_nk (+ bias_n)
-// The sums are exact 32-bit integers (|q|, |w| <= 128: K up to 131071), on v_mfma_i32_16x16x64_i8.
+// The sums are exact 32-bit integers (|q|, |w| <= 128: K up to 131071).
 //
 // Three kernels share the work by rows:
 //   - up to 64 rows (one per decoded sequence): the weights' bytes bound it. i8_rows_kernel reads
-//     every weight row once, straight into registers, the k of a row shared by its waves.
-//   - more rows: the matrix cores bound it. i8_gemm_kernel is a tiled product out of LDS.
-//   - rows that are not 16-byte aligned are laid out in the workspace first (lay_rows_kernel).
+//     every weight row once, straight into registers, the k of a row shared by its waves
+//     (v_mfma_i32_16x16x64_i8).
+//   - more rows: the matrix cores bound it. i8_gemm_kernel and, where every CU has a tile of 256 x 256,
+//     i8_gemm_big_kernel are tiled products out of LDS (v_mfma_i32_32x32x32_i8).
+// Rows that these cannot read in place (not 16-byte aligned, x's of few rows in the operands' order) are laid
+// out in the workspace first, in every call (lay_rows_kernel): weights kept at a stride of 16 bytes save that.
 #include <algorithm>
 #include <type_traits>
 
@@ -539,8 +542,8 @@ __device__ __forceinline__ void to_lds16(__amdgpu_buffer_rsrc_t r, char* lds, un
 // products behind and ahead of it, and a load has three blocks' time to land. At a tile's end these
 // are the next tile's first blocks: its operands land while the outputs are written.
 //
-// Bound by the matrix cores and the LDS reads that feed them: 8192 x 8512 x 2048 to bf16 takes 154 us, 1.86
-// POP/s (a library's product of the integers alone 164 us), 8192 x 8192 x 8192 477 us, 2.3 POP/s (457).
+// Bound by the matrix cores and the LDS reads that feed them: 8192 x 8512 x 2048 to bf16 takes 152 to 164 us
+// on different cards, 1.74 POP/s and more (a library's product of the integers alone 164 us), 8192 x 8192 x 8192 477 us, 2.3 POP/s (457).
 //
 // The outputs go through LDS, so that they are written 128 bytes of a row at a time: as they lie in the
 // accumulators (16 bytes of 32 rows an instruction) they took 17 us of a tile's 40 at K 2048.

@@ -85,8 +85,8 @@ __device__ __forceinline__ int seq_len(const LaArgs& a, int b) {
 
 // Workgroup order: those that read the same keys and values (the parts of V and the heads of a group) on one
 // XCD, the groups, then the sequences and segments, dealt out over the XCDs: a padded batch's long
-// sequences are then shared by all of them (8 sequences of up to 1500 tokens, 32 heads: 112 -> 84 us against
-// a range of ids an XCD). Few groups would leave XCDs idle: then single heads are dealt out.
+// sequences are then shared by all of them (8 sequences of up to 1500 tokens, 32 heads: a range of ids an XCD
+// took 1.3 times as long). Few groups would leave XCDs idle: then single heads are dealt out.
 struct Place {
     int part, h, grp, b, seg;   // seg past the last: none
     __device__ __forceinline__ explicit Place(const LaArgs& a) {
@@ -114,13 +114,15 @@ inline unsigned la_groups(LaArgs& a, int segments) {
 // the block taken in the order (16 t + 4 g + r, 16 (t + 1) + 4 g + r); q is read from LDS in that
 // order. The 64 x 64 products q k^T are shared out over the waves by rows i and go through LDS.
 //
-// 8 sequences of 4096 tokens, 16 heads, K = V = 128: the state pass takes 57 us (268 MB, 4.7 TB/s), the full
-// pass 140, of which its loads and stores alone are 120: it is bound by memory and by the three barriers a
-// chunk, between which two waves a SIMD cannot keep the matrix cores fed (a third of their time). Eight
-// waves of 16 columns read S q's queries twice as often: 190 us.
+// 8 sequences of 4096 tokens, 16 heads, K = V = 128, in four segments: the state pass, over three of them,
+// takes 60 us (201 MB of rows in, 25 MB of states out: 3.8 TB/s, short of memory speed), the full pass 165, of
+// which its loads and stores alone are 120 and the matrix cores' work 51: it is bound by memory and by the
+// three barriers a chunk, between which two waves a SIMD cannot keep either busy. Eight waves of 16 columns
+// read S q's queries twice as often (1.36 times as long).
 //
 // Roundings to bf16: the output's alone. What enters a product with 24 bits (S with q, the products q k^T with
-// v, and the values of the state update, e^{..} v, with k) enters in three parts of eight bits each.
+// v, and the values of the state update, e^{..} v, with k) enters in three parts of eight bits each. (Two parts
+// took 196 us of the 225 in all and left 2^-17 of a term out, which is all that a sum that cancels holds.)
 __device__ __forceinline__ floatx4 mfma(bf16x8 a, bf16x8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
         for (int u = 0; u < NV; ++u) rv[u] = fetch_b<VEC>(dv, voff + u * vdown, part * VT + vcol, a.V);
         if constexpr (!STATE) {
             // (read once: out of the way of k and v, which the state pass has read before and the other
-            // heads of the group read; 5 sequences of 4096 tokens 146 -> 140 us)
+            // heads of the group read; 4% at 5 sequences of 4096 tokens)
             const auto dq = ssm::rsrc(base(a.q, a.ldq, h, a.K, tt), bytes(a.ldq, a.K, n));
 #pragma unroll
             for (int u = 0; u < NK; ++u) rq[u] = fetch_b<VEC, true>(dq, qoff + u * qdown, kcol, a.K);
@@ -614,7 +616,7 @@ __global__ __launch_bounds__(256, KD == 256 ? 1 : 2) void la_bf16_kernel(LaArgs 
 // nothing else, as S stays in the accumulators. MFMA r of a 16-k block takes k = 4 (lane / 16) + r
 // from every lane, so that S and the products q k^T are read as they lie in the accumulators and
 // q and k as 16-byte pieces. Bound by the matrix cores: 8 sequences of 4096 tokens, 16 heads, K = V = 128 take
-// 513 us, 105 TFLOP/s of the 154 that a large product reaches (5.5 K V + 48 (K + V) operations a token, the
+// 530 us, 101 TFLOP/s of the 154 that a large product reaches (5.5 K V + 48 (K + V) operations a token, the
 // state pass's among them).
 constexpr int CF = 32;
 
@@ -949,16 +951,16 @@ __global__ __launch_bounds__(256) void la_combine_kernel(LaArgs a) {
 
 // ---------------------------------------------------------------- plan
 // Segments: as many as fill the chip once, two workgroups a CU (one more turn for the rest costs as much
-// as a whole one: 80 sequences and heads of 4096 tokens ran 171 us in 7 segments, 144 in 6), each of
+// as a whole one: 80 sequences and heads of 4096 tokens take 163 us in 7 segments, 158 in 6), each of
 // at least so many tokens that its states' traffic stays small beside its rows'. bf16: 512 where that
-// leaves a workgroup for every CU (128 sequences and heads of 1024: 72 -> 63 us against 256), else 256.
-// fp32 chunks take four times as long on the matrix cores: 64 (24 of 2000: 95 -> 84 us against 256).
+// leaves a workgroup for every CU (128 sequences and heads of 1024: 71 us, 73 in segments of 256), else 256.
+// fp32 chunks take longer on the matrix cores: 64 (24 of 2000: 83 us, 95 in segments of 256).
 //
 // Columns of V a workgroup: 128, which share a chunk's q k^T and its rows of q and k (512 sequences and
-// heads of 4096 tokens: 484 us, 600 in parts of 64). 64 where V or the registers (K above 128) ask for
+// heads of 4096 tokens: 624 us, 765 in parts of 64). 64 where V or the registers (K above 128) ask for
 // it; where whole sequences fill the chip in parts of 64 and need no state pass (256 sequences and heads
-// of 1500 tokens: 111 us, 130 in two segments of 128 columns; of 4096: 303, 307); and where the shortest
-// segments would leave CUs idle (8 of 4096: 37 us, 45).
+// of 1500 tokens: 144 us, 149 in two segments of 128 columns; of 4096: 385, 398); and where the shortest
+// segments would leave CUs idle (8 of 4096: 38 us, 46).
 constexpr int kSlots = 512, kCUs = 256;
 struct LaPlan { int nseg, seglen, vt, vparts; };
 LaPlan la_plan(int dtype, int B, int L, int H, int K, int V) {
@@ -978,7 +980,7 @@ LaPlan la_plan(int dtype, int B, int L, int H, int K, int V) {
 }
 
 // A chain of more segments than this is combined once, by a pass of its own (8 sequences of 1500 tokens, 16
-// heads, 3 segments: 94 us in a chain, 100 combined; 24 heads of 4096 tokens, 16 segments: 103 and 64).
+// heads, 3 segments: 97 us in a chain, 107 combined; 24 heads of 4096 tokens, 16 segments: 98 and 71).
 constexpr int kChain = 4;
 
 template <int KD, int VT, bool VEC>
@@ -1016,7 +1018,7 @@ ssm_status la_dispatch(int dtype, const LaArgs& a, int vt, hipStream_t st) {
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // ---------------------------------------------------------------- one token
-// S is read and written once: memory bound (64 sequences of 32 heads, K = V = 128, 270 MB: 50 us, 5.4
+// S is read and written once: memory bound (64 sequences of 32 heads, K = V = 128, 270 MB: 51 us, 5.3
 // TB/s), past the caches, as the next token's call comes after the layer's other work. 16 lanes hold a row of S (LV x 64 columns in float4
 // pieces, or one by one), a wave four rows, a workgroup 16 RV rows of one (sequence, head); the
 // loads of all RV rows are in flight before the first is used.
@@ -1202,7 +1204,7 @@ extern "C" ssm_status ssm_linear_attention_step(int dtype, const void* q, long l
                 "ssm_linear_attention_step: row stride below row width");
     LaStepArgs a{q, ldq, k, ldk, v, ldv, g, scale, y, ldy, H, G, K, V, 0, h};
     // four rows a lane group where that still leaves a workgroup for every CU (K = V = 128: 64 sequences of
-    // 32 heads 50 us, 68 with one row; one of 12 heads 3.8 us with one, 4.5 with four)
+    // 32 heads 51 us, 68 with one row; one of 12 heads 3.8 us with one, 4.5 with four)
     const int rv = (long)B * H * ssm::cdiv(V, 64) >= 256 ? 4 : 1;
     a.blocks = (int)ssm::cdiv(V, 16 * rv);
     const long n = (long)B * H * a.blocks;
