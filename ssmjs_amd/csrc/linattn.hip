@@ -121,8 +121,8 @@ inline unsigned la_groups(LaArgs& a, int segments) {
 // read S q's queries twice as often (1.36 times as long).
 //
 // Roundings to bf16: the output's alone. What enters a product with 24 bits (S with q, the products q k^T with
-// v, and the values of the state update, e^{..} v, with k) enters in three parts of eight bits each. (Two parts
-// took 196 us of the 225 in all and left 2^-17 of a term out, which is all that a sum that cancels holds.)
+// v, and the values of the state update, e^{..} v, with k) enters in three parts of eight bits each. (In two
+// parts a call took 196 us in all, now 225, and 2^-17 of a term was left out: all that a sum that cancels holds.)
 __device__ __forceinline__ floatx4 mfma(bf16x8 a, bf16x8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
