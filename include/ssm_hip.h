@@ -284,6 +284,40 @@ ssm_status ssm_linear_q8(int in_dtype, const void* x, long ldx, const int8_t* W,
                          int N, int K, float beta, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/* ---- A gated-recurrence layer, in both directions (no counterpart in the reference). Element types are SSM_F32
+ * and SSM_BF16; one call's activations and their gradients share theirs. */
+
+/* Gated linear recurrence over whole prompts, for every channel d:
+ *   z_t = c softplus(lam_d) sigmoid(r_t),  a_t = e^{-z_t}
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t,  y_t = h_t   (h in fp32)
+ * x, r, i, y (B,L,D) with row strides; lam (D) float; c >= 0. lengths (B) int32 on the device or NULL: sequence b
+ * has lengths[b] tokens (held to 0 .. L); rows of y from there on become zeros with `pad`, else are not written, and
+ * what x, r and i hold there is not used. h0, hT (B,D) float: the states before the first and after each sequence's last token; either may be
+ * NULL, hT may be h0. states (B, ceil(L / 64), D) float or NULL: the states entering tokens 0, 64, 128 .. of each
+ * sequence, which the backward pass needs (those behind a sequence's end are not written). An infinite state
+ * stays infinite; an inf or NaN changes no earlier token and no other channel. Outputs, states and the workspace
+ * overlap nothing else. Row strides below 2^20, L <= 2^30. `workspace` (16-byte aligned) holds
+ * ssm_gated_recurrence_workspace(...) bytes (0 where no sequence is cut) and serves one stream at a time. */
+size_t ssm_gated_recurrence_workspace(int B, int L, int D);
+ssm_status ssm_gated_recurrence(int dtype, const void* x, long ldx, const void* r, long ldr, const void* i, long ldi,
+                                const float* lam, float c, const int* lengths, int pad, void* y, long ldy, int B, int L,
+                                int D, const float* h0, float* hT, float* states, void* workspace, size_t workspace_bytes,
+                                void* stream);
+/* Its gradients: dy (B,L,D) and dhT (B,D; NULL: zeros) are those of y and hT; dx, dr, di (B,L,D; rows behind a
+ * sequence's end as y's), dlam (D) and dh0 (B,D; may be NULL or dhT) those of the inputs. `states` as the
+ * forward call with the same x, r, i, lam, c and lengths left them. Sums over tokens are in one order: the same call
+ * gives the same bits. workspace: 16-byte aligned, ssm_gated_recurrence_backward_workspace(...) bytes, never 0. */
+size_t ssm_gated_recurrence_backward_workspace(int B, int L, int D);
+ssm_status ssm_gated_recurrence_backward(int dtype, const void* dy, long lddy, const void* x, long ldx, const void* r,
+                                         long ldr, const void* i, long ldi, const float* lam, float c,
+                                         const int* lengths, int pad, const float* states, const float* dhT, void* dx, long lddx,
+                                         void* dr, long lddr, void* di, long lddi, float* dlam, float* dh0, int B, int L,
+                                         int D, void* workspace, size_t workspace_bytes, void* stream);
+/* One token of B sequences, h (B,D) float in place: x, r, i, y (B,D) with row strides. */
+ssm_status ssm_gated_recurrence_step(int dtype, const void* x, long ldx, const void* r, long ldr, const void* i,
+                                     long ldi, const float* lam, float c, void* y, long ldy, float* h, int B, int D,
+                                     void* stream);
+
 /* Greedy pick per row (sampleToken with topK = 1, src/session/streaming.ts:74-75): index
  * of the largest value, lowest index among equal maxima; NaN never wins (0 for an all-NaN
  * row). x (rows, n) with row stride ldx; out (rows) uint32. */

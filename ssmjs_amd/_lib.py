@@ -122,6 +122,14 @@ PROTOTYPES = {
     "ssm_linear_q8_workspace": (_sz, [_vp, _l, _i, _i, _i]),
     "ssm_linear_q8": (_i, [_i, _vp, _l, _vp, _l, _fp, _fp, _i, _vp, _l, _i, _i, _i, _f, _vp, _sz,
                            _vp]),
+    "ssm_gated_recurrence_workspace": (_sz, [_i, _i, _i]),
+    "ssm_gated_recurrence": (_i, [_i, _vp, _l, _vp, _l, _vp, _l, _fp, _f, _vp, _i, _vp, _l, _i, _i, _i,
+                                  _fp, _fp, _fp, _vp, _sz, _vp]),
+    "ssm_gated_recurrence_backward_workspace": (_sz, [_i, _i, _i]),
+    "ssm_gated_recurrence_backward": (_i, [_i, _vp, _l, _vp, _l, _vp, _l, _vp, _l, _fp, _f, _vp, _i, _fp, _fp,
+                                           _vp, _l, _vp, _l, _vp, _l, _fp, _fp, _i, _i, _i, _vp, _sz,
+                                           _vp]),
+    "ssm_gated_recurrence_step": (_i, [_i, _vp, _l, _vp, _l, _vp, _l, _fp, _f, _vp, _l, _fp, _i, _i, _vp]),
     "ssm_argmax": (_i, [_fp, _l, _i, _i, _vp, _vp]),
     "ssm_sample_workspace": (_sz, [_i, _i]),
     "ssm_sample": (_i, [_fp, _l, _i, _i, _d, _i, _d, _vp, _vp, _vp, _sz, _vp]),

@@ -10,6 +10,7 @@ Shapes (row-major):
   ssd_chunk_scan   x (B,L,H,P); dt (B,L,H); B, C (B,L,G,N); A (H); state (B,H,P,N)
   linear_attention q (B,L,H,K); k (B,L,G,K); v (B,L,G,V); g (H); state (B,H,V,K)
   linear_i8/q8     x (M,K), W (N,K) -> y (M,N)
+  gated_recurrence x, r, i (B,L,D); lam (D); state (B,D)
 """
 from __future__ import annotations
 
@@ -501,3 +502,103 @@ def linear_q8(x, W, sw, bias=None, out=None, out_dtype=None, beta=0.0, workspace
               py, ldy, M, N, K, beta, pws, nbytes,
               _raw_stream(dev) if _raw_stream is not None else _stream())
     return y
+
+
+# ---------------------------------------------------------------- a gated-recurrence layer, both directions
+def _steps(name, t):
+    """Row stride of (B,L,D): rows are contiguous and lie at one distance through the batch."""
+    B, L, D = t.shape
+    if t.is_contiguous():
+        return D
+    sb, st, sd = t.stride()
+    if D > 1 and sd != 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    ld = st if L > 1 else (sb if B > 1 else D)
+    if B > 1 and L > 1 and sb != L * ld:
+        raise ValueError(f"{name}: rows must lie at one distance")
+    return ld
+
+
+def _on(dev):
+    return _raw_stream(dev) if _raw_stream is not None else _stream()
+
+
+def gated_recurrence_states(B, L, D, device):
+    """Room for the states that gated_recurrence keeps for its backward pass: one every 64 tokens."""
+    return torch.empty(B, -(-L // 64), D, device=device, dtype=_f32_t)
+
+
+def gated_recurrence(x, r, i, lam, c=8.0, lengths=None, h0=None, hT=None, out=None, states=None, workspace=None):
+    """Gated linear recurrence over whole prompts (ssm_gated_recurrence): a = e^{-c softplus(lam) sigmoid(r)},
+    h <- a h + sqrt(1 - a^2) sigmoid(i) x, y = h. x, r, i (B,L,D) float32 or bfloat16, y in their type; lam (D)
+    float32. lengths (B) int32: rows of y from a sequence's length on are zeros, or, in an `out` of the caller's,
+    not written. h0, hT (B,D) float32, hT may be h0; `states` (gated_recurrence_states) is filled for the
+    backward pass."""
+    if x.dim() != 3:
+        raise ValueError("x, r, i (B,L,D)")
+    shape, dt = x.shape, x.dtype
+    B, L, D = shape
+    code, dev = _code(dt), _current("x", x)
+    pr, pi = _at("r", r, shape, dt, dev), _at("i", i, shape, dt, dev)
+    pad = out is None
+    if pad:
+        out = x.new_empty(shape)
+    py = _at("out", out, shape, dt, dev)
+    state = (B, D)
+    ws, pws, nbytes = _own_scratch(workspace, _lib.lib().ssm_gated_recurrence_workspace(B, L, D), x)
+    _lib.call("ssm_gated_recurrence", code, x.data_ptr(), _steps("x", x), pr, _steps("r", r), pi, _steps("i", i),
+              _packed("lam", lam, (D,), _f32_t, dev), c, _packed("lengths", lengths, (B,), _i32_t, dev), int(pad),
+              py, _steps("out", out), B, L, D, _packed("h0", h0, state, _f32_t, dev),
+              _packed("hT", hT, state, _f32_t, dev),
+              _packed("states", states, (B, -(-L // 64), D), _f32_t, dev), pws, nbytes, _on(dev))
+    return out
+
+
+def gated_recurrence_backward(dy, x, r, i, lam, states, c=8.0, lengths=None, dhT=None, dh0=None, out=None,
+                              workspace=None):
+    """Gradients of gated_recurrence (ssm_gated_recurrence_backward): returns (dx, dr, di, dlam). dy and the first
+    three (B,L,D) in x's type, dlam (D) float32; `states` as the forward call filled them. dhT, the gradient of hT,
+    and dh0, which receives that of h0: (B,D) float32 or None, dh0 may be dhT. `out`: tensors for dx, dr, di, whose
+    rows from a sequence's length on are not written (else zeros)."""
+    if x.dim() != 3:
+        raise ValueError("x, r, i (B,L,D)")
+    shape, dt = x.shape, x.dtype
+    B, L, D = shape
+    code, dev = _code(dt), _current("x", x)
+    pg, pr, pi = _at("dy", dy, shape, dt, dev), _at("r", r, shape, dt, dev), _at("i", i, shape, dt, dev)
+    pad = out is None
+    if pad:
+        out = x.new_empty(shape), x.new_empty(shape), x.new_empty(shape)
+    dx, dr, di = out
+    pdx, pdr, pdi = (_at(f"out[{n}]", t, shape, dt, dev) for n, t in enumerate(out))
+    dlam = lam.new_empty(D, dtype=_f32_t)
+    state = (B, D)
+    ps = _packed("states", states, (B, -(-L // 64), D), _f32_t, dev)
+    ws, pws, nbytes = _own_scratch(workspace, _lib.lib().ssm_gated_recurrence_backward_workspace(B, L, D), x)
+    _lib.call("ssm_gated_recurrence_backward", code, pg, _steps("dy", dy), x.data_ptr(), _steps("x", x), pr,
+              _steps("r", r), pi, _steps("i", i), _packed("lam", lam, (D,), _f32_t, dev), c,
+              _packed("lengths", lengths, (B,), _i32_t, dev), int(pad), ps,
+              _packed("dhT", dhT, state, _f32_t, dev), pdx, _steps("out[0]", dx), pdr, _steps("out[1]", dr), pdi,
+              _steps("out[2]", di), dlam.data_ptr(), _packed("dh0", dh0, state, _f32_t, dev), B, L, D, pws, nbytes,
+              _on(dev))
+    return dx, dr, di, dlam
+
+
+def gated_recurrence_step(x, r, i, lam, h, c=8.0, out=None):
+    """One token of gated_recurrence for every sequence, h (B,D) float32 in place (ssm_gated_recurrence_step):
+    x, r, i (B,D) -> y (B,D)."""
+    shape, dt = x.shape, x.dtype
+    B, D = shape
+    code, dev = _code(dt), _current("x", x)
+    pr, pi = _at("r", r, shape, dt, dev), _at("i", i, shape, dt, dev)
+    if h is None:
+        raise ValueError("gated_recurrence_step needs a state")
+    ph = _packed("h", h, shape, _f32_t, dev)
+    if out is None:
+        out = x.new_empty(shape)
+        py, ldy = out.data_ptr(), D
+    else:
+        py, ldy = _at("out", out, shape, dt, dev), _ld("out", out)
+    _lib.call("ssm_gated_recurrence_step", code, x.data_ptr(), _ld("x", x), pr, _ld("r", r), pi, _ld("i", i),
+              _packed("lam", lam, (D,), _f32_t, dev), c, py, ldy, ph, B, D, _on(dev))
+    return out
