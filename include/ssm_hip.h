@@ -318,6 +318,45 @@ ssm_status ssm_gated_recurrence_step(int dtype, const void* x, long ldx, const v
                                      long ldi, const float* lam, float c, void* y, long ldy, float* h, int B, int D,
                                      void* stream);
 
+/* The norms around a block, with its gate, residual scale and residual, over T rows of D elements:
+ *   v = y / sqrt(mean y^2 + eps) post silu(z),  x' = x + scale v,  n = x' / sqrt(mean x'^2 + eps) pre
+ * x, y, z (NULL: no gate), x', n with row strides; post, scale, pre (D) float or NULL (ones). x' may be x and n may
+ * be y; outputs overlap nothing else. Rows need no alignment. D <= 16384 (SSM_ERR_UNSUPPORTED above). fp32 in between; n is
+ * formed from x' before that is rounded. */
+ssm_status ssm_block_norm(int dtype, const void* x, long ldx, const void* y, long ldy, const void* z, long ldz,
+                          const float* post, const float* scale, const float* pre, float eps, void* x1, long ldx1, void* n,
+                          long ldn, int T, int D, void* stream);
+/* Its gradients from dx1 (of x'; NULL: zeros) and dn: dx, dy and, with z, dz (T,D), and over all rows dpost, dscale,
+ * dpre (D) float (each may be NULL). dx may be dx1; outputs and the workspace overlap nothing else. Sums over rows are in one
+ * order. T >= 1. workspace: 16-byte aligned, ssm_block_norm_backward_workspace(...) bytes, one stream at a time. */
+size_t ssm_block_norm_backward_workspace(int T, int D);
+ssm_status ssm_block_norm_backward(int dtype, const void* dx1, long lddx1, const void* dn, long lddn, const void* x,
+                                   long ldx, const void* y, long ldy, const void* z, long ldz, const float* post,
+                                   const float* scale, const float* pre, float eps, void* dx, long lddx, void* dy,
+                                   long lddy, void* dz, long lddz, float* dpost, float* dscale, float* dpre, int T, int D,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Log probabilities of given tokens, entropy and the k likeliest tokens of M rows of N logits (`dtype`, row stride ldx):
+ *   log p_j = x_j - log sum e^x,  logp[m] = log p_id,  entropy[m] = -sum p log p
+ * ids (M) int32; one outside 0 .. N - 1 (padding) gives logp 0. logp (needs ids) and entropy (M) float, either may be
+ * NULL. stats (M,2) float, 8-byte aligned, or NULL: max x and log sum e^{x - max}, which the backward pass needs.
+ * top_ids, top_logp (M,k): in descending order, of equal logits the lowest index first; k <= min(N, 64)
+ * (SSM_ERR_UNSUPPORTED above 64). Logits of -inf are tokens that cannot be; a row of nothing else gives logp and
+ * top_logp -inf and entropy 0. A NaN or +inf makes its row's probabilities NaN. One pass over the logits, fp32 sums in
+ * one order. Rows need no alignment. N <= 2^30. workspace: 16-byte aligned, ssm_token_logprobs_workspace(...) bytes (0 where
+ * no row is cut), one stream at a time. */
+size_t ssm_token_logprobs_workspace(int M, int N, int k);
+ssm_status ssm_token_logprobs(int dtype, const void* x, long ldx, const int* ids, int M, int N, int k, float* logp,
+                              float* entropy, float* stats, int* top_ids, float* top_logp, void* workspace,
+                              size_t workspace_bytes, void* stream);
+/* Gradient of the logits from those of logp (dlogp, needs ids) and of the entropy (dentropy, needs entropy), either NULL:
+ *   dx_j = dlogp (delta_{j,id} - p_j) - dentropy p_j (log p_j + entropy)
+ * stats and entropy as the forward call left them; dx (M,N) in x's type, may be x. An id outside 0 .. N - 1 has no
+ * gradient of logp; a row of nothing but -inf gets zeros. */
+ssm_status ssm_token_logprobs_backward(int dtype, const void* x, long ldx, const int* ids, const float* stats,
+                                       const float* entropy, const float* dlogp, const float* dentropy, void* dx,
+                                       long lddx, int M, int N, void* stream);
+
 /* Greedy pick per row (sampleToken with topK = 1, src/session/streaming.ts:74-75): index
  * of the largest value, lowest index among equal maxima; NaN never wins (0 for an all-NaN
  * row). x (rows, n) with row stride ldx; out (rows) uint32. */

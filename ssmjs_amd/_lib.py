@@ -130,6 +130,14 @@ PROTOTYPES = {
                                            _vp, _l, _vp, _l, _vp, _l, _fp, _fp, _i, _i, _i, _vp, _sz,
                                            _vp]),
     "ssm_gated_recurrence_step": (_i, [_i, _vp, _l, _vp, _l, _vp, _l, _fp, _f, _vp, _l, _fp, _i, _i, _vp]),
+    "ssm_block_norm": (_i, [_i, _vp, _l, _vp, _l, _vp, _l, _fp, _fp, _fp, _f, _vp, _l, _vp, _l, _i, _i,
+                            _vp]),
+    "ssm_block_norm_backward_workspace": (_sz, [_i, _i]),
+    "ssm_block_norm_backward": (_i, [_i, _vp, _l, _vp, _l, _vp, _l, _vp, _l, _vp, _l, _fp, _fp, _fp, _f,
+                                     _vp, _l, _vp, _l, _vp, _l, _fp, _fp, _fp, _i, _i, _vp, _sz, _vp]),
+    "ssm_token_logprobs_workspace": (_sz, [_i, _i, _i]),
+    "ssm_token_logprobs": (_i, [_i, _vp, _l, _vp, _i, _i, _i, _fp, _fp, _fp, _vp, _fp, _vp, _sz, _vp]),
+    "ssm_token_logprobs_backward": (_i, [_i, _vp, _l, _vp, _fp, _fp, _fp, _fp, _vp, _l, _i, _i, _vp]),
     "ssm_argmax": (_i, [_fp, _l, _i, _i, _vp, _vp]),
     "ssm_sample_workspace": (_sz, [_i, _i]),
     "ssm_sample": (_i, [_fp, _l, _i, _i, _d, _i, _d, _vp, _vp, _vp, _sz, _vp]),

@@ -1,0 +1,439 @@
+// The norms around a block, one pass over its rows: with y the block's output, x the residual stream and z its gate,
+//   w = y / sqrt(mean y^2 + eps),  u = w post,  v = u silu(z),  x' = x + scale v,  n = x' / sqrt(mean x'^2 + eps) pre
+// and the gradients of all of it: with g that of x' (its own and the one through n),
+//   d = dn pre,  g = dx' + (d - n^ mean(d n^)) / rms(x')   (n^ = x' / rms(x'))
+//   dx = g,  t = g scale,  dz = t u s (1 + z (1 - s)),  s = sigmoid(z),  c = t silu(z) post
+//   dy = (c - w mean(c w)) / rms(y);  dscale = sum g v,  dpre = sum dn n^,  dpost = sum t silu(z) w  over the rows.
+// Sums and everything between the loads and the stores are in fp32; x' enters n before its own rounding.
+//
+// Memory bound. A row lies in the registers of one wave, or of a few where it is long: each element is read once and
+// written once, and the sums over a row are lane exchanges. Rows need no alignment: vector loads and stores of
+// eight elements are made at the elements' own alignment, which the hardware splits where it must.
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace {
+
+constexpr int kMaxD = 16384;
+
+// Eight elements of a row, as they lie in memory; `left` of them exist.
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+    float v[8];
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    __device__ __forceinline__ void load(const float* p, int left) {
+        if (left >= 8) {
+            const f4 a = __builtin_nontemporal_load(reinterpret_cast<const f4*>(p)),
+                     b = __builtin_nontemporal_load(reinterpret_cast<const f4*>(p) + 1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.f;
+        }
+    }
+    __device__ __forceinline__ float operator[](int j) const { return v[j]; }
+    static __device__ __forceinline__ void store(const float (&f)[8], float* p, int left) {
+        if (left >= 8) {
+            reinterpret_cast<f4*>(p)[0] = f4{f[0], f[1], f[2], f[3]};
+            reinterpret_cast<f4*>(p)[1] = f4{f[4], f[5], f[6], f[7]};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < left) p[j] = f[j];
+        }
+    }
+};
+template <> struct Eight<__bf16> {
+    typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    unsigned v[4];
+    __device__ __forceinline__ void load(const __bf16* p, int left) {
+        if (left >= 8) {
+            const u4 a = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = a[j];
+        } else {
+            const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j] = (2 * j < left ? h[2 * j] : 0u) | (2 * j + 1 < left ? (unsigned)h[2 * j + 1] << 16 : 0u);
+        }
+    }
+    __device__ __forceinline__ float operator[](int j) const {
+        return __builtin_bit_cast(float, j % 2 ? v[j / 2] & 0xffff0000u : v[j / 2] << 16);
+    }
+    static __device__ __forceinline__ void store(const float (&f)[8], __bf16* p, int left) {
+        if (left >= 8) {
+            b8 b;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = (__bf16)f[j];
+            *reinterpret_cast<u4*>(p) = __builtin_bit_cast(u4, b);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < left) p[j] = (__bf16)f[j];
+        }
+    }
+};
+
+// Eight weights (none: ones).
+__device__ __forceinline__ void weights(const float* w, int e, int left, float (&f)[8]) {
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    if (!w) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = 1.f;
+    } else if (left >= 8) {
+        const f4 a = *reinterpret_cast<const f4*>(w + e), b = *reinterpret_cast<const f4*>(w + e + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = a[j], f[4 + j] = b[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = j < left ? w[e + j] : 0.f;
+    }
+}
+
+struct NormArgs {
+    const void* x; long ldx;
+    const void* y; long ldy;
+    const void* z; long ldz;      // (null: no gate)
+    const float* post; const float* scale; const float* pre;
+    void* x1; long ldx1;          // x', or dx
+    void* n; long ldn;            // n, or dy
+    const void* dx1; long lddx1;  // (null: zeros)
+    const void* dn; long lddn;
+    void* dz; long lddz;
+    float* part;                  // the workgroups' column sums: dpost, dscale, dpre of D each
+    int T, D;
+    float eps;
+};
+
+// Sum over the lanes of a row: one wave, or WPR waves through `red` (two buffers in turn: one barrier a sum).
+template <int WPR>
+__device__ __forceinline__ float row_sum(float s, float (&red)[2][WPR], int& turn) {
+#pragma unroll
+    for (int k = 32; k > 0; k /= 2) s += __shfl_xor(s, k);
+    if constexpr (WPR > 1) {
+        if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = 0.f;
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) s += red[turn][w];
+        turn ^= 1;
+    }
+    return s;
+}
+
+template <typename T> __device__ __forceinline__ const T* row_of(const void* p, long ld, long t) {
+    return static_cast<const T*>(p) + t * ld;
+}
+template <typename T> __device__ __forceinline__ T* row_of(void* p, long ld, long t) { return static_cast<T*>(p) + t * ld; }
+
+// 512 NC WPR elements a row at most; four rows a workgroup where a row is one wave's.
+template <typename T, int NC, int WPR, bool GATE>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_kernel(NormArgs a) {
+    __shared__ float red[2][WPR];
+    int turn = 0;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const long t = WPR == 1 ? (long)blockIdx.x * 4 + w : blockIdx.x;
+    if (t >= a.T) return;
+    const int e0 = ((WPR == 1 ? 0 : w * NC) * 64 + lane) * 8;   // chunk c begins at e0 + 512 c
+    const T* px = row_of<T>(a.x, a.ldx, t) + e0;
+    const T* py = row_of<T>(a.y, a.ldy, t) + e0;
+    const T* pz = GATE ? row_of<T>(a.z, a.ldz, t) + e0 : nullptr;
+    Eight<T> x[NC], y[NC], z[NC];
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        y[c].load(py + 512 * c, a.D - e0 - 512 * c);
+        x[c].load(px + 512 * c, a.D - e0 - 512 * c);
+        if constexpr (GATE) z[c].load(pz + 512 * c, a.D - e0 - 512 * c);
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fmaf(y[c][j], y[c][j], ss);
+    const float inv = 1.f / (float)a.D;
+    const float ry = __builtin_amdgcn_rsqf(fmaf(row_sum<WPR>(ss, red, turn), inv, a.eps));
+    float x1[NC][8];
+    ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int e = e0 + 512 * c;
+        float post[8], scale[8];
+        weights(a.post, e, a.D - e, post);
+        weights(a.scale, e, a.D - e, scale);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float u = y[c][j] * ry * post[j];
+            if constexpr (GATE) u *= ssm::silu_fast(z[c][j]);
+            x1[c][j] = fmaf(scale[j], u, x[c][j]);
+            ss = fmaf(x1[c][j], x1[c][j], ss);
+        }
+    }
+    const float rx = __builtin_amdgcn_rsqf(fmaf(row_sum<WPR>(ss, red, turn), inv, a.eps));
+    T* p1 = row_of<T>(a.x1, a.ldx1, t);
+    T* pn = row_of<T>(a.n, a.ldn, t);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int e = e0 + 512 * c;
+        float pre[8], n[8];
+        weights(a.pre, e, a.D - e, pre);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) n[j] = x1[c][j] * rx * pre[j];
+        Eight<T>::store(x1[c], p1 + e, a.D - e);
+        Eight<T>::store(n, pn + e, a.D - e);
+    }
+}
+
+template <typename T, int NC, int WPR, bool GATE>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_backward(NormArgs a) {
+    __shared__ float red[2][WPR];
+    __shared__ float cols[WPR == 1 ? 4 : 1][WPR == 1 ? 512 * NC : 1];
+    int turn = 0;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int e0 = ((WPR == 1 ? 0 : w * NC) * 64 + lane) * 8;
+    const float inv = 1.f / (float)a.D;
+    float spost[NC][8] = {}, sscale[NC][8] = {}, spre[NC][8] = {};
+    const long step = WPR == 1 ? 4L * gridDim.x : gridDim.x;
+    for (long t = WPR == 1 ? (long)blockIdx.x * 4 + w : blockIdx.x; t < a.T; t += step) {
+        Eight<T> x[NC], y[NC], z[NC], dn[NC], g0[NC];
+        float ss = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int e = e0 + 512 * c, left = a.D - e;
+            y[c].load(row_of<T>(a.y, a.ldy, t) + e, left);
+            x[c].load(row_of<T>(a.x, a.ldx, t) + e, left);
+            if constexpr (GATE) z[c].load(row_of<T>(a.z, a.ldz, t) + e, left);
+            dn[c].load(row_of<T>(a.dn, a.lddn, t) + e, left);
+            g0[c].load(a.dx1 ? row_of<T>(a.dx1, a.lddx1, t) + e : nullptr, a.dx1 ? left : 0);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss = fmaf(y[c][j], y[c][j], ss);
+        const float ry = __builtin_amdgcn_rsqf(fmaf(row_sum<WPR>(ss, red, turn), inv, a.eps));
+        float x1[NC][8];
+        float s1 = 0.f, sd = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int e = e0 + 512 * c;
+            float post[8], scale[8], pre[8];
+            weights(a.post, e, a.D - e, post);
+            weights(a.scale, e, a.D - e, scale);
+            weights(a.pre, e, a.D - e, pre);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float u = y[c][j] * ry * post[j];
+                if constexpr (GATE) u *= ssm::silu_fast(z[c][j]);
+                x1[c][j] = fmaf(scale[j], u, x[c][j]);
+                s1 = fmaf(x1[c][j], x1[c][j], s1);
+                sd = fmaf(dn[c][j] * pre[j], x1[c][j], sd);
+            }
+        }
+        const float rx = __builtin_amdgcn_rsqf(fmaf(row_sum<WPR>(s1, red, turn), inv, a.eps));
+        const float m1 = row_sum<WPR>(sd, red, turn) * rx * inv;   // mean of d n^
+        float s2 = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int e = e0 + 512 * c;
+            float post[8], scale[8], pre[8], dz[8];
+            weights(a.post, e, a.D - e, post);
+            weights(a.scale, e, a.D - e, scale);
+            weights(a.pre, e, a.D - e, pre);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float nh = x1[c][j] * rx, g = fmaf(rx, dn[c][j] * pre[j] - nh * m1, g0[c][j]);
+                const float wv = y[c][j] * ry, u = wv * post[j];
+                spre[c][j] = fmaf(dn[c][j], nh, spre[c][j]);
+                float t1 = g * scale[j], v = u;
+                if constexpr (GATE) {
+                    const float zj = z[c][j], s = __builtin_amdgcn_rcpf(1.f + __expf(-zj)), sl = zj * s;
+                    dz[j] = t1 * u * (s * fmaf(zj, 1.f - s, 1.f));
+                    v = u * sl;
+                    t1 *= sl;
+                }
+                sscale[c][j] = fmaf(g, v, sscale[c][j]);
+                spost[c][j] = fmaf(t1, wv, spost[c][j]);
+                s2 = fmaf(t1 * post[j], wv, s2);
+                x1[c][j] = g;
+            }
+            Eight<T>::store(x1[c], row_of<T>(a.x1, a.ldx1, t) + e, a.D - e);
+            if constexpr (GATE) Eight<T>::store(dz, row_of<T>(a.dz, a.lddz, t) + e, a.D - e);
+        }
+        const float m2 = row_sum<WPR>(s2, red, turn) * inv;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int e = e0 + 512 * c;
+            float post[8], scale[8], dy[8];
+            weights(a.post, e, a.D - e, post);
+            weights(a.scale, e, a.D - e, scale);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float t1 = x1[c][j] * scale[j];
+                if constexpr (GATE) t1 *= ssm::silu_fast(z[c][j]);
+                dy[j] = ry * (t1 * post[j] - y[c][j] * ry * m2);
+            }
+            Eight<T>::store(dy, row_of<T>(a.n, a.ldn, t) + e, a.D - e);
+        }
+    }
+    // the workgroup's column sums
+    float* part = a.part + (long)blockIdx.x * 3 * a.D;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        float (&s)[NC][8] = k == 0 ? spost : k == 1 ? sscale : spre;
+        if constexpr (WPR == 1) {
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) cols[w][512 * c + lane * 8 + j] = s[c][j];
+            __syncthreads();
+            for (int e = threadIdx.x; e < a.D; e += 256)
+                part[(long)k * a.D + e] = (cols[0][e] + cols[1][e]) + (cols[2][e] + cols[3][e]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (e0 + 512 * c + j < a.D) part[(long)k * a.D + e0 + 512 * c + j] = s[c][j];
+        }
+    }
+}
+
+// Column sums of n rows of 3 D partial sums, in one order: dpost, dscale, dpre (null: not wanted).
+__global__ __launch_bounds__(1024) void norm_columns(const float* __restrict__ part, int n, int D, float* dpost,
+                                                     float* dscale, float* dpre) {
+    __shared__ float sum[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, k = blockIdx.y, e = blockIdx.x * 64 + lane;
+    float* out = k == 0 ? dpost : k == 1 ? dscale : dpre;
+    if (!out) return;
+    float s = 0.f;
+    if (e < D)
+#pragma unroll 4
+        for (int r = w; r < n; r += 16) s += part[((long)r * 3 + k) * D + e];
+    sum[w][lane] = s;
+    __syncthreads();
+    if (w || e >= D) return;
+#pragma unroll
+    for (int r = 8; r > 0; r /= 2)
+        for (int q = 0; q < r; ++q) sum[q][lane] += sum[q + r][lane];
+    out[e] = sum[0][lane];
+}
+
+template <typename T, int NC, int WPR>
+void go_forward(const NormArgs& a, hipStream_t st) {
+    const unsigned n = (unsigned)(WPR == 1 ? ssm::cdiv(a.T, 4) : a.T), threads = WPR == 1 ? 256 : 64 * WPR;
+    if (a.z) norm_kernel<T, NC, WPR, true><<<n, threads, 0, st>>>(a);
+    else norm_kernel<T, NC, WPR, false><<<n, threads, 0, st>>>(a);
+}
+template <typename T>
+void forward_of(const NormArgs& a, hipStream_t st) {
+    if (a.D <= 512) go_forward<T, 1, 1>(a, st);
+    else if (a.D <= 1024) go_forward<T, 2, 1>(a, st);
+    else if (a.D <= 2048) go_forward<T, 4, 1>(a, st);
+    else if (a.D <= 4096) go_forward<T, 4, 2>(a, st);
+    else if (a.D <= 8192) go_forward<T, 4, 4>(a, st);
+    else go_forward<T, 4, 8>(a, st);
+}
+
+// Workgroups of the backward pass: each keeps column sums, which go to memory once.
+int groups_back(int T, int D) { return (int)std::min(D <= 1024 ? ssm::cdiv(T, 4) : (long)T, 512L); }
+
+template <typename T, int NC, int WPR>
+void go_backward(const NormArgs& a, hipStream_t st) {
+    const unsigned n = (unsigned)groups_back(a.T, a.D), threads = WPR == 1 ? 256 : 64 * WPR;
+    if (a.z) norm_backward<T, NC, WPR, true><<<n, threads, 0, st>>>(a);
+    else norm_backward<T, NC, WPR, false><<<n, threads, 0, st>>>(a);
+}
+template <typename T>
+void backward_of(const NormArgs& a, hipStream_t st) {
+    if (a.D <= 512) go_backward<T, 1, 1>(a, st);
+    else if (a.D <= 1024) go_backward<T, 2, 1>(a, st);
+    else if (a.D <= 2048) go_backward<T, 2, 2>(a, st);
+    else if (a.D <= 4096) go_backward<T, 2, 4>(a, st);
+    else if (a.D <= 8192) go_backward<T, 2, 8>(a, st);
+    else go_backward<T, 2, 16>(a, st);
+}
+
+}  // namespace
+
+extern "C" ssm_status ssm_block_norm(int dtype, const void* x, long ldx, const void* y, long ldy, const void* z,
+                                     long ldz, const float* post, const float* scale, const float* pre, float eps,
+                                     void* x1, long ldx1, void* n, long ldn, int T, int D, void* stream) {
+    SSM_REQUIRE(dtype == SSM_F32 || dtype == SSM_BF16, "ssm_block_norm: bad dtype");
+    SSM_REQUIRE(T >= 0 && D > 0, "ssm_block_norm: bad shape");
+    SSM_REQUIRE(eps >= 0.f, "ssm_block_norm: eps below 0");
+    if (D > kMaxD) return ssm::fail(SSM_ERR_UNSUPPORTED, "ssm_block_norm: rows of %d elements, at most %d", D, kMaxD);
+    if (T == 0) return SSM_OK;
+    SSM_REQUIRE(x && y && x1 && n, "ssm_block_norm: null input");
+    if (T == 1) ldx = ldy = ldz = ldx1 = ldn = D;
+    SSM_REQUIRE(ldx >= D && ldy >= D && (!z || ldz >= D) && ldx1 >= D && ldn >= D, "ssm_block_norm: row stride below row width");
+    SSM_REQUIRE(T <= ssm::kMaxGroups / 4, "ssm_block_norm: too many rows");
+    const long es = dtype == SSM_F32 ? 4 : 2;
+    auto op = [&](const void* p, long ld) { return ssm::Rows{p, ld * es, D * es, T}; };
+    const ssm::Rows rx = op(x, ldx), ry = op(y, ldy), rz = op(z, ldz), o1 = op(x1, ldx1), on = op(n, ldn),
+                    w0 = ssm::block(post, 4L * D), w1 = ssm::block(scale, 4L * D), w2 = ssm::block(pre, 4L * D);
+    // a row is read before it is written: x' may be x, n may be y
+    SSM_REQUIRE(!ssm::meets(o1, ry, rz, on, w0, w1, w2) && !ssm::meets(on, rx, rz, w0, w1, w2) &&
+                    ((x1 == x && ldx1 == ldx) || !ssm::meet(o1, rx)) && ((n == y && ldn == ldy) || !ssm::meet(on, ry)),
+                "ssm_block_norm: an output overlaps an operand that it is not");
+    NormArgs a{};
+    a.x = x; a.ldx = ldx; a.y = y; a.ldy = ldy; a.z = z; a.ldz = ldz; a.post = post; a.scale = scale; a.pre = pre;
+    a.x1 = x1; a.ldx1 = ldx1; a.n = n; a.ldn = ldn; a.T = T; a.D = D; a.eps = eps;
+    if (dtype == SSM_F32) forward_of<float>(a, (hipStream_t)stream);
+    else forward_of<__bf16>(a, (hipStream_t)stream);
+    return ssm::check_launch("ssm_block_norm");
+}
+
+extern "C" size_t ssm_block_norm_backward_workspace(int T, int D) {
+    return T > 0 && D > 0 ? (size_t)groups_back(T, D) * 3 * D * sizeof(float) : 0;
+}
+
+extern "C" ssm_status ssm_block_norm_backward(int dtype, const void* dx1, long lddx1, const void* dn, long lddn,
+                                              const void* x, long ldx, const void* y, long ldy, const void* z, long ldz,
+                                              const float* post, const float* scale, const float* pre, float eps, void* dx,
+                                              long lddx, void* dy, long lddy, void* dz, long lddz, float* dpost,
+                                              float* dscale, float* dpre, int T, int D, void* workspace,
+                                              size_t workspace_bytes, void* stream) {
+    SSM_REQUIRE(dtype == SSM_F32 || dtype == SSM_BF16, "ssm_block_norm_backward: bad dtype");
+    SSM_REQUIRE(T > 0 && D > 0, "ssm_block_norm_backward: bad shape");
+    SSM_REQUIRE(eps >= 0.f, "ssm_block_norm_backward: eps below 0");
+    if (D > kMaxD)
+        return ssm::fail(SSM_ERR_UNSUPPORTED, "ssm_block_norm_backward: rows of %d elements, at most %d", D, kMaxD);
+    SSM_REQUIRE(dn && x && y && dx && dy && (!z || dz), "ssm_block_norm_backward: null input");
+    if (!z) dz = nullptr;
+    if (T == 1) lddx1 = lddn = ldx = ldy = ldz = lddx = lddy = lddz = D;
+    SSM_REQUIRE((!dx1 || lddx1 >= D) && lddn >= D && ldx >= D && ldy >= D && (!z || (ldz >= D && lddz >= D)) &&
+                    lddx >= D && lddy >= D, "ssm_block_norm_backward: row stride below row width");
+    SSM_REQUIRE(T <= ssm::kMaxGroups / 4, "ssm_block_norm_backward: too many rows");
+    const size_t need = ssm_block_norm_backward_workspace(T, D);
+    SSM_REQUIRE(workspace && workspace_bytes >= need, "ssm_block_norm_backward: needs a workspace of %zu bytes", need);
+    SSM_REQUIRE(((uintptr_t)workspace & 15) == 0, "ssm_block_norm_backward: workspace must be 16-byte aligned");
+    const long es = dtype == SSM_F32 ? 4 : 2;
+    auto op = [&](const void* p, long ld) { return ssm::Rows{p, ld * es, D * es, T}; };
+    const ssm::Rows g1 = op(dx1, lddx1), gn = op(dn, lddn), rx = op(x, ldx), ry = op(y, ldy), rz = op(z, ldz),
+                    ox = op(dx, lddx), oy = op(dy, lddy), oz = op(dz, lddz), w0 = ssm::block(post, 4L * D),
+                    w1 = ssm::block(scale, 4L * D), w2 = ssm::block(pre, 4L * D), s0 = ssm::block(dpost, 4L * D),
+                    s1 = ssm::block(dscale, 4L * D), s2 = ssm::block(dpre, 4L * D), ws = ssm::block(workspace, need);
+    auto clear = [&](const ssm::Rows& o) { return !ssm::meets(o, gn, rx, ry, rz, w0, w1, w2); };
+    // a row's gradient dx' is read before dx is written: they may be one
+    SSM_REQUIRE(clear(ox) && clear(oy) && clear(oz) && clear(s0) && clear(s1) && clear(s2) && clear(ws) &&
+                    ((dx == dx1 && lddx == lddx1) || !ssm::meet(ox, g1)) && !ssm::meets(g1, oy, oz, s0, s1, s2, ws) &&
+                    !ssm::meets(ox, oy, oz, s0, s1, s2, ws) && !ssm::meets(oy, oz, s0, s1, s2, ws) &&
+                    !ssm::meets(oz, s0, s1, s2, ws) && !ssm::meets(s0, s1, s2, ws) && !ssm::meets(s1, s2, ws) &&
+                    !ssm::meet(s2, ws),
+                "ssm_block_norm_backward: an output or the workspace overlaps an operand that it is not");
+    NormArgs a{};
+    a.x = x; a.ldx = ldx; a.y = y; a.ldy = ldy; a.z = z; a.ldz = ldz; a.post = post; a.scale = scale; a.pre = pre;
+    a.dx1 = dx1; a.lddx1 = lddx1; a.dn = dn; a.lddn = lddn;
+    a.x1 = dx; a.ldx1 = lddx; a.n = dy; a.ldn = lddy; a.dz = dz; a.lddz = lddz;
+    a.part = static_cast<float*>(workspace); a.T = T; a.D = D; a.eps = eps;
+    if (dtype == SSM_F32) backward_of<float>(a, (hipStream_t)stream);
+    else backward_of<__bf16>(a, (hipStream_t)stream);
+    if (dpost || dscale || dpre)
+        norm_columns<<<dim3((unsigned)ssm::cdiv(D, 64), 3), 1024, 0, (hipStream_t)stream>>>(a.part, groups_back(T, D), D,
+                                                                                          dpost, dscale, dpre);
+    return ssm::check_launch("ssm_block_norm_backward");
+}

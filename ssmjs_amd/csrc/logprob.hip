@@ -1,0 +1,403 @@
+// Log probabilities of given tokens, entropy and the likeliest tokens of rows of logits, in one pass over them, and
+// their gradient. With m = max x, Z = sum e^{x-m}, S = sum e^{x-m} (x - m):
+//   log p_j = x_j - m - log Z,   H = -sum p log p = log Z - S / Z
+//   dx_j = w (delta_{j,id} - p_j) - v p_j (log p_j + H)   for the gradients w of log p_id and v of H
+// A lane keeps its own (m, Z, S) and rescales it where m grows (Milakov & Gimelshein 2018); lanes, waves and
+// slices of a row are joined the same way, in one order.
+//
+// Likeliest tokens: a wave keeps a list of 64 in its lanes, sorted by one key for each logit (larger for larger
+// values and, of equal ones, for lower indices). The first 2048 logits give the maximum of each lane, sorted at once;
+// from there on a logit enters only past the list's k-th, which few do: about k ln(n / 2048) of a random row.
+//
+// Memory bound: one read of the logits; the gradient reads and writes each once.
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace {
+
+constexpr int kMaxTop = 64;
+constexpr int kGroups = 4, kWaveRun = 64 * 8 * kGroups, kRun = 4 * kWaveRun;   // logits of a wave's and a workgroup's turn
+constexpr float kFloor = -200.f;   // e^kFloor is 0 in fp32: differences are held above it where they multiply a 0
+constexpr float kLowest = -3.40282347e38f;
+typedef unsigned long long u64;
+
+template <typename T> __device__ __forceinline__ void load8(const T* p, int left, float (&f)[8]);
+template <> __device__ __forceinline__ void load8(const float* p, int left, float (&f)[8]) {
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    if (left >= 8) {
+        const f4 a = reinterpret_cast<const f4*>(p)[0], b = reinterpret_cast<const f4*>(p)[1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = a[j], f[4 + j] = b[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = j < left ? p[j] : -__builtin_inff();
+    }
+}
+template <> __device__ __forceinline__ void load8(const __bf16* p, int left, float (&f)[8]) {
+    typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(2)));
+    if (left >= 8) {
+        const u4 a = *reinterpret_cast<const u4*>(p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __builtin_bit_cast(float, j % 2 ? a[j / 2] & 0xffff0000u : a[j / 2] << 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = j < left ? (float)p[j] : -__builtin_inff();
+    }
+}
+__device__ __forceinline__ void store8(float* p, int left, const float (&f)[8]) {
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    if (left >= 8) {
+        reinterpret_cast<f4*>(p)[0] = f4{f[0], f[1], f[2], f[3]};
+        reinterpret_cast<f4*>(p)[1] = f4{f[4], f[5], f[6], f[7]};
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) p[j] = f[j];
+    }
+}
+__device__ __forceinline__ void store8(__bf16* p, int left, const float (&f)[8]) {
+    typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    if (left >= 8) {
+        b8 b;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = (__bf16)f[j];
+        *reinterpret_cast<u4*>(p) = __builtin_bit_cast(u4, b);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) p[j] = (__bf16)f[j];
+    }
+}
+
+// ---------------------------------------------------------------- sums
+struct Sums {
+    float m, z, s;
+};
+__device__ __forceinline__ float grow(float d) { return ssm::ex2(ssm::kLog2e * d); }   // e^d
+__device__ __forceinline__ void raise(Sums& a, float m) {   // the same sums from a maximum m >= a.m
+    const float d = fmaxf(a.m - m, kFloor), f = grow(d);
+    a.s = f * fmaf(a.z, d, a.s);
+    a.z *= f;
+    a.m = m;
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+    const float m = fmaxf(a.m, b.m);
+    raise(a, m);
+    raise(b, m);
+    return Sums{m, a.z + b.z, a.s + b.s};
+}
+__device__ __forceinline__ void take8(Sums& a, const float (&x)[8]) {
+    float m = a.m;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, x[j]);
+    raise(a, m);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float d = x[j] - m, e = grow(d);
+        a.z += e;
+        a.s = fmaf(e, fmaxf(d, kFloor), a.s);
+    }
+}
+__device__ __forceinline__ Sums over_wave(Sums a) {
+#pragma unroll
+    for (int k = 32; k > 0; k /= 2) a = join(a, Sums{__shfl_xor(a.m, k), __shfl_xor(a.z, k), __shfl_xor(a.s, k)});
+    return a;
+}
+
+// ---------------------------------------------------------------- keys
+// Larger for larger values and, of equal ones, for lower indices; never 0; a NaN below all else.
+__device__ __forceinline__ u64 key_of(float x, unsigned index) {
+    const unsigned b = __builtin_bit_cast(unsigned, x + 0.f);   // (-0 equals 0)
+    const unsigned o = x != x ? 0u : (b & 0x80000000u ? ~b : b | 0x80000000u);
+    return (u64)o << 32 | (0xffffffffu - index);
+}
+__device__ __forceinline__ float value_of(u64 key) {
+    const unsigned o = (unsigned)(key >> 32);
+    return o == 0u ? __builtin_nanf("") : __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ unsigned index_of(u64 key) { return 0xffffffffu - (unsigned)key; }
+
+__device__ __forceinline__ u64 shfl64(u64 v, int lane) {
+    return (u64)(unsigned)__shfl((int)(v >> 32), lane) << 32 | (unsigned)__shfl((int)v, lane);
+}
+__device__ __forceinline__ u64 lane64(u64 v, int lane) {   // lane: the same in all lanes
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (unsigned)__builtin_amdgcn_readlane((int)v, lane);
+}
+// The lanes' keys in descending order over the lanes.
+__device__ u64 sorted(u64 v, int lane) {
+    for (int k = 2; k <= 64; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            const u64 o = shfl64(v, lane ^ j);
+            const bool high = ((lane & j) == 0) == ((lane & k) == 0);   // this lane takes the larger one
+            v = (v > o) == high ? v : o;
+        }
+    return v;
+}
+// A key enters the sorted list, whose last one leaves it.
+__device__ __forceinline__ u64 entered(u64 list, u64 key, int lane) {
+    const int at = __popcll(__ballot(list > key));
+    const u64 below = shfl64(list, (lane + 63) & 63);
+    return lane < at ? list : lane == at ? key : below;
+}
+
+struct LogArgs {
+    const void* x; long ldx;
+    const int* ids;
+    float* logp; float* ent; float2* stats;
+    int* top; float* toplp;
+    Sums* sums; u64* keys;   // the slices' results
+    int M, N, k, slices, turns;
+};
+
+// What a row's results are, from its sums and its lists' keys (`have` of them in LDS, unique; 0: none).
+template <typename T>
+__device__ void finish(const LogArgs& a, int row, Sums s, const u64* keys, int have) {
+    // (nothing left: Z = 0)
+    const bool none = s.z == 0.f;
+    const float m = fmaxf(s.m, kLowest), logz = none ? -__builtin_inff() : logf(s.z);
+    if (threadIdx.x == 0) {
+        if (a.stats) a.stats[row] = make_float2(m, logz);
+        const float h = logz - s.s / s.z;
+        if (a.ent) a.ent[row] = none || h < 0.f ? 0.f : h;   // (below 0 by rounding)
+        if (a.logp) {
+            const int id = a.ids[row];
+            const bool given = id >= 0 && id < a.N;
+            a.logp[row] = !given ? 0.f : none ? -__builtin_inff() : ((float)static_cast<const T*>(a.x)[row * a.ldx + id] - m) - logz;
+        }
+    }
+    for (int c = threadIdx.x; c < have; c += blockDim.x) {
+        const u64 mine = keys[c];
+        if (!mine) continue;
+        int rank = 0;
+        for (int o = 0; o < have; ++o) rank += keys[o] > mine;
+        if (rank < a.k) {
+            a.top[(long)row * a.k + rank] = (int)index_of(mine);
+            a.toplp[(long)row * a.k + rank] = none ? -__builtin_inff() : (value_of(mine) - m) - logz;
+        }
+    }
+}
+
+template <typename T, bool TOP>
+__global__ __launch_bounds__(256) void logprob_kernel(LogArgs a) {
+    __shared__ Sums ws[4];
+    __shared__ u64 lists[TOP ? 4 * kMaxTop : 1];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    const int begin = slice * a.turns, end = begin + a.turns;
+    Sums s{kLowest, 0.f, 0.f};
+    u64 list = 0, least = 0;   // least: the k-th of the list
+    float bar = 0.f;           // its value
+    bool full = false;
+    for (int turn = begin; turn < end; ++turn) {
+        const int base = turn * kRun + w * kWaveRun;   // (below 2^31: N is at most 2^30)
+        if (base >= a.N) break;
+        float v[kGroups][8];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) load8<T>(x + base + (g * 64 + lane) * 8, a.N - base - (g * 64 + lane) * 8, v[g]);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) take8(s, v[g]);
+        if constexpr (TOP) {
+            u64 own = 0;
+            if (!full) {   // the first turn: the lanes' maxima
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int at = base + (g * 64 + lane) * 8 + j;
+                        const u64 key = at < a.N ? key_of(v[g][j], at) : 0;
+                        own = key > own ? key : own;
+                    }
+                list = sorted(own, lane);
+                least = lane64(list, a.k - 1);
+                bar = least ? value_of(least) : __builtin_nanf("");
+            }
+            bool some = false;   // (all earlier logits of the wave have lower indices: equal ones stay out)
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) some |= full ? !(v[g][j] <= bar) : !(v[g][j] < bar);
+            if (__any(some)) {
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (!__any(!(v[g][j] < bar))) continue;
+                        const int at = base + (g * 64 + lane) * 8 + j;
+                        const u64 key = at < a.N ? key_of(v[g][j], at) : 0;
+                        u64 left = __ballot(key > least && key != own);
+                        while (left) {
+                            const int l = __builtin_ctzll(left);
+                            list = entered(list, lane64(key, l), lane);
+                            least = lane64(list, a.k - 1);
+                            left &= left - 1;
+                            left &= __ballot(key > least);
+                        }
+                        bar = least ? value_of(least) : __builtin_nanf("");
+                    }
+            }
+            full = least != 0;
+        }
+    }
+    s = over_wave(s);
+    if (lane == 0) ws[w] = s;
+    if constexpr (TOP)
+        if (lane < a.k) lists[w * a.k + lane] = list;
+    __syncthreads();
+    s = join(join(ws[0], ws[1]), join(ws[2], ws[3]));
+    if (a.slices == 1) {
+        finish<T>(a, row, s, lists, TOP ? 4 * a.k : 0);
+        return;
+    }
+    if (threadIdx.x == 0) a.sums[blockIdx.x] = s;
+    if constexpr (TOP)
+        for (int c = threadIdx.x; c < 4 * a.k; c += 256) {
+            const u64 mine = lists[c];
+            int rank = 0, there = 0;
+            for (int o = 0; o < 4 * a.k; ++o) rank += lists[o] > mine, there += lists[o] != 0;
+            u64* out = a.keys + (long)blockIdx.x * a.k;
+            if (mine && rank < a.k) out[rank] = mine;
+            if (c < a.k && c >= there) out[c] = 0;
+        }
+}
+
+// The slices of a row together.
+template <typename T>
+__global__ __launch_bounds__(256) void logprob_join(LogArgs a) {
+    extern __shared__ u64 all[];
+    const int row = blockIdx.x, have = a.slices * a.k;
+    for (int c = threadIdx.x; c < have; c += 256) all[c] = a.keys[(long)row * have + c];
+    Sums s{kLowest, 0.f, 0.f};
+    for (int c = 0; c < a.slices; ++c) s = join(s, a.sums[(long)row * a.slices + c]);
+    __syncthreads();
+    finish<T>(a, row, s, all, have);
+}
+
+struct GradArgs {
+    const void* x; long ldx;
+    const int* ids;
+    const float2* stats;
+    const float* ent; const float* dlogp; const float* dent;
+    void* dx; long lddx;
+    int M, N, pieces;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
+    const int row = blockIdx.x / a.pieces, piece = blockIdx.x - row * a.pieces;
+    const float2 st = a.stats[row];
+    const int id = a.ids ? a.ids[row] : -1;
+    const float w = a.dlogp && id >= 0 && id < a.N ? a.dlogp[row] : 0.f;
+    const float v = a.dent ? a.dent[row] : 0.f, h = a.dent ? a.ent[row] : 0.f;
+    const bool none = st.y == -__builtin_inff();
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+    float f[kGroups][8];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int at = piece * kRun + (g * 256 + (int)threadIdx.x) * 8;
+        load8<T>(x + at, a.N - at, f[g]);
+    }
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int at = piece * kRun + (g * 256 + (int)threadIdx.x) * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float lp = (f[g][j] - st.x) - st.y, p = grow(lp);
+            const float d = -p * fmaf(v, fmaxf(lp, kFloor) + h, w);
+            f[g][j] = none ? 0.f : at + j == id ? d + w : d;
+        }
+        store8(dx + at, a.N - at, f[g]);
+    }
+}
+
+// Slices of a row: workgroups enough for the chip (four a CU), each of at least one turn.
+int slices_of(int M, int N) {
+    const long turns = ssm::cdiv(N, kRun);
+    return (int)std::max(1L, std::min(std::min(turns, 64L), 1024L / std::max(1, M)));
+}
+
+size_t sums_bytes(int M, int slices) { return ((size_t)M * slices * sizeof(Sums) + 15) / 16 * 16; }
+
+template <typename T>
+void run_logprobs(const LogArgs& a, hipStream_t st) {
+    const unsigned n = (unsigned)((long)a.M * a.slices);
+    if (a.k) logprob_kernel<T, true><<<n, 256, 0, st>>>(a);
+    else logprob_kernel<T, false><<<n, 256, 0, st>>>(a);
+    if (a.slices > 1) logprob_join<T><<<a.M, 256, std::max(8, a.slices * a.k * 8), st>>>(a);
+}
+
+}  // namespace
+
+extern "C" size_t ssm_token_logprobs_workspace(int M, int N, int k) {
+    if (M <= 0 || N <= 0 || k < 0 || k > kMaxTop) return 0;
+    const int s = slices_of(M, N);
+    return s > 1 ? sums_bytes(M, s) + (size_t)M * s * k * sizeof(u64) : 0;
+}
+
+extern "C" ssm_status ssm_token_logprobs(int dtype, const void* x, long ldx, const int* ids, int M, int N, int k,
+                                         float* logp, float* entropy, float* stats, int* top_ids, float* top_logp,
+                                         void* workspace, size_t workspace_bytes, void* stream) {
+    SSM_REQUIRE(dtype == SSM_F32 || dtype == SSM_BF16, "ssm_token_logprobs: bad dtype");
+    SSM_REQUIRE(M >= 0 && N > 0 && N <= ssm::kMaxSteps && k >= 0, "ssm_token_logprobs: bad shape");
+    SSM_REQUIRE(k <= N, "ssm_token_logprobs: %d alternatives of %d logits", k, N);
+    if (k > kMaxTop) return ssm::fail(SSM_ERR_UNSUPPORTED, "ssm_token_logprobs: %d alternatives, at most %d", k, kMaxTop);
+    if (M == 0) return SSM_OK;
+    SSM_REQUIRE(x && (!logp || ids) && (k == 0 || (top_ids && top_logp)), "ssm_token_logprobs: null input");
+    if (M == 1) ldx = N;
+    SSM_REQUIRE(ldx >= N, "ssm_token_logprobs: row stride below row width");
+    const int slices = slices_of(M, N);
+    SSM_REQUIRE((long)M * slices <= ssm::kMaxGroups, "ssm_token_logprobs: too many rows");
+    const size_t need = ssm_token_logprobs_workspace(M, N, k);
+    SSM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "ssm_token_logprobs: needs a workspace of %zu bytes", need);
+    SSM_REQUIRE(need == 0 || ((uintptr_t)workspace & 15) == 0, "ssm_token_logprobs: workspace must be 16-byte aligned");
+    SSM_REQUIRE(((uintptr_t)stats & 7) == 0, "ssm_token_logprobs: stats must be 8-byte aligned");
+    const long es = dtype == SSM_F32 ? 4 : 2;
+    const ssm::Rows rx{x, ldx * es, N * es, M}, ri = ssm::block(ids, 4L * M), o0 = ssm::block(logp, 4L * M),
+                    o1 = ssm::block(entropy, 4L * M), o2 = ssm::block(stats, 8L * M),
+                    o3 = ssm::block(k ? top_ids : nullptr, 4L * M * k), o4 = ssm::block(k ? top_logp : nullptr, 4L * M * k),
+                    ws = ssm::block(need ? workspace : nullptr, need);
+    SSM_REQUIRE(!ssm::meets(o0, rx, ri, o1, o2, o3, o4, ws) && !ssm::meets(o1, rx, ri, o2, o3, o4, ws) &&
+                    !ssm::meets(o2, rx, ri, o3, o4, ws) && !ssm::meets(o3, rx, ri, o4, ws) &&
+                    !ssm::meets(o4, rx, ri, ws) && !ssm::meets(ws, rx, ri),
+                "ssm_token_logprobs: an output or the workspace overlaps another operand");
+    LogArgs a{};
+    a.x = x; a.ldx = ldx; a.ids = ids; a.logp = logp; a.ent = entropy; a.stats = reinterpret_cast<float2*>(stats);
+    a.top = top_ids; a.toplp = top_logp; a.M = M; a.N = N; a.k = k; a.slices = slices;
+    a.turns = (int)ssm::cdiv(ssm::cdiv(N, kRun), slices);
+    a.sums = static_cast<Sums*>(workspace);
+    a.keys = reinterpret_cast<u64*>(static_cast<char*>(workspace) + sums_bytes(M, slices));
+    if (dtype == SSM_F32) run_logprobs<float>(a, (hipStream_t)stream);
+    else run_logprobs<__bf16>(a, (hipStream_t)stream);
+    return ssm::check_launch("ssm_token_logprobs");
+}
+
+extern "C" ssm_status ssm_token_logprobs_backward(int dtype, const void* x, long ldx, const int* ids, const float* stats,
+                                                  const float* entropy, const float* dlogp, const float* dentropy,
+                                                  void* dx, long lddx, int M, int N, void* stream) {
+    SSM_REQUIRE(dtype == SSM_F32 || dtype == SSM_BF16, "ssm_token_logprobs_backward: bad dtype");
+    SSM_REQUIRE(M >= 0 && N > 0 && N <= ssm::kMaxSteps, "ssm_token_logprobs_backward: bad shape");
+    if (M == 0) return SSM_OK;
+    SSM_REQUIRE(x && stats && dx && (!dlogp || ids) && (!dentropy || entropy), "ssm_token_logprobs_backward: null input");
+    SSM_REQUIRE(((uintptr_t)stats & 7) == 0, "ssm_token_logprobs_backward: stats must be 8-byte aligned");
+    if (M == 1) ldx = lddx = N;
+    SSM_REQUIRE(ldx >= N && lddx >= N, "ssm_token_logprobs_backward: row stride below row width");
+    const long pieces = ssm::cdiv(N, kRun);
+    SSM_REQUIRE(M * pieces <= ssm::kMaxGroups, "ssm_token_logprobs_backward: too many logits");
+    const long es = dtype == SSM_F32 ? 4 : 2;
+    const ssm::Rows rx{x, ldx * es, N * es, M}, ox{dx, lddx * es, N * es, M};
+    SSM_REQUIRE((dx == x && ldx == lddx) || !ssm::meet(ox, rx), "ssm_token_logprobs_backward: dx overlaps x, which it is not");
+    SSM_REQUIRE(!ssm::meets(ox, ssm::block(ids, 4L * M), ssm::block(stats, 8L * M), ssm::block(entropy, 4L * M),
+                            ssm::block(dlogp, 4L * M), ssm::block(dentropy, 4L * M)),
+                "ssm_token_logprobs_backward: dx overlaps another operand");
+    GradArgs a{};
+    a.x = x; a.ldx = ldx; a.ids = ids; a.stats = reinterpret_cast<const float2*>(stats); a.ent = entropy;
+    a.dlogp = dlogp; a.dent = dentropy; a.dx = dx; a.lddx = lddx; a.M = M; a.N = N; a.pieces = (int)pieces;
+    const unsigned n = (unsigned)(M * pieces);
+    if (dtype == SSM_F32) logprob_grad<float><<<n, 256, 0, (hipStream_t)stream>>>(a);
+    else logprob_grad<__bf16><<<n, 256, 0, (hipStream_t)stream>>>(a);
+    return ssm::check_launch("ssm_token_logprobs_backward");
+}

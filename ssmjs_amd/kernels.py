@@ -11,6 +11,8 @@ Shapes (row-major):
   linear_attention q (B,L,H,K); k (B,L,G,K); v (B,L,G,V); g (H); state (B,H,V,K)
   linear_i8/q8     x (M,K), W (N,K) -> y (M,N)
   gated_recurrence x, r, i (B,L,D); lam (D); state (B,D)
+  block_norm       x, y, z (..,D); post, scale, pre (D)
+  token_logprobs   logits (M,N); ids (M)
 """
 from __future__ import annotations
 
@@ -601,4 +603,115 @@ def gated_recurrence_step(x, r, i, lam, h, c=8.0, out=None):
         py, ldy = _at("out", out, shape, dt, dev), _ld("out", out)
     _lib.call("ssm_gated_recurrence_step", code, x.data_ptr(), _ld("x", x), pr, _ld("r", r), pi, _ld("i", i),
               _packed("lam", lam, (D,), _f32_t, dev), c, py, ldy, ph, B, D, _on(dev))
+    return out
+
+
+def _flat(name, t):
+    """Row stride of (..,D): contiguous rows at one distance through all leading dimensions."""
+    size = t.shape
+    if t.is_contiguous():
+        return size[-1]
+    if len(size) == 3:
+        return _steps(name, t)
+    if len(size) != 2:
+        raise ValueError(f"{name}: rows must lie at one distance")
+    return _ld(name, t)
+
+
+def _rows_of(t):
+    n = 1
+    for s in t.shape[:-1]:
+        n *= s
+    return n
+
+
+def block_norm(x, y, z=None, post=None, scale=None, pre=None, eps=1e-6, out=None):
+    """The norms around a block, with its gate and residual scale (ssm_block_norm): returns
+    x' = x + scale norm(y; post) silu(z) and n = norm(x'; pre). x, y, z (..,D) float32 or bfloat16, z None: no
+    gate; post, scale, pre (D) float32 or None (ones). `out`: a pair of tensors, which may be (x, y)."""
+    shape, dt = x.shape, x.dtype
+    D, T = shape[-1], _rows_of(x)
+    code, dev = _code(dt), _current("x", x)
+    py = _at("y", y, shape, dt, dev)
+    pz, ldz = (None, D) if z is None else (_at("z", z, shape, dt, dev), _flat("z", z))
+    if out is None:
+        x1, n = x.new_empty(shape), x.new_empty(shape)
+        p1, pn, ld1, ldn = x1.data_ptr(), n.data_ptr(), D, D
+    else:
+        x1, n = out
+        p1, pn = _at("out[0]", x1, shape, dt, dev), _at("out[1]", n, shape, dt, dev)
+        ld1, ldn = _flat("out[0]", x1), _flat("out[1]", n)
+    w = (D,)
+    _lib.call("ssm_block_norm", code, x.data_ptr(), _flat("x", x), py, _flat("y", y), pz, ldz,
+              _packed("post", post, w, _f32_t, dev), _packed("scale", scale, w, _f32_t, dev),
+              _packed("pre", pre, w, _f32_t, dev), eps, p1, ld1, pn, ldn, T, D, _on(dev))
+    return x1, n
+
+
+def block_norm_backward(dx1, dn, x, y, z=None, post=None, scale=None, pre=None, eps=1e-6, out=None, workspace=None):
+    """Gradients of block_norm (ssm_block_norm_backward) from dx1, that of x' (None: zeros), and dn: returns
+    (dx, dy, dz, dpost, dscale, dpre), None for what was None. `out`: tensors for dx, dy, dz; dx may be dx1."""
+    shape, dt = x.shape, x.dtype
+    D, T = shape[-1], _rows_of(x)
+    code, dev = _code(dt), _current("x", x)
+
+    def side(name, t):
+        return (None, D) if t is None else (_at(name, t, shape, dt, dev), _flat(name, t))
+
+    if out is None:
+        out = x.new_empty(shape), x.new_empty(shape), x.new_empty(shape) if z is not None else None
+    dx, dy, dz = out
+    if z is not None and dz is None:
+        raise ValueError("out[2]: a gate needs its gradient's tensor")
+    if z is None:
+        dz = None
+    grads = [w.new_empty(D, dtype=_f32_t) if w is not None else None for w in (post, scale, pre)]
+    if T == 0:
+        for g in grads:
+            if g is not None:
+                g.zero_()
+        return dx, dy, dz, *grads
+    ws, pws, nbytes = _own_scratch(workspace, _lib.lib().ssm_block_norm_backward_workspace(T, D), x)
+    w = (D,)
+    _lib.call("ssm_block_norm_backward", code, *side("dx1", dx1), *side("dn", dn), x.data_ptr(), _flat("x", x),
+              *side("y", y), *side("z", z), _packed("post", post, w, _f32_t, dev),
+              _packed("scale", scale, w, _f32_t, dev), _packed("pre", pre, w, _f32_t, dev), eps,
+              *side("out[0]", dx), *side("out[1]", dy), *side("out[2]", dz),
+              *(None if g is None else g.data_ptr() for g in grads), T, D, pws, nbytes, _on(dev))
+    return dx, dy, dz, *grads
+
+
+def token_logprobs(logits, ids=None, k=0, stats=None, workspace=None):
+    """Log probabilities of given tokens, entropy and the k likeliest tokens of each row (ssm_token_logprobs):
+    returns (logp (M), entropy (M), top_ids (M,k) int32, top_logp (M,k)), the last two None for k = 0 and the first
+    None without ids. logits (M,N) float32 or bfloat16; ids (M) int32, one outside 0 .. N - 1 has logp 0; of equal
+    logits the lowest index comes first. `stats` (M,2) float32 is filled for the backward pass."""
+    M, N = logits.shape
+    code, dev = _code(logits.dtype), _current("logits", logits)
+    logp = logits.new_empty(M, dtype=_f32_t) if ids is not None else None
+    ent = logits.new_empty(M, dtype=_f32_t)
+    top, toplp = (logits.new_empty((M, k), dtype=_i32_t), logits.new_empty((M, k), dtype=_f32_t)) if k else (None, None)
+    ws, pws, nbytes = _own_scratch(workspace, _lib.lib().ssm_token_logprobs_workspace(M, N, k), logits)
+    _lib.call("ssm_token_logprobs", code, logits.data_ptr(), _ld("logits", logits),
+              _packed("ids", ids, (M,), _i32_t, dev), M, N, k, None if logp is None else logp.data_ptr(),
+              ent.data_ptr(), _packed("stats", stats, (M, 2), _f32_t, dev), None if top is None else top.data_ptr(),
+              None if toplp is None else toplp.data_ptr(), pws, nbytes, _on(dev))
+    return logp, ent, top, toplp
+
+
+def token_logprobs_backward(logits, ids, stats, entropy=None, dlogp=None, dentropy=None, out=None):
+    """Gradient of the logits (ssm_token_logprobs_backward) from those of token_logprobs' logp and entropy (None:
+    zeros), with the `stats` and entropy that it left. `out` may be the logits."""
+    M, N = logits.shape
+    dt = logits.dtype
+    code, dev = _code(dt), _current("logits", logits)
+    if out is None:
+        out = logits.new_empty((M, N))
+    po = _at("out", out, (M, N), dt, dev)
+    if stats is None:
+        raise ValueError("token_logprobs_backward needs stats")
+    _lib.call("ssm_token_logprobs_backward", code, logits.data_ptr(), _ld("logits", logits),
+              _packed("ids", ids, (M,), _i32_t, dev), _packed("stats", stats, (M, 2), _f32_t, dev),
+              _packed("entropy", entropy, (M,), _f32_t, dev), _packed("dlogp", dlogp, (M,), _f32_t, dev),
+              _packed("dentropy", dentropy, (M,), _f32_t, dev), po, _ld("out", out), M, N, _on(dev))
     return out
