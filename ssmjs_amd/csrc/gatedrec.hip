@@ -29,6 +29,7 @@ constexpr float kSeries = 0.2f;  // z up to which 1 - e^-z is summed as a series
 constexpr float kTiny = 1.17549435e-38f;
 
 // ---------------------------------------------------------------- elements
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 template <typename T, int VEC> struct Raw;
 template <> struct Raw<float, 2> {
     float2 v;
@@ -50,23 +51,36 @@ template <> struct Raw<__bf16, 2> {
         f[1] = __builtin_bit_cast(float, v & 0xffff0000u);
     }
 };
+template <> struct Raw<float, 4> {
+    float4 v;
+    __device__ void load(__amdgpu_buffer_rsrc_t r, unsigned o) { v = ssm::bload16<float4>(r, o); }
+    __device__ void get(float (&f)[4]) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+};
+template <> struct Raw<__bf16, 4> {
+    u32x2 v;
+    __device__ void load(__amdgpu_buffer_rsrc_t r, unsigned o) { v = __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0); }
+    __device__ void get(float (&f)[4]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = __builtin_bit_cast(float, j % 2 ? v[j / 2] & 0xffff0000u : v[j / 2] << 16);
+    }
+};
 template <> struct Raw<__bf16, 1> {
     unsigned short v;
     __device__ void load(__amdgpu_buffer_rsrc_t r, unsigned o) { v = __builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0); }
     __device__ void get(float (&f)[1]) const { f[0] = __builtin_bit_cast(float, (unsigned)v << 16); }
 };
 
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+// (stores past the caches: what a second pass reads again stays in them; 1 x 32768 x 1024 113 -> 103 us)
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void put(const float (&f)[2], __amdgpu_buffer_rsrc_t r, unsigned o, float) {
-    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, make_float2(f[0], f[1])), r, o, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, make_float2(f[0], f[1])), r, o, 0, ssm::kPolicyNT);
 }
 __device__ __forceinline__ void put(const float (&f)[1], __amdgpu_buffer_rsrc_t r, unsigned o, float) {
     ssm::bstore4(f[0], r, o);
 }
 __device__ __forceinline__ void put(const float (&f)[2], __amdgpu_buffer_rsrc_t r, unsigned o, __bf16) {
     const bf16x2 b{(__bf16)f[0], (__bf16)f[1]};
-    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, b), r, o, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, b), r, o, 0, ssm::kPolicyNT);
 }
 __device__ __forceinline__ void put(const float (&f)[1], __amdgpu_buffer_rsrc_t r, unsigned o, __bf16) {
     __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (__bf16)f[0]), r, o, 0, 0);
@@ -134,10 +148,10 @@ __device__ __forceinline__ unsigned here(unsigned v) {
     return v;
 }
 
-// A lane's place: VEC channels of one of R = VEC rows of a wave; W waves. A row has S consecutive steps of a block.
-template <typename T, int VEC, int W_>
+// A lane's place: VEC of CH channels, in one of R rows of a wave; W waves. A row has S consecutive steps of a block.
+template <typename T, int VEC, int W_, int CH = kCh>
 struct Place {
-    static constexpr int LC = kCh / VEC, R = 64 / LC, S = 16 / VEC, W = W_, TB = W * R * S;
+    static constexpr int LC = CH / VEC, R = 64 / LC, S = 16 / VEC, W = W_, TB = W * R * S;
     int lane, w, col, row, mine;   // mine: its first step of a block
     int ch, cg, b, part, n;
     bool live;
@@ -148,12 +162,12 @@ struct Place {
         col = lane % LC;
         row = lane / LC;
         mine = (w * R + row) * S;
-        const int groups = (a.D + kCh - 1) / kCh;
+        const int groups = (a.D + CH - 1) / CH;
         cg = blockIdx.x % groups;
         const int rest = blockIdx.x / groups;
         b = rest % a.B;
         part = rest / a.B;
-        ch = cg * kCh + col * VEC;
+        ch = cg * CH + col * VEC;
         live = ch < a.D;
         n = a.L;
         if (a.lengths) n = min(max(a.lengths[b], 0), a.L);
@@ -171,8 +185,8 @@ struct Place {
     // `there` rows of this group's channels from step t0 on (none: nothing is read or written)
     template <typename Q>
     __device__ __amdgpu_buffer_rsrc_t rows(Q* p, long ld, const RecArgs& a, int t0, int there) const {
-        const char* base = (const char*)p + (((long)b * a.L + t0) * ld + cg * kCh) * sizeof(T);
-        return ssm::rsrc(base, there > 0 ? (unsigned)(((long)(there - 1) * ld + min(kCh, a.D - cg * kCh)) * sizeof(T)) : 0u);
+        const char* base = (const char*)p + (((long)b * a.L + t0) * ld + cg * CH) * sizeof(T);
+        return ssm::rsrc(base, there > 0 ? (unsigned)(((long)(there - 1) * ld + min(CH, a.D - cg * CH)) * sizeof(T)) : 0u);
     }
     __device__ unsigned at(long ld, int step) const {   // (dead lanes: past every end)
         return live ? (unsigned)((step * ld + col * VEC) * sizeof(T)) : 0x80000000u;
@@ -253,17 +267,18 @@ __device__ __forceinline__ void runs(int lane, int row, const float (&d)[S][VEC]
 // ---------------------------------------------------------------- the blocks' (A, H)
 // For the segments after them. Without outputs no order binds the lanes: each walks a run of a block on its own, and
 // the runs are composed at the end. BACK: of the adjoint, e_{t-1} = a_t (dy_t + e_t), walked from the end.
-constexpr int kRunWaves = 4;
+constexpr int kRunWaves = 8;
 
-template <typename T, int VEC, int TB, bool BACK>
+// Rows of CH = 128 channels, four a lane, where alignment allows: CHFIG
+template <typename T, int VEC, int CH, int TB, bool BACK>
 __global__ __launch_bounds__(64 * kRunWaves) void rec_runs(RecArgs a) {
-    using P = Place<T, VEC, kRunWaves>;
+    using P = Place<T, VEC, kRunWaves, CH>;
     constexpr int S = P::S, R = P::R, N = kRunWaves * R, RUN = TB / N;
     static_assert(RUN % S == 0, "whole rows of steps");
-    __shared__ float sa[N][kCh], sh[N][kCh];
+    __shared__ float sa[N][CH], sh[N][CH];
     const P p(a);
-    const int chl = p.cg * kCh + (int)threadIdx.x;
-    const bool mine = threadIdx.x < kCh && chl < a.D;
+    const int chl = p.cg * CH + (int)threadIdx.x;
+    const bool mine = threadIdx.x < CH && chl < a.D;
     // the entering states go on from here: the caller's may lie where the final ones are written
     float2* const runs = a.runs + (long)p.b * (a.blocks + 1) * a.D;
     if (p.part == 0 && mine) runs[(long)a.blocks * a.D + chl] = make_float2(a.h0 ? a.h0[(long)p.b * a.D + chl] : 0.f, 0.f);
@@ -658,51 +673,84 @@ __global__ __launch_bounds__(256) void rec_step(RecArgs a) {
 // ---------------------------------------------------------------- plans
 constexpr int kWaves = 16, kWavesBack = 8;
 
-// Blocks and segments of the sequences. PLAN
+// Blocks and segments of the sequences: as many segments as make the kernels' time least, counted in the time of a
+// block on a full chip (one workgroup a CU; us, W = 16 and 8 waves: 7.6, 6.9):
+//   - a turn of 256 workgroups takes the blocks of a segment, a last one of fewer at least 0.77 of that (16 blocks of
+//     128 workgroups 95 us, of 256 122);
+//   - a first pass over the blocks that others follow takes `again` of a block each, spread over the chip, and a launch.
+// Of sequences with lengths about 0.6 are taken to be there. us, one segment / the rule / twice its segments:
+// 1 x 32768 x 1024 588 / 100 / 107, 4 x 2048 x 2048 49.4 / 49.1 / 58.5, 8 x 4096 x 2048 122 / 122 / 155; gradients
+// 1123 / 137 / 143, 87.7 / 69.5 / 75.6, 220 / 220 / 259.
 struct Plan {
     long chains;        // sequences times channel groups
     int blocks, seg;    // blocks of a sequence, and of a segment
     int segments() const { return (blocks + seg - 1) / seg; }
     long groups() const { return chains * segments(); }
 };
-Plan plan_of(int B, int L, int D, int block, double again) {
+Plan plan_of(int B, int L, int D, int block, double again, bool ragged) {
     Plan p{ssm::cdiv(D, kCh) * B, (int)std::max(1L, ssm::cdiv(L, block)), 0};
+    const double chains = p.chains * (ragged ? 0.6 : 1.0);
     double best = 0;
-    for (long n = 1; n <= std::min(64, p.blocks); ++n) {
-        const long per = ssm::cdiv(p.blocks, n), segs = ssm::cdiv(p.blocks, per);
-        // turns of the chip, in blocks; the first pass over all but the last segment costs `again` of a share of the chip
-        double t = (double)ssm::cdiv(p.chains * segs, 256) * per;
-        if (segs > 1) t += 0.5 + again * std::max(1.0, (double)p.chains * (p.blocks - per) / 256);
-        if (n == 1 || t < best) best = t, p.seg = (int)per;
+    for (int n = 1; n <= std::min(64, p.blocks); ++n) {
+        const int per = (p.blocks + n - 1) / n, segs = (p.blocks + per - 1) / per;
+        const double turns = chains * segs / 256, full = (double)(long)turns, rest = turns - full;
+        double t = per * (full + (rest > 0 || full == 0 ? std::max(0.77, rest) : 0.0));
+        if (segs > 1) t += 0.5 + again * std::max(1.0, chains * (p.blocks - per) / 256);
+        if (n == 1 || t < best) best = t, p.seg = per;
     }
     return p;
 }
-Plan plan_forward(int B, int L, int D) { return plan_of(B, L, D, kWaves * 16, 0.7); }
-Plan plan_backward(int B, int L, int D) { return plan_of(B, L, D, kWavesBack * 16, 0.3); }
+Plan plan_forward(int B, int L, int D, bool ragged) { return plan_of(B, L, D, kWaves * 16, 0.7, ragged); }
+Plan plan_backward(int B, int L, int D, bool ragged) { return plan_of(B, L, D, kWavesBack * 16, 0.3, ragged); }
 
 size_t runs_bytes(const Plan& p, int B, int D) {
     return p.segments() > 1 ? ((size_t)B * (p.blocks + 1) * D * sizeof(float2) + 15) / 16 * 16 : 0;
 }
 size_t sums_bytes(const Plan& p, int B, int D) { return (size_t)B * p.segments() * D * sizeof(float); }
+size_t forward_bytes(int B, int L, int D) {
+    return std::max(runs_bytes(plan_forward(B, L, D, false), B, D), runs_bytes(plan_forward(B, L, D, true), B, D));
+}
+size_t backward_bytes(int B, int L, int D) {
+    const Plan p = plan_backward(B, L, D, false), q = plan_backward(B, L, D, true);
+    return std::max(runs_bytes(p, B, D) + sums_bytes(p, B, D), runs_bytes(q, B, D) + sums_bytes(q, B, D));
+}
 
+// VEC channels a lane (4: two in the kernels with outputs).
+template <typename T, int VEC, bool BACK>
+void launch_runs(const RecArgs& a, int parts, hipStream_t st) {
+    constexpr int TB = 16 * (BACK ? kWavesBack : kWaves), CH = VEC == 4 ? 128 : kCh;
+    rec_runs<T, VEC, CH, TB, BACK><<<(unsigned)(ssm::cdiv(a.D, CH) * a.B * parts), 64 * kRunWaves, 0, st>>>(a);
+}
 template <typename T, int VEC>
 void launch_forward(const RecArgs& a, const Plan& p, hipStream_t st) {
-    if (a.runs) rec_runs<T, VEC, kWaves * 16, false><<<(unsigned)(p.chains * (p.segments() - 1) * p.seg), 64 * kRunWaves, 0, st>>>(a);
-    rec_kernel<T, VEC, kWaves><<<(unsigned)p.groups(), 64 * kWaves, 0, st>>>(a);
+    if (a.runs) launch_runs<T, VEC, false>(a, (p.segments() - 1) * p.seg, st);
+    rec_kernel<T, std::min(VEC, 2), kWaves><<<(unsigned)p.groups(), 64 * kWaves, 0, st>>>(a);
 }
 template <typename T, int VEC>
 void launch_backward(const RecArgs& a, const Plan& p, float* dlam, hipStream_t st) {
-    if (a.runs) rec_runs<T, VEC, kWavesBack * 16, true><<<(unsigned)(p.chains * (p.blocks - p.seg)), 64 * kRunWaves, 0, st>>>(a);
-    rec_backward<T, VEC, kWavesBack><<<(unsigned)p.groups(), 64 * kWavesBack, 0, st>>>(a);
+    if (a.runs) launch_runs<T, VEC, true>(a, p.blocks - p.seg, st);
+    rec_backward<T, std::min(VEC, 2), kWavesBack><<<(unsigned)p.groups(), 64 * kWavesBack, 0, st>>>(a);
     rec_dlam<<<(unsigned)ssm::cdiv(a.D, 64), 1024, 0, st>>>(a.sums, a.lam, a.B * p.segments(), a.D, dlam);
 }
 
-// Two channels a lane: D and all strides even, and rows aligned to that.
-bool in_pairs(int dtype, int D, std::initializer_list<std::pair<const void*, long>> ops) {
-    const uintptr_t piece = dtype == SSM_F32 ? 7 : 3;
-    bool ok = D % 2 == 0;
-    for (const auto& o : ops) ok = ok && o.second % 2 == 0 && ((uintptr_t)o.first & piece) == 0;
-    return ok;
+// Channels that a lane may load at a time: four or two where D, all strides and the rows' alignment are whole ones.
+int vector_of(int dtype, int D, std::initializer_list<std::pair<const void*, long>> ops) {
+    const uintptr_t es = dtype == SSM_F32 ? 4 : 2;
+    uintptr_t all = (uintptr_t)D;
+    for (const auto& o : ops) all |= (uintptr_t)o.second | ((uintptr_t)o.first & (4 * es - 1)) / es | ((uintptr_t)o.first % es ? 1 : 0);
+    return all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
+}
+template <typename T, typename... A>
+void forward_of(int vec, A... a) {
+    if (vec == 4) launch_forward<T, 4>(a...);
+    else if (vec == 2) launch_forward<T, 2>(a...);
+    else launch_forward<T, 1>(a...);
+}
+template <typename T, typename... A>
+void backward_of(int vec, A... a) {
+    if (vec == 4) launch_backward<T, 4>(a...);
+    else if (vec == 2) launch_backward<T, 2>(a...);
+    else launch_backward<T, 1>(a...);
 }
 
 constexpr long kMaxLd = 1L << 20;   // a block's rows within 2^31 bytes
@@ -710,7 +758,7 @@ constexpr long kMaxBlocks = (1L << 22) - 1;   // (launches of 1024 threads in 32
 }  // namespace
 
 extern "C" size_t ssm_gated_recurrence_workspace(int B, int L, int D) {
-    return B > 0 && L > 0 && D > 0 ? runs_bytes(plan_forward(B, L, D), B, D) : 0;
+    return B > 0 && L > 0 && D > 0 ? forward_bytes(B, L, D) : 0;
 }
 
 extern "C" ssm_status ssm_gated_recurrence(int dtype, const void* x, long ldx, const void* r, long ldr, const void* i,
@@ -727,7 +775,7 @@ extern "C" ssm_status ssm_gated_recurrence(int dtype, const void* x, long ldx, c
     SSM_REQUIRE(ldx >= D && ldr >= D && ldi >= D && ldy >= D, "ssm_gated_recurrence: row stride below row width");
     SSM_REQUIRE(ldx < kMaxLd && ldr < kMaxLd && ldi < kMaxLd && ldy < kMaxLd && L <= ssm::kMaxSteps,
                 "ssm_gated_recurrence: row strides of %ld elements, or sequences, too large", kMaxLd);
-    const Plan p = plan_forward(B, L, D);
+    const Plan p = plan_forward(B, L, D, lengths != nullptr);
     SSM_REQUIRE(p.chains * p.blocks <= kMaxBlocks, "ssm_gated_recurrence: too many sequences, steps or channels");
     const size_t need = ssm_gated_recurrence_workspace(B, L, D);
     SSM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
@@ -746,19 +794,17 @@ extern "C" ssm_status ssm_gated_recurrence(int dtype, const void* x, long ldx, c
     RecArgs a{};
     a.x = x; a.ldx = ldx; a.r = r; a.ldr = ldr; a.i = i; a.ldi = ldi; a.y = y; a.ldy = ldy;
     a.lam = lam; a.lengths = lengths; a.pad = lengths && pad; a.h0 = h0; a.hT = hT; a.states = states; a.c = c;
-    a.runs = need ? static_cast<float2*>(workspace) : nullptr;
+    a.runs = p.segments() > 1 ? static_cast<float2*>(workspace) : nullptr;
     a.B = B; a.L = L; a.D = D; a.blocks = p.blocks; a.seg = p.seg;
-    const bool two = in_pairs(dtype, D, {{x, ldx}, {r, ldr}, {i, ldi}, {y, ldy}});
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype == SSM_F32) two ? launch_forward<float, 2>(a, p, st) : launch_forward<float, 1>(a, p, st);
-    else two ? launch_forward<__bf16, 2>(a, p, st) : launch_forward<__bf16, 1>(a, p, st);
+    const int vec = vector_of(dtype, D, {{x, ldx}, {r, ldr}, {i, ldi}, {y, ldy}});
+    if (dtype == SSM_F32) forward_of<float>(vec, a, p, (hipStream_t)stream);
+    else forward_of<__bf16>(vec, a, p, (hipStream_t)stream);
     return ssm::check_launch("ssm_gated_recurrence");
 }
 
 extern "C" size_t ssm_gated_recurrence_backward_workspace(int B, int L, int D) {
     if (B <= 0 || L < 0 || D <= 0) return 0;
-    const Plan p = plan_backward(B, L, D);
-    return runs_bytes(p, B, D) + sums_bytes(p, B, D);
+    return backward_bytes(B, L, D);
 }
 
 extern "C" ssm_status ssm_gated_recurrence_backward(int dtype, const void* dy, long lddy, const void* x, long ldx,
@@ -778,7 +824,7 @@ extern "C" ssm_status ssm_gated_recurrence_backward(int dtype, const void* dy, l
         SSM_REQUIRE(ld >= D, "ssm_gated_recurrence_backward: row stride below row width");
         SSM_REQUIRE(ld < kMaxLd, "ssm_gated_recurrence_backward: row strides of %ld elements are too large", kMaxLd);
     }
-    const Plan p = plan_backward(B, L, D);
+    const Plan p = plan_backward(B, L, D, lengths != nullptr);
     SSM_REQUIRE(L <= ssm::kMaxSteps && p.chains * p.blocks <= kMaxBlocks,
                 "ssm_gated_recurrence_backward: too many sequences, steps or channels");
     const size_t need = ssm_gated_recurrence_backward_workspace(B, L, D);
@@ -804,10 +850,9 @@ extern "C" ssm_status ssm_gated_recurrence_backward(int dtype, const void* dy, l
     a.runs = runs ? static_cast<float2*>(workspace) : nullptr;
     a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + runs);
     a.B = B; a.L = L; a.D = D; a.blocks = p.blocks; a.seg = p.seg;
-    const bool two = in_pairs(dtype, D, {{dy, lddy}, {x, ldx}, {r, ldr}, {i, ldi}, {dx, lddx}, {dr, lddr}, {di, lddi}});
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype == SSM_F32) two ? launch_backward<float, 2>(a, p, dlam, st) : launch_backward<float, 1>(a, p, dlam, st);
-    else two ? launch_backward<__bf16, 2>(a, p, dlam, st) : launch_backward<__bf16, 1>(a, p, dlam, st);
+    const int vec = vector_of(dtype, D, {{dy, lddy}, {x, ldx}, {r, ldr}, {i, ldi}, {dx, lddx}, {dr, lddr}, {di, lddi}});
+    if (dtype == SSM_F32) backward_of<float>(vec, a, p, dlam, (hipStream_t)stream);
+    else backward_of<__bf16>(vec, a, p, dlam, (hipStream_t)stream);
     return ssm::check_launch("ssm_gated_recurrence_backward");
 }
 
