@@ -152,6 +152,16 @@ struct LogArgs {
     int M, N, k, slices, turns;
 };
 
+// How many of a list's keys are larger.
+__device__ __forceinline__ int rank_of(u64 mine, const u64* keys, int have) {
+    int rank = 0, o = 0;
+    for (; o + 8 <= have; o += 8)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rank += keys[o + j] > mine;
+    for (; o < have; ++o) rank += keys[o] > mine;
+    return rank;
+}
+
 // What a row's results are, from its sums and its lists' keys (`have` of them in LDS, unique; 0: none).
 template <typename T>
 __device__ void finish(const LogArgs& a, int row, Sums s, const u64* keys, int have) {
@@ -170,10 +180,8 @@ __device__ void finish(const LogArgs& a, int row, Sums s, const u64* keys, int h
     }
     for (int c = threadIdx.x; c < have; c += blockDim.x) {
         const u64 mine = keys[c];
-        if (!mine) continue;
-        int rank = 0;
-        for (int o = 0; o < have; ++o) rank += keys[o] > mine;
-        if (rank < a.k) {
+        const int rank = rank_of(mine, keys, have);
+        if (mine && rank < a.k) {
             a.top[(long)row * a.k + rank] = (int)index_of(mine);
             a.toplp[(long)row * a.k + rank] = none ? -__builtin_inff() : (value_of(mine) - m) - logz;
         }
@@ -202,15 +210,19 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogArgs a) {
         for (int g = 0; g < kGroups; ++g) take8(s, v[g]);
         if constexpr (TOP) {
             u64 own = 0;
-            if (!full) {   // the first turn: the lanes' maxima
+            if (!full) {   // the first turn: the lanes' maxima (any of a lane's logits would do)
+                float most = v[0][0];
+                int at = 0;
 #pragma unroll
                 for (int g = 0; g < kGroups; ++g)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int at = base + (g * 64 + lane) * 8 + j;
-                        const u64 key = at < a.N ? key_of(v[g][j], at) : 0;
-                        own = key > own ? key : own;
+                        const bool up = v[g][j] > most;
+                        most = up ? v[g][j] : most;
+                        at = up ? g * 512 + j : at;
                     }
+                at += base + lane * 8;
+                own = at < a.N ? key_of(most, at) : 0;
                 list = sorted(own, lane);
                 least = lane64(list, a.k - 1);
                 bar = least ? value_of(least) : __builtin_nanf("");
@@ -256,22 +268,22 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogArgs a) {
     if constexpr (TOP)
         for (int c = threadIdx.x; c < 4 * a.k; c += 256) {
             const u64 mine = lists[c];
-            int rank = 0, there = 0;
-            for (int o = 0; o < 4 * a.k; ++o) rank += lists[o] > mine, there += lists[o] != 0;
+            const int rank = rank_of(mine, lists, 4 * a.k);
             u64* out = a.keys + (long)blockIdx.x * a.k;
             if (mine && rank < a.k) out[rank] = mine;
-            if (c < a.k && c >= there) out[c] = 0;
+            if (c < a.k && c >= rank_of(0, lists, 4 * a.k)) out[c] = 0;   // (fewer logits than k)
         }
 }
 
 // The slices of a row together.
 template <typename T>
-__global__ __launch_bounds__(256) void logprob_join(LogArgs a) {
+__global__ __launch_bounds__(1024) void logprob_join(LogArgs a) {
     extern __shared__ u64 all[];
-    const int row = blockIdx.x, have = a.slices * a.k;
-    for (int c = threadIdx.x; c < have; c += 256) all[c] = a.keys[(long)row * have + c];
+    const int row = blockIdx.x, have = a.slices * a.k, lane = threadIdx.x & 63;
+    for (int c = threadIdx.x; c < have; c += blockDim.x) all[c] = a.keys[(long)row * have + c];
     Sums s{kLowest, 0.f, 0.f};
-    for (int c = 0; c < a.slices; ++c) s = join(s, a.sums[(long)row * a.slices + c]);
+    if (lane < a.slices) s = a.sums[(long)row * a.slices + lane];
+    s = over_wave(s);
     __syncthreads();
     finish<T>(a, row, s, all, have);
 }
@@ -327,7 +339,9 @@ void run_logprobs(const LogArgs& a, hipStream_t st) {
     const unsigned n = (unsigned)((long)a.M * a.slices);
     if (a.k) logprob_kernel<T, true><<<n, 256, 0, st>>>(a);
     else logprob_kernel<T, false><<<n, 256, 0, st>>>(a);
-    if (a.slices > 1) logprob_join<T><<<a.M, 256, std::max(8, a.slices * a.k * 8), st>>>(a);
+    // a thread for each slice's key
+    const int have = a.slices * a.k, threads = std::min(1024, std::max(64, (have + 63) / 64 * 64));
+    if (a.slices > 1) logprob_join<T><<<a.M, threads, std::max(8, have * 8), st>>>(a);
 }
 
 }  // namespace
