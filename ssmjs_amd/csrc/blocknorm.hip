@@ -94,6 +94,13 @@ __device__ __forceinline__ void weights(const float* w, int e, int left, float (
     }
 }
 
+// Keeps loads through `p` where they are: the backward pass needs its registers for rows, and the weights lie in
+// the caches.
+__device__ __forceinline__ const float* again(const float* p) {
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
 struct NormArgs {
     const void* x; long ldx;
     const void* y; long ldy;
@@ -109,17 +116,32 @@ struct NormArgs {
     float eps;
 };
 
-// Sum over the lanes of a row: one wave, or WPR waves through `red` (two buffers in turn: one barrier a sum).
-template <int WPR>
-__device__ __forceinline__ float row_sum(float s, float (&red)[2][WPR], int& turn) {
-#pragma unroll
-    for (int k = 32; k > 0; k /= 2) s += __shfl_xor(s, k);
+// Sum over a wave: rotations within its rows of 16 lanes, then two exchanges between them.
+template <int N>
+__device__ __forceinline__ float rotated(float v) {   // by N lanes of 16 (row_ror)
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float wave_sum(float s) {
+    s += rotated<8>(s);
+    s += rotated<4>(s);
+    s += rotated<2>(s);
+    s += rotated<1>(s);
+    s += __shfl_xor(s, 16);
+    return s + __shfl_xor(s, 32);
+}
+
+// Sum over the lanes of a row: one wave, or WPR waves (the workgroup's waves are W, its rows W / WPR) through `red`
+// (two buffers in turn: one barrier a sum).
+template <int WPR, int W>
+__device__ __forceinline__ float row_sum(float s, float (&red)[2][W], int& turn) {
+    s = wave_sum(s);
     if constexpr (WPR > 1) {
         if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = s;
         __syncthreads();
         s = 0.f;
+        const int first = (threadIdx.x >> 6) / WPR * WPR;
 #pragma unroll
-        for (int w = 0; w < WPR; ++w) s += red[turn][w];
+        for (int w = 0; w < WPR; ++w) s += red[turn][first + w];
         turn ^= 1;
     }
     return s;
@@ -155,7 +177,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_kernel(NormArg
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(y[c][j], y[c][j], ss);
     const float inv = 1.f / (float)a.D;
-    const float ry = __builtin_amdgcn_rsqf(fmaf(row_sum<WPR>(ss, red, turn), inv, a.eps));
+    const float ry = __builtin_amdgcn_rsqf(fmaf(row_sum<WPR, WPR>(ss, red, turn), inv, a.eps));
     float x1[NC][8];
     ss = 0.f;
 #pragma unroll
@@ -172,7 +194,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_kernel(NormArg
             ss = fmaf(x1[c][j], x1[c][j], ss);
         }
     }
-    const float rx = __builtin_amdgcn_rsqf(fmaf(row_sum<WPR>(ss, red, turn), inv, a.eps));
+    const float rx = __builtin_amdgcn_rsqf(fmaf(row_sum<WPR, WPR>(ss, red, turn), inv, a.eps));
     T* p1 = row_of<T>(a.x1, a.ldx1, t);
     T* pn = row_of<T>(a.n, a.ldn, t);
 #pragma unroll
@@ -187,42 +209,58 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_kernel(NormArg
     }
 }
 
+// W = 8 waves (16 for one row) a workgroup and one workgroup a CU, which walks its rows and keeps the column sums of
+// its lanes' elements: few partial sums, and they go to memory once.
 template <typename T, int NC, int WPR, bool GATE>
-__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_backward(NormArgs a) {
-    __shared__ float red[2][WPR];
-    __shared__ float cols[WPR == 1 ? 4 : 1][WPR == 1 ? 512 * NC : 1];
+__global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArgs a) {
+    constexpr int W = WPR > 8 ? WPR : 8, RPG = W / WPR;   // rows at a time
+    __shared__ float red[2][W];
+    __shared__ float cols[RPG][512 * NC * WPR];
     int turn = 0;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int e0 = ((WPR == 1 ? 0 : w * NC) * 64 + lane) * 8;
+    const int e0 = (w % WPR * NC * 64 + lane) * 8;
     const float inv = 1.f / (float)a.D;
     float spost[NC][8] = {}, sscale[NC][8] = {}, spre[NC][8] = {};
-    const long step = WPR == 1 ? 4L * gridDim.x : gridDim.x;
-    for (long t = WPR == 1 ? (long)blockIdx.x * 4 + w : blockIdx.x; t < a.T; t += step) {
-        Eight<T> x[NC], y[NC], z[NC], dn[NC], g0[NC];
-        float ss = 0.f;
+    const long step = (long)RPG * gridDim.x;
+    constexpr bool kAhead = NC == 1 || (!GATE && sizeof(T) == 2);   // (registers for the next row too)
+    Eight<T> x[NC], y[NC], z[NC], dn[NC], g0[NC], nx[NC], ny[NC], nz[NC], ndn[NC], ng0[NC];
+    auto fetch = [&](long t) {   // the next row, on its way while this one is worked on
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int e = e0 + 512 * c, left = a.D - e;
-            y[c].load(row_of<T>(a.y, a.ldy, t) + e, left);
-            x[c].load(row_of<T>(a.x, a.ldx, t) + e, left);
-            if constexpr (GATE) z[c].load(row_of<T>(a.z, a.ldz, t) + e, left);
-            dn[c].load(row_of<T>(a.dn, a.lddn, t) + e, left);
-            g0[c].load(a.dx1 ? row_of<T>(a.dx1, a.lddx1, t) + e : nullptr, a.dx1 ? left : 0);
+            const int e = e0 + 512 * c, left = t < a.T ? a.D - e : 0;
+            ny[c].load(row_of<T>(a.y, a.ldy, t) + e, left);
+            nx[c].load(row_of<T>(a.x, a.ldx, t) + e, left);
+            if constexpr (GATE) nz[c].load(row_of<T>(a.z, a.ldz, t) + e, left);
+            ndn[c].load(row_of<T>(a.dn, a.lddn, t) + e, left);
+            ng0[c].load(a.dx1 ? row_of<T>(a.dx1, a.lddx1, t) + e : nullptr, a.dx1 ? left : 0);
         }
+    };
+    long t = (long)blockIdx.x * RPG + w / WPR;
+    if constexpr (kAhead) fetch(t);
+    for (long group = (long)blockIdx.x * RPG; group < a.T; group += step, t += step) {
+        const bool on = t < a.T;   // (all waves take part in the sums)
+        if constexpr (!kAhead) fetch(t);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            x[c] = nx[c], y[c] = ny[c], dn[c] = ndn[c], g0[c] = ng0[c];
+            if constexpr (GATE) z[c] = nz[c];
+        }
+        if constexpr (kAhead) fetch(t + step);
+        float ss = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int j = 0; j < 8; ++j) ss = fmaf(y[c][j], y[c][j], ss);
-        const float ry = __builtin_amdgcn_rsqf(fmaf(row_sum<WPR>(ss, red, turn), inv, a.eps));
+        const float sy = row_sum<WPR, W>(ss, red, turn), ry = on ? __builtin_amdgcn_rsqf(fmaf(sy, inv, a.eps)) : 0.f;
         float x1[NC][8];
         float s1 = 0.f, sd = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int e = e0 + 512 * c;
             float post[8], scale[8], pre[8];
-            weights(a.post, e, a.D - e, post);
-            weights(a.scale, e, a.D - e, scale);
-            weights(a.pre, e, a.D - e, pre);
+            weights(again(a.post), e, a.D - e, post);
+            weights(again(a.scale), e, a.D - e, scale);
+            weights(again(a.pre), e, a.D - e, pre);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float u = y[c][j] * ry * post[j];
@@ -232,16 +270,16 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_backward(NormA
                 sd = fmaf(dn[c][j] * pre[j], x1[c][j], sd);
             }
         }
-        const float rx = __builtin_amdgcn_rsqf(fmaf(row_sum<WPR>(s1, red, turn), inv, a.eps));
-        const float m1 = row_sum<WPR>(sd, red, turn) * rx * inv;   // mean of d n^
+        const float sx = row_sum<WPR, W>(s1, red, turn), rx = on ? __builtin_amdgcn_rsqf(fmaf(sx, inv, a.eps)) : 0.f;
+        const float m1 = row_sum<WPR, W>(sd, red, turn) * rx * inv;   // mean of d n^
         float s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int e = e0 + 512 * c;
             float post[8], scale[8], pre[8], dz[8];
-            weights(a.post, e, a.D - e, post);
-            weights(a.scale, e, a.D - e, scale);
-            weights(a.pre, e, a.D - e, pre);
+            weights(again(a.post), e, a.D - e, post);
+            weights(again(a.scale), e, a.D - e, scale);
+            weights(again(a.pre), e, a.D - e, pre);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float nh = x1[c][j] * rx, g = fmaf(rx, dn[c][j] * pre[j] - nh * m1, g0[c][j]);
@@ -259,23 +297,24 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_backward(NormA
                 s2 = fmaf(t1 * post[j], wv, s2);
                 x1[c][j] = g;
             }
-            Eight<T>::store(x1[c], row_of<T>(a.x1, a.ldx1, t) + e, a.D - e);
-            if constexpr (GATE) Eight<T>::store(dz, row_of<T>(a.dz, a.lddz, t) + e, a.D - e);
+            const int left = on ? a.D - e : 0;
+            Eight<T>::store(x1[c], row_of<T>(a.x1, a.ldx1, t) + e, left);
+            if constexpr (GATE) Eight<T>::store(dz, row_of<T>(a.dz, a.lddz, t) + e, left);
         }
-        const float m2 = row_sum<WPR>(s2, red, turn) * inv;
+        const float m2 = row_sum<WPR, W>(s2, red, turn) * inv;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int e = e0 + 512 * c;
             float post[8], scale[8], dy[8];
-            weights(a.post, e, a.D - e, post);
-            weights(a.scale, e, a.D - e, scale);
+            weights(again(a.post), e, a.D - e, post);
+            weights(again(a.scale), e, a.D - e, scale);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float t1 = x1[c][j] * scale[j];
                 if constexpr (GATE) t1 *= ssm::silu_fast(z[c][j]);
                 dy[j] = ry * (t1 * post[j] - y[c][j] * ry * m2);
             }
-            Eight<T>::store(dy, row_of<T>(a.n, a.ldn, t) + e, a.D - e);
+            Eight<T>::store(dy, row_of<T>(a.n, a.ldn, t) + e, on ? a.D - e : 0);
         }
     }
     // the workgroup's column sums
@@ -283,21 +322,17 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_backward(NormA
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
         float (&s)[NC][8] = k == 0 ? spost : k == 1 ? sscale : spre;
-        if constexpr (WPR == 1) {
-            __syncthreads();
+        __syncthreads();
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) cols[w][512 * c + lane * 8 + j] = s[c][j];
-            __syncthreads();
-            for (int e = threadIdx.x; e < a.D; e += 256)
-                part[(long)k * a.D + e] = (cols[0][e] + cols[1][e]) + (cols[2][e] + cols[3][e]);
-        } else {
+            for (int j = 0; j < 8; ++j) cols[w / WPR][e0 + 512 * c + j] = s[c][j];
+        __syncthreads();
+        for (int e = threadIdx.x; e < a.D; e += blockDim.x) {
+            float t = cols[0][e];
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (e0 + 512 * c + j < a.D) part[(long)k * a.D + e0 + 512 * c + j] = s[c][j];
+            for (int r = 1; r < RPG; ++r) t += cols[r][e];
+            part[(long)k * a.D + e] = t;
         }
     }
 }
@@ -338,12 +373,13 @@ void forward_of(const NormArgs& a, hipStream_t st) {
     else go_forward<T, 4, 8>(a, st);
 }
 
-// Workgroups of the backward pass: each keeps column sums, which go to memory once.
-int groups_back(int T, int D) { return (int)std::min(D <= 1024 ? ssm::cdiv(T, 4) : (long)T, 512L); }
+// Workgroups of the backward pass: one a CU.
+int rows_at_a_time(int D) { return D <= 1024 ? 8 : D <= 2048 ? 4 : D <= 4096 ? 2 : 1; }
+int groups_back(int T, int D) { return (int)std::min(ssm::cdiv(T, rows_at_a_time(D)), 256L); }
 
 template <typename T, int NC, int WPR>
 void go_backward(const NormArgs& a, hipStream_t st) {
-    const unsigned n = (unsigned)groups_back(a.T, a.D), threads = WPR == 1 ? 256 : 64 * WPR;
+    const unsigned n = (unsigned)groups_back(a.T, a.D), threads = 64 * std::max(WPR, 8);
     if (a.z) norm_backward<T, NC, WPR, true><<<n, threads, 0, st>>>(a);
     else norm_backward<T, NC, WPR, false><<<n, threads, 0, st>>>(a);
 }
