@@ -22,8 +22,8 @@ constexpr float kFloor = -200.f;   // e^kFloor is 0 in fp32: differences are hel
 constexpr float kLowest = -3.40282347e38f;
 typedef unsigned long long u64;
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, int left, float (&f)[8]);
-template <> __device__ __forceinline__ void load8(const float* p, int left, float (&f)[8]) {
+// WHOLE: rows of whole eights (`left` is at least 8, or nothing is there), which keeps the code short.
+template <bool WHOLE> __device__ __forceinline__ void load8(const float* p, int left, float (&f)[8]) {
     typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
     if (left >= 8) {
         const f4 a = reinterpret_cast<const f4*>(p)[0], b = reinterpret_cast<const f4*>(p)[1];
@@ -31,10 +31,10 @@ template <> __device__ __forceinline__ void load8(const float* p, int left, floa
         for (int j = 0; j < 4; ++j) f[j] = a[j], f[4 + j] = b[j];
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = j < left ? p[j] : -__builtin_inff();
+        for (int j = 0; j < 8; ++j) f[j] = !WHOLE && j < left ? p[j] : -__builtin_inff();
     }
 }
-template <> __device__ __forceinline__ void load8(const __bf16* p, int left, float (&f)[8]) {
+template <bool WHOLE> __device__ __forceinline__ void load8(const __bf16* p, int left, float (&f)[8]) {
     typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(2)));
     if (left >= 8) {
         const u4 a = *reinterpret_cast<const u4*>(p);
@@ -42,10 +42,10 @@ template <> __device__ __forceinline__ void load8(const __bf16* p, int left, flo
         for (int j = 0; j < 8; ++j) f[j] = __builtin_bit_cast(float, j % 2 ? a[j / 2] & 0xffff0000u : a[j / 2] << 16);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = j < left ? (float)p[j] : -__builtin_inff();
+        for (int j = 0; j < 8; ++j) f[j] = !WHOLE && j < left ? (float)p[j] : -__builtin_inff();
     }
 }
-__device__ __forceinline__ void store8(float* p, int left, const float (&f)[8]) {
+template <bool WHOLE> __device__ __forceinline__ void store8(float* p, int left, const float (&f)[8]) {
     typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
     if (left >= 8) {
         reinterpret_cast<f4*>(p)[0] = f4{f[0], f[1], f[2], f[3]};
@@ -53,10 +53,10 @@ __device__ __forceinline__ void store8(float* p, int left, const float (&f)[8]) 
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (j < left) p[j] = f[j];
+            if (!WHOLE && j < left) p[j] = f[j];
     }
 }
-__device__ __forceinline__ void store8(__bf16* p, int left, const float (&f)[8]) {
+template <bool WHOLE> __device__ __forceinline__ void store8(__bf16* p, int left, const float (&f)[8]) {
     typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(2)));
     typedef __bf16 b8 __attribute__((ext_vector_type(8)));
     if (left >= 8) {
@@ -67,7 +67,7 @@ __device__ __forceinline__ void store8(__bf16* p, int left, const float (&f)[8])
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (j < left) p[j] = (__bf16)f[j];
+            if (!WHOLE && j < left) p[j] = (__bf16)f[j];
     }
 }
 
@@ -126,20 +126,46 @@ __device__ __forceinline__ u64 lane64(u64 v, int lane) {   // lane: the same in 
     return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
            (unsigned)__builtin_amdgcn_readlane((int)v, lane);
 }
+// The key of lane ^ J (J a power of two): within a row of 16 lanes by the moves that the vector unit has.
+template <int CTRL> __device__ __forceinline__ u64 moved(u64 v) {
+    return (u64)(unsigned)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, 0xf, 0xf, true) << 32 |
+           (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ u64 across(u64 v, int lane, int j) {   // j: a constant after unrolling
+    switch (j) {
+        case 1: return moved<0xb1>(v);                  // quad_perm 1 0 3 2
+        case 2: return moved<0x4e>(v);                  // quad_perm 2 3 0 1
+        case 4: return moved<0x1b>(moved<0x141>(v));    // row_half_mirror (^ 7), then quad_perm 3 2 1 0 (^ 3)
+        case 8: return moved<0x128>(v);                 // row_ror 8
+        default: return shfl64(v, lane ^ j);
+    }
+}
 // The lanes' keys in descending order over the lanes.
-__device__ u64 sorted(u64 v, int lane) {
+__device__ __forceinline__ u64 sorted(u64 v, int lane) {
+#pragma unroll
     for (int k = 2; k <= 64; k *= 2)
+#pragma unroll
         for (int j = k / 2; j > 0; j /= 2) {
-            const u64 o = shfl64(v, lane ^ j);
+            const u64 o = across(v, lane, j);
             const bool high = ((lane & j) == 0) == ((lane & k) == 0);   // this lane takes the larger one
             v = (v > o) == high ? v : o;
         }
     return v;
 }
+// The 64 largest of two sorted lists, sorted: the larger of each pair of one and the other's mirror, then six levels.
+__device__ __forceinline__ u64 merged(u64 a, u64 b, int lane) {
+    u64 o = shfl64(b, 63 - lane), v = a > o ? a : o;
+#pragma unroll
+    for (int j = 32; j > 0; j /= 2) {
+        o = across(v, lane, j);
+        v = (v > o) == ((lane & j) == 0) ? v : o;
+    }
+    return v;
+}
 // A key enters the sorted list, whose last one leaves it.
 __device__ __forceinline__ u64 entered(u64 list, u64 key, int lane) {
     const int at = __popcll(__ballot(list > key));
-    const u64 below = shfl64(list, (lane + 63) & 63);
+    const u64 below = moved<0x138>(list);   // wave_shr 1
     return lane < at ? list : lane == at ? key : below;
 }
 
@@ -152,23 +178,13 @@ struct LogArgs {
     int M, N, k, slices, turns;
 };
 
-// How many of a list's keys are larger.
-__device__ __forceinline__ int rank_of(u64 mine, const u64* keys, int have) {
-    int rank = 0, o = 0;
-    for (; o + 8 <= have; o += 8)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) rank += keys[o + j] > mine;
-    for (; o < have; ++o) rank += keys[o] > mine;
-    return rank;
-}
-
-// What a row's results are, from its sums and its lists' keys (`have` of them in LDS, unique; 0: none).
+// By one wave: a row's results from its sums and its sorted list (0: none).
 template <typename T>
-__device__ void finish(const LogArgs& a, int row, Sums s, const u64* keys, int have) {
+__device__ __forceinline__ void finish(const LogArgs& a, int row, Sums s, u64 list, int lane) {
     // (nothing left: Z = 0)
     const bool none = s.z == 0.f;
     const float m = fmaxf(s.m, kLowest), logz = none ? -__builtin_inff() : logf(s.z);
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
         if (a.stats) a.stats[row] = make_float2(m, logz);
         const float h = logz - s.s / s.z;
         if (a.ent) a.ent[row] = none || h < 0.f ? 0.f : h;   // (below 0 by rounding)
@@ -178,20 +194,16 @@ __device__ void finish(const LogArgs& a, int row, Sums s, const u64* keys, int h
             a.logp[row] = !given ? 0.f : none ? -__builtin_inff() : ((float)static_cast<const T*>(a.x)[row * a.ldx + id] - m) - logz;
         }
     }
-    for (int c = threadIdx.x; c < have; c += blockDim.x) {
-        const u64 mine = keys[c];
-        const int rank = rank_of(mine, keys, have);
-        if (mine && rank < a.k) {
-            a.top[(long)row * a.k + rank] = (int)index_of(mine);
-            a.toplp[(long)row * a.k + rank] = none ? -__builtin_inff() : (value_of(mine) - m) - logz;
-        }
+    if (lane < a.k) {
+        a.top[(long)row * a.k + lane] = (int)index_of(list);
+        a.toplp[(long)row * a.k + lane] = none ? -__builtin_inff() : (value_of(list) - m) - logz;
     }
 }
 
-template <typename T, bool TOP>
-__global__ __launch_bounds__(256) void logprob_kernel(LogArgs a) {
+template <typename T, bool TOP, bool WHOLE>
+__global__ __launch_bounds__(256, 8) void logprob_kernel(LogArgs a) {
     __shared__ Sums ws[4];
-    __shared__ u64 lists[TOP ? 4 * kMaxTop : 1];
+    __shared__ u64 lists[4][TOP ? 64 : 1], near[4][TOP ? 512 : 1];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -205,11 +217,11 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogArgs a) {
         if (base >= a.N) break;
         float v[kGroups][8];
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) load8<T>(x + base + (g * 64 + lane) * 8, a.N - base - (g * 64 + lane) * 8, v[g]);
+        for (int g = 0; g < kGroups; ++g) load8<WHOLE>(x + base + (g * 64 + lane) * 8, a.N - base - (g * 64 + lane) * 8, v[g]);
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) take8(s, v[g]);
         if constexpr (TOP) {
-            u64 own = 0;
+            int own = -1;
             if (!full) {   // the first turn: the lanes' maxima (any of a lane's logits would do)
                 float most = v[0][0];
                 int at = 0;
@@ -221,71 +233,92 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogArgs a) {
                         most = up ? v[g][j] : most;
                         at = up ? g * 512 + j : at;
                     }
-                at += base + lane * 8;
-                own = at < a.N ? key_of(most, at) : 0;
-                list = sorted(own, lane);
+                own = at + base + lane * 8;
+                list = sorted(own < a.N ? key_of(most, own) : 0, lane);
                 least = lane64(list, a.k - 1);
                 bar = least ? value_of(least) : __builtin_nanf("");
             }
-            bool some = false;   // (all earlier logits of the wave have lower indices: equal ones stay out)
+            // Logits that may enter (of an unfilled list: equal ones too; later, all earlier logits of the wave have
+            // lower indices) are written side by side, a group at a time, and entered from there.
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g)
+            for (int g = 0; g < kGroups; ++g) {
+                bool some = false;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) some |= full ? !(v[g][j] <= bar) : !(v[g][j] < bar);
-            if (__any(some)) {
+                if (!__any(some)) continue;
+                int n = 0;
 #pragma unroll
-                for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        if (!__any(!(v[g][j] < bar))) continue;
-                        const int at = base + (g * 64 + lane) * 8 + j;
-                        const u64 key = at < a.N ? key_of(v[g][j], at) : 0;
-                        u64 left = __ballot(key > least && key != own);
-                        while (left) {
-                            const int l = __builtin_ctzll(left);
-                            list = entered(list, lane64(key, l), lane);
-                            least = lane64(list, a.k - 1);
-                            left &= left - 1;
-                            left &= __ballot(key > least);
-                        }
-                        bar = least ? value_of(least) : __builtin_nanf("");
+                for (int j = 0; j < 8; ++j) {
+                    const int at = base + (g * 64 + lane) * 8 + j;
+                    const bool in = (full ? !(v[g][j] <= bar) : !(v[g][j] < bar)) && at < a.N && at != own;   // (own: in the list)
+                    const u64 which = __ballot(in);
+                    if (in) near[w][n + __builtin_amdgcn_mbcnt_hi((unsigned)(which >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)which, 0))] = key_of(v[g][j], at);
+                    n += __popcll(which);
+                }
+                __builtin_amdgcn_wave_barrier();
+                for (int k = 0; k < n; k += 64) {
+                    const u64 key = k + lane < n ? near[w][k + lane] : 0;
+                    u64 left = __ballot(key > least);
+                    if (__popcll(left) > 8) {   // (an entry takes about an eighth of a sort and merge)
+                        list = merged(list, sorted(key, lane), lane);
+                        least = lane64(list, a.k - 1);
+                        left = 0;
                     }
+                    while (left) {
+                        const int l = __builtin_ctzll(left);
+                        list = entered(list, lane64(key, l), lane);
+                        least = lane64(list, a.k - 1);
+                        left &= left - 1;
+                        left &= __ballot(key > least);
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
+                bar = least ? value_of(least) : __builtin_nanf("");
             }
             full = least != 0;
         }
     }
     s = over_wave(s);
     if (lane == 0) ws[w] = s;
-    if constexpr (TOP)
-        if (lane < a.k) lists[w * a.k + lane] = list;
+    if constexpr (TOP) lists[w][lane] = list;
     __syncthreads();
+    if (w) return;
     s = join(join(ws[0], ws[1]), join(ws[2], ws[3]));
+    if constexpr (TOP)
+        for (int o = 1; o < 4; ++o) list = merged(list, lists[o][lane], lane);
     if (a.slices == 1) {
-        finish<T>(a, row, s, lists, TOP ? 4 * a.k : 0);
+        finish<T>(a, row, s, list, lane);
         return;
     }
-    if (threadIdx.x == 0) a.sums[blockIdx.x] = s;
+    if (lane == 0) a.sums[blockIdx.x] = s;
     if constexpr (TOP)
-        for (int c = threadIdx.x; c < 4 * a.k; c += 256) {
-            const u64 mine = lists[c];
-            const int rank = rank_of(mine, lists, 4 * a.k);
-            u64* out = a.keys + (long)blockIdx.x * a.k;
-            if (mine && rank < a.k) out[rank] = mine;
-            if (c < a.k && c >= rank_of(0, lists, 4 * a.k)) out[c] = 0;   // (fewer logits than k)
-        }
+        if (lane < a.k) a.keys[(long)blockIdx.x * a.k + lane] = list;
 }
 
 // The slices of a row together.
 template <typename T>
-__global__ __launch_bounds__(1024) void logprob_join(LogArgs a) {
-    extern __shared__ u64 all[];
-    const int row = blockIdx.x, have = a.slices * a.k, lane = threadIdx.x & 63;
-    for (int c = threadIdx.x; c < have; c += blockDim.x) all[c] = a.keys[(long)row * have + c];
+__global__ __launch_bounds__(256) void logprob_join(LogArgs a) {
+    __shared__ u64 lists[4][64];
+    const int row = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     Sums s{kLowest, 0.f, 0.f};
     if (lane < a.slices) s = a.sums[(long)row * a.slices + lane];
-    s = over_wave(s);
-    __syncthreads();
-    finish<T>(a, row, s, all, have);
+    u64 list = 0;
+    if (a.k) {
+        const u64* keys = a.keys + (long)row * a.slices * a.k + lane;
+        u64 next = lane < a.k && w < a.slices ? keys[(long)w * a.k] : 0;
+        for (int c = w; c < a.slices; c += 4) {
+            const u64 here = next;
+            next = lane < a.k && c + 4 < a.slices ? keys[(long)(c + 4) * a.k] : 0;
+            list = merged(list, here, lane);
+        }
+        lists[w][lane] = list;
+        __syncthreads();
+        if (w) return;
+        for (int o = 1; o < 4; ++o) list = merged(list, lists[o][lane], lane);
+    } else if (w) {
+        return;
+    }
+    finish<T>(a, row, over_wave(s), list, lane);
 }
 
 struct GradArgs {
@@ -297,7 +330,7 @@ struct GradArgs {
     int M, N, pieces;
 };
 
-template <typename T>
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
     const int row = blockIdx.x / a.pieces, piece = blockIdx.x - row * a.pieces;
     const float2 st = a.stats[row];
@@ -311,7 +344,7 @@ __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
         const int at = piece * kRun + (g * 256 + (int)threadIdx.x) * 8;
-        load8<T>(x + at, a.N - at, f[g]);
+        load8<WHOLE>(x + at, a.N - at, f[g]);
     }
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
@@ -322,7 +355,7 @@ __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
             const float d = -p * fmaf(v, fmaxf(lp, kFloor) + h, w);
             f[g][j] = none ? 0.f : at + j == id ? d + w : d;
         }
-        store8(dx + at, a.N - at, f[g]);
+        store8<WHOLE>(dx + at, a.N - at, f[g]);
     }
 }
 
@@ -334,14 +367,18 @@ int slices_of(int M, int N) {
 
 size_t sums_bytes(int M, int slices) { return ((size_t)M * slices * sizeof(Sums) + 15) / 16 * 16; }
 
-template <typename T>
+template <typename T, bool WHOLE>
 void run_logprobs(const LogArgs& a, hipStream_t st) {
     const unsigned n = (unsigned)((long)a.M * a.slices);
-    if (a.k) logprob_kernel<T, true><<<n, 256, 0, st>>>(a);
-    else logprob_kernel<T, false><<<n, 256, 0, st>>>(a);
-    // a thread for each slice's key
-    const int have = a.slices * a.k, threads = std::min(1024, std::max(64, (have + 63) / 64 * 64));
-    if (a.slices > 1) logprob_join<T><<<a.M, threads, std::max(8, have * 8), st>>>(a);
+    if (a.k) logprob_kernel<T, true, WHOLE><<<n, 256, 0, st>>>(a);
+    else logprob_kernel<T, false, WHOLE><<<n, 256, 0, st>>>(a);
+    if (a.slices > 1) logprob_join<T><<<a.M, 256, 0, st>>>(a);
+}
+template <typename T>
+void run_grad(const GradArgs& a, hipStream_t st) {
+    const unsigned n = (unsigned)((long)a.M * a.pieces);
+    if (a.N % 8 == 0) logprob_grad<T, true><<<n, 256, 0, st>>>(a);
+    else logprob_grad<T, false><<<n, 256, 0, st>>>(a);
 }
 
 }  // namespace
@@ -384,8 +421,9 @@ extern "C" ssm_status ssm_token_logprobs(int dtype, const void* x, long ldx, con
     a.turns = (int)ssm::cdiv(ssm::cdiv(N, kRun), slices);
     a.sums = static_cast<Sums*>(workspace);
     a.keys = reinterpret_cast<u64*>(static_cast<char*>(workspace) + sums_bytes(M, slices));
-    if (dtype == SSM_F32) run_logprobs<float>(a, (hipStream_t)stream);
-    else run_logprobs<__bf16>(a, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == SSM_F32) N % 8 ? run_logprobs<float, false>(a, st) : run_logprobs<float, true>(a, st);
+    else N % 8 ? run_logprobs<__bf16, false>(a, st) : run_logprobs<__bf16, true>(a, st);
     return ssm::check_launch("ssm_token_logprobs");
 }
 
@@ -410,8 +448,7 @@ extern "C" ssm_status ssm_token_logprobs_backward(int dtype, const void* x, long
     GradArgs a{};
     a.x = x; a.ldx = ldx; a.ids = ids; a.stats = reinterpret_cast<const float2*>(stats); a.ent = entropy;
     a.dlogp = dlogp; a.dent = dentropy; a.dx = dx; a.lddx = lddx; a.M = M; a.N = N; a.pieces = (int)pieces;
-    const unsigned n = (unsigned)(M * pieces);
-    if (dtype == SSM_F32) logprob_grad<float><<<n, 256, 0, (hipStream_t)stream>>>(a);
-    else logprob_grad<__bf16><<<n, 256, 0, (hipStream_t)stream>>>(a);
+    if (dtype == SSM_F32) run_grad<float>(a, (hipStream_t)stream);
+    else run_grad<__bf16>(a, (hipStream_t)stream);
     return ssm::check_launch("ssm_token_logprobs_backward");
 }
