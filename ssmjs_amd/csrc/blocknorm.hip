@@ -17,9 +17,10 @@ namespace {
 
 constexpr int kMaxD = 16384;
 
-// Eight elements of a row, as they lie in memory; `left` of them exist.
-template <typename T> struct Eight;
-template <> struct Eight<float> {
+// Eight elements of a row, as they lie in memory; `left` of them exist. WHOLE: at least eight, or none, which keeps the
+// code short.
+template <typename T, bool WHOLE> struct Eight;
+template <bool WHOLE> struct Eight<float, WHOLE> {
     float v[8];
     typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
     __device__ __forceinline__ void load(const float* p, int left) {
@@ -30,7 +31,7 @@ template <> struct Eight<float> {
             for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.f;
+            for (int j = 0; j < 8; ++j) v[j] = !WHOLE && j < left ? p[j] : 0.f;
         }
     }
     __device__ __forceinline__ float operator[](int j) const { return v[j]; }
@@ -41,11 +42,11 @@ template <> struct Eight<float> {
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (j < left) p[j] = f[j];
+                if (!WHOLE && j < left) p[j] = f[j];
         }
     }
 };
-template <> struct Eight<__bf16> {
+template <bool WHOLE> struct Eight<__bf16, WHOLE> {
     typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(2)));
     typedef __bf16 b8 __attribute__((ext_vector_type(8)));
     unsigned v[4];
@@ -58,7 +59,7 @@ template <> struct Eight<__bf16> {
             const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                v[j] = (2 * j < left ? h[2 * j] : 0u) | (2 * j + 1 < left ? (unsigned)h[2 * j + 1] << 16 : 0u);
+                v[j] = (!WHOLE && 2 * j < left ? h[2 * j] : 0u) | (!WHOLE && 2 * j + 1 < left ? (unsigned)h[2 * j + 1] << 16 : 0u);
         }
     }
     __device__ __forceinline__ float operator[](int j) const {
@@ -73,12 +74,13 @@ template <> struct Eight<__bf16> {
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (j < left) p[j] = (__bf16)f[j];
+                if (!WHOLE && j < left) p[j] = (__bf16)f[j];
         }
     }
 };
 
 // Eight weights (none: ones).
+template <bool WHOLE>
 __device__ __forceinline__ void weights(const float* w, int e, int left, float (&f)[8]) {
     typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
     if (!w) {
@@ -90,7 +92,7 @@ __device__ __forceinline__ void weights(const float* w, int e, int left, float (
         for (int j = 0; j < 4; ++j) f[j] = a[j], f[4 + j] = b[j];
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = j < left ? w[e + j] : 0.f;
+        for (int j = 0; j < 8; ++j) f[j] = !WHOLE && j < left ? w[e + j] : 0.f;
     }
 }
 
@@ -153,7 +155,7 @@ template <typename T> __device__ __forceinline__ const T* row_of(const void* p, 
 template <typename T> __device__ __forceinline__ T* row_of(void* p, long ld, long t) { return static_cast<T*>(p) + t * ld; }
 
 // 512 NC WPR elements a row at most; four rows a workgroup where a row is one wave's.
-template <typename T, int NC, int WPR, bool GATE>
+template <typename T, int NC, int WPR, bool GATE, bool WHOLE>
 __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_kernel(NormArgs a) {
     __shared__ float red[2][WPR];
     int turn = 0;
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_kernel(NormArg
     const T* px = row_of<T>(a.x, a.ldx, t) + e0;
     const T* py = row_of<T>(a.y, a.ldy, t) + e0;
     const T* pz = GATE ? row_of<T>(a.z, a.ldz, t) + e0 : nullptr;
-    Eight<T> x[NC], y[NC], z[NC];
+    Eight<T, WHOLE> x[NC], y[NC], z[NC];
     float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -176,6 +178,13 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_kernel(NormArg
     for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(y[c][j], y[c][j], ss);
+    // (the weights with the row where there is one piece of each: one trip to memory)
+    float post[8], scale[8], pre[8];
+    if constexpr (NC == 1) {
+        weights<WHOLE>(a.post, e0, a.D - e0, post);
+        weights<WHOLE>(a.scale, e0, a.D - e0, scale);
+        weights<WHOLE>(a.pre, e0, a.D - e0, pre);
+    }
     const float inv = 1.f / (float)a.D;
     const float ry = __builtin_amdgcn_rsqf(fmaf(row_sum<WPR, WPR>(ss, red, turn), inv, a.eps));
     float x1[NC][8];
@@ -183,9 +192,10 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_kernel(NormArg
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int e = e0 + 512 * c;
-        float post[8], scale[8];
-        weights(a.post, e, a.D - e, post);
-        weights(a.scale, e, a.D - e, scale);
+        if constexpr (NC > 1) {
+            weights<WHOLE>(a.post, e, a.D - e, post);
+            weights<WHOLE>(a.scale, e, a.D - e, scale);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             float u = y[c][j] * ry * post[j];
@@ -200,18 +210,18 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_kernel(NormArg
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int e = e0 + 512 * c;
-        float pre[8], n[8];
-        weights(a.pre, e, a.D - e, pre);
+        float n[8];
+        if constexpr (NC > 1) weights<WHOLE>(a.pre, e, a.D - e, pre);
 #pragma unroll
         for (int j = 0; j < 8; ++j) n[j] = x1[c][j] * rx * pre[j];
-        Eight<T>::store(x1[c], p1 + e, a.D - e);
-        Eight<T>::store(n, pn + e, a.D - e);
+        Eight<T, WHOLE>::store(x1[c], p1 + e, a.D - e);
+        Eight<T, WHOLE>::store(n, pn + e, a.D - e);
     }
 }
 
 // W = 8 waves (16 for one row) a workgroup and one workgroup a CU, which walks its rows and keeps the column sums of
 // its lanes' elements: few partial sums, and they go to memory once.
-template <typename T, int NC, int WPR, bool GATE>
+template <typename T, int NC, int WPR, bool GATE, bool WHOLE>
 __global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArgs a) {
     constexpr int W = WPR > 8 ? WPR : 8, RPG = W / WPR;   // rows at a time
     __shared__ float red[2][W];
@@ -223,7 +233,7 @@ __global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArg
     float spost[NC][8] = {}, sscale[NC][8] = {}, spre[NC][8] = {};
     const long step = (long)RPG * gridDim.x;
     constexpr bool kAhead = NC == 1 || (!GATE && sizeof(T) == 2);   // (registers for the next row too)
-    Eight<T> x[NC], y[NC], z[NC], dn[NC], g0[NC], nx[NC], ny[NC], nz[NC], ndn[NC], ng0[NC];
+    Eight<T, WHOLE> x[NC], y[NC], z[NC], dn[NC], g0[NC], nx[NC], ny[NC], nz[NC], ndn[NC], ng0[NC];
     auto fetch = [&](long t) {   // the next row, on its way while this one is worked on
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -258,9 +268,9 @@ __global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArg
         for (int c = 0; c < NC; ++c) {
             const int e = e0 + 512 * c;
             float post[8], scale[8], pre[8];
-            weights(again(a.post), e, a.D - e, post);
-            weights(again(a.scale), e, a.D - e, scale);
-            weights(again(a.pre), e, a.D - e, pre);
+            weights<WHOLE>(again(a.post), e, a.D - e, post);
+            weights<WHOLE>(again(a.scale), e, a.D - e, scale);
+            weights<WHOLE>(again(a.pre), e, a.D - e, pre);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float u = y[c][j] * ry * post[j];
@@ -277,9 +287,9 @@ __global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArg
         for (int c = 0; c < NC; ++c) {
             const int e = e0 + 512 * c;
             float post[8], scale[8], pre[8], dz[8];
-            weights(again(a.post), e, a.D - e, post);
-            weights(again(a.scale), e, a.D - e, scale);
-            weights(again(a.pre), e, a.D - e, pre);
+            weights<WHOLE>(again(a.post), e, a.D - e, post);
+            weights<WHOLE>(again(a.scale), e, a.D - e, scale);
+            weights<WHOLE>(again(a.pre), e, a.D - e, pre);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float nh = x1[c][j] * rx, g = fmaf(rx, dn[c][j] * pre[j] - nh * m1, g0[c][j]);
@@ -298,23 +308,23 @@ __global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArg
                 x1[c][j] = g;
             }
             const int left = on ? a.D - e : 0;
-            Eight<T>::store(x1[c], row_of<T>(a.x1, a.ldx1, t) + e, left);
-            if constexpr (GATE) Eight<T>::store(dz, row_of<T>(a.dz, a.lddz, t) + e, left);
+            Eight<T, WHOLE>::store(x1[c], row_of<T>(a.x1, a.ldx1, t) + e, left);
+            if constexpr (GATE) Eight<T, WHOLE>::store(dz, row_of<T>(a.dz, a.lddz, t) + e, left);
         }
         const float m2 = row_sum<WPR, W>(s2, red, turn) * inv;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int e = e0 + 512 * c;
             float post[8], scale[8], dy[8];
-            weights(again(a.post), e, a.D - e, post);
-            weights(again(a.scale), e, a.D - e, scale);
+            weights<WHOLE>(again(a.post), e, a.D - e, post);
+            weights<WHOLE>(again(a.scale), e, a.D - e, scale);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float t1 = x1[c][j] * scale[j];
                 if constexpr (GATE) t1 *= ssm::silu_fast(z[c][j]);
                 dy[j] = ry * (t1 * post[j] - y[c][j] * ry * m2);
             }
-            Eight<T>::store(dy, row_of<T>(a.n, a.ldn, t) + e, on ? a.D - e : 0);
+            Eight<T, WHOLE>::store(dy, row_of<T>(a.n, a.ldn, t) + e, on ? a.D - e : 0);
         }
     }
     // the workgroup's column sums
@@ -360,17 +370,19 @@ __global__ __launch_bounds__(1024) void norm_columns(const float* __restrict__ p
 template <typename T, int NC, int WPR>
 void go_forward(const NormArgs& a, hipStream_t st) {
     const unsigned n = (unsigned)(WPR == 1 ? ssm::cdiv(a.T, 4) : a.T), threads = WPR == 1 ? 256 : 64 * WPR;
-    if (a.z) norm_kernel<T, NC, WPR, true><<<n, threads, 0, st>>>(a);
-    else norm_kernel<T, NC, WPR, false><<<n, threads, 0, st>>>(a);
+    if (a.D % 8) a.z ? norm_kernel<T, NC, WPR, true, false><<<n, threads, 0, st>>>(a) : norm_kernel<T, NC, WPR, false, false><<<n, threads, 0, st>>>(a);
+    else a.z ? norm_kernel<T, NC, WPR, true, true><<<n, threads, 0, st>>>(a) : norm_kernel<T, NC, WPR, false, true><<<n, threads, 0, st>>>(a);
 }
 template <typename T>
 void forward_of(const NormArgs& a, hipStream_t st) {
+    // eight elements a lane, as many waves as that takes (us, against four times the elements and a quarter of the
+    // waves: 64 x 2048 bf16 2.9 / 5.0, 16384 x 2048 55.8 / 65.7, 4096 x 8192 61 / 67)
     if (a.D <= 512) go_forward<T, 1, 1>(a, st);
-    else if (a.D <= 1024) go_forward<T, 2, 1>(a, st);
-    else if (a.D <= 2048) go_forward<T, 4, 1>(a, st);
-    else if (a.D <= 4096) go_forward<T, 4, 2>(a, st);
-    else if (a.D <= 8192) go_forward<T, 4, 4>(a, st);
-    else go_forward<T, 4, 8>(a, st);
+    else if (a.D <= 1024) go_forward<T, 1, 2>(a, st);
+    else if (a.D <= 2048) go_forward<T, 1, 4>(a, st);
+    else if (a.D <= 4096) go_forward<T, 1, 8>(a, st);
+    else if (a.D <= 8192) go_forward<T, 1, 16>(a, st);
+    else go_forward<T, 2, 16>(a, st);
 }
 
 // Workgroups of the backward pass: one a CU.
@@ -380,8 +392,8 @@ int groups_back(int T, int D) { return (int)std::min(ssm::cdiv(T, rows_at_a_time
 template <typename T, int NC, int WPR>
 void go_backward(const NormArgs& a, hipStream_t st) {
     const unsigned n = (unsigned)groups_back(a.T, a.D), threads = 64 * std::max(WPR, 8);
-    if (a.z) norm_backward<T, NC, WPR, true><<<n, threads, 0, st>>>(a);
-    else norm_backward<T, NC, WPR, false><<<n, threads, 0, st>>>(a);
+    if (a.D % 8) a.z ? norm_backward<T, NC, WPR, true, false><<<n, threads, 0, st>>>(a) : norm_backward<T, NC, WPR, false, false><<<n, threads, 0, st>>>(a);
+    else a.z ? norm_backward<T, NC, WPR, true, true><<<n, threads, 0, st>>>(a) : norm_backward<T, NC, WPR, false, true><<<n, threads, 0, st>>>(a);
 }
 template <typename T>
 void backward_of(const NormArgs& a, hipStream_t st) {

@@ -656,29 +656,35 @@ def block_norm_backward(dx1, dn, x, y, z=None, post=None, scale=None, pre=None, 
     code, dev = _code(dt), _current("x", x)
 
     def side(name, t):
-        return (None, D) if t is None else (_at(name, t, shape, dt, dev), _flat(name, t))
+        if t is None:
+            return None, D
+        return _at(name, t, shape, dt, dev), D if t.is_contiguous() else _flat(name, t)
 
     if out is None:
-        out = x.new_empty(shape), x.new_empty(shape), x.new_empty(shape) if z is not None else None
-    dx, dy, dz = out
-    if z is not None and dz is None:
-        raise ValueError("out[2]: a gate needs its gradient's tensor")
-    if z is None:
-        dz = None
-    grads = [w.new_empty(D, dtype=_f32_t) if w is not None else None for w in (post, scale, pre)]
+        dx, dy, dz = torch.empty_like(y), torch.empty_like(y), torch.empty_like(y) if z is not None else None
+        if not y.is_contiguous():
+            dx, dy, dz = (t if t is None else t.new_empty(shape) for t in (dx, dy, dz))
+    else:
+        dx, dy, dz = out
+        if z is None:
+            dz = None
+        elif dz is None:
+            raise ValueError("out[2]: a gate needs its gradient's tensor")
+    # (one piece of memory each, as a program keeps or drops them one by one)
+    dpost, dscale, dpre = (None if w is None else torch.empty_like(w) for w in (post, scale, pre))
     if T == 0:
-        for g in grads:
+        for g in (dpost, dscale, dpre):
             if g is not None:
                 g.zero_()
-        return dx, dy, dz, *grads
+        return dx, dy, dz, dpost, dscale, dpre
     ws, pws, nbytes = _own_scratch(workspace, _lib.lib().ssm_block_norm_backward_workspace(T, D), x)
     w = (D,)
-    _lib.call("ssm_block_norm_backward", code, *side("dx1", dx1), *side("dn", dn), x.data_ptr(), _flat("x", x),
-              *side("y", y), *side("z", z), _packed("post", post, w, _f32_t, dev),
-              _packed("scale", scale, w, _f32_t, dev), _packed("pre", pre, w, _f32_t, dev), eps,
-              *side("out[0]", dx), *side("out[1]", dy), *side("out[2]", dz),
-              *(None if g is None else g.data_ptr() for g in grads), T, D, pws, nbytes, _on(dev))
-    return dx, dy, dz, *grads
+    _lib.call("ssm_block_norm_backward", code, *side("dx1", dx1), *side("dn", dn), *side("x", x), *side("y", y),
+              *side("z", z), _packed("post", post, w, _f32_t, dev), _packed("scale", scale, w, _f32_t, dev),
+              _packed("pre", pre, w, _f32_t, dev), eps, *side("out[0]", dx), *side("out[1]", dy), *side("out[2]", dz),
+              None if dpost is None else dpost.data_ptr(), None if dscale is None else dscale.data_ptr(),
+              None if dpre is None else dpre.data_ptr(), T, D, pws, nbytes, _on(dev))
+    return dx, dy, dz, dpost, dscale, dpre
 
 
 def token_logprobs(logits, ids=None, k=0, stats=None, workspace=None):
