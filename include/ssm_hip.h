@@ -426,7 +426,14 @@ ssm_status ssm_model_export_weights(ssm_model* m, int f16, void* buf, size_t cap
 /* model.forward(ids, batch, seqLen) (streaming.ts:31-35): host ids (B,L) -> host logits
  * (B,L,V), zero initial state. */
 ssm_status ssm_forward(ssm_model* m, const uint32_t* ids, int B, int L, float* logits);
-/* Same with device buffers, enqueued on the context stream (no host synchronisation). */
+/* One forward of host ids (B,L) and what it says of them, without their logits on the host (the MambaTrainer's
+ * evaluation, session.ts:504-507, reads all B L V of them): for every position the log probability of the token that
+ * follows (0 at a sequence's last), the entropy of its prediction (natural logarithms) and the k <= 64 likeliest next
+ * tokens, as ssm_token_logprobs. logp, entropy (B,L), top_ids, top_logp (B,L,k) host; logp and entropy may be NULL, the
+ * others with k = 0. B L < 2^24. */
+ssm_status ssm_score(ssm_model* m, const uint32_t* ids, int B, int L, int k, float* logp, float* entropy,
+                     uint32_t* top_ids, float* top_logp);
+/* Same as ssm_forward with device buffers, enqueued on the context stream (no host synchronisation). */
 ssm_status ssm_forward_device(ssm_model* m, const uint32_t* d_ids, int B, int L,
                               float* d_logits);
 /* One mixer (layer `layer`, no norm / residual) over device hidden states (B,L,d_model). */

@@ -148,6 +148,7 @@ PROTOTYPES = {
     "ssm_model_load_weights": (_i, [_vp, _vp, _sz]),
     "ssm_model_export_weights": (_i, [_vp, _i, _vp, _sz, C.POINTER(_sz)]),
     "ssm_forward": (_i, [_vp, _vp, _i, _i, _vp]),
+    "ssm_score": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "ssm_forward_device": (_i, [_vp, _vp, _i, _i, _vp]),
     "ssm_mixer_forward_device": (_i, [_vp, _i, _vp, _vp, _i, _i]),
     "ssm_mixer_forward_device_bf16": (_i, [_vp, _i, _vp, _vp, _i, _i]),

@@ -128,6 +128,20 @@ class Model:
         _lib.call("ssm_forward", self._h, _ptr(ids), B, L, _ptr(out))
         return out
 
+    def score(self, ids, k: int = 0):
+        """One forward of ids (B,L) and what it says of them (ssm_score): (logp, entropy, top_ids, top_logp),
+        the log probability of the token after each position (0 at the last) and the entropy of its prediction,
+        (B,L), and the k <= 64 likeliest next tokens, (B,L,k)."""
+        ids = np.ascontiguousarray(ids, dtype=np.uint32)
+        if ids.ndim == 1:
+            ids = ids[None]
+        B, L = ids.shape
+        logp, ent = np.zeros((B, L), np.float32), np.zeros((B, L), np.float32)
+        top, toplp = np.zeros((B, L, k), np.uint32), np.zeros((B, L, k), np.float32)
+        _lib.call("ssm_score", self._h, _ptr(ids), B, L, int(k), _ptr(logp), _ptr(ent), _ptr(top) if k else None,
+                  _ptr(toplp) if k else None)
+        return logp, ent, top, toplp
+
     def new_state(self, B: int) -> "State":
         return State(self, B)
 

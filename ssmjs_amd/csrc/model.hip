@@ -21,7 +21,9 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <tuple>
 #include <string>
 #include <vector>
@@ -558,6 +560,8 @@ struct ssm_model {
     int* d_flag = nullptr;   // out-of-range token id flag
     uint32_t* d_ids = nullptr;
     size_t ids_cap = 0;
+    char* score = nullptr;   // ssm_score's outputs and workspace
+    size_t score_bytes = 0;
     bool destroyed = false;
 };
 
@@ -1639,7 +1643,7 @@ extern "C" ssm_status ssm_model_destroy(ssm_model* m) {
     if (!m->ctx->destroyed) {
         hipSetDevice(m->ctx->device);
         hipStreamSynchronize(m->ctx->stream);
-        hipFree(m->w); hipFree(m->Ab); hipFree(m->ws); hipFree(m->d_flag); hipFree(m->d_ids);
+        hipFree(m->w); hipFree(m->Ab); hipFree(m->ws); hipFree(m->d_flag); hipFree(m->d_ids); hipFree(m->score);
         hipFree(m->rg); hipFree(m->wp); hipFree(m->wb); hipFree(m->wh); hipFree(m->wh_emb);
     }
     m->destroyed = true;
@@ -1761,6 +1765,62 @@ extern "C" ssm_status ssm_forward(ssm_model* m, const uint32_t* ids, int B, int 
     SSM_HIP_TRY(hipMemcpyAsync(logits, w.logits, T * m->dm.V * 4, hipMemcpyDeviceToHost,
                                m->ctx->stream));
     return check_flag(m);
+}
+
+extern "C" ssm_status ssm_score(ssm_model* m, const uint32_t* ids, int B, int L, int k, float* logp,
+                                float* entropy, uint32_t* top_ids, float* top_logp) {
+    CtxLock lk;
+    SSM_TRY(model_enter(m, lk));
+    SSM_REQUIRE(ids && B >= 0 && L >= 0 && k >= 0 && (k == 0 || (top_ids && top_logp)), "ssm_score: bad args");
+    SSM_REQUIRE(k <= m->dm.V, "ssm_score: %d alternatives of %d tokens", k, m->dm.V);
+    if (k > 64) return ssm::fail(SSM_ERR_UNSUPPORTED, "ssm_score: %d alternatives, at most 64", k);
+    if (B == 0 || L == 0) return SSM_OK;
+    SSM_REQUIRE((long)B * L < (1L << 24), "ssm_score: too many tokens");
+    SSM_TRY(derived_current(m));
+    const size_t T = (size_t)B * L;
+    SSM_TRY(ensure_ids(m, 2 * T));
+    Ws w;
+    SSM_TRY(ensure_ws(m, B, L, true, &w));
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    const size_t row = up(4 * T), tops = up(4 * T * k), ws = ssm_token_logprobs_workspace((int)T, m->dm.V, k),
+                 need = 2 * row + 2 * tops + ws;
+    if (need > m->score_bytes) {
+        SSM_HIP_TRY(hipStreamSynchronize(m->ctx->stream));
+        if (m->score) SSM_HIP_TRY(hipFree(m->score));
+        m->score = nullptr;
+        m->score_bytes = 0;
+        SSM_HIP_TRY(ssm::dev_malloc((void**)&m->score, need));
+        m->score_bytes = need;
+    }
+    // the token that each position predicts: the next one; none at a sequence's last
+    const std::unique_ptr<int[]> next(new (std::nothrow) int[T]);
+    if (!next) return ssm::fail(SSM_ERR_OUT_OF_MEMORY, "ssm_score: %zu tokens", T);
+    for (size_t t = 0; t < T; ++t) next[t] = (t + 1) % L ? (int)ids[t + 1] : -1;
+    hipStream_t st = m->ctx->stream;
+    float* lp = (float*)m->score;
+    float* en = (float*)(m->score + row);
+    int* ti = (int*)(m->score + 2 * row);
+    float* tl = (float*)(m->score + 2 * row + tops);
+    auto run = [&]() -> ssm_status {
+        SSM_HIP_TRY(hipMemcpyAsync(m->d_ids, ids, T * 4, hipMemcpyHostToDevice, st));
+        SSM_HIP_TRY(hipMemcpyAsync(m->d_ids + T, next.get(), T * 4, hipMemcpyHostToDevice, st));
+        const bool own = own_head_ok(m, w, (long)T);
+        SSM_TRY(trunk(m, m->d_ids, B, L, nullptr, w, !own));
+        if (own) SSM_TRY(head_rows(m, w, w.hid, m->dm.d, (int)T, w.logits, nullptr));
+        else SSM_TRY(head_many(m, w, w.nrm, (int)T, w.logits));
+        SSM_TRY(ssm_token_logprobs(SSM_F32, w.logits, m->dm.V, (const int*)(m->d_ids + T), (int)T, m->dm.V, k, lp, en,
+                                   nullptr, k ? ti : nullptr, k ? tl : nullptr, m->score + 2 * row + 2 * tops, ws, st));
+        if (logp) SSM_HIP_TRY(hipMemcpyAsync(logp, lp, 4 * T, hipMemcpyDeviceToHost, st));
+        if (entropy) SSM_HIP_TRY(hipMemcpyAsync(entropy, en, 4 * T, hipMemcpyDeviceToHost, st));
+        if (k) {
+            SSM_HIP_TRY(hipMemcpyAsync(top_ids, ti, 4 * T * k, hipMemcpyDeviceToHost, st));
+            SSM_HIP_TRY(hipMemcpyAsync(top_logp, tl, 4 * T * k, hipMemcpyDeviceToHost, st));
+        }
+        return check_flag(m);   // (waits for the stream)
+    };
+    const ssm_status s = run();
+    if (s != SSM_OK) (void)hipStreamSynchronize(st);   // (`next` is read until then)
+    return s;
 }
 
 extern "C" ssm_status ssm_mixer_forward_device(ssm_model* m, int layer, const float* d_x,

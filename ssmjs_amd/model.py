@@ -78,6 +78,13 @@ class HybridMambaModel:
         logits = self._m.forward(a)
         return {"logits": logits.reshape(-1)}
 
+    # -- score: what one forward says of the ids, without the logits (no counterpart in the reference, whose
+    #    evaluation reads them all: session.ts:504-507)
+    def score(self, ids, batch: int, seq_len: int, top: int = 0) -> dict:
+        a = np.ascontiguousarray(ids, dtype=np.uint32).reshape(batch, seq_len)
+        logp, ent, top_ids, top_logp = self._m.score(a, top)
+        return {"logprobs": logp, "entropies": ent, "topIds": top_ids, "topLogprobs": top_logp}
+
     # -- generate: recurrent decode (prefill once, one state update per token)
     def generate(self, prompt_ids, max_new_tokens: int = 200, sampling: dict | None = None,
                  rng=None) -> list:
