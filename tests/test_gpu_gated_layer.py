@@ -1,0 +1,269 @@
+"""A small gated-recurrence model made of gated_recurrence, block_norm and token_logprobs: trained on a padded batch,
+then answering token by token, eager and captured, against the same model in 64 bits.
+
+Bounds: an operator's or a product's result is within 100 * 2^-24 of its value and of the magnitudes it adds up (the
+operators' own tests hold them to less; products here add up 64 to 97 terms). The model in 64 bits with each such
+result moved by that much, the signs drawn, tells what this does to any later value; four times the largest of eight
+draws is the bound, over a tensor's largest.
+A row's log S, S = sum e^{x - max} >= 1, takes the rounding of S over as 2^-24 in the absolute, however small log S is:
+log probabilities and entropies, which add it, are moved by NOISE of 1 + their value."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+V, D, LAYERS, B, L = 97, 64, 2, 3, 200
+NOISE = 100 * 2.0 ** -24
+EPS, C = 1e-6, 8.0
+
+
+def model(seed, size=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    f = lambda *s: torch.randn(*s, generator=gen, device="cuda")   # noqa: E731
+    p = {"emb": size * f(V, D), "pre0": 1 + 0.1 * f(D)}
+    for n in range(LAYERS):
+        p |= {f"in{n}": f(D, 4 * D) / 8, f"out{n}": f(D, D) / 8, f"lam{n}": 2 * f(D) - 3, f"post{n}": 1 + 0.1 * f(D),
+              f"scale{n}": 0.5 + 0.1 * f(D), f"pre{n + 1}": 1 + 0.1 * f(D)}
+    ids = torch.randint(0, V, (B, L), generator=gen, device="cuda")
+    lengths = torch.tensor([L, 1, 131], dtype=torch.int32, device="cuda")
+    nxt = torch.full((B, L), -1, dtype=torch.int32, device="cuda")
+    nxt[:, :-1] = ids[:, 1:].int()
+    nxt[torch.arange(L, device="cuda") >= lengths[:, None] - 1] = -1
+    return p, ids, lengths, nxt
+
+
+# ---- in 64 bits
+def plain(p, ids, lengths, nxt, jog=lambda t, m=None: t):
+    """Logits, logp, entropy and the loss; jog(result, magnitudes) moves a result."""
+    p = {k: v.double() for k, v in p.items()}
+    on = (torch.arange(L, device="cuda") < lengths[:, None])[..., None]
+
+    def mm(a, b):
+        return jog((a.reshape(-1, a.shape[-1]) @ b).view(*a.shape[:-1], -1), a.detach().abs().reshape(-1, a.shape[-1]) @ b.detach().abs())
+
+    def norm(t, w):
+        return t / (t.square().mean(-1, keepdim=True) + EPS).sqrt() * w
+
+    x = p["emb"][ids]
+    n = jog(norm(x, p["pre0"]))
+    for k in range(LAYERS):
+        v, r, i, z = mm(n, p[f"in{k}"]).split(D, -1)
+        zz = C * torch.nn.functional.softplus(p[f"lam{k}"]) * torch.sigmoid(r)
+        a, b = torch.exp(-zz), (-torch.expm1(-2 * zz)).sqrt() * torch.sigmoid(i) * v
+        h, hs = torch.zeros(B, D, dtype=torch.float64, device="cuda"), []
+        for t in range(L):
+            h = a[:, t] * h + b[:, t]
+            hs.append(h)
+        y = jog(torch.where(on, torch.stack(hs, 1), 0.0))
+        x = jog(x + p[f"scale{k}"] * norm(mm(y, p[f"out{k}"]), p[f"post{k}"]) * torch.nn.functional.silu(z))
+        n = jog(norm(x, p[f"pre{k + 1}"]))
+    lg = mm(n, p["emb"].t())
+    ls = torch.log_softmax(lg, -1)
+    ls = jog(ls, 1 + ls.detach().abs())
+    ent = -(ls.exp() * ls).sum(-1)
+    ent = jog(ent, 1 + ent.detach().abs())
+    given = nxt >= 0
+    logp = torch.where(given, ls.gather(-1, nxt.clamp(min=0).long()[..., None])[..., 0], 0.0)
+    return lg, logp, ent, -logp.sum() + 0.1 * torch.where(given, ent, 0.0).sum()
+
+
+def plain_grads(p, *batch, jog=lambda t, m=None: t):
+    leaves = {k: v.double().requires_grad_() for k, v in p.items()}
+    lg, logp, ent, loss = plain(leaves, *batch, jog=jog)
+    g = torch.autograd.grad(loss, list(leaves.values()))
+    return {"logits": lg.detach(), "logp": logp.detach(), "entropy": ent.detach()} | dict(zip(leaves, g))
+
+
+class _Jog(torch.autograd.Function):
+    """Moves a result, and what comes back to it."""
+    @staticmethod
+    def forward(ctx, t, m, gen):
+        ctx.gen = gen
+        sign = torch.randint(0, 2, t.shape, generator=gen, device="cuda") * 2 - 1
+        return t + NOISE * sign * (t.abs() if m is None else m.reshape(t.shape))
+
+    @staticmethod
+    def backward(ctx, g):
+        return g * (1 + NOISE * (torch.randint(0, 2, g.shape, generator=ctx.gen, device="cuda") * 2 - 1)), None, None
+
+
+def bounds(p, *batch):
+    ref = plain_grads(p, *batch)
+    worst = {k: 0.0 for k in ref}
+    for s in range(8):
+        gen = torch.Generator(device="cuda").manual_seed(s)
+        moved = plain_grads(p, *batch, jog=lambda t, m=None: _Jog.apply(t, m, gen))
+        worst = {k: max(w, float((moved[k] - ref[k]).abs().max())) for k, w in worst.items()}
+    return ref, {k: 4 * w for k, w in worst.items()}
+
+
+# ---- with the operators
+def run(p, ids, lengths, nxt):
+    """A training step: logits, logp, entropy and the gradients of every parameter."""
+    from ssmjs_amd import kernels as k
+    x = p["emb"][ids]
+    zero = torch.zeros_like(x)
+    kept = []
+    x1, n = k.block_norm(x, zero, pre=p["pre0"], eps=EPS)
+    for q in range(LAYERS):
+        u = (n.view(-1, D) @ p[f"in{q}"]).view(B, L, 4 * D)
+        v, r, i, z = u.split(D, -1)
+        st = k.gated_recurrence_states(B, L, D, "cuda")
+        y = k.gated_recurrence(v, r, i, p[f"lam{q}"], lengths=lengths, states=st)
+        o = (y.view(-1, D) @ p[f"out{q}"]).view(B, L, D)
+        kept.append((x1, n, u, st, y, o))
+        x1, n = k.block_norm(x1, o, z, p[f"post{q}"], p[f"scale{q}"], p[f"pre{q + 1}"], EPS)
+    lg = n.view(-1, D) @ p["emb"].t()
+    stats = torch.empty(B * L, 2, device="cuda")
+    logp, ent, _, _ = k.token_logprobs(lg, nxt.view(-1), stats=stats)
+    given = (nxt.view(-1) >= 0).float()
+    g = {}
+    dlg = k.token_logprobs_backward(lg, nxt.view(-1), stats, ent, -given, 0.1 * given)
+    g["emb"] = dlg.t() @ n.view(-1, D)
+    dn, dx1 = (dlg @ p["emb"]).view(B, L, D), None
+    for q in reversed(range(LAYERS)):
+        x0, n0, u, st, y, o = kept[q]
+        v, r, i, z = u.split(D, -1)
+        du = torch.empty_like(u)
+        dx = torch.empty_like(x0)
+        do = torch.empty_like(x0)
+        _, _, _, g[f"post{q}"], g[f"scale{q}"], g[f"pre{q + 1}"] = k.block_norm_backward(
+            dx1, dn, x0, o, z, p[f"post{q}"], p[f"scale{q}"], p[f"pre{q + 1}"], EPS, out=(dx, do, du[..., 3 * D:]))
+        dx1 = dx
+        g[f"out{q}"] = y.view(-1, D).t() @ do.view(-1, D)
+        dy = (do.view(-1, D) @ p[f"out{q}"].t()).view(B, L, D)
+        du[..., :3 * D] = 0      # (rows behind a sequence stay so)
+        *_, g[f"lam{q}"] = k.gated_recurrence_backward(dy, v, r, i, p[f"lam{q}"], st, lengths=lengths,
+                                                       out=du[..., :3 * D].split(D, -1))
+        g[f"in{q}"] = n0.view(-1, D).t() @ du.view(-1, 4 * D)
+        dn = (du.view(-1, 4 * D) @ p[f"in{q}"].t()).view(B, L, D)
+    dx, _, _, _, _, g["pre0"] = k.block_norm_backward(dx1, dn, x, zero, pre=p["pre0"], eps=EPS)
+    g["emb"] = g["emb"].index_add(0, ids.view(-1), dx.view(-1, D)) if not torch.cuda.is_current_stream_capturing() else \
+        g["emb"] + torch.nn.functional.one_hot(ids.view(-1), V).float().t() @ dx.view(-1, D)
+    return {"logits": lg.view(B, L, V), "logp": logp.view(B, L), "entropy": ent.view(B, L)} | g
+
+
+@pytest.mark.parametrize("size", [1.0, 0.1])     # rows of a likeliest token, and of many
+def test_training_step(size):
+    print(f"[case] gated model, training step {size}", flush=True)
+    p, *batch = model(1, size)
+    ref, bound = bounds(p, *batch)
+    got = run(p, *batch)
+    torch.cuda.synchronize()
+    for k, want in ref.items():
+        worst = float((got[k].double() - want).abs().max()) / bound[k]
+        print(f"  {k}: worst |err| / bound {worst:.3f}", flush=True)
+        assert worst <= 1, k
+
+
+@pytest.mark.parametrize("size", [1.0, 0.1])
+def test_prompt_then_tokens(size):
+    """A prompt leaves its states, from which tokens follow one by one, eager and as a captured call."""
+    from ssmjs_amd import kernels as k
+    print("[case] gated model, prompt then tokens", flush=True)
+    p, ids, _, nxt = model(2, size)
+    whole = torch.full((B,), L, dtype=torch.int32, device="cuda")
+    ref, bound = bounds(p, ids, whole, nxt)
+    cut = L - 8
+
+    def trunk(x, recur):
+        x1, n = k.block_norm(x, torch.zeros_like(x), pre=p["pre0"], eps=EPS)
+        for q in range(LAYERS):
+            u = (n.view(-1, D) @ p[f"in{q}"]).view(*x.shape[:-1], 4 * D)
+            v, r, i, z = u.split(D, -1)
+            o = (recur(q, v, r, i).view(-1, D) @ p[f"out{q}"]).view_as(x)
+            x1, n = k.block_norm(x1, o, z, p[f"post{q}"], p[f"scale{q}"], p[f"pre{q + 1}"], EPS)
+        return n.view(-1, D) @ p["emb"].t()
+
+    h = torch.zeros(LAYERS, B, D, device="cuda")
+    lg = trunk(p["emb"][ids[:, :cut]], lambda q, v, r, i: k.gated_recurrence(v, r, i, p[f"lam{q}"], h0=h[q], hT=h[q]))
+    torch.cuda.synchronize()
+    assert float((lg.view(B, cut, V).double() - ref["logits"][:, :cut]).abs().max()) <= bound["logits"]
+    after = h.clone()
+    token = torch.zeros(B, dtype=torch.long, device="cuda")
+
+    def answer():
+        lg = trunk(p["emb"][token], lambda q, v, r, i: k.gated_recurrence_step(v, r, i, p[f"lam{q}"], h[q]))
+        return [lg, *k.token_logprobs(lg, None, 5)[1:]]
+
+    eager = []
+    for t in range(cut, L):
+        token.copy_(ids[:, t])
+        eager.append(answer())
+        torch.cuda.synchronize()
+        lg, ent, top, toplp = eager[-1]
+        want = ref["logits"][:, t]
+        assert float((lg.double() - want).abs().max()) <= bound["logits"]
+        assert float((ent.double() - ref["entropy"][:, t]).abs().max()) <= bound["entropy"]
+        ls = torch.log_softmax(want, -1)
+        # a listed token is as likely as any that is not, but for the bound on either side
+        assert float((toplp.double() - ls.gather(1, top.long())).abs().max()) <= bound["logits"] * 2 + bound["entropy"]
+        rest = ls.scatter(1, top.long(), -1e9).amax(1)
+        assert bool((ls.gather(1, top.long()).amin(1) >= rest - 2 * bound["logits"]).all())
+    last = h.clone()
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        answer()
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        out = answer()
+    for _ in range(2):
+        h.copy_(after)
+        for n, t in enumerate(range(cut, L)):
+            token.copy_(ids[:, t])
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(out, eager[n]):
+                assert torch.equal(a, b)
+        assert torch.equal(h, last)
+
+
+def test_training_step_captured():
+    """A captured step beside live eager work gives the eager bits, replay after replay, and so do two streams."""
+    print("[case] gated model, captured training step", flush=True)
+    p, ids, lengths, nxt = model(3)
+    keep = [n for n in ("logits", "logp", "entropy", "lam0", "pre0", "post1", "scale0", "pre2")]
+    want = run(p, ids, lengths, nxt)
+    torch.cuda.synchronize()
+    side, graph = [torch.cuda.Stream(), torch.cuda.Stream()], torch.cuda.CUDAGraph()
+    got = []
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(run(p, ids, lengths, nxt))
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(g[n], want[n]) for n in keep)
+    with torch.cuda.graph(graph):
+        out = run(p, ids, lengths, nxt)
+    for _ in range(3):
+        graph.replay()
+        run(p, ids, lengths, nxt)
+        torch.cuda.synchronize()
+        assert all(torch.equal(out[n], want[n]) for n in keep)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_states_in_place(ragged):
+    """hT in h0's place and dh0 in dhT's, over one segment and several, whole and ragged."""
+    from ssmjs_amd import kernels as k
+    for b, n, d in ((3, 50, 68), (2, 5000, 64), (3, 3000, 33)):
+        print(f"[case] states in place {b} {n} {d} {ragged}", flush=True)
+        gen = torch.Generator(device="cuda").manual_seed(n)
+        f = lambda *s: torch.randn(*s, generator=gen, device="cuda")   # noqa: E731
+        x, r, i, dy, lam, h0, dhT = f(b, n, d), f(b, n, d), f(b, n, d), f(b, n, d), f(d) - 3, f(b, d), f(b, d)
+        lengths = torch.tensor([n - 1, 0, 7][:b], dtype=torch.int32, device="cuda") if ragged else None
+        st, hT, dh0 = k.gated_recurrence_states(b, n, d, "cuda"), torch.empty_like(h0), torch.empty_like(h0)
+        y = k.gated_recurrence(x, r, i, lam, lengths=lengths, h0=h0, hT=hT, states=st)
+        grads = k.gated_recurrence_backward(dy, x, r, i, lam, st, lengths=lengths, dhT=dhT, dh0=dh0)
+        h, e = h0.clone(), dhT.clone()
+        y2 = k.gated_recurrence(x, r, i, lam, lengths=lengths, h0=h, hT=h)
+        grads2 = k.gated_recurrence_backward(dy, x, r, i, lam, st, lengths=lengths, dhT=e, dh0=e)
+        torch.cuda.synchronize()
+        assert torch.equal(y, y2) and torch.equal(h, hT) and torch.equal(e, dh0)
+        assert all(torch.equal(a, c) for a, c in zip(grads, grads2))
+        if ragged:      # (a sequence of nothing hands its state on)
+            assert torch.equal(hT[1], h0[1]) and torch.equal(dh0[1], dhT[1])
