@@ -485,8 +485,8 @@ template <typename T, int VEC, int W>
 __global__ __launch_bounds__(64 * W, 2) void rec_backward(RecArgs a) {
     using P = Place<T, VEC, W>;
     constexpr int S = P::S, R = P::R, TB = P::TB;
-    constexpr int WK = kKept / (R * S);   // waves of a kept state
-    static_assert(TB % kKept == 0 && WK >= 1 && W % WK == 0, "whole kept spans");
+    constexpr int WK = std::min(W, kKept / (R * S));   // waves of a kept state (fewer: sequences of one block)
+    static_assert(WK >= 1 && W % WK == 0, "whole kept spans");
     __shared__ float aggA[2][W][kCh], aggH[2][W][kCh], aggG[2][W][kCh];
     __shared__ float2 share[W][kCh];
     const P p(a);
@@ -681,14 +681,25 @@ constexpr int kWaves = 16, kWavesBack = 8;
 // Of sequences with lengths about 0.6 are taken to be there. us, one segment / the rule / twice its segments:
 // 1 x 32768 x 1024 588 / 100 / 107, 4 x 2048 x 2048 49.4 / 49.1 / 58.5, 8 x 4096 x 2048 122 / 122 / 155; gradients
 // 1123 / 137 / 143, 87.7 / 69.5 / 75.6, 220 / 220 / 259.
+// Short sequences leave most of a block of 256 steps empty: up to 16 steps go to single waves, and up to half a block, or 512
+// where two workgroups a CU are there to share it, to four waves. fp32, us, 16 waves / fewer: 64 x 16 x 1024 42 / 9,
+// 256 x 4 x 1024 163 / 12, 64 x 64 x 1024 48 / 16, 64 x 400 x 1024 103 / 77, but 8 x 200 x 1024 12.5 / 13.8 and
+// 256 x 1000 x 1024 805 / 829; gradients, 8 waves / fewer: 63 / 15, 201 / 30, 73 / 42, 272 / 246, 28 / 35, 2081 / 2109.
 struct Plan {
     long chains;        // sequences times channel groups
     int blocks, seg;    // blocks of a sequence, and of a segment
+    int waves;          // of a workgroup
     int segments() const { return (blocks + seg - 1) / seg; }
     long groups() const { return chains * segments(); }
 };
-Plan plan_of(int B, int L, int D, int block, double again, bool ragged) {
-    Plan p{ssm::cdiv(D, kCh) * B, (int)std::max(1L, ssm::cdiv(L, block)), 0};
+Plan plan_of(int B, int L, int D, int waves, double again, bool ragged) {
+    const long chain = ssm::cdiv(D, kCh) * B;
+    if (L <= 16) return Plan{chain, 1, 1, 1};
+    if (L <= 8 * waves || (L <= 512 && chain * (ragged ? 0.6 : 1.0) >= 512)) {
+        const int n = (int)ssm::cdiv(L, 64);
+        return Plan{chain, n, n, 4};
+    }
+    Plan p{chain, (int)ssm::cdiv(L, 16 * waves), 0, waves};
     const double chains = p.chains * (ragged ? 0.6 : 1.0);
     double best = 0;
     for (int n = 1; n <= std::min(64, p.blocks); ++n) {
@@ -700,8 +711,8 @@ Plan plan_of(int B, int L, int D, int block, double again, bool ragged) {
     }
     return p;
 }
-Plan plan_forward(int B, int L, int D, bool ragged) { return plan_of(B, L, D, kWaves * 16, 0.7, ragged); }
-Plan plan_backward(int B, int L, int D, bool ragged) { return plan_of(B, L, D, kWavesBack * 16, 0.3, ragged); }
+Plan plan_forward(int B, int L, int D, bool ragged) { return plan_of(B, L, D, kWaves, 0.7, ragged); }
+Plan plan_backward(int B, int L, int D, bool ragged) { return plan_of(B, L, D, kWavesBack, 0.3, ragged); }
 
 size_t runs_bytes(const Plan& p, int B, int D) {
     return p.segments() > 1 ? ((size_t)B * (p.blocks + 1) * D * sizeof(float2) + 15) / 16 * 16 : 0;
@@ -724,12 +735,20 @@ void launch_runs(const RecArgs& a, int parts, hipStream_t st) {
 template <typename T, int VEC>
 void launch_forward(const RecArgs& a, const Plan& p, hipStream_t st) {
     if (a.runs) launch_runs<T, VEC, false>(a, (p.segments() - 1) * p.seg, st);
-    rec_kernel<T, std::min(VEC, 2), kWaves><<<(unsigned)p.groups(), 64 * kWaves, 0, st>>>(a);
+    constexpr int V = std::min(VEC, 2);
+    const unsigned n = (unsigned)p.groups();
+    if (p.waves == 1) rec_kernel<T, V, 1><<<n, 64, 0, st>>>(a);
+    else if (p.waves == 4) rec_kernel<T, V, 4><<<n, 256, 0, st>>>(a);
+    else rec_kernel<T, V, kWaves><<<n, 64 * kWaves, 0, st>>>(a);
 }
 template <typename T, int VEC>
 void launch_backward(const RecArgs& a, const Plan& p, float* dlam, hipStream_t st) {
     if (a.runs) launch_runs<T, VEC, true>(a, p.blocks - p.seg, st);
-    rec_backward<T, std::min(VEC, 2), kWavesBack><<<(unsigned)p.groups(), 64 * kWavesBack, 0, st>>>(a);
+    constexpr int V = std::min(VEC, 2);
+    const unsigned n = (unsigned)p.groups();
+    if (p.waves == 1) rec_backward<T, V, 1><<<n, 64, 0, st>>>(a);
+    else if (p.waves == 4) rec_backward<T, V, 4><<<n, 256, 0, st>>>(a);
+    else rec_backward<T, V, kWavesBack><<<n, 64 * kWavesBack, 0, st>>>(a);
     rec_dlam<<<(unsigned)ssm::cdiv(a.D, 64), 1024, 0, st>>>(a.sums, a.lam, a.B * p.segments(), a.D, dlam);
 }
 

@@ -267,3 +267,51 @@ def test_states_in_place(ragged):
         assert all(torch.equal(a, c) for a, c in zip(grads, grads2))
         if ragged:      # (a sequence of nothing hands its state on)
             assert torch.equal(hT[1], h0[1]) and torch.equal(dh0[1], dhT[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,n,d", [(3, 16, 66), (70, 13, 64), (2, 17, 130), (3, 128, 64), (2, 129, 64), (40, 150, 1024), (17, 512, 2048)])
+def test_short_prompts(b, n, d, dtype):
+    """Short prompts, few and many, whole and ragged, are what the same tokens one by one give, and their gradients
+    those of the same tokens in a longer, padded batch: the steps' order of sums differs, which is worth
+    n / 2 + 32 roundings of each of the magnitudes added (here bounded by a walk over magnitudes)."""
+    from ssmjs_amd import kernels as k
+    print(f"[case] short prompts {b} {n} {d} {dtype}", flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    f = lambda *s: torch.randn(*s, generator=gen, device="cuda")   # noqa: E731
+    x, r, i, dy = (f(b, n, d).to(dtype) for _ in range(4))
+    lam, h0, dhT = f(d) - 3, f(b, d), f(b, d)
+    half = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
+    lengths = torch.randint(0, n + 1, (b,), generator=gen, device="cuda").to(torch.int32)
+    lengths[0] = n
+    for ln in (None, lengths):
+        st, hT = k.gated_recurrence_states(b, n, d, "cuda"), torch.empty_like(h0)
+        y = k.gated_recurrence(x, r, i, lam, lengths=ln, h0=h0, hT=hT, states=st)
+        # (the gates are the same numbers either way; every state adds up |h0| and the steps' inputs, sqrt(n) of |x| <= 6)
+        scale = 6 * (n ** 0.5 + 1)
+        tol = (n / 2 + 32) * 2.0 ** -24 * scale
+        h, end = h0.clone(), h0.clone()
+        for t in range(n):
+            yt = k.gated_recurrence_step(x[:, t], r[:, t], i[:, t], lam, h)
+            on = (torch.ones(b, dtype=torch.bool, device="cuda") if ln is None else t < ln)[:, None]
+            want = torch.where(on, yt, 0).double()
+            assert bool(((y[:, t].double() - want).abs() <= tol + 2 * half * want.abs()).all()), t
+            end = torch.where(on, h, end)
+        assert float((hT - end).abs().max()) <= tol
+        # the same batch behind more padding: workgroups of another size
+        more = 1400
+        pad = lambda t: torch.cat([t, torch.full((b, more - n, d), float("nan"), device="cuda", dtype=dtype)], 1)   # noqa: E731
+        whole = torch.full((b,), n, dtype=torch.int32, device="cuda") if ln is None else ln
+        big = [pad(t) for t in (x, r, i, dy)]
+        st2, dh0, dh02 = k.gated_recurrence_states(b, more, d, "cuda"), torch.empty_like(h0), torch.empty_like(h0)
+        y2 = k.gated_recurrence(*big[:3], lam, lengths=whole, h0=h0, states=st2)
+        assert bool(((y2[:, :n].double() - y.double()).abs() <= tol + 2 * half * y.double().abs()).all()) and bool((y2[:, n:] == 0).all())
+        g = k.gated_recurrence_backward(dy, x, r, i, lam, st, lengths=ln, dhT=dhT, dh0=dh0)
+        g2 = k.gated_recurrence_backward(big[3], *big[:3], lam, st2, lengths=whole, dhT=dhT, dh0=dh02)
+        torch.cuda.synchronize()
+        # adjoints add up like states; dr multiplies one by a state (and by at most 1)
+        for a, c, m in ((g[0], g2[0], scale), (g[1], g2[1], scale * scale), (g[2], g2[2], 6 * scale), (dh0, dh02, scale)):
+            c = c[:, :n] if c.dim() == 3 else c
+            far = (a.double() - c.double()).abs()
+            assert bool((far <= 4 * (n / 2 + 32) * 2.0 ** -24 * m + 2 * half * c.double().abs()).all())
+        assert float((g[3] - g2[3]).abs().max()) <= 4 * (n / 2 + 32) * 2.0 ** -24 * scale * scale * b * n
