@@ -219,30 +219,54 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void norm_kernel(NormArg
     }
 }
 
-// W = 8 waves (16 for one row) a workgroup and one workgroup a CU, which walks its rows and keeps the column sums of
+// Keeps what follows, and what is formed from `e`, in its place: moved up over it, it would take registers.
+__device__ __forceinline__ int apart(int e) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" : "+v"(e)::"memory");
+    return e;
+}
+
+// W = 8 waves a workgroup and one workgroup a CU, which walks its rows and keeps the column sums of
 // its lanes' elements: few partial sums, and they go to memory once.
 template <typename T, int NC, int WPR, bool GATE, bool WHOLE>
-__global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArgs a) {
-    constexpr int W = WPR > 8 ? WPR : 8, RPG = W / WPR;   // rows at a time
+__global__ __launch_bounds__(512, 2) void norm_backward(NormArgs a) {
+    constexpr int W = 8, RPG = W / WPR;   // rows at a time
+    // Rows above 8192 elements have more than fits in registers: two of the column sums stay in LDS, and of a row's operands
+    // y alone is held, the others read again from the cache where they are wanted (1024 x 16384, all held by 16 waves / this:
+    // bf16 311 / 176 us, fp32 325 / 254)
+    constexpr bool kHeld = NC > 2;
     __shared__ float red[2][W];
-    __shared__ float cols[RPG][512 * NC * WPR];
+    __shared__ alignas(16) float cols[kHeld ? 2 : RPG][512 * NC * WPR];
     int turn = 0;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int e0 = (w % WPR * NC * 64 + lane) * 8;
     const float inv = 1.f / (float)a.D;
     float spost[NC][8] = {}, sscale[NC][8] = {}, spre[NC][8] = {};
+    if constexpr (kHeld)   // (its own lane's alone, up to the end)
+        for (int c = 0; c < NC; ++c)
+            for (int j = 0; j < 8; ++j) cols[0][e0 + 512 * c + j] = cols[1][e0 + 512 * c + j] = 0.f;
     const long step = (long)RPG * gridDim.x;
-    constexpr bool kAhead = NC == 1 || (!GATE && sizeof(T) == 2);   // (registers for the next row too)
+    constexpr bool kAhead = NC == 1 || (!GATE && sizeof(T) == 2 && !kHeld);   // (registers for the next row too)
     Eight<T, WHOLE> x[NC], y[NC], z[NC], dn[NC], g0[NC], nx[NC], ny[NC], nz[NC], ndn[NC], ng0[NC];
+    auto fetch_y = [&](int c, int e, long t, int left) { ny[c].load(row_of<T>(a.y, a.ldy, t) + e, left); };
+    auto fetch_x = [&](int c, int e, long t, int left) { nx[c].load(row_of<T>(a.x, a.ldx, t) + e, left); };
+    auto fetch_z = [&](int c, int e, long t, int left) {
+        if constexpr (GATE) nz[c].load(row_of<T>(a.z, a.ldz, t) + e, left);
+    };
+    auto fetch_n = [&](int c, int e, long t, int left) { ndn[c].load(row_of<T>(a.dn, a.lddn, t) + e, left); };
+    auto fetch_g = [&](int c, int e, long t, int left) {
+        ng0[c].load(a.dx1 ? row_of<T>(a.dx1, a.lddx1, t) + e : nullptr, a.dx1 ? left : 0);
+    };
     auto fetch = [&](long t) {   // the next row, on its way while this one is worked on
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int e = e0 + 512 * c, left = t < a.T ? a.D - e : 0;
-            ny[c].load(row_of<T>(a.y, a.ldy, t) + e, left);
-            nx[c].load(row_of<T>(a.x, a.ldx, t) + e, left);
-            if constexpr (GATE) nz[c].load(row_of<T>(a.z, a.ldz, t) + e, left);
-            ndn[c].load(row_of<T>(a.dn, a.lddn, t) + e, left);
-            ng0[c].load(a.dx1 ? row_of<T>(a.dx1, a.lddx1, t) + e : nullptr, a.dx1 ? left : 0);
+            fetch_y(c, e, t, left);
+            if constexpr (kHeld) continue;
+            fetch_x(c, e, t, left);
+            fetch_z(c, e, t, left);
+            fetch_n(c, e, t, left);
+            fetch_g(c, e, t, left);
         }
     };
     long t = (long)blockIdx.x * RPG + w / WPR;
@@ -252,7 +276,9 @@ __global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArg
         if constexpr (!kAhead) fetch(t);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            x[c] = nx[c], y[c] = ny[c], dn[c] = ndn[c], g0[c] = ng0[c];
+            y[c] = ny[c];
+            if constexpr (kHeld) continue;
+            x[c] = nx[c], dn[c] = ndn[c], g0[c] = ng0[c];
             if constexpr (GATE) z[c] = nz[c];
         }
         if constexpr (kAhead) fetch(t + step);
@@ -266,7 +292,12 @@ __global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArg
         float s1 = 0.f, sd = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int e = e0 + 512 * c;
+            const int e = kHeld ? apart(e0 + 512 * c) : e0 + 512 * c;
+            if constexpr (kHeld) {
+                const int left = on ? a.D - e : 0;
+                fetch_x(c, e, t, left), fetch_z(c, e, t, left), fetch_n(c, e, t, left);
+                x[c] = nx[c], z[c] = nz[c], dn[c] = ndn[c];
+            }
             float post[8], scale[8], pre[8];
             weights<WHOLE>(again(a.post), e, a.D - e, post);
             weights<WHOLE>(again(a.scale), e, a.D - e, scale);
@@ -285,11 +316,18 @@ __global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArg
         float s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int e = e0 + 512 * c;
+            const int e = kHeld ? apart(e0 + 512 * c) : e0 + 512 * c;
             float post[8], scale[8], pre[8], dz[8];
             weights<WHOLE>(again(a.post), e, a.D - e, post);
             weights<WHOLE>(again(a.scale), e, a.D - e, scale);
             weights<WHOLE>(again(a.pre), e, a.D - e, pre);
+            if constexpr (kHeld) {
+                const int left = on ? a.D - e : 0;
+                fetch_z(c, e, t, left), fetch_n(c, e, t, left), fetch_g(c, e, t, left);
+                z[c] = nz[c], dn[c] = ndn[c], g0[c] = ng0[c];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) spost[c][j] = cols[0][e + j], sscale[c][j] = cols[1][e + j];
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float nh = x1[c][j] * rx, g = fmaf(rx, dn[c][j] * pre[j] - nh * m1, g0[c][j]);
@@ -307,6 +345,10 @@ __global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArg
                 s2 = fmaf(t1 * post[j], wv, s2);
                 x1[c][j] = g;
             }
+            if constexpr (kHeld) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) cols[0][e + j] = spost[c][j], cols[1][e + j] = sscale[c][j];
+            }
             const int left = on ? a.D - e : 0;
             Eight<T, WHOLE>::store(x1[c], row_of<T>(a.x1, a.ldx1, t) + e, left);
             if constexpr (GATE) Eight<T, WHOLE>::store(dz, row_of<T>(a.dz, a.lddz, t) + e, left);
@@ -314,7 +356,11 @@ __global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArg
         const float m2 = row_sum<WPR, W>(s2, red, turn) * inv;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int e = e0 + 512 * c;
+            const int e = kHeld ? apart(e0 + 512 * c) : e0 + 512 * c;
+            if constexpr (kHeld) {
+                fetch_z(c, e, t, on ? a.D - e : 0);
+                z[c] = nz[c];
+            }
             float post[8], scale[8], dy[8];
             weights<WHOLE>(again(a.post), e, a.D - e, post);
             weights<WHOLE>(again(a.scale), e, a.D - e, scale);
@@ -332,14 +378,17 @@ __global__ __launch_bounds__(WPR > 8 ? 1024 : 512, 2) void norm_backward(NormArg
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
         float (&s)[NC][8] = k == 0 ? spost : k == 1 ? sscale : spre;
-        __syncthreads();
+        const bool there = kHeld && k < 2;
+        if (!there) {
+            __syncthreads();
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) cols[w / WPR][e0 + 512 * c + j] = s[c][j];
+                for (int j = 0; j < 8; ++j) cols[w / WPR][e0 + 512 * c + j] = s[c][j];
+        }
         __syncthreads();
         for (int e = threadIdx.x; e < a.D; e += blockDim.x) {
-            float t = cols[0][e];
+            float t = cols[kHeld ? k % 2 : 0][e];
 #pragma unroll
             for (int r = 1; r < RPG; ++r) t += cols[r][e];
             part[(long)k * a.D + e] = t;
@@ -391,7 +440,7 @@ int groups_back(int T, int D) { return (int)std::min(ssm::cdiv(T, rows_at_a_time
 
 template <typename T, int NC, int WPR>
 void go_backward(const NormArgs& a, hipStream_t st) {
-    const unsigned n = (unsigned)groups_back(a.T, a.D), threads = 64 * std::max(WPR, 8);
+    const unsigned n = (unsigned)groups_back(a.T, a.D), threads = 512;
     if (a.D % 8) a.z ? norm_backward<T, NC, WPR, true, false><<<n, threads, 0, st>>>(a) : norm_backward<T, NC, WPR, false, false><<<n, threads, 0, st>>>(a);
     else a.z ? norm_backward<T, NC, WPR, true, true><<<n, threads, 0, st>>>(a) : norm_backward<T, NC, WPR, false, true><<<n, threads, 0, st>>>(a);
 }
@@ -402,7 +451,7 @@ void backward_of(const NormArgs& a, hipStream_t st) {
     else if (a.D <= 2048) go_backward<T, 2, 2>(a, st);
     else if (a.D <= 4096) go_backward<T, 2, 4>(a, st);
     else if (a.D <= 8192) go_backward<T, 2, 8>(a, st);
-    else go_backward<T, 2, 16>(a, st);
+    else go_backward<T, 4, 8>(a, st);
 }
 
 }  // namespace
