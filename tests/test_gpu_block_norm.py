@@ -95,7 +95,7 @@ def inputs(shape, dtype, seed, strided):
 CASES = [((1, 1), False), ((3, 5), True), ((2, 3, 64), True), ((7, 512), False), ((9, 513), False), ((5, 768), True),
          ((33, 1000), False), ((1, 1024), False), ((6, 1027), True), ((4, 2048), True), ((5, 2049), False),
          ((3, 4096), False), ((3, 4100), True), ((2, 8193), False), ((2, 16384), False), ((2500, 66), False),
-         ((1300, 1100), False)]
+         ((1300, 1100), False), ((300, 8200), True), ((520, 16384), False)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
