@@ -13,7 +13,12 @@
 // Where the sequences' channels are too few to fill the chip, sequences are cut into segments of whole blocks: a
 // first pass forms the (A, H) of every block that others follow, and each segment starts from the composition of
 // those before it. (One pass, with workgroups that wait for the results of those before them, read the inputs once
-// and took as long: the waiting ones' looks at memory cost what the second reading costs.)
+// and took as long, the waiting ones' looks at memory costing what the second reading costs. us, two passes / one:
+// 1 x 32768 x 1024 bf16 100 / 122, 8 x 4096 x 2048 130 / 155, 5 x 1500 x 1536 fp32 ragged 37 / 40.)
+//
+// Memory bound: 8 x 4096 x 2048 bf16 takes 130 us, 4.1 TB/s; rows' pieces of 128 bytes read and written with nothing
+// else done take 118, whole rows 106. The gradients of 4 x 2048 x 2048 bf16 take 68 us (51 without the first pass: 4.6
+// TB/s). Small calls are launches: 64 tokens of 4096 channels 4.2 us.
 //
 // 1 - a^2 from a rounded a would lose its digits where a is near 1 (0.999 and more in use): with
 // q = 1 - e^{-z} by its series below z = 0.2, a = 1 - q and 1 - a^2 = q (1 + a).
@@ -269,7 +274,8 @@ __device__ __forceinline__ void runs(int lane, int row, const float (&d)[S][VEC]
 // the runs are composed at the end. BACK: of the adjoint, e_{t-1} = a_t (dy_t + e_t), walked from the end.
 constexpr int kRunWaves = 8;
 
-// Rows of CH = 128 channels, four a lane, where alignment allows: CHFIG
+// Rows of CH = 128 channels, four a lane, where alignment allows: 1 x 32768 x 1024 bf16 42 us, against 53 with
+// rows of 64, one or two a lane, which other rows take.
 template <typename T, int VEC, int CH, int TB, bool BACK>
 __global__ __launch_bounds__(64 * kRunWaves) void rec_runs(RecArgs a) {
     using P = Place<T, VEC, kRunWaves, CH>;
