@@ -315,3 +315,84 @@ def test_short_prompts(b, n, d, dtype):
             far = (a.double() - c.double()).abs()
             assert bool((far <= 4 * (n / 2 + 32) * 2.0 ** -24 * m + 2 * half * c.double().abs()).all())
         assert float((g[3] - g2[3]).abs().max()) <= 4 * (n / 2 + 32) * 2.0 ** -24 * scale * scale * b * n
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_nothing_to_do(dtype):
+    """Batches of no sequences and of no tokens: states go through, gradients of nothing are zeros."""
+    from ssmjs_amd import kernels as k
+    print(f"[case] nothing to do {dtype}", flush=True)
+    e = lambda *s: torch.empty(*s, device="cuda", dtype=dtype)   # noqa: E731
+    lam, w = torch.randn(70, device="cuda"), torch.ones(70, device="cuda")
+    for b, n in ((0, 9), (3, 0), (0, 0)):
+        x = e(b, n, 70)
+        h0 = torch.randn(b, 70, device="cuda")
+        hT, dh0 = torch.full_like(h0, 7.0), torch.full_like(h0, 7.0)
+        st = k.gated_recurrence_states(b, n, 70, "cuda")
+        for ln in (None, torch.zeros(b, dtype=torch.int32, device="cuda")):
+            y = k.gated_recurrence(x, x, x, lam, lengths=ln, h0=h0, hT=hT, states=st)
+            torch.cuda.synchronize()
+            assert y.shape == x.shape and torch.equal(hT, h0)
+            if b:
+                g = k.gated_recurrence_backward(x, x, x, x, lam, st, lengths=ln, dhT=h0, dh0=dh0)
+                torch.cuda.synchronize()
+                assert torch.equal(dh0, h0) and bool((g[3] == 0).all())
+    h = torch.empty(0, 70, device="cuda")
+    assert k.gated_recurrence_step(e(0, 70), e(0, 70), e(0, 70), lam, h).shape == (0, 70)
+    x1, n1 = k.block_norm(e(0, 70), e(0, 70), e(0, 70), w, w, w)
+    assert x1.shape == n1.shape == (0, 70)
+    g = k.block_norm_backward(x1, n1, e(0, 70), e(0, 70), e(0, 70), w, w, w)
+    torch.cuda.synchronize()
+    assert all(bool((t == 0).all()) and t.shape == (70,) for t in g[3:])
+    ids, stats = torch.empty(0, dtype=torch.int32, device="cuda"), torch.empty(0, 2, device="cuda")
+    lp, ent, top, _ = k.token_logprobs(e(0, 70), ids, 3, stats)
+    assert lp.shape == ent.shape == (0,) and top.shape == (0, 3)
+    assert k.token_logprobs_backward(e(0, 70), ids, stats, ent, lp, ent).shape == (0, 70)
+
+
+def test_far_apart():
+    """Rows whose offsets pass 2^31 elements give the bits of rows side by side."""
+    from ssmjs_amd import kernels as k
+    print("[case] far apart", flush=True)
+    room = torch.empty((1 << 33) + (1 << 21), dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    f = lambda *s: torch.randn(*s, generator=gen, device="cuda").bfloat16()   # noqa: E731
+    b, n, d, ld = 5, 3000, 130, (1 << 19) + 1000          # 5 * 3000 rows of 2^19: 2^32.9 elements
+    x, r, i, dy = f(b, n, d), f(b, n, d), f(b, n, d), f(b, n, d)
+    lam = torch.randn(d, generator=gen, device="cuda") - 3
+    far = [room.as_strided((b, n, d), (n * ld, ld, 1), 1000 * j) for j in range(8)]
+    for t, v in zip(far, (x, r, i, dy)):
+        t.copy_(v)
+    st, st2 = k.gated_recurrence_states(b, n, d, "cuda"), k.gated_recurrence_states(b, n, d, "cuda")
+    y = k.gated_recurrence(x, r, i, lam, states=st)
+    k.gated_recurrence(*far[:3], lam, states=st2, out=far[4])
+    g = k.gated_recurrence_backward(dy, x, r, i, lam, st)
+    g2 = k.gated_recurrence_backward(far[3], *far[:3], lam, st2, out=far[5:8])
+    torch.cuda.synchronize()
+    assert torch.equal(y, far[4]) and torch.equal(st, st2) and all(torch.equal(a, c) for a, c in zip(g, g2))
+    # norms of the same rows, with x as z, r as x, i as y
+    w = [torch.randn(d, generator=gen, device="cuda") for _ in range(3)]
+    want = k.block_norm(r, i, x, *w)
+    back = k.block_norm_backward(dy, y, r, i, x, *w)
+    flat = lambda t: t.as_strided((b * n, d), (ld, 1), t.storage_offset())   # noqa: E731
+    fx, fr, fi, fd, fy = (flat(t) for t in far[:5])
+    got = k.block_norm(fr, fi, fx, *w, out=(flat(far[5]), flat(far[6])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a.view(-1, d), c) for a, c in zip(want, got))
+    got = k.block_norm_backward(fd, fy, fr, fi, fx, *w, out=[flat(t) for t in far[5:8]])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a.view(c.shape), c) for a, c in zip(back, got))
+    # logits: nine rows 2^30 - 8 apart, and in place of them their gradient
+    m, v = 9, 1001
+    lg = f(m, v)
+    wide = room.as_strided((m, v), ((1 << 30) - 8, 1), 5)
+    wide.copy_(lg)
+    ids = torch.arange(m, device="cuda").int() * 100
+    stats, stats2 = torch.empty(m, 2, device="cuda"), torch.empty(m, 2, device="cuda")
+    want, got = k.token_logprobs(lg, ids, 7, stats), k.token_logprobs(wide, ids, 7, stats2)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(want, got))
+    a = k.token_logprobs_backward(lg, ids, stats, want[1], want[0], want[1])
+    k.token_logprobs_backward(wide, ids, stats2, want[1], want[0], want[1], out=wide)
+    torch.cuda.synchronize()
+    assert torch.equal(a, wide)
