@@ -5,7 +5,7 @@
 //
 // The recurrence is associative: a run of steps maps its entering state h to A h + H with A the product
 // of its decays and H its result from a zero state. A workgroup of W waves walks 64 channels of one sequence in
-// blocks of TB = 16 W steps: a lane holds 16 (step, channel) elements of consecutive steps, forms their a and
+// blocks of TB = 16 W steps (32 channels in blocks of 32 W where that fills more of the chip): a lane holds 16 (step, channel) elements of consecutive steps, forms their a and
 // b once, in registers, and its run's (A, H); runs are composed over the lanes of a wave (lane exchanges) and over the
 // waves (LDS, one barrier a block), and each lane then walks its steps from its true entering state, as
 // the formula says. The next block's inputs are on their way meanwhile.
@@ -23,6 +23,7 @@
 // 1 - a^2 from a rounded a would lose its digits where a is near 1 (0.999 and more in use): with
 // q = 1 - e^{-z} by its series below z = 0.2, a = 1 - q and 1 - a^2 = q (1 + a).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -121,6 +122,15 @@ __device__ __forceinline__ void decay(float z, bool near, float& a, float& q) {
     }
 }
 
+// f(std::true_type) where `near`, else f(std::false_type). As selects, the choice takes a sixth of a block's instructions,
+// and in the gradients' kernel registers that spill (us, selects / this: 4 x 2048 x 2048 fp32 gradients 165 / 116, bf16
+// 72 / 68; 5 x 1500 x 1536 fp32 forward, narrow groups, 29.7 / 27.4).
+template <typename F>
+__device__ __forceinline__ void by_gates(bool near, F f) {
+    if (near) f(std::true_type());
+    else f(std::false_type());
+}
+
 // A run's result from entering state h. An infinite state stays infinite: its decay is positive, however
 // far below fp32's range.
 __device__ __forceinline__ float onto(float A, float H, float h) {
@@ -168,8 +178,11 @@ struct Place {
         row = lane / LC;
         mine = (w * R + row) * S;
         const int groups = (a.D + CH - 1) / CH;
-        cg = blockIdx.x % groups;
-        const int rest = blockIdx.x / groups;
+        int j = blockIdx.x;
+        // (two groups of 32 channels share memory's lines of 128 bytes: on one XCD, of 8 that take workgroups in turn)
+        if (CH < kCh && (j | 15) < (int)gridDim.x) j = (j & ~15) | (j & 7) << 1 | (j >> 3 & 1);
+        cg = j % groups;
+        const int rest = j / groups;
         b = rest % a.B;
         part = rest / a.B;
         ch = cg * CH + col * VEC;
@@ -230,13 +243,13 @@ __device__ __forceinline__ bool any_nan(const float (&h)[N]) {
     return __any(no);
 }
 
-// A lane's runs, and their composition over the (one or two) rows of a wave: (A, H) becomes the run of all rows up to
+// A lane's runs, and their composition over the R rows of a wave: (A, H) becomes the run of all rows up to
 // this one, (Ae, He) that of the rows before it. BACK: from this one on, and after it; H the adjoint's.
 // SAFE: infinities go through `onto`.
-template <int VEC, int S, bool BACK, bool SAFE>
+template <int VEC, int S, int R, bool BACK, bool SAFE>
 __device__ __forceinline__ void runs(int lane, int row, const float (&d)[S][VEC], const float (&b)[S][VEC], float (&A)[VEC],
                                      float (&H)[VEC], float (&Ae)[VEC], float (&He)[VEC]) {
-    static_assert(VEC <= 2, "at most two rows");
+    static_assert(R <= 2 || (R == 4 && !BACK), "rows of a wave");
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
         if (BACK) {   // e <- d (dy + e)
@@ -258,13 +271,26 @@ __device__ __forceinline__ void runs(int lane, int row, const float (&d)[S][VEC]
         }
         Ae[v] = 1.f;
         He[v] = 0.f;
-        if constexpr (VEC == 2) {
+        if constexpr (R == 2) {
             const float A1 = of_lane(A[v], lane + 32), H1 = of_lane(H[v], lane + 32);   // the other row's
             const bool after = row == (BACK ? 0 : 1);
             Ae[v] = after ? A1 : 1.f;
             He[v] = after ? H1 : 0.f;
             H[v] = SAFE ? onto(A[v], H[v], He[v]) : fmaf(A[v], He[v], H[v]);
             A[v] *= Ae[v];
+        }
+        if constexpr (R == 4) {
+#pragma unroll
+            for (int k = 1; k < 4; k *= 2) {   // those of the k rows before
+                const float A1 = of_lane(A[v], lane - 16 * k), H1 = of_lane(H[v], lane - 16 * k);
+                if (row >= k) {
+                    H[v] = SAFE ? onto(A[v], H[v], H1) : fmaf(A[v], H1, H[v]);
+                    A[v] *= A1;
+                }
+            }
+            const float A1 = of_lane(A[v], lane - 16), H1 = of_lane(H[v], lane - 16);
+            Ae[v] = row ? A1 : 1.f;
+            He[v] = row ? H1 : 0.f;
         }
     }
 }
@@ -357,8 +383,8 @@ __global__ __launch_bounds__(64 * kRunWaves) void rec_runs(RecArgs a) {
 
 // By all waves of a workgroup: the state that enters (BACK: leaves) a segment, of channel `lane`. Each wave composes a
 // share of the blocks before it (after it); the shares are chained in order.
-template <int W, bool BACK>
-__device__ float enter_segment(const RecArgs& a, float2 (&share)[W][kCh], int b, int ch, bool has, int from, int to, int w,
+template <int W, int CH, bool BACK>
+__device__ float enter_segment(const RecArgs& a, float2 (&share)[W][CH], int b, int ch, bool has, int from, int to, int w,
                                int lane) {
     const float2* runs = a.runs + (long)b * (a.blocks + 1) * a.D + ch;
     const float h0 = !has ? 0.f : a.runs ? runs[(long)a.blocks * a.D].x : a.h0 ? a.h0[(long)b * a.D + ch] : 0.f;
@@ -380,17 +406,17 @@ __device__ float enter_segment(const RecArgs& a, float2 (&share)[W][kCh], int b,
 }
 
 // ---------------------------------------------------------------- prompts
-template <typename T, int VEC, int W>
+template <typename T, int VEC, int W, int CH = kCh>
 __global__ __launch_bounds__(64 * W, 4) void rec_kernel(RecArgs a) {
-    using P = Place<T, VEC, W>;
+    using P = Place<T, VEC, W, CH>;
     constexpr int S = P::S, R = P::R, TB = P::TB;
-    __shared__ float aggA[2][W][kCh], aggH[2][W][kCh];
-    __shared__ float2 share[W][kCh];
+    __shared__ float aggA[2][W][CH], aggH[2][W][CH];
+    __shared__ float2 share[W][CH];
     const P p(a);
     if (a.pad) p.clear(a.y, a.ldy, a);
     const int last = p.n > 0 ? (p.n - 1) / TB / a.seg : 0;   // the segment of the last token
     if (p.part > last) return;
-    const int chl = p.cg * kCh + p.lane;   // the channel of what a wave holds by lanes
+    const int cl = p.lane % CH, chl = p.cg * CH + cl;   // the channel of what a wave holds by lanes
     const bool has = chl < a.D;
     const int s0 = p.part * a.seg * TB, s1 = min((long)p.n, (long)s0 + (long)a.seg * TB);
     Raw<T, VEC> qx[S], qr[S], qi[S];
@@ -403,24 +429,26 @@ __global__ __launch_bounds__(64 * W, 4) void rec_kernel(RecArgs a) {
     fetch(s0);
     float kd[VEC];
     const bool near = p.decays(a, kd);
-    float st = enter_segment<W, false>(a, share, p.b, chl, has, 0, p.part * a.seg, p.w, p.lane);
+    float st = enter_segment<W, CH, false>(a, share, p.b, chl, has, 0, p.part * a.seg, p.w, cl);
     int buf = 0;
     for (int t0 = s0; t0 < s1; t0 += TB, buf ^= 1) {
         float d[S][VEC], bt[S][VEC];
+        by_gates(near, [&](auto close) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            float x[VEC], r[VEC], i[VEC];
-            qx[s].get(x);
-            qr[s].get(r);
-            qi[s].get(i);
+            for (int s = 0; s < S; ++s) {
+                float x[VEC], r[VEC], i[VEC];
+                qx[s].get(x);
+                qr[s].get(r);
+                qi[s].get(i);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                float q;
-                decay(kd[v] * open(fall(r[v])), near, d[s][v], q);
-                bt[s][v] = __builtin_amdgcn_sqrtf(fmaf(q, d[s][v], q)) * (open(fall(i[v])) * x[v]);
+                for (int v = 0; v < VEC; ++v) {
+                    float u;
+                    decay(kd[v] * open(fall(r[v])), close(), d[s][v], u);
+                    bt[s][v] = __builtin_amdgcn_sqrtf(fmaf(u, d[s][v], u)) * (open(fall(i[v])) * x[v]);
+                }
+                if ((s + 1) * VEC % 4 == 0) __builtin_amdgcn_sched_barrier(0);   // (four elements at a time)
             }
-            if ((s + 1) * VEC % 4 == 0) __builtin_amdgcn_sched_barrier(0);   // (four elements at a time)
-        }
+        });
         if (t0 + TB > s1) {   // past the end the state stays
 #pragma unroll
             for (int s = 0; s < S; ++s)
@@ -430,8 +458,8 @@ __global__ __launch_bounds__(64 * W, 4) void rec_kernel(RecArgs a) {
         }
         fetch(min(t0 + TB, s1));
         float A[VEC], H[VEC], Ae[VEC], He[VEC];
-        runs<VEC, S, false, false>(p.lane, p.row, d, bt, A, H, Ae, He);
-        if (any_nan(H)) runs<VEC, S, false, true>(p.lane, p.row, d, bt, A, H, Ae, He);
+        runs<VEC, S, R, false, false>(p.lane, p.row, d, bt, A, H, Ae, He);
+        if (any_nan(H)) runs<VEC, S, R, false, true>(p.lane, p.row, d, bt, A, H, Ae, He);
         if (p.row == R - 1) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
@@ -444,20 +472,20 @@ __global__ __launch_bounds__(64 * W, 4) void rec_kernel(RecArgs a) {
 #pragma unroll 4
         for (int w = 0; w < W; ++w) {
             if (w == p.w) enter = next;
-            next = fmaf(aggA[buf][w][p.lane], next, aggH[buf][w][p.lane]);
+            next = fmaf(aggA[buf][w][cl], next, aggH[buf][w][cl]);
         }
         if (__any(next != next)) {
             next = st;
             for (int w = 0; w < W; ++w) {
                 if (w == p.w) enter = next;
-                next = onto(aggA[buf][w][p.lane], aggH[buf][w][p.lane], next);
+                next = onto(aggA[buf][w][cl], aggH[buf][w][cl], next);
             }
         }
         st = next;
         float h[VEC], g[VEC], y[S][VEC];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            h[v] = g[v] = onto(Ae[v], He[v], VEC == 1 ? enter : of_lane(enter, p.col * VEC + v));
+            h[v] = g[v] = onto(Ae[v], He[v], CH == 64 && VEC == 1 ? enter : of_lane(enter, p.col * VEC + v));
 #pragma unroll
             for (int s = 0; s < S; ++s) y[s][v] = g[v] = fmaf(d[s][v], g[v], bt[s][v]);
         }
@@ -525,35 +553,37 @@ __global__ __launch_bounds__(64 * W, 2) void rec_backward(RecArgs a) {
         const int t1 = s1 > s0 ? s0 + (s1 - s0 - 1) / TB * TB : s0 - TB;
         if (t1 >= s0) fetch(t1);
         // the adjoint that leaves a block's first step, of channel `lane`
-        float e = enter_segment<W, true>(a, share, p.b, chl, has, (p.part + 1) * a.seg, p.n > 0 ? (p.n - 1) / TB + 1 : 0, p.w,
-                                         p.lane);
+        float e = enter_segment<W, kCh, true>(a, share, p.b, chl, has, (p.part + 1) * a.seg, p.n > 0 ? (p.n - 1) / TB + 1 : 0, p.w,
+                                              p.lane);
         int buf = 0;
         for (int t0 = t1; t0 >= s0; t0 -= TB, buf ^= 1) {
             float d[S][VEC], bt[S][VEC], bi[S][VEC], bj[S][VEC], k1[S][VEC], k2[S][VEC], cr[S][VEC], gy[S][VEC];
+            by_gates(near, [&](auto close) __attribute__((always_inline)) {
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-                float x[VEC], r[VEC], i[VEC];
-                qx[s].get(x);
-                qr[s].get(r);
-                qi[s].get(i);
-                qg[s].get(gy[s]);
+                for (int s = 0; s < S; ++s) {
+                    float x[VEC], r[VEC], i[VEC];
+                    qx[s].get(x);
+                    qr[s].get(r);
+                    qi[s].get(i);
+                    qg[s].get(gy[s]);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const float er = fall_held(r[v]), ei = fall_held(i[v]);
-                    const float gr = open(er), gi = open(ei), z = kd[v] * gr;
-                    float q;
-                    decay(z, near, d[s][v], q);
-                    const float b2 = fmaf(q, d[s][v], q), inv = __builtin_amdgcn_rsqf(fmaxf(b2, kTiny)), be = b2 * inv;
-                    const float u = gi * x[v];
-                    bi[s][v] = be * gi;
-                    bt[s][v] = be * u;
-                    bj[s][v] = bt[s][v] * (ei * gi);
-                    k2[s][v] = d[s][v] * z;
-                    k1[s][v] = u * d[s][v] * d[s][v] * (z * inv);
-                    cr[s][v] = er * gr;
+                    for (int v = 0; v < VEC; ++v) {
+                        const float er = fall_held(r[v]), ei = fall_held(i[v]);
+                        const float gr = open(er), gi = open(ei), z = kd[v] * gr;
+                        float q;
+                        decay(z, close(), d[s][v], q);
+                        const float b2 = fmaf(q, d[s][v], q), inv = __builtin_amdgcn_rsqf(fmaxf(b2, kTiny)), be = b2 * inv;
+                        const float u = gi * x[v];
+                        bi[s][v] = be * gi;
+                        bt[s][v] = be * u;
+                        bj[s][v] = bt[s][v] * (ei * gi);
+                        k2[s][v] = d[s][v] * z;
+                        k1[s][v] = u * d[s][v] * d[s][v] * (z * inv);
+                        cr[s][v] = er * gr;
+                    }
+                    if ((s + 1) * VEC % 4 == 0) __builtin_amdgcn_sched_barrier(0);   // (four elements at a time)
                 }
-                if ((s + 1) * VEC % 4 == 0) __builtin_amdgcn_sched_barrier(0);   // (four elements at a time)
-            }
+            });
             if (t0 + TB > s1) {
 #pragma unroll
                 for (int s = 0; s < S; ++s)
@@ -564,8 +594,8 @@ __global__ __launch_bounds__(64 * W, 2) void rec_backward(RecArgs a) {
             float hl = ks;
             fetch(t0 - TB);
             float A[VEC], H[VEC], Ae[VEC], He[VEC], Ab[VEC], G[VEC], Ax[VEC], Gx[VEC];
-            runs<VEC, S, false, false>(p.lane, p.row, d, bt, A, H, Ae, He);
-            runs<VEC, S, true, false>(p.lane, p.row, d, gy, Ab, G, Ax, Gx);
+            runs<VEC, S, R, false, false>(p.lane, p.row, d, bt, A, H, Ae, He);
+            runs<VEC, S, R, true, false>(p.lane, p.row, d, gy, Ab, G, Ax, Gx);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 if (p.row == R - 1) {
@@ -678,6 +708,7 @@ __global__ __launch_bounds__(256) void rec_step(RecArgs a) {
 
 // ---------------------------------------------------------------- plans
 constexpr int kWaves = 16, kWavesBack = 8;
+constexpr int kNarrow = 32, kWavesNarrow = 8;   // channels and waves of narrow groups
 
 // Blocks and segments of the sequences: as many segments as make the kernels' time least, counted in the time of a
 // block on a full chip (one workgroup a CU; us, W = 16 and 8 waves: 7.6, 6.9):
@@ -695,17 +726,18 @@ struct Plan {
     long chains;        // sequences times channel groups
     int blocks, seg;    // blocks of a sequence, and of a segment
     int waves;          // of a workgroup
+    int ch;             // channels of a group
     int segments() const { return (blocks + seg - 1) / seg; }
     long groups() const { return chains * segments(); }
 };
-Plan plan_of(int B, int L, int D, int waves, double again, bool ragged) {
+Plan plan_of(int B, int L, int D, int waves, double again, bool ragged, double* cost = nullptr) {
     const long chain = ssm::cdiv(D, kCh) * B;
-    if (L <= 16) return Plan{chain, 1, 1, 1};
+    if (L <= 16) return Plan{chain, 1, 1, 1, kCh};
     if (L <= 8 * waves || (L <= 512 && chain * (ragged ? 0.6 : 1.0) >= 512)) {
         const int n = (int)ssm::cdiv(L, 64);
-        return Plan{chain, n, n, 4};
+        return Plan{chain, n, n, 4, kCh};
     }
-    Plan p{chain, (int)ssm::cdiv(L, 16 * waves), 0, waves};
+    Plan p{chain, (int)ssm::cdiv(L, 16 * waves), 0, waves, kCh};
     const double chains = p.chains * (ragged ? 0.6 : 1.0);
     double best = 0;
     for (int n = 1; n <= std::min(64, p.blocks); ++n) {
@@ -715,9 +747,21 @@ Plan plan_of(int B, int L, int D, int waves, double again, bool ragged) {
         if (segs > 1) t += 0.5 + again * std::max(1.0, chains * (p.blocks - per) / 256);
         if (n == 1 || t < best) best = t, p.seg = per;
     }
+    if (cost) *cost = best;
     return p;
 }
-Plan plan_forward(int B, int L, int D, bool ragged) { return plan_of(B, L, D, kWaves, 0.7, ragged); }
+// Groups of 32 channels put twice the workgroups on sequences that are walked whole, where those are few enough for one a CU:
+// a block then takes 0.4 (up to 80 workgroups) to 0.73 (256) of a full chip's. us, wide groups by the rule above / narrow:
+// 4 x 2048 x 2048 bf16 50 / 45, fp32 81 / 61, 5 x 1500 x 1536 fp32 with lengths 39 / 27, 2 x 600 x 2048 bf16 24 / 14, but
+// 2 x 4096 x 2048 bf16 56 / 71 and 1 x 8192 x 512 fp32 33 / 99. With lengths the segments' share is the less even one.
+Plan plan_forward(int B, int L, int D, bool ragged) {
+    double best = 0;
+    const Plan p = plan_of(B, L, D, kWaves, 0.7, ragged, &best);
+    const long n = ssm::cdiv(D, kNarrow) * B;
+    if (p.waves != kWaves || n > 256) return p;
+    const double there = n * (ragged ? 0.6 : 1.0), t = p.blocks * (0.4 + 0.33 * std::max(0.0, there - 80) / 176);
+    return t < best * (ragged ? 1.25 : 1.0) ? Plan{n, p.blocks, p.blocks, kWavesNarrow, kNarrow} : p;
+}
 Plan plan_backward(int B, int L, int D, bool ragged) { return plan_of(B, L, D, kWavesBack, 0.3, ragged); }
 
 size_t runs_bytes(const Plan& p, int B, int D) {
@@ -745,6 +789,7 @@ void launch_forward(const RecArgs& a, const Plan& p, hipStream_t st) {
     const unsigned n = (unsigned)p.groups();
     if (p.waves == 1) rec_kernel<T, V, 1><<<n, 64, 0, st>>>(a);
     else if (p.waves == 4) rec_kernel<T, V, 4><<<n, 256, 0, st>>>(a);
+    else if (p.ch == kNarrow) rec_kernel<T, V, kWavesNarrow, kNarrow><<<n, 64 * kWavesNarrow, 0, st>>>(a);
     else rec_kernel<T, V, kWaves><<<n, 64 * kWaves, 0, st>>>(a);
 }
 template <typename T, int VEC>

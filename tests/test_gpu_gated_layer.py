@@ -11,6 +11,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+import test_gpu_gated_recurrence as recurrence  # noqa: E402
+
 pytestmark = pytest.mark.gpu
 
 V, D, LAYERS, B, L = 97, 64, 2, 3, 200
@@ -396,3 +398,21 @@ def test_far_apart():
     k.token_logprobs_backward(wide, ids, stats2, want[1], want[0], want[1], out=wide)
     torch.cuda.synchronize()
     assert torch.equal(a, wide)
+
+
+@pytest.mark.parametrize("L", [9, 200, 700])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_infinities_at_other_lengths(bad, L):
+    """Infinities and NaN in workgroups of one wave and in those of 32 channels."""
+    print(f"[case] infinities {L} {bad}", flush=True)
+    recurrence.test_an_infinity_stays_where_it_is(bad, L)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [
+    (1, 129, 1, False, True, False, False), (3, 700, 33, True, True, True, False), (2, 256, 34, False, False, True, True),
+    (2, 513, 66, True, True, False, True), (5, 1025, 100, True, True, True, False), (4, 900, 2048, False, True, False, False),
+    (1, 1024, 68, False, True, False, True), (1, 10, 66, False, True, True, True), (2, 60, 33, True, True, False, True)])
+def test_other_groups(case, dtype):
+    """The recurrence and its gradients, to the bounds of its own tests, where groups of 32 channels and few waves run."""
+    recurrence.test_forward_backward(case, dtype)
