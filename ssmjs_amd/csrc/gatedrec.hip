@@ -718,10 +718,10 @@ constexpr int kNarrow = 32, kWavesNarrow = 8;   // channels and waves of narrow 
 // Of sequences with lengths about 0.6 are taken to be there. us, one segment / the rule / twice its segments:
 // 1 x 32768 x 1024 588 / 100 / 107, 4 x 2048 x 2048 49.4 / 49.1 / 58.5, 8 x 4096 x 2048 122 / 122 / 155; gradients
 // 1123 / 137 / 143, 87.7 / 69.5 / 75.6, 220 / 220 / 259.
-// Short sequences leave most of a block of 256 steps empty: up to 16 steps go to single waves, and up to half a block, or 512
-// where two workgroups a CU are there to share it, to four waves. fp32, us, 16 waves / fewer: 64 x 16 x 1024 42 / 9,
-// 256 x 4 x 1024 163 / 12, 64 x 64 x 1024 48 / 16, 64 x 400 x 1024 103 / 77, but 8 x 200 x 1024 12.5 / 13.8 and
-// 256 x 1000 x 1024 805 / 829; gradients, 8 waves / fewer: 63 / 15, 201 / 30, 73 / 42, 272 / 246, 28 / 35, 2081 / 2109.
+// Short sequences leave most of a block of 256 steps empty: up to 16 steps go to single waves, and up to half a block, or four
+// blocks where two workgroups a CU are there to share it, to four waves. fp32, us, 16 waves / fewer: 64 x 16 x 1024 46 / 9,
+// 256 x 4 x 1024 168 / 12, 64 x 64 x 1024 47 / 16, 64 x 400 x 1024 103 / 78, 32 x 1000 x 1024 113 / 106, but 8 x 200 x 1024
+// 12.5 / 13.8 and 64 x 2000 x 1024 416 / 421; gradients, 8 waves / fewer: 41 / 15, 143 / 21, 45 / 27, 161 / 154, 182 / 189.
 struct Plan {
     long chains;        // sequences times channel groups
     int blocks, seg;    // blocks of a sequence, and of a segment
@@ -733,7 +733,7 @@ struct Plan {
 Plan plan_of(int B, int L, int D, int waves, double again, bool ragged, double* cost = nullptr) {
     const long chain = ssm::cdiv(D, kCh) * B;
     if (L <= 16) return Plan{chain, 1, 1, 1, kCh};
-    if (L <= 8 * waves || (L <= 512 && chain * (ragged ? 0.6 : 1.0) >= 512)) {
+    if (L <= 8 * waves || (L <= 64 * waves && chain * (ragged ? 0.6 : 1.0) >= 512)) {
         const int n = (int)ssm::cdiv(L, 64);
         return Plan{chain, n, n, 4, kCh};
     }
