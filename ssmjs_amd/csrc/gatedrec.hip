@@ -5,20 +5,21 @@
 //
 // The recurrence is associative: a run of steps maps its entering state h to A h + H with A the product
 // of its decays and H its result from a zero state. A workgroup of W waves walks 64 channels of one sequence in
-// blocks of TB = 16 W steps (32 channels in blocks of 32 W where that fills more of the chip): a lane holds 16 (step, channel) elements of consecutive steps, forms their a and
-// b once, in registers, and its run's (A, H); runs are composed over the lanes of a wave (lane exchanges) and over the
-// waves (LDS, one barrier a block), and each lane then walks its steps from its true entering state, as
-// the formula says. The next block's inputs are on their way meanwhile.
+// blocks of TB = 16 W steps (32 channels in blocks of 32 W where that fills more of the chip): a lane holds 16 (step,
+// channel) elements of consecutive steps, forms their a and b once, in registers, and its run's (A, H); runs are composed
+// over the lanes of a wave (lane exchanges) and over the waves (LDS, one barrier a block), and each lane then walks its
+// steps from its true entering state, as the formula says. The next block's inputs are on their way meanwhile.
 //
 // Where the sequences' channels are too few to fill the chip, sequences are cut into segments of whole blocks: a
 // first pass forms the (A, H) of every block that others follow, and each segment starts from the composition of
 // those before it. (One pass, with workgroups that wait for the results of those before them, read the inputs once
 // and took as long, the waiting ones' looks at memory costing what the second reading costs. us, two passes / one:
-// 1 x 32768 x 1024 bf16 100 / 122, 8 x 4096 x 2048 130 / 155, 5 x 1500 x 1536 fp32 ragged 37 / 40.)
+// 1 x 32768 x 1024 bf16 100 / 122, 8 x 4096 x 2048 130 / 155, 4 x 2048 x 2048 49 / 52.)
 //
-// Memory bound: 8 x 4096 x 2048 bf16 takes 130 us, 4.1 TB/s; rows' pieces of 128 bytes read and written with nothing
-// else done take 118, whole rows 106. The gradients of 4 x 2048 x 2048 bf16 take 68 us (51 without the first pass: 4.6
-// TB/s). Small calls are launches: 64 tokens of 4096 channels 4.2 us.
+// Bound by memory where the chip is full, 8 x 4096 x 2048 bf16 131 us, 4.1 TB/s (rows' pieces of 128 bytes read and written
+// with nothing else done take 118, whole rows 106), 256 x 1000 x 1024 fp32 832 us, 5.0 TB/s; with one workgroup a CU as much
+// by its instructions, about 60 an element. The gradients of 4 x 2048 x 2048 bf16 take 68 us (50 without the first pass:
+// 4.7 TB/s), of 256 x 1000 x 1024 fp32 1420, 5.2 TB/s. Small calls are launches: 64 tokens of 4096 channels 4.2 us.
 //
 // 1 - a^2 from a rounded a would lose its digits where a is near 1 (0.999 and more in use): with
 // q = 1 - e^{-z} by its series below z = 0.2, a = 1 - q and 1 - a^2 = q (1 + a).
@@ -715,9 +716,9 @@ constexpr int kNarrow = 32, kWavesNarrow = 8;   // channels and waves of narrow 
 //   - a turn of 256 workgroups takes the blocks of a segment, a last one of fewer at least 0.77 of that (16 blocks of
 //     128 workgroups 95 us, of 256 122);
 //   - a first pass over the blocks that others follow takes `again` of a block each, spread over the chip, and a launch.
-// Of sequences with lengths about 0.6 are taken to be there. us, one segment / the rule / twice its segments:
-// 1 x 32768 x 1024 588 / 100 / 107, 4 x 2048 x 2048 49.4 / 49.1 / 58.5, 8 x 4096 x 2048 122 / 122 / 155; gradients
-// 1123 / 137 / 143, 87.7 / 69.5 / 75.6, 220 / 220 / 259.
+// Of sequences with lengths about 0.6 are taken to be there. us, groups of 64 channels in one segment / by the rule / in twice
+// its segments: 1 x 32768 x 1024 633 / 110 / 112, 4 x 2048 x 2048 51 / 51 / 59, 8 x 4096 x 2048 132 / 132 / 173;
+// gradients 1090 / 142 / 146, 86 / 70 / 77, 225 / 225 / 278.
 // Short sequences leave most of a block of 256 steps empty: up to 16 steps go to single waves, and up to half a block, or four
 // blocks where two workgroups a CU are there to share it, to four waves. fp32, us, 16 waves / fewer: 64 x 16 x 1024 46 / 9,
 // 256 x 4 x 1024 168 / 12, 64 x 64 x 1024 47 / 16, 64 x 400 x 1024 103 / 78, 32 x 1000 x 1024 113 / 106, but 8 x 200 x 1024
