@@ -248,7 +248,9 @@ __global__ __launch_bounds__(512, 2) void norm_backward(NormArgs a) {
         for (int c = 0; c < NC; ++c)
             for (int j = 0; j < 8; ++j) cols[0][e0 + 512 * c + j] = cols[1][e0 + 512 * c + j] = 0.f;
     const long step = (long)RPG * gridDim.x;
-    constexpr bool kAhead = NC == 1 || (!GATE && sizeof(T) == 2 && !kHeld);   // (registers for the next row too)
+    // The next row is on its way where registers hold it too (fp32 rows of whole eights in one wave: 8192 x 768 42.6 / 41.4 us
+    // without / with; in two waves 4096 x 2048 51.6 / 53.7, which spills).
+    constexpr bool kAhead = NC == 1 || (!GATE && !kHeld && (sizeof(T) == 2 || (WPR == 1 && WHOLE)));
     Eight<T, WHOLE> x[NC], y[NC], z[NC], dn[NC], g0[NC], nx[NC], ny[NC], nz[NC], ndn[NC], ng0[NC];
     auto fetch_y = [&](int c, int e, long t, int left) { ny[c].load(row_of<T>(a.y, a.ldy, t) + e, left); };
     auto fetch_x = [&](int c, int e, long t, int left) { nx[c].load(row_of<T>(a.x, a.ldx, t) + e, left); };
