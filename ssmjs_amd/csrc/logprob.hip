@@ -10,7 +10,7 @@
 // from there on a logit enters only past the list's k-th, which few do: about k ln(n / 2048) of a random row.
 //
 // Memory bound: one read of the logits; the gradient reads and writes each once. 4096 x 50257 bf16 is read in 121 to
-// 127 us (3.3 TB/s, odd rows at the elements' alignment) and its gradient written in 134 to 142 (5.9 TB/s of both, part of it
+// 127 us (3.3 TB/s, odd rows at the elements' alignment) and its gradient written in 134 to 138 (6.0 TB/s of both, part of it
 // still in the caches); 2047 x 32000 fp32 with five alternatives takes 52 us (5.0 TB/s). Fewer rows with lists are bound by
 // the lists: 64 x 128000 fp32 with 20 alternatives 15 us and 5 for the joining, without 7 and 3.
 #include <algorithm>
@@ -25,44 +25,45 @@ constexpr float kFloor = -200.f;   // e^kFloor is 0 in fp32: differences are hel
 constexpr float kLowest = -3.40282347e38f;
 typedef unsigned long long u64;
 
-// WHOLE: rows of whole eights (`left` is at least 8, or nothing is there), which keeps the code short.
-template <bool WHOLE> __device__ __forceinline__ void load8(const float* p, int left, float (&f)[8]) {
+// Eight elements at p, from element `at` of a row of n on. WHOLE: rows of whole eights, all or none of which is there.
+template <bool WHOLE> __device__ __forceinline__ bool inside(int at, int n) { return WHOLE ? at < n : at >= 0 && at <= n - 8; }
+template <bool WHOLE> __device__ __forceinline__ void load8(const float* p, int at, int n, float (&f)[8]) {
     typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-    if (left >= 8) {
+    if (inside<WHOLE>(at, n)) {
         const f4 a = reinterpret_cast<const f4*>(p)[0], b = reinterpret_cast<const f4*>(p)[1];
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = a[j], f[4 + j] = b[j];
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = !WHOLE && j < left ? p[j] : -__builtin_inff();
+        for (int j = 0; j < 8; ++j) f[j] = !WHOLE && (unsigned)(at + j) < (unsigned)n ? p[j] : -__builtin_inff();
     }
 }
-template <bool WHOLE> __device__ __forceinline__ void load8(const __bf16* p, int left, float (&f)[8]) {
+template <bool WHOLE> __device__ __forceinline__ void load8(const __bf16* p, int at, int n, float (&f)[8]) {
     typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(2)));
-    if (left >= 8) {
+    if (inside<WHOLE>(at, n)) {
         const u4 a = *reinterpret_cast<const u4*>(p);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = __builtin_bit_cast(float, j % 2 ? a[j / 2] & 0xffff0000u : a[j / 2] << 16);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = !WHOLE && j < left ? (float)p[j] : -__builtin_inff();
+        for (int j = 0; j < 8; ++j) f[j] = !WHOLE && (unsigned)(at + j) < (unsigned)n ? (float)p[j] : -__builtin_inff();
     }
 }
-template <bool WHOLE> __device__ __forceinline__ void store8(float* p, int left, const float (&f)[8]) {
+template <bool WHOLE> __device__ __forceinline__ void store8(float* p, int at, int n, const float (&f)[8]) {
     typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-    if (left >= 8) {
+    if (inside<WHOLE>(at, n)) {
         reinterpret_cast<f4*>(p)[0] = f4{f[0], f[1], f[2], f[3]};
         reinterpret_cast<f4*>(p)[1] = f4{f[4], f[5], f[6], f[7]};
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (!WHOLE && j < left) p[j] = f[j];
+            if (!WHOLE && (unsigned)(at + j) < (unsigned)n) p[j] = f[j];
     }
 }
-template <bool WHOLE> __device__ __forceinline__ void store8(__bf16* p, int left, const float (&f)[8]) {
+template <bool WHOLE> __device__ __forceinline__ void store8(__bf16* p, int at, int n, const float (&f)[8]) {
     typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(2)));
     typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-    if (left >= 8) {
+    if (inside<WHOLE>(at, n)) {
         b8 b;
 #pragma unroll
         for (int j = 0; j < 8; ++j) b[j] = (__bf16)f[j];
@@ -70,8 +71,14 @@ template <bool WHOLE> __device__ __forceinline__ void store8(__bf16* p, int left
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (!WHOLE && j < left) p[j] = (__bf16)f[j];
+            if (!WHOLE && (unsigned)(at + j) < (unsigned)n) p[j] = (__bf16)f[j];
     }
+}
+// Where a row of bf16 begins in its 16 bytes. The gradient takes rows from there on, with all but their first and last eight
+// elements in place (us, eights from the row's first element on / this: 4096 x 50257 bf16 168 / 162, but 2048 x 50257 fp32
+// 157 / 163). The sums do not: their order would go by where a row lies.
+template <bool WHOLE, typename T> __device__ __forceinline__ int lead(const T* row) {
+    return WHOLE || sizeof(T) == 4 ? 0 : (int)((uintptr_t)row / sizeof(T) & 7);
 }
 
 // ---------------------------------------------------------------- sums
@@ -223,7 +230,7 @@ __global__ __launch_bounds__(256, TOP && sizeof(T) == 4 ? 5 : 8) void logprob_ke
         if (base >= a.N) break;
         float v[kGroups][8];
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) load8<WHOLE>(x + base + (g * 64 + lane) * 8, a.N - base - (g * 64 + lane) * 8, v[g]);
+        for (int g = 0; g < kGroups; ++g) load8<WHOLE>(x + base + (g * 64 + lane) * 8, base + (g * 64 + lane) * 8, a.N, v[g]);
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) take8(s, v[g]);
         if constexpr (TOP) {
@@ -351,22 +358,23 @@ __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
     const bool none = st.y == -__builtin_inff();
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+    const int base = piece * kRun - lead<WHOLE>(dx);
     float f[kGroups][8];
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-        const int at = piece * kRun + (g * 256 + (int)threadIdx.x) * 8;
-        load8<WHOLE>(x + at, a.N - at, f[g]);
+        const int at = base + (g * 256 + (int)threadIdx.x) * 8;
+        load8<WHOLE>(x + at, at, a.N, f[g]);
     }
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-        const int at = piece * kRun + (g * 256 + (int)threadIdx.x) * 8;
+        const int at = base + (g * 256 + (int)threadIdx.x) * 8;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float lp = (f[g][j] - st.x) - st.y, p = grow(lp);
             const float d = -p * fmaf(v, fmaxf(lp, kFloor) + h, w);
             f[g][j] = none ? 0.f : at + j == id ? d + w : d;
         }
-        store8<WHOLE>(dx + at, a.N - at, f[g]);
+        store8<WHOLE>(dx + at, at, a.N, f[g]);
     }
 }
 
@@ -376,6 +384,9 @@ int slices_of(int M, int N) {
     const long turns = ssm::cdiv(N, kRun);
     return (int)std::max(1L, std::min(std::min(turns, 64L), 1024L / std::max(1, M)));
 }
+
+// Rows on 16-byte places.
+bool in_place(const void* p, long bytes) { return (((uintptr_t)p | (uintptr_t)bytes) & 15) == 0; }
 
 size_t sums_bytes(int M, int slices) { return ((size_t)M * slices * sizeof(Sums) + 15) / 16 * 16; }
 
@@ -387,9 +398,9 @@ void run_logprobs(const LogArgs& a, hipStream_t st) {
     if (a.slices > 1) logprob_join<T><<<a.M, 256, 0, st>>>(a);
 }
 template <typename T>
-void run_grad(const GradArgs& a, hipStream_t st) {
+void run_grad(const GradArgs& a, bool whole, hipStream_t st) {
     const unsigned n = (unsigned)((long)a.M * a.pieces);
-    if (a.N % 8 == 0) logprob_grad<T, true><<<n, 256, 0, st>>>(a);
+    if (whole) logprob_grad<T, true><<<n, 256, 0, st>>>(a);
     else logprob_grad<T, false><<<n, 256, 0, st>>>(a);
 }
 
@@ -449,9 +460,10 @@ extern "C" ssm_status ssm_token_logprobs_backward(int dtype, const void* x, long
     SSM_REQUIRE(((uintptr_t)stats & 7) == 0, "ssm_token_logprobs_backward: stats must be 8-byte aligned");
     if (M == 1) ldx = lddx = N;
     SSM_REQUIRE(ldx >= N && lddx >= N, "ssm_token_logprobs_backward: row stride below row width");
-    const long pieces = ssm::cdiv(N, kRun);
-    SSM_REQUIRE(M * pieces <= ssm::kMaxGroups, "ssm_token_logprobs_backward: too many logits");
     const long es = dtype == SSM_F32 ? 4 : 2;
+    const bool whole = N % 8 == 0 && (dtype == SSM_F32 || in_place(dx, lddx * es));
+    const long pieces = ssm::cdiv(whole ? N : N + 7, kRun);
+    SSM_REQUIRE(M * pieces <= ssm::kMaxGroups, "ssm_token_logprobs_backward: too many logits");
     const ssm::Rows rx{x, ldx * es, N * es, M}, ox{dx, lddx * es, N * es, M};
     SSM_REQUIRE((dx == x && ldx == lddx) || !ssm::meet(ox, rx), "ssm_token_logprobs_backward: dx overlaps x, which it is not");
     SSM_REQUIRE(!ssm::meets(ox, ssm::block(ids, 4L * M), ssm::block(stats, 8L * M), ssm::block(entropy, 4L * M),
@@ -460,7 +472,7 @@ extern "C" ssm_status ssm_token_logprobs_backward(int dtype, const void* x, long
     GradArgs a{};
     a.x = x; a.ldx = ldx; a.ids = ids; a.stats = reinterpret_cast<const float2*>(stats); a.ent = entropy;
     a.dlogp = dlogp; a.dent = dentropy; a.dx = dx; a.lddx = lddx; a.M = M; a.N = N; a.pieces = (int)pieces;
-    if (dtype == SSM_F32) run_grad<float>(a, (hipStream_t)stream);
-    else run_grad<__bf16>(a, (hipStream_t)stream);
+    if (dtype == SSM_F32) run_grad<float>(a, whole, (hipStream_t)stream);
+    else run_grad<__bf16>(a, whole, (hipStream_t)stream);
     return ssm::check_launch("ssm_token_logprobs_backward");
 }

@@ -416,3 +416,32 @@ def test_infinities_at_other_lengths(bad, L):
 def test_other_groups(case, dtype):
     """The recurrence and its gradients, to the bounds of its own tests, where groups of 32 channels and few waves run."""
     recurrence.test_forward_backward(case, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_of_logits_wherever_rows_lie(dtype):
+    """Rows at every place in 16 bytes, of lengths around whole eights, gradients beside and in place: the bits of
+    contiguous rows, and nothing beside the rows written."""
+    from ssmjs_amd import kernels as k
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    for n in (1, 5, 8, 9, 16, 23, 8184, 8185, 8192, 8199, 16384):
+        print(f"[case] logits' gradient, {n} {dtype}", flush=True)
+        lg = torch.randn(3, n, generator=gen, device="cuda").to(dtype)
+        ids = torch.tensor([0, n // 2, n - 1], dtype=torch.int32, device="cuda")
+        stats = torch.empty(3, 2, device="cuda")
+        lp, ent, _, _ = k.token_logprobs(lg, ids, stats=stats)
+        w, v = torch.randn(3, generator=gen, device="cuda"), torch.randn(3, generator=gen, device="cuda")
+        want = k.token_logprobs_backward(lg, ids, stats, ent, w, v)
+        for shift in range(9):
+            for ld in (n, n + 3, n + 8):
+                a = torch.full((3 * ld + 40,), 5.0, dtype=dtype, device="cuda")
+                b = torch.full((3 * ld + 40,), 5.0, dtype=dtype, device="cuda")
+                xs, out = (t.as_strided((3, n), (ld, 1), 8 + o) for t, o in ((a, shift), (b, (shift * 5 + 3) % 9)))
+                xs.copy_(lg)
+                k.token_logprobs_backward(xs, ids, stats, ent, w, v, out=out)
+                k.token_logprobs_backward(xs, ids, stats, ent, w, v, out=xs)
+                torch.cuda.synchronize()
+                assert torch.equal(out, want) and torch.equal(xs, want)
+                for t, r in ((a, xs), (b, out)):
+                    r.fill_(5.0)
+                    assert bool((t == 5).all())
