@@ -7,10 +7,10 @@
 // Sums and everything between the loads and the stores are in fp32; x' enters n before its own rounding.
 //
 // Memory bound. A row lies in the registers of one wave, or of a few where it is long: each element is read once and
-// written once, and the sums over a row are lane exchanges. Rows need no alignment: vector loads and stores of
-// eight elements are made at the elements' own alignment, which the hardware splits where it must.
-// Measured: 16384 x 2048 bf16 62 us (5.4 TB/s), 8192 x 768 fp32 without gate 24 us (4.2 TB/s) and its gradients 40 (3.7 TB/s) and 5
-// for the columns' sums; 64 x 2048 3.5 us, two trips to memory and a launch.
+// written once (gradients of rows above 8192 elements read some again), and the sums over a row are lane exchanges. Rows
+// need no alignment: vector loads and stores of eight elements are made at the elements' own alignment, which the hardware
+// splits where it must. Measured: 16384 x 2048 bf16 62 us (5.4 TB/s), 8192 x 768 fp32 without gate 24 us (4.2 TB/s) and its
+// gradients 40 (3.7 TB/s) and 5 for the columns' sums; 64 x 2048 3.5 us, two trips to memory and a launch.
 #include <algorithm>
 
 #include "common.hpp"

@@ -445,3 +445,21 @@ def test_gradient_of_logits_wherever_rows_lie(dtype):
                 for t, r in ((a, xs), (b, out)):
                     r.fill_(5.0)
                     assert bool((t == 5).all())
+
+
+@pytest.mark.parametrize("n", [12, 100, 700, 5000])
+def test_lengths_out_of_range(n):
+    """Lengths below 0 are 0, lengths above L are L."""
+    from ssmjs_amd import kernels as k
+    print(f"[case] lengths out of range {n}", flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    f = lambda *s: torch.randn(*s, generator=gen, device="cuda")   # noqa: E731
+    x, r, i, dy, lam, h0 = f(4, n, 66), f(4, n, 66), f(4, n, 66), f(4, n, 66), f(66) - 3, f(4, 66)
+    got = []
+    for ln in ([-5, n + 7, 3, 2**31 - 1], [0, n, 3, n]):
+        ln = torch.tensor(ln, dtype=torch.int32, device="cuda")
+        st, hT, dh0 = k.gated_recurrence_states(4, n, 66, "cuda").zero_(), torch.empty_like(h0), torch.empty_like(h0)
+        y = k.gated_recurrence(x, r, i, lam, lengths=ln, h0=h0, hT=hT, states=st)
+        got.append([y, hT, st, dh0, *k.gated_recurrence_backward(dy, x, r, i, lam, st, lengths=ln, dhT=h0, dh0=dh0)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
