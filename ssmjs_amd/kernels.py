@@ -550,12 +550,14 @@ def gated_recurrence(x, r, i, lam, c=8.0, lengths=None, h0=None, hT=None, out=No
     pad = out is None
     if pad:
         out = _fresh(x, shape)
-    py = _at("out", out, shape, dt, dev)
+        py, ldy = out.data_ptr(), D
+    else:
+        py, ldy = _at("out", out, shape, dt, dev), _steps("out", out)
     state = (B, D)
     ws, pws, nbytes = _own_scratch(workspace, _lib.lib().ssm_gated_recurrence_workspace(B, L, D), x)
     _lib.call("ssm_gated_recurrence", code, x.data_ptr(), _steps("x", x), pr, _steps("r", r), pi, _steps("i", i),
               _packed("lam", lam, (D,), _f32_t, dev), c, _packed("lengths", lengths, (B,), _i32_t, dev), int(pad),
-              py, _steps("out", out), B, L, D, _packed("h0", h0, state, _f32_t, dev),
+              py, ldy, B, L, D, _packed("h0", h0, state, _f32_t, dev),
               _packed("hT", hT, state, _f32_t, dev),
               _packed("states", states, (B, -(-L // 64), D), _f32_t, dev), pws, nbytes, _on(dev))
     return out
@@ -575,9 +577,11 @@ def gated_recurrence_backward(dy, x, r, i, lam, states, c=8.0, lengths=None, dhT
     pg, pr, pi = _at("dy", dy, shape, dt, dev), _at("r", r, shape, dt, dev), _at("i", i, shape, dt, dev)
     pad = out is None
     if pad:
-        out = _fresh(x, shape), _fresh(x, shape), _fresh(x, shape)
-    dx, dr, di = out
-    pdx, pdr, pdi = (_at(f"out[{n}]", t, shape, dt, dev) for n, t in enumerate(out))
+        dx, dr, di = _fresh(x, shape), _fresh(x, shape), _fresh(x, shape)
+        places = dx.data_ptr(), D, dr.data_ptr(), D, di.data_ptr(), D
+    else:
+        dx, dr, di = out
+        places = [v for n, t in enumerate(out) for v in (_at(f"out[{n}]", t, shape, dt, dev), _steps(f"out[{n}]", t))]
     dlam = _fresh(lam, (D,))
     state = (B, D)
     ps = _packed("states", states, (B, -(-L // 64), D), _f32_t, dev)
@@ -585,8 +589,8 @@ def gated_recurrence_backward(dy, x, r, i, lam, states, c=8.0, lengths=None, dhT
     _lib.call("ssm_gated_recurrence_backward", code, pg, _steps("dy", dy), x.data_ptr(), _steps("x", x), pr,
               _steps("r", r), pi, _steps("i", i), _packed("lam", lam, (D,), _f32_t, dev), c,
               _packed("lengths", lengths, (B,), _i32_t, dev), int(pad), ps,
-              _packed("dhT", dhT, state, _f32_t, dev), pdx, _steps("out[0]", dx), pdr, _steps("out[1]", dr), pdi,
-              _steps("out[2]", di), dlam.data_ptr(), _packed("dh0", dh0, state, _f32_t, dev), B, L, D, pws, nbytes,
+              _packed("dhT", dhT, state, _f32_t, dev), *places, dlam.data_ptr(),
+              _packed("dh0", dh0, state, _f32_t, dev), B, L, D, pws, nbytes,
               _on(dev))
     return dx, dr, di, dlam
 
@@ -667,12 +671,14 @@ def block_norm_backward(dx1, dn, x, y, z=None, post=None, scale=None, pre=None, 
 
     if out is None:
         dx, dy, dz = _fresh(x, shape), _fresh(x, shape), _fresh(x, shape) if z is not None else None
+        places = dx.data_ptr(), D, dy.data_ptr(), D, None if dz is None else dz.data_ptr(), D
     else:
         dx, dy, dz = out
         if z is None:
             dz = None
         elif dz is None:
             raise ValueError("out[2]: a gate needs its gradient's tensor")
+        places = *side("out[0]", dx), *side("out[1]", dy), *side("out[2]", dz)
     # (one piece of memory each, as a program keeps or drops them one by one)
     dpost, dscale, dpre = (None if w is None else torch.empty_like(w) for w in (post, scale, pre))
     if T == 0:
@@ -684,7 +690,7 @@ def block_norm_backward(dx1, dn, x, y, z=None, post=None, scale=None, pre=None, 
     w = (D,)
     _lib.call("ssm_block_norm_backward", code, *side("dx1", dx1), *side("dn", dn), *side("x", x), *side("y", y),
               *side("z", z), _packed("post", post, w, _f32_t, dev), _packed("scale", scale, w, _f32_t, dev),
-              _packed("pre", pre, w, _f32_t, dev), eps, *side("out[0]", dx), *side("out[1]", dy), *side("out[2]", dz),
+              _packed("pre", pre, w, _f32_t, dev), eps, *places,
               None if dpost is None else dpost.data_ptr(), None if dscale is None else dscale.data_ptr(),
               None if dpre is None else dpre.data_ptr(), T, D, pws, nbytes, _on(dev))
     return dx, dy, dz, dpost, dscale, dpre
@@ -716,11 +722,13 @@ def token_logprobs_backward(logits, ids, stats, entropy=None, dlogp=None, dentro
     code, dev = _code(dt), _current("logits", logits)
     if out is None:
         out = _fresh(logits, (M, N))
-    po = _at("out", out, (M, N), dt, dev)
+        po, ldo = out.data_ptr(), N
+    else:
+        po, ldo = _at("out", out, (M, N), dt, dev), _ld("out", out)
     if stats is None:
         raise ValueError("token_logprobs_backward needs stats")
     _lib.call("ssm_token_logprobs_backward", code, logits.data_ptr(), _ld("logits", logits),
               _packed("ids", ids, (M,), _i32_t, dev), _packed("stats", stats, (M, 2), _f32_t, dev),
               _packed("entropy", entropy, (M,), _f32_t, dev), _packed("dlogp", dlogp, (M,), _f32_t, dev),
-              _packed("dentropy", dentropy, (M,), _f32_t, dev), po, _ld("out", out), M, N, _on(dev))
+              _packed("dentropy", dentropy, (M,), _f32_t, dev), po, ldo, M, N, _on(dev))
     return out
