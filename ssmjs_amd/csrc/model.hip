@@ -956,6 +956,7 @@ ssm_status ensure_ids(ssm_model* m, size_t n) {
         SSM_HIP_TRY(hipStreamSynchronize(m->ctx->stream));
         if (m->d_ids) SSM_HIP_TRY(hipFree(m->d_ids));
         m->d_ids = nullptr;
+        m->ids_cap = 0;
         SSM_HIP_TRY(ssm::dev_malloc((void**)&m->d_ids, n * sizeof(uint32_t)));
         m->ids_cap = n;
     }

@@ -219,6 +219,38 @@ def test_no_room_for_packed_operands(device, inject, nth, what):
     m.destroy()
 
 
+@pytest.mark.parametrize("nth", [1, 2, 3, 4])
+def test_score_goes_on_after_a_failed_allocation(device, inject, nth):
+    """A larger score whose nth allocation fails (the ids', which take the place of a smaller piece, first), then calls
+    that the smaller piece was enough for, and the larger one again."""
+    case(f"injected fault: allocation {nth} of a score")
+    from ssmjs_amd import _lib, backend
+    m = backend.Model(device, CFG, seed=8)
+    few = np.array([[5, 9, 33, 2]], np.uint32)
+    many = (np.arange(60, dtype=np.uint32) * 7 % 64)[None]
+    om = O.Model(m.export_weights())
+    small, before = m.score(few, k=3), m.forward(few)
+    inject(f"alloc:{nth}")
+    failed = False
+    try:
+        m.score(many, k=3)
+    except _lib.SsmError as e:
+        failed = True
+        assert e.status == 6
+    inject(None)
+    assert failed or nth > 1
+    again = m.score(few, k=3)
+    st = m.new_state(1)
+    st.prefill(few)
+    for got, ref in ((m.forward(few), before), (m.forward(many), om.forward(many))):
+        assert np.abs(got - ref).max() <= 1e-4 * max(1.0, np.abs(ref).max())
+    if nth == 1:      # (nothing else changed: the same bits)
+        for a, b in zip(small, again):
+            np.testing.assert_array_equal(a, b)
+    assert np.isfinite(m.score(many, k=3)[0]).all()
+    m.destroy()
+
+
 def test_session_create_reports_model_failure(inject):
     """MambaSession.create with every allocation failing: the device opens (no allocation), the
     model construction fails and the session raises SessionError('UNKNOWN') as session.ts
