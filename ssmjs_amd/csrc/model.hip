@@ -2006,6 +2006,7 @@ ssm_status ensure_gen(ssm_state* s, size_t n) {
         SSM_HIP_TRY(hipStreamSynchronize(s->m->ctx->stream));
         if (s->d_gen) SSM_HIP_TRY(hipFree(s->d_gen));
         s->d_gen = nullptr;
+        s->gen_cap = 0;
         SSM_HIP_TRY(ssm::dev_malloc((void**)&s->d_gen, n * 4));
         s->gen_cap = n;
     }
@@ -2211,6 +2212,7 @@ extern "C" ssm_status ssm_generate_sample(ssm_model* m, ssm_state* s, const uint
         SSM_HIP_TRY(hipStreamSynchronize(st));
         if (s->d_u) SSM_HIP_TRY(hipFree(s->d_u));
         s->d_u = nullptr;
+        s->u_cap = 0;
         SSM_HIP_TRY(ssm::dev_malloc((void**)&s->d_u, nu * sizeof(double)));
         s->u_cap = nu;
     }

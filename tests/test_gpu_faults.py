@@ -251,6 +251,33 @@ def test_score_goes_on_after_a_failed_allocation(device, inject, nth):
     m.destroy()
 
 
+@pytest.mark.parametrize("nth", [1, 2])
+def test_generation_goes_on_after_a_failed_allocation(device, inject, nth):
+    """A longer generation that has no room for its tokens (nth = 1) or, sampled, its draws (2), then one as long as before."""
+    case(f"injected fault: allocation {nth} of a generation")
+    from ssmjs_amd import _lib, backend
+    m = backend.Model(device, CFG, seed=9)
+    st = m.new_state(2)
+    prompt = np.array([[5, 9, 33], [2, 7, 60]], np.uint32)
+    u = np.random.default_rng(3).random((40, 2))
+    greedy = lambda n: (st.reset(), st.generate_greedy(prompt, n))[1]   # noqa: E731
+    sample = lambda n: (st.reset(), st.generate_sample(prompt, n, 0.8, 20, 0.9, u[:n]))[1]   # noqa: E731
+    short = [sample(3), greedy(3)]
+    for call in (sample, greedy)[:3 - nth]:
+        inject(f"alloc:{nth}")
+        with pytest.raises(_lib.SsmError) as e:
+            call(20 if call == sample else 40)
+        assert e.value.status == 6
+        inject(None)
+        for got, want in zip((sample(3), greedy(3)), short):
+            np.testing.assert_array_equal(got, want)
+        for long in (sample(20), greedy(20)):
+            assert (long < CFG["vocabSize"]).all()
+    np.testing.assert_array_equal(sample(20)[:, :3], short[0])
+    np.testing.assert_array_equal(greedy(20)[:, :3], short[1])
+    m.destroy()
+
+
 def test_session_create_reports_model_failure(inject):
     """MambaSession.create with every allocation failing: the device opens (no allocation), the
     model construction fails and the session raises SessionError('UNKNOWN') as session.ts
