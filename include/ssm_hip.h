@@ -306,7 +306,7 @@ ssm_status ssm_gated_recurrence(int dtype, const void* x, long ldx, const void* 
 /* Its gradients: dy (B,L,D) and dhT (B,D; NULL: zeros) are those of y and hT; dx, dr, di (B,L,D; rows behind a
  * sequence's end as y's), dlam (D) and dh0 (B,D; may be NULL or dhT) those of the inputs. `states` as the
  * forward call with the same x, r, i, lam, c and lengths left them. Sums over tokens are in one order: the same call
- * gives the same bits. workspace: 16-byte aligned, ssm_gated_recurrence_backward_workspace(...) bytes, never 0. */
+ * gives the same bits. B >= 1. workspace: 16-byte aligned, ssm_gated_recurrence_backward_workspace(...) bytes, never 0. */
 size_t ssm_gated_recurrence_backward_workspace(int B, int L, int D);
 ssm_status ssm_gated_recurrence_backward(int dtype, const void* dy, long lddy, const void* x, long ldx, const void* r,
                                          long ldr, const void* i, long ldi, const float* lam, float c,

@@ -568,7 +568,8 @@ def gated_recurrence_backward(dy, x, r, i, lam, states, c=8.0, lengths=None, dhT
     """Gradients of gated_recurrence (ssm_gated_recurrence_backward): returns (dx, dr, di, dlam). dy and the first
     three (B,L,D) in x's type, dlam (D) float32; `states` as the forward call filled them. dhT, the gradient of hT,
     and dh0, which receives that of h0: (B,D) float32 or None, dh0 may be dhT. `out`: tensors for dx, dr, di, whose
-    rows from a sequence's length on are not written (else zeros)."""
+    rows from a sequence's length on are not written (else zeros). A batch
+    of no sequences gives zeros for dlam."""
     if x.dim() != 3:
         raise ValueError("x, r, i (B,L,D)")
     shape, dt = x.shape, x.dtype
@@ -584,14 +585,15 @@ def gated_recurrence_backward(dy, x, r, i, lam, states, c=8.0, lengths=None, dhT
         places = [v for n, t in enumerate(out) for v in (_at(f"out[{n}]", t, shape, dt, dev), _steps(f"out[{n}]", t))]
     dlam = _fresh(lam, (D,))
     state = (B, D)
-    ps = _packed("states", states, (B, -(-L // 64), D), _f32_t, dev)
+    ps, pl = _packed("states", states, (B, -(-L // 64), D), _f32_t, dev), _packed("lam", lam, (D,), _f32_t, dev)
+    pn = _packed("lengths", lengths, (B,), _i32_t, dev)
+    pT, p0 = _packed("dhT", dhT, state, _f32_t, dev), _packed("dh0", dh0, state, _f32_t, dev)
+    if B == 0:
+        return dx, dr, di, dlam.zero_()
     ws, pws, nbytes = _own_scratch(workspace, _lib.lib().ssm_gated_recurrence_backward_workspace(B, L, D), x)
     _lib.call("ssm_gated_recurrence_backward", code, pg, _steps("dy", dy), x.data_ptr(), _steps("x", x), pr,
-              _steps("r", r), pi, _steps("i", i), _packed("lam", lam, (D,), _f32_t, dev), c,
-              _packed("lengths", lengths, (B,), _i32_t, dev), int(pad), ps,
-              _packed("dhT", dhT, state, _f32_t, dev), *places, dlam.data_ptr(),
-              _packed("dh0", dh0, state, _f32_t, dev), B, L, D, pws, nbytes,
-              _on(dev))
+              _steps("r", r), pi, _steps("i", i), pl, c, pn, int(pad), ps, pT, *places, dlam.data_ptr(), p0, B, L, D,
+              pws, nbytes, _on(dev))
     return dx, dr, di, dlam
 
 
