@@ -149,6 +149,16 @@ def test_workspaces_agree_with_the_launches():
     assert f"{need} bytes".encode() in L.ssm_last_error()
 
 
+@pytest.mark.parametrize("B,L,D,cut", [
+    (8, 4096, 2048, False), (4, 2048, 2048, False), (256, 1000, 1024, False), (64, 16, 1024, False), (1, 256, 64, False),
+    (1, 32768, 1024, True), (1, 5000, 516, True), (2, 4000, 392, True), (3, 3000, 392, True)])
+def test_room_for_segments(B, L, D, cut):
+    """A forward call whose sequences are cut keeps a pair of floats for each block of 256 steps and one more, of every
+    channel and sequence, to whole 16 bytes; one whose sequences are walked whole keeps nothing."""
+    need = _lib.lib().ssm_gated_recurrence_workspace(B, L, D)
+    assert need == ((B * (-(-L // 256) + 1) * D * 8 + 15) // 16 * 16 if cut else 0)
+
+
 # What each operand covers, of the calls above: bytes from its first to past its last
 ROWS, WIDE = 15 * 200 + 200, 15 * 400 + 200
 SIZES = {
