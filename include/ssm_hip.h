@@ -290,7 +290,7 @@ ssm_status ssm_linear_q8(int in_dtype, const void* x, long ldx, const int8_t* W,
 /* Gated linear recurrence over whole prompts, for every channel d:
  *   z_t = c softplus(lam_d) sigmoid(r_t),  a_t = e^{-z_t}
  *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t,  y_t = h_t   (h in fp32)
- * x, r, i, y (B,L,D) with row strides; lam (D) float; c >= 0. lengths (B) int32 on the device or NULL: sequence b
+ * x, r, i, y (B,L,D) with row strides; lam (D) float; c >= 0, c softplus(lam) counted up to 2^64. lengths (B) int32 on the device or NULL: sequence b
  * has lengths[b] tokens (held to 0 .. L); rows of y from there on become zeros with `pad`, else are not written, and
  * what x, r and i hold there is not used. h0, hT (B,D) float: the states before the first and after each sequence's last token; either may be
  * NULL, hT may be h0. states (B, ceil(L / 64), D) float or NULL: the states entering tokens 0, 64, 128 .. of each

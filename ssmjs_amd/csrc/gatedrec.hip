@@ -102,6 +102,13 @@ __device__ __forceinline__ float fall_held(float v) {
 }
 __device__ __forceinline__ float open(float e) { return __builtin_amdgcn_rcpf(1.f + e); }   // sigmoid of e = e^-v
 
+// c softplus(lam), counted up to 2^64: its product with any gate is then finite, and with one below fp32's range (0, or
+// 2^-126 by fall_held) next to 0. (A NaN stays one.)
+__device__ __forceinline__ float rate(float c, float lam) {
+    const float k = c * ssm::softplus(lam);
+    return k > 0x1p64f ? 0x1p64f : k;
+}
+
 // 1 - e^-z for z <= kSeries: its first six terms, whose rest is below 0.2^6 / 7! = 1.3e-8 of it.
 __device__ __forceinline__ float lost_small(float z) {
     float p = fmaf(z, -1.f / 720, 1.f / 120);
@@ -196,7 +203,7 @@ struct Place {
         bool near = true;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            kd[v] = live ? a.c * ssm::softplus(a.lam[ch + v]) : 0.f;
+            kd[v] = live ? rate(a.c, a.lam[ch + v]) : 0.f;
             near &= kd[v] <= kSeries;
         }
         return __all(near);
@@ -698,7 +705,7 @@ __global__ __launch_bounds__(256) void rec_step(RecArgs a) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
         float d, q;
-        decay(a.c * ssm::softplus(lam[v]) * open(fall((float)r[v])), false, d, q);
+        decay(rate(a.c, lam[v]) * open(fall((float)r[v])), false, d, q);
         const float bt = __builtin_amdgcn_sqrtf(fmaf(q, d, q)) * (open(fall((float)i[v])) * (float)x[v]);
         h[v] = onto(d, bt, h[v]);
         y[v] = (T)h[v];
