@@ -290,10 +290,10 @@ ssm_status ssm_linear_q8(int in_dtype, const void* x, long ldx, const int8_t* W,
 /* Gated linear recurrence over whole prompts, for every channel d:
  *   z_t = c softplus(lam_d) sigmoid(r_t),  a_t = e^{-z_t}
  *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t,  y_t = h_t   (h in fp32)
- * x, r, i, y (B,L,D) with row strides; lam (D) float; c >= 0, c softplus(lam) counted up to 2^64. lengths (B) int32 on the device or NULL: sequence b
- * has lengths[b] tokens (held to 0 .. L); rows of y from there on become zeros with `pad`, else are not written, and
- * what x, r and i hold there is not used. h0, hT (B,D) float: the states before the first and after each sequence's last token; either may be
- * NULL, hT may be h0. states (B, ceil(L / 64), D) float or NULL: the states entering tokens 0, 64, 128 .. of each
+ * x, r, i, y (B,L,D) with row strides; lam (D) float; c >= 0, c softplus(lam) counted up to 2^64. lengths (B) int32
+ * on the device or NULL: sequence b has lengths[b] tokens (held to 0 .. L); rows of y from there on become zeros with
+ * `pad`, else are not written, and what x, r and i hold there is not used. h0, hT (B,D) float: the states before the
+ * first and after each sequence's last token; either may be NULL, hT may be h0. states (B, ceil(L / 64), D) float or NULL: the states entering tokens 0, 64, 128 .. of each
  * sequence, which the backward pass needs (those behind a sequence's end are not written). An infinite state
  * stays infinite; an inf or NaN changes no earlier token and no other channel. Outputs, states and the workspace
  * overlap nothing else. Row strides below 2^20, L <= 2^30. `workspace` (16-byte aligned) holds
@@ -327,8 +327,9 @@ ssm_status ssm_block_norm(int dtype, const void* x, long ldx, const void* y, lon
                           const float* post, const float* scale, const float* pre, float eps, void* x1, long ldx1, void* n,
                           long ldn, int T, int D, void* stream);
 /* Its gradients from dx1 (of x'; NULL: zeros) and dn: dx, dy and, with z, dz (T,D), and over all rows dpost, dscale,
- * dpre (D) float (each may be NULL). dx may be dx1; outputs and the workspace overlap nothing else. Sums over rows are in one
- * order. T >= 1. workspace: 16-byte aligned, ssm_block_norm_backward_workspace(...) bytes, one stream at a time. */
+ * dpre (D) float (each may be NULL); x and y as the forward call read them. dx may be dx1; outputs and the workspace
+ * overlap nothing else. Sums over rows are in one order. T >= 1. workspace: 16-byte aligned,
+ * ssm_block_norm_backward_workspace(...) bytes, one stream at a time. */
 size_t ssm_block_norm_backward_workspace(int T, int D);
 ssm_status ssm_block_norm_backward(int dtype, const void* dx1, long lddx1, const void* dn, long lddn, const void* x,
                                    long ldx, const void* y, long ldy, const void* z, long ldz, const float* post,

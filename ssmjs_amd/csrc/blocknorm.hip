@@ -9,8 +9,9 @@
 // Memory bound. A row lies in the registers of one wave, or of a few where it is long: each element is read once and
 // written once (gradients of rows above 8192 elements read some again), and the sums over a row are lane exchanges. Rows
 // need no alignment: vector loads and stores of eight elements are made at the elements' own alignment, which the hardware
-// splits where it must. Measured: 16384 x 2048 bf16 62 us (5.4 TB/s), 8192 x 768 fp32 without gate 24 us (4.2 TB/s) and its
-// gradients 40 (3.7 TB/s) and 5 for the columns' sums; 64 x 2048 3.5 us, two trips to memory and a launch.
+// splits where it must. Measured: 16384 x 2048 bf16 63 us (5.3 TB/s) and its gradients 137 (3.9 TB/s), 8192 x 768 fp32 without
+// gate 24 us (4.2 TB/s) and its gradients 40 (3.7 TB/s) and 5 for the columns' sums; 64 x 2048 3.4 us, two trips to memory
+// and a launch.
 #include <algorithm>
 
 #include "common.hpp"
@@ -235,7 +236,7 @@ __global__ __launch_bounds__(512, 2) void norm_backward(NormArgs a) {
     constexpr int W = 8, RPG = W / WPR;   // rows at a time
     // Rows above 8192 elements have more than fits in registers: two of the column sums stay in LDS, and of a row's operands
     // y alone is held, the others read again from the cache where they are wanted (1024 x 16384, all held by 16 waves / this:
-    // bf16 311 / 176 us, fp32 325 / 254)
+    // bf16 311 / 177 us, fp32 325 / 260)
     constexpr bool kHeld = NC > 2;
     __shared__ float red[2][W];
     __shared__ alignas(16) float cols[kHeld ? 2 : RPG][512 * NC * WPR];
@@ -429,7 +430,7 @@ void go_forward(const NormArgs& a, hipStream_t st) {
 template <typename T>
 void forward_of(const NormArgs& a, hipStream_t st) {
     // eight elements a lane, as many waves as that takes (us, against four times the elements and a quarter of the
-    // waves: 64 x 2048 bf16 2.9 / 5.0, 16384 x 2048 55.8 / 65.7, 4096 x 8192 61 / 67)
+    // waves: 64 x 2048 bf16 3.4 / 5.8, 16384 x 2048 62.9 / 64.6, 4096 x 8192 63.8 / 69.0)
     if (a.D <= 512) go_forward<T, 1, 1>(a, st);
     else if (a.D <= 1024) go_forward<T, 1, 2>(a, st);
     else if (a.D <= 2048) go_forward<T, 1, 4>(a, st);

@@ -13,13 +13,14 @@
 // Where the sequences' channels are too few to fill the chip, sequences are cut into segments of whole blocks: a
 // first pass forms the (A, H) of every block that others follow, and each segment starts from the composition of
 // those before it. (One pass, with workgroups that wait for the results of those before them, read the inputs once
-// and took as long, the waiting ones' looks at memory costing what the second reading costs. us, two passes / one:
-// 1 x 32768 x 1024 bf16 100 / 122, 8 x 4096 x 2048 130 / 155, 4 x 2048 x 2048 49 / 52.)
+// and took longer, the waiting ones' looks at memory costing more than the second reading. us, two passes / one, when both
+// were built: 1 x 32768 x 1024 bf16 100 / 122 to 134, 8 x 4096 x 2048 130 / 155 to 160, 4 x 2048 x 2048 49 / 52.)
 //
-// Bound by memory where the chip is full, 8 x 4096 x 2048 bf16 131 us, 4.1 TB/s (rows' pieces of 128 bytes read and written
-// with nothing else done take 118, whole rows 106), 256 x 1000 x 1024 fp32 832 us, 5.0 TB/s; with one workgroup a CU as much
-// by its instructions, about 60 an element. The gradients of 4 x 2048 x 2048 bf16 take 68 us (50 without the first pass:
-// 4.7 TB/s), of 256 x 1000 x 1024 fp32 1420, 5.2 TB/s. Small calls are launches: 64 tokens of 4096 channels 4.2 us.
+// Bound by memory where the chip is full, 8 x 4096 x 2048 bf16 131 to 135 us, 4.1 TB/s (rows' pieces of 128 bytes read and
+// written with nothing else done take 118, whole rows 106), 256 x 1000 x 1024 fp32 827 us, 5.1 TB/s; with one workgroup a CU as
+// much by its instructions, about 60 an element. The gradients of 4 x 2048 x 2048 bf16 take 68 to 73 us (50 to 52 without the
+// first pass and the last sum: 4.6 TB/s), of 256 x 1000 x 1024 fp32 1412, 5.2 TB/s. Small calls are launches: 64 tokens of 4096
+// channels 4.2 to 4.5 us.
 //
 // 1 - a^2 from a rounded a would lose its digits where a is near 1 (0.999 and more in use): with
 // q = 1 - e^{-z} by its series below z = 0.2, a = 1 - q and 1 - a^2 = q (1 + a).
@@ -761,7 +762,8 @@ Plan plan_of(int B, int L, int D, int waves, double again, bool ragged, double* 
 // Groups of 32 channels put twice the workgroups on sequences that are walked whole, where those are few enough for one a CU:
 // a block then takes 0.4 (up to 80 workgroups) to 0.73 (256) of a full chip's. us, wide groups by the rule above / narrow:
 // 4 x 2048 x 2048 bf16 50 / 45, fp32 81 / 61, 5 x 1500 x 1536 fp32 with lengths 39 / 27, 2 x 600 x 2048 bf16 24 / 14, but
-// 2 x 4096 x 2048 bf16 56 / 71 and 1 x 8192 x 512 fp32 33 / 99. With lengths the segments' share is the less even one.
+// 2 x 4096 x 2048 bf16 56 / 71 and 1 x 8192 x 512 fp32 33 / 99. With lengths the segments' share is the less even one: the
+// 1.25, and the 0.6 above, are from the ragged batch named here alone.
 Plan plan_forward(int B, int L, int D, bool ragged) {
     double best = 0;
     const Plan p = plan_of(B, L, D, kWaves, 0.7, ragged, &best);

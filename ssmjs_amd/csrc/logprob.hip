@@ -9,10 +9,11 @@
 // values and, of equal ones, for lower indices). The first 2048 logits give the maximum of each lane, sorted at once;
 // from there on a logit enters only past the list's k-th, which few do: about k ln(n / 2048) of a random row.
 //
-// Memory bound: one read of the logits; the gradient reads and writes each once. 4096 x 50257 bf16 is read in 121 to
-// 127 us (3.3 TB/s, odd rows at the elements' alignment) and its gradient written in 134 to 138 (6.0 TB/s of both, part of it
-// still in the caches); 2047 x 32000 fp32 with five alternatives takes 52 us (5.0 TB/s). Fewer rows with lists are bound by
-// the lists: 64 x 128000 fp32 with 20 alternatives 15 us and 5 for the joining, without 7 and 3.
+// Memory bound: one read of the logits; the gradient reads and writes each once. 4096 x 50257 bf16 (odd rows at the
+// elements' alignment) is read in 93 us (4.4 TB/s), in 121 to 127 behind a gradient's writes, and its gradient takes 151
+// (5.4 TB/s), or 134 to 138 behind its forward call, with part of the logits still in the caches; 2047 x 32000 fp32 with five
+// alternatives takes 52 us (5.0 TB/s). Lists bound bf16 rows, 45 us for 2047 x 32000 (2.9 TB/s), 117 for 4096 x 50257, and
+// few rows: 64 x 128000 fp32 with 20 alternatives 15 us and 5 for the joining, without 7 and 3.
 #include <algorithm>
 
 #include "common.hpp"
@@ -75,8 +76,9 @@ template <bool WHOLE> __device__ __forceinline__ void store8(__bf16* p, int at, 
     }
 }
 // Where a row of bf16 begins in its 16 bytes. The gradient takes rows from there on, with all but their first and last eight
-// elements in place (us, eights from the row's first element on / this: 4096 x 50257 bf16 168 / 162, but 2048 x 50257 fp32
-// 157 / 163). The sums do not: their order would go by where a row lies.
+// elements in place (us, eights from the row's first element on / this: 4096 x 32001 bf16 111 / 105, 4096 x 50257 152 / 152, with
+// its forward call 262.4 / 261.7, 16000 x 5003 69 / 74; 2048 x 50257 fp32 156 / 163). The sums do not: their order would go by
+// where a row lies.
 template <bool WHOLE, typename T> __device__ __forceinline__ int lead(const T* row) {
     return WHOLE || sizeof(T) == 4 ? 0 : (int)((uintptr_t)row / sizeof(T) & 7);
 }
@@ -210,7 +212,8 @@ __device__ __forceinline__ void finish(const LogArgs& a, int row, Sums s, u64 li
     }
 }
 
-// (waves a SIMD for its registers, us: 4096 x 50257 bf16, five alternatives, 8 waves 117, 5 138; 2047 x 32000 fp32 58, 52)
+// (waves a SIMD for its registers, us, five alternatives, 8 waves / 5: bf16 4096 x 50257 117 / 137, 2047 x 32000 45 / 51, but fp32
+// 2047 x 32000 58 / 52)
 template <typename T, bool TOP, bool WHOLE>
 __global__ __launch_bounds__(256, TOP && sizeof(T) == 4 ? 5 : 8) void logprob_kernel(LogArgs a) {
     __shared__ Sums ws[4];

@@ -661,7 +661,8 @@ def block_norm(x, y, z=None, post=None, scale=None, pre=None, eps=1e-6, out=None
 
 def block_norm_backward(dx1, dn, x, y, z=None, post=None, scale=None, pre=None, eps=1e-6, out=None, workspace=None):
     """Gradients of block_norm (ssm_block_norm_backward) from dx1, that of x' (None: zeros), and dn: returns
-    (dx, dy, dz, dpost, dscale, dpre), None for what was None. `out`: tensors for dx, dy, dz; dx may be dx1."""
+    (dx, dy, dz, dpost, dscale, dpre), None for what was None. x and y as block_norm read them: a call whose outputs took
+    their places has no gradients any more. `out`: tensors for dx, dy, dz; dx may be dx1."""
     shape, dt = x.shape, x.dtype
     D, T = shape[-1], _rows_of(x)
     code, dev = _code(dt), _current("x", x)
