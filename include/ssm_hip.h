@@ -293,11 +293,12 @@ ssm_status ssm_linear_q8(int in_dtype, const void* x, long ldx, const int8_t* W,
  * x, r, i, y (B,L,D) with row strides; lam (D) float; c >= 0, c softplus(lam) counted up to 2^64. lengths (B) int32
  * on the device or NULL: sequence b has lengths[b] tokens (held to 0 .. L); rows of y from there on become zeros with
  * `pad`, else are not written, and what x, r and i hold there is not used. h0, hT (B,D) float: the states before the
- * first and after each sequence's last token; either may be NULL, hT may be h0. states (B, ceil(L / 64), D) float or NULL: the states entering tokens 0, 64, 128 .. of each
- * sequence, which the backward pass needs (those behind a sequence's end are not written). An infinite state
- * stays infinite; an inf or NaN changes no earlier token and no other channel. Outputs, states and the workspace
- * overlap nothing else. Row strides below 2^20, L <= 2^30. `workspace` (16-byte aligned) holds
- * ssm_gated_recurrence_workspace(...) bytes (0 where no sequence is cut) and serves one stream at a time. */
+ * first and after each sequence's last token; either may be NULL, hT may be h0. states (B, ceil(L / 64), D) float or
+ * NULL: the states entering tokens 0, 64, 128 .. of each sequence, which the backward pass needs (those behind a
+ * sequence's end are not written). An infinite state stays infinite; an inf or NaN changes no earlier token and no
+ * other channel. Outputs, states and the workspace overlap nothing else. Row strides below 2^20, L <= 2^30.
+ * `workspace` (16-byte aligned) holds ssm_gated_recurrence_workspace(...) bytes (0 where no sequence is cut) and serves
+ * one stream at a time. */
 size_t ssm_gated_recurrence_workspace(int B, int L, int D);
 ssm_status ssm_gated_recurrence(int dtype, const void* x, long ldx, const void* r, long ldr, const void* i, long ldi,
                                 const float* lam, float c, const int* lengths, int pad, void* y, long ldy, int B, int L,
